@@ -1,0 +1,45 @@
+"""Cache pages in 8 bits: codes with one scale per token and kv head.
+
+A head's row x of a token is kept as codes c = round(127 x / a), a = max |x|, and the float32 scale a / 127; it is read as
+c * scale (`csrc/cache_q8.cu` writes and reads them, `csrc/attention_q8*.cu` attends over them).  A `QuantisedPages` stands
+wherever the kernels take a layer's keys or values: `rope_kv_write`, `kv_write`, `kv_read` and `paged_attention`.
+Azimml/shrike's pool has one form, the model's dtype (shrike/engine/model_runner.py:52-60).
+"""
+
+from __future__ import annotations
+
+import torch
+
+
+class QuantisedPages:
+    """`codes` int8 [pages, page_size, kv heads, head size], `scales` float32 [pages, kv heads, page_size], on one device."""
+
+    __slots__ = ("codes", "scales")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor):
+        if codes.dtype != torch.int8 or codes.dim() != 4 or not codes.is_contiguous():
+            raise ValueError("codes must be a contiguous int8 [pages, page_size, kv heads, head size]")
+        pages, page_size, heads, _dim = codes.shape
+        if scales.dtype != torch.float32 or tuple(scales.shape) != (pages, heads, page_size) or not scales.is_contiguous():
+            raise ValueError(f"scales must be a contiguous float32 [{pages}, {heads}, {page_size}], are "
+                             f"{scales.dtype} {list(scales.shape)}")
+        if codes.device != scales.device:
+            raise ValueError(f"codes are on {codes.device}, scales on {scales.device}")
+        self.codes, self.scales = codes, scales
+
+    @classmethod
+    def zeros(cls, pages: int, page_size: int, kv_heads: int, head_dim: int, device) -> "QuantisedPages":
+        return cls(torch.zeros(pages, page_size, kv_heads, head_dim, dtype=torch.int8, device=device),
+                   torch.zeros(pages, kv_heads, page_size, dtype=torch.float32, device=device))
+
+    @property
+    def shape(self) -> torch.Size:
+        """That of the codes: [pages, page_size, kv heads, head size], as a pool in the engine's type has it."""
+        return self.codes.shape
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
+
+    def bytes(self) -> int:
+        return self.codes.numel() + 4 * self.scales.numel()

@@ -1,0 +1,738 @@
+// Paged attention over keys and values in 8 bits, for any head size up to 256, any page size, queries in bfloat16 or float32.
+//
+// With codes c and scales s (keys: c^k_j, s^k_j; values: c^v_j, s^v_j) a row q of head h sees
+//   z_j = scale s^k_j (q . c^k_j),   p_j = 2^(log2e z_j - m),   o = sum_j (p_j s^v_j) c^v_j / sum_j p_j
+// Codes are integers up to 127: exact in float16.  Both products run on mma.sync m16n8k16 with float16 operands and float32
+// sums, and nothing but the queries and the weights is ever rounded:
+//   queries   scaled by a power of two per row (largest magnitude in [2^14, 2^15)); bfloat16 queries are then exact, float32
+//             ones are split in two float16 parts (22 bits) whose products are added in the accumulator
+//   weights   w_j = p_j s^v_j.  The base m of the exponentials is a row's largest score plus an exponent F that puts the largest
+//             value scale the row has seen at 2^13 ... 2^14 (the sums and the outputs are all in units of 2^m, so F costs
+//             nothing): float16 then keeps 11 bits of a weight down to 2^-27 of the largest possible one (bfloat16 would keep 8
+//             bits), and 22 bits in two parts for float32
+// A warp takes 16 query rows (the heads that share a kv head side by side, token by token) against 32 keys a step.
+//
+// The keys' order inside a product is free as long as scores and values agree on it, and so is the order of a head's elements
+// in q . c: both are chosen so that a lane's operands are consecutive bytes.  Element order: a lane reads 16 codes of a key
+// with one load and they are its operands of four products.  Key order: column n of a group of eight is key n ^ ((n >> 1) & 1),
+// and 16-byte chunks of a row are swizzled with it, so that neither the keys' nor the values' loads meet in a bank.
+// Four codes become two registers of float16 pairs by a byte permutation (1024 + code + 128, exact) and a subtraction.
+//
+// Two forms.  Few rows (single tokens): the rows' keys are dealt to `splits` CTAs and to each CTA's four warps, each with its
+// own ring of cp.async copies (no barrier in the loop); the warps' results meet in shared memory, the CTAs' in global memory,
+// where the last CTA to arrive adds them up in the order of the splits.  Many rows (portions): four warps of 16 rows each share
+// one ring of key tiles.
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+
+#ifndef SHRIKE_HEAD_DIM
+#error "compile with -DSHRIKE_HEAD_DIM=<head size>"
+#endif
+
+namespace attnq8 {
+
+constexpr int D = SHRIKE_HEAD_DIM;
+static_assert(D % 16 == 0 && D >= 16 && D <= 256, "head sizes are multiples of 16 up to 256");
+constexpr int WARPS = 4, THREADS = WARPS * 32;
+constexpr int ROWS = 16;                 // query rows of a warp
+constexpr int KEYS = 32;                 // keys of a step
+constexpr int CHUNKS = D / 16;           // 16-byte chunks of a key's codes
+constexpr int STEPS_K = D / 16;          // products along the head size, for 8 keys
+constexpr int BLOCKS_V = (D + 31) / 32;  // runs of 32 elements of the output
+constexpr bool WIDE = D % 64 == 0;       // keys are read 16 bytes a lane (else 4)
+constexpr int TILE = KEYS * D;           // bytes of a step's key (or value) codes
+constexpr int STAGE = 2 * TILE + 2 * KEYS * 4;   // keys, values, and their scales
+constexpr int STAGES = 3;
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr int MAX_SPLITS = 64;
+
+struct Args {
+  const signed char* k_codes;
+  const float* k_scales;
+  const signed char* v_codes;
+  const float* v_scales;
+  const int* block_table;
+  const int* q_start;
+  const int* ctx_len;
+  const void* q;
+  void* out;
+  int max_blocks, num_heads, num_kv_heads, page_size, num_pages, window;
+  int only;            // 1: entries of one token, 2: longer ones, 0: all
+  float scale_log2;
+  int splits;
+  float* scratch;      // [(entry, kv head, row tile)][split][16][D + 2]: unnormalised rows, then each row's base and sum
+  int* arrivals;       // [(entry, kv head, row tile)]: CTAs that have left their share; zero between launches
+};
+
+__device__ __forceinline__ float fast_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ unsigned smem_u32(const void* p) { return static_cast<unsigned>(__cvta_generic_to_shared(p)); }
+__device__ __forceinline__ void copy16(unsigned dst, const void* src, bool there) {   // zeros where there is nothing
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy4(unsigned dst, const void* src, bool there) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(there ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
+
+__device__ __forceinline__ void mma(float (&c)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ unsigned pack_half(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const unsigned*>(&h);
+}
+__device__ __forceinline__ float low_half(unsigned v) { return __low2float(*reinterpret_cast<const __half2*>(&v)); }
+__device__ __forceinline__ float high_half(unsigned v) { return __high2float(*reinterpret_cast<const __half2*>(&v)); }
+// Two codes, biased by 128 in bytes 0, 1 (or 2, 3) of `biased`, as float16: byte b under 0x64 is 1024 + b.
+template <int SELECT> __device__ __forceinline__ unsigned codes_to_half(unsigned biased) {
+  const unsigned raw = __byte_perm(biased, 0x64646464u, SELECT), offset = 0x64806480u;   // 1152 twice
+  const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&raw), *reinterpret_cast<const __half2*>(&offset));
+  return *reinterpret_cast<const unsigned*>(&h);
+}
+// The key of column n of a group of eight columns.
+__device__ __forceinline__ constexpr int key_of(int n) { return n ^ ((n >> 1) & 1); }
+// What the 16-byte chunks of a row are exchanged by.
+__device__ __forceinline__ int swizzle(int row) {
+  if (D % 128 == 0) return (((((row ^ (row >> 1) ^ (row >> 2)) & 1) << 1) | ((row >> 1) & 1)) << 1);
+  if (D == 64) return ((row >> 2) & 1) << 1;
+  return 0;
+}
+__device__ __forceinline__ int chunk_at(int row, int chunk) { return row * D + ((chunk ^ swizzle(row)) << 4); }
+
+// F's range: sums of 2^(z - m) stay within float32 for any count of keys, and weights of 2^-20 of the largest above its least.
+constexpr int LEAST_EXPONENT = -93, MOST_EXPONENT = 107;
+// A magnitude's bits (which order as the magnitudes do), 0 for infinities and NaN.
+__device__ __forceinline__ unsigned finite_bits(float x) {
+  const unsigned bits = __float_as_uint(x) & 0x7fffffffu;
+  return bits < 0x7f800000u ? bits : 0u;
+}
+
+// 2^e for e in [-126, 127].
+__device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e + 127) << 23); }
+
+// Brings the codes and scales of the 32 keys from `key0` on into a stage; `threads` threads of which this is number `id` share
+// the work, and each of their warps holds in lane l the slot of key key0 + l (-1: no such key).
+template <int COUNT>
+__device__ __forceinline__ void load_step(const Args& args, int kv_head, int slot_of_lane, unsigned stage, int id) {
+#pragma unroll
+  for (int k = 0; k < (KEYS * CHUNKS + COUNT - 1) / COUNT; ++k) {
+    const int idx = id + k * COUNT;
+    const int key = idx / CHUNKS, chunk = idx - key * CHUNKS;
+    const int slot = __shfl_sync(0xffffffffu, slot_of_lane, key & 31);
+    if (KEYS * CHUNKS % COUNT == 0 || idx < KEYS * CHUNKS) {
+      const bool there = slot >= 0;
+      const size_t at = (static_cast<size_t>(there ? slot : 0) * args.num_kv_heads + kv_head) * D + chunk * 16;
+      const unsigned to = stage + chunk_at(key, chunk);
+      copy16(to, args.k_codes + at, there);
+      copy16(to + TILE, args.v_codes + at, there);
+    }
+  }
+  if (id < KEYS) {
+    const bool there = slot_of_lane >= 0;
+    const int page = there ? slot_of_lane / args.page_size : 0, within = there ? slot_of_lane - page * args.page_size : 0;
+    const size_t at = (static_cast<size_t>(page) * args.num_kv_heads + kv_head) * args.page_size + within;
+    copy4(stage + 2 * TILE + id * 4, args.k_scales + at, there);
+    copy4(stage + 2 * TILE + KEYS * 4 + id * 4, args.v_scales + at, there);
+  }
+}
+
+// The slot of a key, -1 where it lies behind `last_key` or its page is not one of the pool's.
+__device__ __forceinline__ int slot_of(const Args& args, const int* table, int key, int last_key) {
+  if (key > last_key) return -1;
+  const int block = key / args.page_size;
+  if (block >= args.max_blocks) return -1;
+  const int page = table[block];
+  return page < 0 || page >= args.num_pages ? -1 : page * args.page_size + key % args.page_size;
+}
+
+template <typename T> struct Parts { static constexpr int COUNT = 1; };
+template <> struct Parts<float> { static constexpr int COUNT = 2; };
+
+// A warp's 16 rows: queries as operands, running base, sum and output.
+template <typename T>
+struct Rows {
+  static constexpr int PARTS = Parts<T>::COUNT;
+  static constexpr bool IN_SHARED = STEPS_K * PARTS > 8;   // query operands in shared memory, else in registers
+  static constexpr int SHARED_BYTES = IN_SHARED ? STEPS_K * PARTS * 512 : 0;   // for one warp's rows
+  unsigned q[IN_SHARED ? 1 : STEPS_K * PARTS][4];
+  float factor[2];      // what a score is multiplied by, for rows g and g + 8
+  int first[2], last[2];   // the keys those rows see
+  float most[2], base[2], sum[2];   // largest score, base m = most + F, sum of 2^(z - m)
+  int exponent[2];      // F
+  float o[BLOCKS_V * 4][4];
+
+  __device__ __forceinline__ static int element_of(int step, int t) {   // a lane's first element of four in a product
+    return WIDE ? 16 * (t + 4 * (step / 4)) + 4 * (step % 4) : 4 * (t + 4 * step);
+  }
+
+  // Rows row0 ... row0 + 15 of an entry whose tokens begin at `start`; `group` heads share kv head `kv_head`.
+  __device__ void begin(const Args& args, int row0, int rows, int start, int group, int kv_head, int pos0, uint4* shared, int lane) {
+    const int g = lane >> 2, t = lane & 3;
+    const T* src[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int row = row0 + g + 8 * r, token = row / group, head = kv_head * group + row - token * group;
+      const bool there = row < rows;
+      src[r] = there ? static_cast<const T*>(args.q) + (static_cast<size_t>(start + token) * args.num_heads + head) * D : nullptr;
+      last[r] = pos0 + (there ? token : (rows - 1) / group);   // a row that is not there sees what the last one sees: nobody reads it
+      first[r] = first_visible_key(last[r], args.window);
+      most[r] = base[r] = -INFINITY;
+      sum[r] = 0.f;
+      exponent[r] = LEAST_EXPONENT;
+    }
+    float lift[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      unsigned top = 0u;   // the largest magnitude's bits, of finite elements
+#pragma unroll
+      for (int s = 0; s < STEPS_K; ++s) {
+        float x[4] = {0.f, 0.f, 0.f, 0.f};
+        if (src[r] != nullptr) load4<T>(src[r] + element_of(s, t), x);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const unsigned bits = __float_as_uint(x[e]) & 0x7fffffffu;
+          top = bits < 0x7f800000u && bits > top ? bits : top;
+        }
+      }
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const int e = min(max(static_cast<int>(top >> 23) - 127, -100), 126);
+      lift[r] = power_of_two(14 - e);
+      factor[r] = args.scale_log2 * power_of_two(e - 14);
+    }
+#pragma unroll
+    for (int s = 0; s < STEPS_K; ++s) {
+      unsigned a[PARTS][4];
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        float x[4] = {0.f, 0.f, 0.f, 0.f};
+        if (src[r] != nullptr) load4<T>(src[r] + element_of(s, t), x);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] *= lift[r];
+#pragma unroll
+        for (int part = 0; part < PARTS; ++part) {
+          a[part][r] = pack_half(x[0], x[1]);
+          a[part][r + 2] = pack_half(x[2], x[3]);
+          if (part + 1 < PARTS) {
+            x[0] -= low_half(a[part][r]);
+            x[1] -= high_half(a[part][r]);
+            x[2] -= low_half(a[part][r + 2]);
+            x[3] -= high_half(a[part][r + 2]);
+          }
+        }
+      }
+#pragma unroll
+      for (int part = 0; part < PARTS; ++part) {
+        if (IN_SHARED) {
+          shared[(s * PARTS + part) * 32 + lane] = make_uint4(a[part][0], a[part][1], a[part][2], a[part][3]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) q[IN_SHARED ? 0 : s * PARTS + part][i] = a[part][i];
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < BLOCKS_V * 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
+  }
+
+  __device__ __forceinline__ void operand(unsigned (&a)[4], int index, const uint4* shared, int lane) const {
+    if (IN_SHARED) {
+      const uint4 v = shared[index * 32 + lane];
+      a[0] = v.x; a[1] = v.y; a[2] = v.z; a[3] = v.w;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) a[i] = q[IN_SHARED ? 0 : index][i];
+    }
+  }
+
+  // The 32 keys from `key0` on, which lie in `stage`.
+  __device__ __forceinline__ void step(const unsigned char* stage, int key0, const uint4* shared, int lane) {
+    const int g = lane >> 2, t = lane & 3;
+    const unsigned char* k_tile = stage;
+    const unsigned char* v_tile = stage + TILE;
+    const float* k_scales = reinterpret_cast<const float*>(stage + 2 * TILE);
+    const float* v_scales = k_scales + KEYS;
+    float s[4][4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) s[j][c] = 0.f;
+    // scores
+#pragma unroll
+    for (int i = 0; i < (WIDE ? D / 64 : STEPS_K); ++i) {
+      unsigned words[4][WIDE ? 4 : 1];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int key = 8 * j + key_of(g);
+        if (WIDE) {
+          const uint4 v = *reinterpret_cast<const uint4*>(k_tile + chunk_at(key, t + 4 * i));
+          words[j][0] = v.x;
+          words[j][WIDE ? 1 : 0] = WIDE ? v.y : v.x;
+          words[j][WIDE ? 2 : 0] = WIDE ? v.z : v.x;
+          words[j][WIDE ? 3 : 0] = WIDE ? v.w : v.x;
+        } else {
+          words[j][0] = *reinterpret_cast<const unsigned*>(k_tile + chunk_at(key, i) + 4 * t);
+        }
+      }
+#pragma unroll
+      for (int w = 0; w < (WIDE ? 4 : 1); ++w) {
+        unsigned a[PARTS][4];
+#pragma unroll
+        for (int part = 0; part < PARTS; ++part) operand(a[part], ((WIDE ? 4 * i : i) + w) * PARTS + part, shared, lane);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const unsigned biased = words[j][w] ^ 0x80808080u;
+          const unsigned b0 = codes_to_half<0x4140>(biased), b1 = codes_to_half<0x4342>(biased);
+#pragma unroll
+          for (int part = 0; part < PARTS; ++part) mma(s[j], a[part], b0, b1);
+        }
+      }
+    }
+    // what each row sees, and the largest value scale among that
+    const bool edge = __any_sync(0xffffffffu, key0 < first[0] || key0 < first[1] || key0 + KEYS - 1 > last[0] || key0 + KEYS - 1 > last[1]);
+    unsigned top[2];
+    if (!edge) {
+      top[0] = top[1] = __reduce_max_sync(0xffffffffu, finite_bits(v_scales[lane]));
+    } else {
+#pragma unroll
+      for (int r = 0; r < 2; ++r) top[r] = 0u;
+    }
+    float correction[2];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int within = 8 * j + key_of(2 * t + c), key = key0 + within;
+        const float k_scale = k_scales[within];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          s[j][2 * r + c] *= k_scale * factor[r];
+          if (edge) {
+            if (key >= first[r] && key <= last[r]) top[r] = max(top[r], finite_bits(v_scales[within]));
+            else s[j][2 * r + c] = -INFINITY;
+          }
+        }
+      }
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      float largest = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) largest = fmaxf(largest, s[j][2 * r + c]);
+      largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
+      largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
+      if (edge) {
+        top[r] = max(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
+        top[r] = max(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
+      }
+      exponent[r] = max(exponent[r], min(static_cast<int>(top[r] >> 23) - 127 - 13, MOST_EXPONENT));
+      most[r] = fmaxf(most[r], largest);
+      const float next = most[r] + static_cast<float>(exponent[r]), from = most[r] == -INFINITY ? 0.f : next;
+      correction[r] = base[r] == next ? 1.f : fast_exp2(base[r] - from);
+      base[r] = next;
+      float total = 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const float p = fast_exp2(s[j][2 * r + c] - from);
+          s[j][2 * r + c] = p;
+          total += p;
+        }
+      sum[r] = sum[r] * correction[r] + total;
+    }
+    if (__any_sync(0xffffffffu, correction[0] != 1.f || correction[1] != 1.f)) {
+#pragma unroll
+      for (int i = 0; i < BLOCKS_V * 4; ++i)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) o[i][c] *= correction[c >> 1];
+    }
+    // weights
+    unsigned w[2][PARTS][4];   // [16 keys][part]
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float lo = v_scales[8 * j + key_of(2 * t)], hi = v_scales[8 * j + key_of(2 * t + 1)];
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        // a key that a row does not see has no part in it, whatever its scale
+        float x = s[j][2 * r] == 0.f ? 0.f : s[j][2 * r] * lo, y = s[j][2 * r + 1] == 0.f ? 0.f : s[j][2 * r + 1] * hi;
+#pragma unroll
+        for (int part = 0; part < PARTS; ++part) {
+          const unsigned packed = pack_half(x, y);
+          w[j >> 1][part][(j & 1) * 2 + r] = packed;
+          if (part + 1 < PARTS) {
+            x -= low_half(packed);
+            y -= high_half(packed);
+          }
+        }
+      }
+    }
+    // output
+#pragma unroll
+    for (int b = 0; b < BLOCKS_V; ++b) {
+      const int chunk = 2 * b + (g >> 2);
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk) {
+        unsigned rows[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {   // keys 2 t, 2 t + 1 of the first eight, then of the second
+          const int key = 16 * kk + 8 * (i >> 1) + key_of(2 * t + (i & 1));
+          rows[i] = D % 32 == 0 || chunk < CHUNKS ? *reinterpret_cast<const unsigned*>(v_tile + chunk_at(key, chunk) + 4 * (g & 3)) : 0u;
+          rows[i] ^= 0x80808080u;
+        }
+        const unsigned lo01 = __byte_perm(rows[0], rows[1], 0x5140), lo23 = __byte_perm(rows[0], rows[1], 0x7362);
+        const unsigned hi01 = __byte_perm(rows[2], rows[3], 0x5140), hi23 = __byte_perm(rows[2], rows[3], 0x7362);
+        const unsigned b0[4] = {codes_to_half<0x4140>(lo01), codes_to_half<0x4342>(lo01), codes_to_half<0x4140>(lo23), codes_to_half<0x4342>(lo23)};
+        const unsigned b1[4] = {codes_to_half<0x4140>(hi01), codes_to_half<0x4342>(hi01), codes_to_half<0x4140>(hi23), codes_to_half<0x4342>(hi23)};
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int part = 0; part < PARTS; ++part) mma(o[b * 4 + j], w[kk][part], b0[j], b1[j]);
+      }
+    }
+  }
+
+  // Sums of whole rows.
+  __device__ __forceinline__ void finish() {
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 1);
+      sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 2);
+    }
+  }
+  // The element of the head that o[b * 4 + j][c] belongs to (c's low bit: which of a lane's two columns).
+  __device__ __forceinline__ static int out_element(int b, int j, int c, int t) { return 32 * b + 4 * (2 * t + (c & 1)) + j; }
+};
+
+// Which entry this is, and whether it is this launch's.
+__device__ __forceinline__ bool entry_of(const Args& args, int seq, int& start, int& q_len, int& context) {
+  start = args.q_start[seq];
+  q_len = args.q_start[seq + 1] - start;
+  context = args.ctx_len[seq];
+  return q_len > 0 && !(args.only == 1 && q_len > 1) && !(args.only == 2 && q_len == 1);
+}
+
+// Few rows: grid (splits, kv heads * row tiles, entries).
+template <typename T>
+__global__ void __launch_bounds__(THREADS)
+split_keys_kernel(const Args args) {
+  extern __shared__ __align__(128) unsigned char smem[];
+  let_dependents_start();
+  const int seq = blockIdx.z, split = blockIdx.x;
+  const int kv_head = blockIdx.y % args.num_kv_heads, tile = blockIdx.y / args.num_kv_heads;
+  const int group = args.num_heads / args.num_kv_heads;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  wait_for_previous();
+  int start, q_len, context;
+  if (!entry_of(args, seq, start, q_len, context)) return;
+  const int rows = q_len * group, row0 = tile * ROWS;
+  if (row0 >= rows) return;
+  const int pos0 = context - q_len;
+  const int tile_rows = min(ROWS, rows - row0);
+  const int last_key = pos0 + (row0 + tile_rows - 1) / group, first_key = first_visible_key(pos0 + row0 / group, args.window);
+  const int step_lo = max(first_key, 0) / KEYS, steps = last_key < 0 ? 0 : last_key / KEYS + 1 - step_lo;
+  const int per = (steps + args.splits - 1) / args.splits;
+  const int mine_lo = step_lo + min(steps, split * per), mine_hi = step_lo + min(steps, (split + 1) * per);
+
+  using R = Rows<T>;
+  uint4* shared_q = reinterpret_cast<uint4*>(smem + WARPS * STAGES * STAGE);
+  unsigned char* ring = smem + warp * STAGES * STAGE;
+  const unsigned ring_at = smem_u32(ring);
+  const int* table = args.block_table + static_cast<size_t>(seq) * args.max_blocks;
+  R r;
+  // this warp's steps: mine_lo + warp, + WARPS, ...
+  const int begin = mine_lo + warp;
+  int loaded = begin;
+  int next_slot = slot_of(args, table, loaded * KEYS + lane, loaded < mine_hi ? last_key : -1);
+#pragma unroll
+  for (int i = 0; i < STAGES - 1; ++i) {
+    if (loaded < mine_hi) load_step<32>(args, kv_head, next_slot, ring_at + i * STAGE, lane);
+    copies_commit();
+    loaded += WARPS;
+    next_slot = slot_of(args, table, loaded * KEYS + lane, loaded < mine_hi ? last_key : -1);
+  }
+  r.begin(args, row0, rows, start, group, kv_head, pos0, shared_q, lane);   // all warps write the same operands
+  __syncwarp();
+  int stage = 0;
+  for (int step = begin; step < mine_hi; step += WARPS) {
+    copies_wait<STAGES - 2>();
+    __syncwarp();
+    const int into = stage + STAGES - 1 >= STAGES ? stage - 1 : stage + STAGES - 1;
+    if (loaded < mine_hi) load_step<32>(args, kv_head, next_slot, ring_at + into * STAGE, lane);
+    copies_commit();
+    loaded += WARPS;
+    next_slot = slot_of(args, table, loaded * KEYS + lane, loaded < mine_hi ? last_key : -1);
+    r.step(ring + stage * STAGE, step * KEYS, shared_q, lane);
+    __syncwarp();
+    stage = stage + 1 == STAGES ? 0 : stage + 1;
+  }
+  copies_wait<0>();
+  r.finish();
+  __syncthreads();
+  // the warps' rows meet: [warp][16][D] and [warp][16][base, sum]
+  float* all_o = reinterpret_cast<float*>(smem);
+  float* all_m = all_o + WARPS * ROWS * D;
+#pragma unroll
+  for (int b = 0; b < BLOCKS_V; ++b)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int element = R::out_element(b, j, c, t);
+        if (D % 32 == 0 || element < D) all_o[(warp * ROWS + g + 8 * (c >> 1)) * D + element] = r.o[b * 4 + j][c];
+      }
+  if (t == 0) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      all_m[(warp * ROWS + g + 8 * i) * 2] = r.base[i];
+      all_m[(warp * ROWS + g + 8 * i) * 2 + 1] = r.sum[i];
+    }
+  }
+  __syncthreads();
+  const size_t pair = (static_cast<size_t>(seq) * gridDim.y + blockIdx.y);
+  float* share = args.splits > 1 ? args.scratch + (pair * args.splits + split) * ROWS * (D + 2) : nullptr;
+  T* out = static_cast<T*>(args.out);
+  for (int i = threadIdx.x; i < tile_rows * (D / 4); i += THREADS) {
+    const int row = i / (D / 4), element = (i - row * (D / 4)) * 4;
+    float base = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) base = fmaxf(base, all_m[(w * ROWS + row) * 2]);
+    float total = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      const float m = all_m[(w * ROWS + row) * 2];
+      const float weight = m == -INFINITY ? 0.f : fast_exp2(m - base);
+      if (weight == 0.f) continue;
+      total += all_m[(w * ROWS + row) * 2 + 1] * weight;
+      const float4 v = *reinterpret_cast<const float4*>(all_o + (w * ROWS + row) * D + element);
+      acc[0] += v.x * weight; acc[1] += v.y * weight; acc[2] += v.z * weight; acc[3] += v.w * weight;
+    }
+    if (share != nullptr) {
+      *reinterpret_cast<float4*>(share + row * D + element) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+      if (element == 0) {
+        share[ROWS * D + 2 * row] = base;
+        share[ROWS * D + 2 * row + 1] = total;
+      }
+    } else {
+      const float inv = total == 0.f ? 0.f : 1.f / total;   // a row that sees nothing is zeros
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[e] *= inv;
+      const int at = row0 + row, token = at / group, head = kv_head * group + at - token * group;
+      store4<T>(out + (static_cast<size_t>(start + token) * args.num_heads + head) * D + element, acc);
+    }
+  }
+  if (args.splits == 1) return;
+  __threadfence();
+  __syncthreads();
+  __shared__ int arrived;
+  if (threadIdx.x == 0) arrived = atomicAdd(args.arrivals + pair, 1);
+  __syncthreads();
+  if (arrived != args.splits - 1) return;
+  __threadfence();
+  const float* shares = args.scratch + pair * args.splits * ROWS * (D + 2);
+  for (int i = threadIdx.x; i < tile_rows * (D / 4); i += THREADS) {
+    const int row = i / (D / 4), element = (i - row * (D / 4)) * 4;
+    float base = -INFINITY;
+    for (int s = 0; s < args.splits; ++s) base = fmaxf(base, __ldcg(shares + static_cast<size_t>(s) * ROWS * (D + 2) + ROWS * D + 2 * row));
+    float total = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < args.splits; ++s) {
+      const float* share_s = shares + static_cast<size_t>(s) * ROWS * (D + 2);
+      const float m = __ldcg(share_s + ROWS * D + 2 * row);
+      const float weight = m == -INFINITY ? 0.f : fast_exp2(m - base);
+      if (weight == 0.f) continue;
+      total += __ldcg(share_s + ROWS * D + 2 * row + 1) * weight;
+      const float4 v = __ldcg(reinterpret_cast<const float4*>(share_s + row * D + element));
+      acc[0] += v.x * weight; acc[1] += v.y * weight; acc[2] += v.z * weight; acc[3] += v.w * weight;
+    }
+    const float inv = total == 0.f ? 0.f : 1.f / total;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[e] *= inv;
+    const int at = row0 + row, token = at / group, head = kv_head * group + at - token * group;
+    store4<T>(out + (static_cast<size_t>(start + token) * args.num_heads + head) * D + element, acc);
+  }
+  if (threadIdx.x == 0) args.arrivals[pair] = 0;
+}
+
+// Many rows: grid (row tiles of 64, kv heads, entries); the CTA's warps share the key tiles.
+template <typename T>
+__global__ void __launch_bounds__(THREADS)
+portion_rows_kernel(const Args args) {
+  extern __shared__ __align__(128) unsigned char smem[];
+  let_dependents_start();
+  const int seq = blockIdx.z, kv_head = blockIdx.y;
+  const int group = args.num_heads / args.num_kv_heads;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  wait_for_previous();
+  int start, q_len, context;
+  if (!entry_of(args, seq, start, q_len, context)) return;
+  const int rows = q_len * group;
+  const int tiles = (rows + WARPS * ROWS - 1) / (WARPS * ROWS);
+  if (static_cast<int>(blockIdx.x) >= tiles) return;
+  const int cta_row0 = (tiles - 1 - static_cast<int>(blockIdx.x)) * WARPS * ROWS;   // the longest first
+  const int row0 = cta_row0 + warp * ROWS;
+  const int pos0 = context - q_len;
+  const int last_key = pos0 + (min(cta_row0 + WARPS * ROWS, rows) - 1) / group;
+  const int first_key = first_visible_key(pos0 + cta_row0 / group, args.window);
+  const int step_lo = max(first_key, 0) / KEYS, step_hi = last_key < 0 ? step_lo : last_key / KEYS + 1;
+  // this warp's own part of that range
+  const int my_last = row0 < rows ? pos0 + (min(row0 + ROWS, rows) - 1) / group : -1;
+  const int my_first = first_visible_key(pos0 + row0 / group, args.window);
+
+  using R = Rows<T>;
+  uint4* shared_q = reinterpret_cast<uint4*>(smem + STAGES * STAGE + warp * R::SHARED_BYTES);
+  const unsigned ring_at = smem_u32(smem);
+  const int* table = args.block_table + static_cast<size_t>(seq) * args.max_blocks;
+  R r;
+  int next_slot = slot_of(args, table, step_lo * KEYS + lane, last_key);
+#pragma unroll
+  for (int i = 0; i < STAGES - 1; ++i) {
+    if (step_lo + i < step_hi) load_step<THREADS>(args, kv_head, next_slot, ring_at + i * STAGE, threadIdx.x);
+    copies_commit();
+    next_slot = slot_of(args, table, (step_lo + i + 1) * KEYS + lane, last_key);
+  }
+  r.begin(args, row0, rows, start, group, kv_head, pos0, shared_q, lane);
+  __syncwarp();
+  int stage = 0;
+  for (int step = step_lo; step < step_hi; ++step) {
+    copies_wait<STAGES - 2>();
+    __syncthreads();   // this step's copies of all threads have landed; everyone has left the stage that is loaded next
+    const int into = stage + STAGES - 1 >= STAGES ? stage - 1 : stage + STAGES - 1;
+    if (step + STAGES - 1 < step_hi) load_step<THREADS>(args, kv_head, next_slot, ring_at + into * STAGE, threadIdx.x);
+    copies_commit();
+    next_slot = slot_of(args, table, (step + STAGES) * KEYS + lane, last_key);
+    if (step * KEYS <= my_last && step * KEYS + KEYS > my_first) r.step(smem + stage * STAGE, step * KEYS, shared_q, lane);
+    stage = stage + 1 == STAGES ? 0 : stage + 1;
+  }
+  copies_wait<0>();
+  r.finish();
+  T* out = static_cast<T*>(args.out);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int row = row0 + g + 8 * i;
+    if (row >= rows) continue;
+    const int token = row / group, head = kv_head * group + row - token * group;
+    T* dst = out + (static_cast<size_t>(start + token) * args.num_heads + head) * D;
+    const float inv = r.sum[i] == 0.f ? 0.f : 1.f / r.sum[i];
+#pragma unroll
+    for (int b = 0; b < BLOCKS_V; ++b)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {   // a lane's four elements of a run are neighbours
+        const int element = R::out_element(b, 0, c, t);
+        float v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = r.o[b * 4 + j][2 * i + c] * inv;
+        if (D % 32 == 0 || element < D) store4<T>(dst + element, v);
+      }
+  }
+}
+
+template <typename T> constexpr size_t split_keys_smem() {
+  const size_t ring = static_cast<size_t>(WARPS) * STAGES * STAGE + Rows<T>::SHARED_BYTES;
+  const size_t merge = static_cast<size_t>(WARPS) * ROWS * (D + 2) * 4;
+  return ring > merge ? ring : merge;
+}
+template <typename T> constexpr size_t portion_rows_smem() { return static_cast<size_t>(STAGES) * STAGE + WARPS * Rows<T>::SHARED_BYTES; }
+
+template <typename T>
+static int resident() {
+  static PerDevice raised;
+  if (shrike_raise_smem(raised, split_keys_kernel<T>, split_keys_smem<T>()) != 0) return shrike_device().sm_count;
+  int per_sm = 0;
+  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, split_keys_kernel<T>, THREADS, split_keys_smem<T>()) != cudaSuccess || per_sm < 1) per_sm = 1;
+  return per_sm * shrike_device().sm_count;
+}
+
+template <typename T>
+static int launch(const Args& base, int num_seqs, int max_q_len, int has_single, int has_portions, cudaStream_t stream) {
+  Args args = base;
+  const int group = args.num_heads / args.num_kv_heads;
+  if (has_single) {
+    static PerDevice raised;
+    const int rc = shrike_raise_smem(raised, split_keys_kernel<T>, split_keys_smem<T>());
+    if (rc != 0) return rc;
+    args.only = has_portions ? 1 : 0;
+    const long long tiles = (static_cast<long long>(has_portions ? 1 : max_q_len) * group + ROWS - 1) / ROWS;
+    if (tiles * args.num_kv_heads > 65535) return SHRIKE_BAD_ARGUMENT;
+    const cudaError_t err = launch_dependent(split_keys_kernel<T>, dim3(args.splits, static_cast<unsigned>(tiles * args.num_kv_heads), num_seqs),
+                                             dim3(THREADS), split_keys_smem<T>(), stream, args);
+    if (err != cudaSuccess) return static_cast<int>(err);
+  }
+  if (has_portions) {
+    static PerDevice raised;
+    const int rc = shrike_raise_smem(raised, portion_rows_kernel<T>, portion_rows_smem<T>());
+    if (rc != 0) return rc;
+    args.only = has_single ? 2 : 0;
+    const long long tiles = (static_cast<long long>(max_q_len) * group + WARPS * ROWS - 1) / (WARPS * ROWS);
+    if (tiles > 0x7fffffff) return SHRIKE_BAD_ARGUMENT;
+    const cudaError_t err = launch_dependent(portion_rows_kernel<T>, dim3(static_cast<unsigned>(tiles), args.num_kv_heads, num_seqs),
+                                             dim3(THREADS), portion_rows_smem<T>(), stream, args);
+    if (err != cudaSuccess) return static_cast<int>(err);
+  }
+  return shrike_launch_status();
+}
+
+}  // namespace attnq8
+
+// CTAs of the few-rows form that the device holds at once, for queries of `dtype`.
+SHRIKE_API int shrike_attention_q8_resident_ctas(int dtype) {
+  return dtype == SHRIKE_F32 ? attnq8::resident<float>() : attnq8::resident<__nv_bfloat16>();
+}
+// Floats of scratch for a (entry, kv head, row tile) and split, and the most splits.
+SHRIKE_API int shrike_attention_q8_share_floats() { return attnq8::ROWS * (attnq8::D + 2); }
+SHRIKE_API int shrike_attention_q8_max_splits() { return attnq8::MAX_SPLITS; }
+
+// q and out [tokens, heads * D] of `dtype`, 16-byte aligned; codes [pages, page_size, kv heads, D], 16-byte aligned, scales
+// [pages, kv heads, page_size].  `has_single`: entries of one token (every entry, where has_portions is 0: then `max_q_len`
+// tokens at most) run on the few-rows form with `splits` CTAs a row tile; `has_portions`: the longer ones (all of them where
+// has_single is 0) on the other.  splits > 1 needs `scratch` (share_floats() a pair of (entry, kv head, row tile) and split)
+// and `arrivals` (an int a pair, zero before the first launch).
+SHRIKE_API int shrike_paged_attention_q8(const void* q, const void* k_codes, const float* k_scales, const void* v_codes,
+                                         const float* v_scales, const int* block_table, int max_blocks, const int* q_start,
+                                         const int* ctx_len, int dtype, int num_seqs, int num_heads, int num_kv_heads, int page_size,
+                                         int num_pages, float scale, int window, void* out, int has_single, int has_portions,
+                                         int max_q_len, int splits, float* scratch, int* arrivals, cudaStream_t stream) {
+  if (num_seqs <= 0) return SHRIKE_OK;
+  if (num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads || num_kv_heads > 65535 || max_blocks <= 0 || page_size <= 0 ||
+      num_pages <= 0 || static_cast<long long>(num_pages) * page_size > 0x7fffffff ||
+      static_cast<long long>(max_blocks) * page_size > 0x7fffffff - 4096 || max_q_len < 1 || num_seqs > 65535 || splits < 1 ||
+      splits > attnq8::MAX_SPLITS || (splits > 1 && (scratch == nullptr || arrivals == nullptr)) ||
+      (reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(k_codes) |
+       reinterpret_cast<uintptr_t>(v_codes) | reinterpret_cast<uintptr_t>(scratch)) % 16)
+    return SHRIKE_BAD_ARGUMENT;
+  attnq8::Args args;
+  args.k_codes = static_cast<const signed char*>(k_codes);
+  args.k_scales = k_scales;
+  args.v_codes = static_cast<const signed char*>(v_codes);
+  args.v_scales = v_scales;
+  args.block_table = block_table;
+  args.q_start = q_start;
+  args.ctx_len = ctx_len;
+  args.q = q;
+  args.out = out;
+  args.max_blocks = max_blocks;
+  args.num_heads = num_heads;
+  args.num_kv_heads = num_kv_heads;
+  args.page_size = page_size;
+  args.num_pages = num_pages;
+  args.window = window;
+  args.only = 0;
+  args.scale_log2 = scale * attnq8::LOG2E;
+  args.splits = splits;
+  args.scratch = scratch;
+  args.arrivals = arrivals;
+  if (dtype == SHRIKE_F32) return attnq8::launch<float>(args, num_seqs, max_q_len, has_single, has_portions, stream);
+  if (dtype == SHRIKE_BF16) return attnq8::launch<__nv_bfloat16>(args, num_seqs, max_q_len, has_single, has_portions, stream);
+  return SHRIKE_BAD_ARGUMENT;
+}

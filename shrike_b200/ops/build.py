@@ -163,8 +163,9 @@ def load_library(name: str, sources, defines=None, extra_flags=()) -> ctypes.CDL
 
 
 # The libraries of this package.
-CORE_SOURCES = ["elementwise.cu", "branch_ops.cu", "parallel_ops.cu", "decay_ops.cu", "stream_ops.cu", "delta_ops.cu", "gemm_fp32.cu", "sampling.cu"]
+CORE_SOURCES = ["elementwise.cu", "branch_ops.cu", "parallel_ops.cu", "decay_ops.cu", "stream_ops.cu", "delta_ops.cu", "gemm_fp32.cu", "sampling.cu", "cache_q8.cu"]
 ATTENTION_SOURCES = ["attention_fp32.cu", "attention_bf16.cu", "attention_tcgen05.cu"]
+ATTENTION_Q8_SOURCES = ["attention_q8.cu"]
 
 
 def core_library() -> ctypes.CDLL:
@@ -179,6 +180,11 @@ def attention_library(head_dim: int) -> ctypes.CDLL:
     if head_dim > TENSOR_CORE_HEAD_DIM:
         return load_library(f"shrike_attention_wide_d{head_dim}", ["attention_generic.cu"], {"SHRIKE_HEAD_DIM": head_dim})
     return load_library(f"shrike_attention_d{head_dim}", ATTENTION_SOURCES, {"SHRIKE_HEAD_DIM": head_dim})
+
+
+def attention_q8_library(head_dim: int) -> ctypes.CDLL:
+    """The attention kernels over 8-bit cache pages for one head size."""
+    return load_library(f"shrike_attention_q8_d{head_dim}", ATTENTION_Q8_SOURCES, {"SHRIKE_HEAD_DIM": head_dim})
 
 
 def tensor_core_gemm_library() -> ctypes.CDLL:
@@ -200,4 +206,5 @@ def build_all(head_dims=(16, 32, 48, 64, 128, 256)) -> list[Path]:
     for head_dim in head_dims:
         built.append(compile_library(f"shrike_attention_d{head_dim}", ATTENTION_SOURCES,
                                      {"SHRIKE_HEAD_DIM": head_dim}))
+        built.append(compile_library(f"shrike_attention_q8_d{head_dim}", ATTENTION_Q8_SOURCES, {"SHRIKE_HEAD_DIM": head_dim}))
     return built

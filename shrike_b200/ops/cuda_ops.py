@@ -18,6 +18,7 @@ import torch
 from torch.multiprocessing.reductions import StorageWeakRef
 
 from . import build
+from .quantised_cache import QuantisedCacheOps, quantised
 
 _DTYPE_CODE = {torch.float32: 0, torch.bfloat16: 1}
 _c = ctypes
@@ -71,6 +72,10 @@ _LIMITS = {
     "element_gate": "the gate's columns inside the row, the padded head at least as wide as its values",
     "act_blocks": "an activation the kernels know, a weight column per expert",
     "act_mul_blocks": "experts * each columns at most, the rest the shared expert's, which needs the weights' last column",
+    "kv_write_q8": "heads of 16 to 256 elements in sixteens, codes on 16-byte borders",
+    "rope_kv_write_q8": "heads of 16 to 256 elements in sixteens, codes on 16-byte borders",
+    "kv_read_q8": "heads in sixteens, codes and outputs on 16-byte borders",
+    "paged_attention_q8": "at most 65535 sequences and kv heads, heads a multiple of kv heads, everything on 16-byte borders",
     "paged_attention_bf16": "at most 65535 sequences and heads, heads a multiple of kv heads, at most 32 splits",
 }
 
@@ -91,7 +96,7 @@ def _dense(tensor, dtype, what):
         raise KernelError(f"{what} must be contiguous")
 
 
-class CudaOps:
+class CudaOps(QuantisedCacheOps):
     PORTION_SCRATCH_FLOATS = 32 << 20   # at most 128 MiB of partial rows for the split portions kernel
 
     def __init__(self, dtype: torch.dtype, device="cuda"):
@@ -226,6 +231,7 @@ class CudaOps:
         for name in ("shrike_embed_scaled", "shrike_act_mul_limit", "shrike_tanh_norm", "shrike_head_prep",
                      "shrike_matrix_memory_scan", "shrike_matrix_memory_out", "shrike_route_top", "shrike_act_mul_blocks"):
             getattr(lib, name).restype = _I
+        self._declare_q8_core(lib)
         lib.shrike_sample_slices.argtypes = [_I]
         lib.shrike_sample_slices.restype = _I
         for name in ("shrike_embed", "shrike_add_rmsnorm", "shrike_silu_mul", "shrike_rope_kv_write",
@@ -670,7 +676,14 @@ class CudaOps:
         """Bias, rotation and cache store of a fused q/k/v projection ([N, W] or a K-split stack).
         `positions`, `slots`, `bias` and `inv_freq` are read while the kernels launched before may
         still run (the angles are formed meanwhile): they must be the step's metadata or
-        parameters, not something a kernel of this step computes."""
+        parameters, not something a kernel of this step computes.  With `QuantisedPages` keys and values are
+        quantised as they are stored (`positions`, `slots` and `inv_freq` are read early then; every stored slot at
+        most once in a call)."""
+        if quantised(keys, values):
+            if k_out is not None or v_out is not None:
+                raise KernelError("rope_kv_write: rotated keys go to 8-bit pages or to k_out and v_out, not to both")
+            self._rope_kv_write_q8(qkv, bias, positions, inv_freq, q_out, keys, values, slots, num_heads, num_kv_heads, head_dim)
+            return
         _dense(qkv, torch.float32, "qkv")
         _dense(q_out, self.dtype, "q")
         partials, stride = self._stack(qkv)
@@ -687,6 +700,12 @@ class CudaOps:
             num_slots, partials, stride, self._stream()), "rope_kv_write")
 
     def kv_write(self, k_new, v_new, keys, values, slots):
+        """Stores rows of keys and values ([N, kv heads * head size] in the engine's type) at their slots; a row whose slot is none
+        of the pool's (a negative one, say) is left out, the others' slots differ from one another.  Into `QuantisedPages` rows
+        are quantised on the way, and may be part of wider ones (`k_new` and `v_new` with a row stride)."""
+        if quantised(keys, values):
+            self._kv_write_q8(k_new, v_new, keys, values, slots)
+            return
         _dense(keys, self.dtype, "key cache")
         n, kv_width = k_new.shape
         self.launches += 1
@@ -710,7 +729,17 @@ class CudaOps:
         `keep_first` (with a window): the sequence's first `keep_first` keys stay visible to every later query.
         `early_metadata`: `block_table`, `q_start`, `ctx_len` and `seq_of_token` were last written by a copy or an earlier step
         (which have finished), not by a kernel of this step; they are then read while the kernel before this one runs.  In
-        bfloat16 (heads of up to 256) they always are, and have to be such."""
+        bfloat16 (heads of up to 256) they always are, and have to be such.
+        With `QuantisedPages` for keys and values: heads of up to 256, a window or a chunk, and none of the other changes to
+        scores; `max_q_len` is needed, and a query that sees no key (a context shorter than its new tokens) gets zeros."""
+        if quantised(keys, values):
+            if softcap or slopes is not None or sinks is not None or keep_first:
+                raise KernelError("attention over 8-bit pages takes a window or a chunk; no soft cap, slopes, sinks or kept keys")
+            if chunk and window:
+                raise KernelError("attention takes a window or a chunk, not both")
+            self._paged_attention_q8(q, keys, values, block_table, q_start, ctx_len, seq_of_token, num_heads, num_kv_heads, head_dim,
+                                     scale, -int(chunk) if chunk else window, out, max_q_len, min_q_len)
+            return
         _dense(q, self.dtype, "q")
         if sinks is not None:
             _dense(sinks, torch.float32, "softmax sinks")

@@ -1,0 +1,195 @@
+"""The 8-bit cache on the GPU: what is stored, what is read back, and attention over it, against 64 bits."""
+
+import math
+
+import pytest
+import torch
+
+from shrike_b200.cache.quantised import QuantisedPages
+from tests import cache_q8_oracle as oracle
+from tests.gpu_common import cuda_ops
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+TYPES = [torch.bfloat16, torch.float32]
+
+
+def rnd(*shape, seed=0, dtype=torch.float32):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed)).to(DEV, dtype)
+
+
+def empty_pages(pages, page, heads, dim):
+    """Pages whose every place is marked, so that what is stored beside its slot shows."""
+    return QuantisedPages(torch.full((pages, page, heads, dim), 77, dtype=torch.int8, device=DEV),
+                          torch.full((pages, heads, page), 7.5, device=DEV))
+
+
+def check_stored(pages, x, slots, heads, dim):
+    page = pages.codes.shape[1]
+    codes, scales = oracle.quantise(x.view(-1, heads, dim))
+    want_codes, want_scales = torch.full_like(pages.codes, 77), torch.full_like(pages.scales, 7.5)
+    for row, slot in enumerate(slots.tolist()):
+        if 0 <= slot < pages.codes.shape[0] * page:
+            want_codes[slot // page, slot % page] = codes[row]
+            want_scales[slot // page, :, slot % page] = scales[row]
+    assert torch.equal(pages.codes, want_codes)
+    assert torch.equal(pages.scales.nan_to_num(nan=-1.0), want_scales.nan_to_num(nan=-1.0))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,heads,dim,page", [(1, 4, 128, 16), (7, 1, 16, 1), (33, 3, 32, 8), (70, 2, 48, 5), (130, 2, 64, 64),
+                                              (9, 3, 80, 16), (5, 2, 192, 7), (600, 2, 256, 16), (2500, 8, 128, 32)])
+def test_store_and_read_back(dtype, n, heads, dim, page):
+    ops = cuda_ops(dtype)
+    pages = -(-n // page) + 2
+    g = torch.Generator().manual_seed(n)
+    slots = torch.randperm(pages * page, generator=g)[:n].to(torch.int32)
+    if n > 5:
+        slots[2], slots[4] = -1, pages * page   # none of the pool's: left out
+    slots = slots.to(DEV)
+    k, v = rnd(n, heads * dim, seed=1, dtype=dtype), rnd(n, heads * dim, seed=2, dtype=dtype)
+    k[0, :dim] = 0                                       # a row of zeros
+    k[0, dim - 1] = 0.5
+    v[n - 1, -dim:] = 0
+    v[n // 2, :4] = torch.tensor([2.0, 1.0, -1.0, -2.0])   # halves of the largest lie between two codes
+    v[n // 2, 4: dim] = v[n // 2, 4: dim].clamp(-2, 2)
+    keys, values = empty_pages(pages, page, heads, dim), empty_pages(pages, page, heads, dim)
+    ops.kv_write(k, v, keys, values, slots)
+    check_stored(keys, k, slots, heads, dim)
+    check_stored(values, v, slots, heads, dim)
+    k_out, v_out = (torch.full((n, heads * dim), math.nan, dtype=dtype, device=DEV) for _ in range(2))
+    ops.kv_read(keys, values, slots, k_out, v_out)
+    good = ((slots >= 0) & (slots < pages * page))[:, None, None]
+    for x, out in ((k, k_out), (v, v_out)):
+        codes, scales = oracle.quantise(x.view(n, heads, dim))
+        want = torch.where(good, codes.float() * scales[..., None], 0.0).to(dtype)   # a product of 32-bit numbers, rounded once more
+        assert torch.equal(out.view(n, heads, dim), want)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_store_takes_rows_of_a_wider_array_at_any_element(dtype):
+    ops = cuda_ops(dtype)
+    n, heads, dim, page = 19, 2, 64, 16
+    for first in (0, 8, 3):
+        wide = rnd(n, 2 * heads * dim + 12, seed=first, dtype=dtype)
+        k, v = wide[:, first: first + heads * dim], wide[:, -heads * dim:]
+        keys, values = empty_pages(2, page, heads, dim), empty_pages(2, page, heads, dim)
+        slots = torch.arange(n, dtype=torch.int32, device=DEV).flip(0).contiguous()
+        ops.kv_write(k, v, keys, values, slots)
+        check_stored(keys, k.contiguous(), slots, heads, dim)
+        check_stored(values, v.contiguous(), slots, heads, dim)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_rows_of_extreme_elements(dtype):
+    """Tiny, denormal and huge rows keep the nearest codes; a row with an infinity or a NaN is read as NaN and harms nobody else."""
+    ops = cuda_ops(dtype)
+    heads, dim, page = 1, 32, 4
+    base = rnd(12, dim, seed=5)
+    factors = torch.tensor([1e-38, 1e-36, 1e-30, 1e-20, 1.0, 1e20, 1e30, 1e37, 0.0, 1.0, 1.0, 1.0], device=DEV)
+    x = (base * factors[:, None]).to(dtype)
+    x[0] = torch.where(x[0].abs() < 1e-44, torch.zeros_like(x[0]), x[0])
+    x[9, 3], x[10, 31], x[11, 0] = math.inf, math.nan, -math.inf
+    keys, values = empty_pages(3, page, heads, dim), empty_pages(3, page, heads, dim)
+    slots = torch.arange(12, dtype=torch.int32, device=DEV)
+    ops.kv_write(x, x, keys, values, slots)
+    check_stored(keys, x, slots, heads, dim)
+    k_out, v_out = torch.empty_like(x), torch.empty_like(x)
+    ops.kv_read(keys, values, slots, k_out, v_out)
+    assert torch.isnan(k_out[9:]).all() and torch.isfinite(k_out[:9]).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,heads,kv_heads,dim,partials,with_bias,rotate", [
+    (1, 28, 4, 128, 3, True, True), (5, 4, 2, 16, 1, True, True), (40, 14, 2, 64, 2, False, True), (300, 6, 3, 32, 1, True, False),
+    (513, 12, 2, 128, 1, True, True), (3, 2, 2, 256, 5, False, True)])
+def test_rotation_and_store(dtype, n, heads, kv_heads, dim, partials, with_bias, rotate):
+    """Queries get the bits of the call over a cache in the engine's type; keys and values the codes of what that call would
+    have kept in 32 bits."""
+    ops, wide = cuda_ops(dtype), cuda_ops(torch.float32)
+    width = (heads + 2 * kv_heads) * dim
+    qkv = rnd(partials, n, width, seed=3) if partials > 1 else rnd(n, width, seed=3)
+    bias = rnd(width, seed=4) if with_bias else None
+    positions = torch.randint(0, 30000, (n,), generator=torch.Generator().manual_seed(1)).to(torch.int32).to(DEV)
+    inv_freq = (10000.0 ** (-torch.arange(0, dim, 2).double() / dim)).float().to(DEV) if rotate else None
+    page = 8
+    pages = -(-n // page) + 1
+    slots = torch.randperm(pages * page, generator=torch.Generator().manual_seed(2))[:n].to(torch.int32).to(DEV)
+    if n > 4:
+        slots[3] = -1
+    q, q_same = (torch.empty(n, heads * dim, dtype=dtype, device=DEV) for _ in range(2))
+    keys, values = empty_pages(pages, page, kv_heads, dim), empty_pages(pages, page, kv_heads, dim)
+    ops.rope_kv_write(qkv, bias, positions, inv_freq, q, keys, values, slots, heads, kv_heads, dim)
+    plain = [torch.zeros(pages, page, kv_heads, dim, dtype=dtype, device=DEV) for _ in range(2)]
+    ops.rope_kv_write(qkv, bias, positions, inv_freq, q_same, *plain, slots, heads, kv_heads, dim)
+    assert torch.equal(q, q_same)
+    exact = [torch.zeros(pages, page, kv_heads, dim, device=DEV) for _ in range(2)]
+    wide.rope_kv_write(qkv, bias, positions, inv_freq, torch.empty(n, heads * dim, device=DEV), *exact, slots, heads, kv_heads, dim)
+    there = slots[slots >= 0].long()
+    for pool, x in ((keys, exact[0]), (values, exact[1])):
+        check_stored(pool, x.view(-1, kv_heads * dim)[there], there, kv_heads, dim)
+
+
+def attend(ops, case, heads, kv_heads, dim, q_lens, ctx_lens, window=None, chunk=None, scale=None, known=True):
+    out = torch.full_like(case["q"], math.nan)
+    ops.paged_attention(case["q"], QuantisedPages(case["codes_k"], case["scales_k"]), QuantisedPages(case["codes_v"], case["scales_v"]),
+                        case["table"], case["q_start"], case["ctx_len"], case["seq_of"], heads, kv_heads, dim,
+                        dim ** -0.5 if scale is None else scale, window, out, max_q_len=max(q_lens), max_ctx_len=max(ctx_lens),
+                        min_q_len=min(q_lens) if known else 0, q_lens=list(q_lens) if known else None, chunk=chunk)
+    return out
+
+
+def check_attention(dtype, heads, kv_heads, dim, page, q_lens, ctx_lens, seed=0, q_scale=1.0, splits=0, known=True, **options):
+    ops = cuda_ops(dtype)
+    ops.q8_splits = splits
+    case = oracle.pages_case(heads, kv_heads, dim, page, q_lens, ctx_lens, dtype, seed, DEV, q_scale)
+    got = attend(ops, case, heads, kv_heads, dim, q_lens, ctx_lens, known=known, **options)
+    scale = options.pop("scale", None)
+    want, bound = oracle.attention(case["q"], case["sequences"], q_lens, ctx_lens, heads, kv_heads, dim, dim ** -0.5 if scale is None else scale,
+                                   **options)
+    assert torch.isfinite(got).all()
+    excess = ((got.double() - want).abs() - bound)
+    assert excess.max().item() <= 0, f"off by {excess.max().item():.3e} more than the bound at {divmod(int(excess.argmax()), heads * dim)}"
+    again = attend(ops, case, heads, kv_heads, dim, q_lens, ctx_lens, known=known, scale=scale, **options)
+    assert torch.equal(got, again)   # no result depends on who comes first
+
+
+HEADS = [(7, 1, 128, 16), (14, 2, 64, 16), (6, 3, 32, 8), (4, 2, 16, 5), (40, 8, 128, 64), (17, 1, 48, 7), (2, 2, 256, 16), (33, 1, 80, 1)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,kv_heads,dim,page", HEADS)
+def test_single_tokens(dtype, heads, kv_heads, dim, page):
+    ctx_lens = [1, 2, 15, 31, 32, 33, 64, 65, 127, 128, 129, 300, 517]
+    check_attention(dtype, heads, kv_heads, dim, page, [1] * len(ctx_lens), ctx_lens, seed=heads)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("splits", [1, 2, 3, 16, 64])
+@pytest.mark.parametrize("options", [{}, {"window": 40}, {"chunk": 48}])
+def test_single_tokens_in_any_number_of_splits(dtype, splits, options):
+    ctx_lens = [1, 33, 700, 1900]
+    check_attention(dtype, 7, 1, 64, 16, [1] * 4, ctx_lens, splits=splits, **options)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,kv_heads,dim,page", HEADS)
+@pytest.mark.parametrize("options", [{}, {"window": 40}, {"chunk": 48}])
+def test_portions(dtype, heads, kv_heads, dim, page, options):
+    q_lens, ctx_lens = [2, 5, 33, 64, 70, 130, 3], [2, 40, 33, 129, 300, 130, 517]
+    check_attention(dtype, heads, kv_heads, dim, page, q_lens, ctx_lens, seed=dim, **options)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("known", [True, False])
+@pytest.mark.parametrize("options", [{}, {"window": 70}])
+def test_portions_beside_single_tokens(dtype, dim, known, options):
+    q_lens, ctx_lens = [1, 200, 1, 1, 37, 1], [700, 611, 1, 129, 37, 64]
+    check_attention(dtype, 12, 2, dim, 16, q_lens, ctx_lens, known=known, **options)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_large_scores(dtype):
+    """Scores of some hundreds: one key takes all the weight."""
+    check_attention(dtype, 4, 2, 64, 16, [1, 20, 1], [300, 90, 5], q_scale=60.0)
