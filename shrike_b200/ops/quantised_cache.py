@@ -21,7 +21,7 @@ DTYPE_CODE = {torch.float32: 0, torch.bfloat16: 1}
 MOST_HEAD_DIM = 256   # of the kernels over 8-bit pages
 
 
-@dataclass(frozen=True)
+@dataclass(frozen=True, slots=True)
 class QuantisedPlan:
     """How a batch's attention over 8-bit pages is cut."""
 
@@ -57,7 +57,7 @@ class QuantisedCacheOps:
         lib.shrike_kv_read_q8.argtypes = [_P] * 7 + [_I] * 5 + [_LL, _P]
         for name in ("shrike_kv_write_q8", "shrike_rope_kv_write_q8", "shrike_kv_read_q8"):
             getattr(lib, name).restype = _I
-        self._q8_libs = {}
+        self._q8_libs, self._q8_plans = {}, {}
         self._q8_scratch = self._q8_arrivals = None
         self.q8_splits = 0   # 0: the rule of `q8_plan`; n: that many splits for few rows (tests)
 
@@ -78,112 +78,143 @@ class QuantisedCacheOps:
         return lib
 
     # ---- checks
-    def _q8_here(self, *tensors):
-        """Every tensor on the GPU that this call launches on."""
-        current = torch.cuda.current_device()
-        for tensor in tensors:
-            if tensor is not None and (tensor.device.type != "cuda" or tensor.device.index != current):
-                raise _error(f"a tensor is on {tensor.device}, the current device is cuda:{current}")
-
-    def _q8_pages(self, keys, values, num_kv_heads=None, head_dim=None):
-        if keys.shape != values.shape:
-            raise _error(f"key pages {list(keys.shape)} and value pages {list(values.shape)} differ")
-        pages, page_size, heads, dim = keys.shape
-        if (num_kv_heads is not None and heads != num_kv_heads) or (head_dim is not None and dim != head_dim):
-            raise _error(f"key cache {tuple(keys.shape)} does not fit {num_kv_heads} heads of {head_dim}")
-        if dim % 16 or not 16 <= dim <= MOST_HEAD_DIM:
-            raise _error(f"head size {dim} is not served: 8-bit pages take multiples of 16 from 16 to {MOST_HEAD_DIM}")
-        if pages * page_size > 0x7FFFFFFF:
-            raise _error(f"{pages} pages of {page_size} tokens: slots are 32-bit numbers")
-        self._q8_here(keys.codes, keys.scales, values.codes, values.scales)
-        return pages, page_size, heads, dim
+    # A call of the engine's takes longer on the host than its kernel takes for few tokens, so what is right is seen in one
+    # expression of cheap questions; which of them failed is looked up only then.
+    def _q8_stream(self):
+        """The current stream's handle and device (asking torch for the stream object costs more than a launch)."""
+        device = torch._C._cuda_getDevice()
+        return device, self._held_stream if self._held_stream is not None else torch._C._cuda_getCurrentRawStream(device)
 
     @staticmethod
-    def _q8_ints(tensor, count, what):
-        if tensor.dtype != torch.int32 or not tensor.is_contiguous() or tensor.numel() != count:
-            raise _error(f"{what} must be {count} contiguous int32, is {tensor.dtype} {list(tensor.shape)}")
+    def _q8_refuse(device, named, ints=(), pages=None):
+        """Says what is wrong: `named` (tensor, dtype, what), each dense; `ints` (tensor, count, what); `pages` (keys, values, kv
+        heads, head size)."""
+        if pages is not None:
+            keys, values, num_kv_heads, head_dim = pages
+            count, page_size, heads, dim = keys.shape
+            if keys.shape != values.shape:
+                raise _error(f"key pages {list(keys.shape)} and value pages {list(values.shape)} differ")
+            if (num_kv_heads is not None and heads != num_kv_heads) or (head_dim is not None and dim != head_dim):
+                raise _error(f"key cache {tuple(keys.shape)} does not fit {num_kv_heads} heads of {head_dim}")
+            if dim % 16 or not 16 <= dim <= MOST_HEAD_DIM:
+                raise _error(f"head size {dim} is not served: 8-bit pages take multiples of 16 from 16 to {MOST_HEAD_DIM}")
+            if count * page_size > 0x7FFFFFFF:
+                raise _error(f"{count} pages of {page_size} tokens: slots are 32-bit numbers")
+            named = [*named, (keys.codes, torch.int8, "key codes"), (values.codes, torch.int8, "value codes")]
+        for tensor, dtype, what in named:
+            if tensor.get_device() != device:
+                raise _error(f"{what} must be on the current device cuda:{device}, is on {tensor.device}")
+            if tensor.dtype != dtype:
+                raise _error(f"{what} must be {dtype}, is {tensor.dtype}")
+            if not tensor.is_contiguous():
+                raise _error(f"{what} must be contiguous")
+            if tensor.data_ptr() % 16 and not dtype == torch.int32:
+                raise _error(f"{what} must begin on 16 bytes")
+        for tensor, count, what in ints:
+            if tensor.get_device() != device:
+                raise _error(f"{what} must be on the current device cuda:{device}, is on {tensor.device}")
+            if tensor.dtype != torch.int32 or not tensor.is_contiguous() or tensor.numel() != count:
+                raise _error(f"{what} must be {count} contiguous int32, is {tensor.dtype} {list(tensor.shape)}")
 
-    def _q8_rows(self, x, n, width, what):
+    @staticmethod
+    def _q8_pages_fit(device, keys, values) -> bool:
+        codes, others = keys.codes, values.codes
+        count, page_size, _heads, dim = codes.shape
+        return (codes.shape == others.shape and codes.get_device() == device and others.get_device() == device
+                and not dim % 16 and 16 <= dim <= MOST_HEAD_DIM and count * page_size <= 0x7FFFFFFF)
+
+    @staticmethod
+    def _q8_ints_fit(device, tensor, count) -> bool:
+        return tensor.get_device() == device and tensor.dtype == torch.int32 and tensor.numel() == count and tensor.is_contiguous()
+
+    def _q8_rows(self, device, x, n, width, what):
         """The distance of x's rows in elements; a row's elements lie side by side."""
-        if x.dtype != self.dtype or tuple(x.shape) != (n, width) or (width > 1 and x.stride(1) != 1) or (n > 1 and x.stride(0) < 0):
-            raise _error(f"{what} must be {self.dtype} [{n}, {width}] with adjacent columns, is {x.dtype} {list(x.shape)}")
+        if (x.get_device() != device or x.dtype != self.dtype or tuple(x.shape) != (n, width) or (width > 1 and x.stride(1) != 1)
+                or (n > 1 and x.stride(0) < 0)):
+            raise _error(f"{what} must be {self.dtype} [{n}, {width}] with adjacent columns on cuda:{device}, is {x.dtype} "
+                         f"{list(x.shape)} on {x.device}")
         return x.stride(0) if n > 1 else width
 
     # ---- the cache
     def _kv_write_q8(self, k_new, v_new, keys, values, slots):
-        from .cuda_ops import _check, _ptr
+        from .cuda_ops import _check
 
-        pages, page_size, heads, dim = self._q8_pages(keys, values)
+        device, stream = self._q8_stream()
+        pages, page_size, heads, dim = keys.codes.shape
         n = k_new.shape[0]
-        strides = [self._q8_rows(x, n, heads * dim, what) for x, what in ((k_new, "new keys"), (v_new, "new values"))]
-        self._q8_ints(slots, n, "slots")
-        self._q8_here(k_new, v_new, slots)
+        if not (self._q8_pages_fit(device, keys, values) and self._q8_ints_fit(device, slots, n)):
+            self._q8_refuse(device, (), [(slots, n, "slots")], (keys, values, None, None))
+        k_stride = self._q8_rows(device, k_new, n, heads * dim, "new keys")
+        v_stride = self._q8_rows(device, v_new, n, heads * dim, "new values")
         if n == 0:
             return
         self.launches += 1
         _check(self.core.shrike_kv_write_q8(
-            _ptr(k_new), _ptr(v_new), *strides, _ptr(keys.codes), _ptr(keys.scales), _ptr(values.codes), _ptr(values.scales),
-            _ptr(slots), self.code, n, heads, dim, page_size, pages * page_size, self._stream()), "kv_write_q8")
+            k_new.data_ptr(), v_new.data_ptr(), k_stride, v_stride, keys.codes.data_ptr(), keys.scales.data_ptr(),
+            values.codes.data_ptr(), values.scales.data_ptr(), slots.data_ptr(), self.code, n, heads, dim, page_size,
+            pages * page_size, stream), "kv_write_q8")
 
     def _rope_kv_write_q8(self, qkv, bias, positions, inv_freq, q_out, keys, values, slots, num_heads, num_kv_heads, head_dim):
-        from .cuda_ops import _check, _dense, _ptr
+        from .cuda_ops import _check, _ptr
 
-        pages, page_size, _heads, _dim = self._q8_pages(keys, values, num_kv_heads, head_dim)
-        _dense(q_out, self.dtype, "q")
+        device, stream = self._q8_stream()
+        pages, page_size, _heads, _dim = keys.codes.shape
         partials, stride = self._stack(qkv)
         n, width = qkv.shape[-2], (num_heads + 2 * num_kv_heads) * head_dim
-        if qkv.dtype != torch.float32 or qkv.shape[-1] != width or qkv.stride(-1) != 1 or (n > 1 and qkv.stride(-2) != width):
-            raise _error(f"qkv must be float32 rows of {width}, is {qkv.dtype} {list(qkv.shape)}")
+        self._q8_refuse(device, [(q_out, self.dtype, "q")] + [(x, torch.float32, what) for x, what in (
+            (bias, "bias"), (inv_freq, "inverse frequencies")) if x is not None],
+            [(positions, n, "positions"), (slots, n, "slots")], (keys, values, num_kv_heads, head_dim))
+        if (qkv.get_device() != device or qkv.dtype != torch.float32 or qkv.shape[-1] != width or qkv.stride(-1) != 1
+                or (n > 1 and qkv.stride(-2) != width)):
+            raise _error(f"qkv must be float32 rows of {width} on cuda:{device}, is {qkv.dtype} {list(qkv.shape)} on {qkv.device}")
         if q_out.numel() != n * num_heads * head_dim:
             raise _error(f"q {list(q_out.shape)} does not fit {n} tokens of {num_heads} heads of {head_dim}")
-        if bias is not None:
-            _dense(bias, torch.float32, "bias")
-            if bias.numel() != width:
-                raise _error(f"a bias of {bias.numel()} for rows of {width}")
-        if inv_freq is not None:
-            _dense(inv_freq, torch.float32, "inverse frequencies")
-            if inv_freq.numel() != head_dim // 2:
-                raise _error(f"{inv_freq.numel()} inverse frequencies for heads of {head_dim}")
-        self._q8_ints(positions, n, "positions")
-        self._q8_ints(slots, n, "slots")
-        self._q8_here(qkv, bias, positions, inv_freq, q_out, slots)
+        if bias is not None and bias.numel() != width:
+            raise _error(f"a bias of {bias.numel()} for rows of {width}")
+        if inv_freq is not None and inv_freq.numel() != head_dim // 2:
+            raise _error(f"{inv_freq.numel()} inverse frequencies for heads of {head_dim}")
         if n == 0:
             return
         self.launches += 1
         _check(self.core.shrike_rope_kv_write_q8(
             _ptr(qkv), _ptr(bias), _ptr(positions), _ptr(inv_freq), _ptr(q_out), _ptr(keys.codes), _ptr(keys.scales),
             _ptr(values.codes), _ptr(values.scales), _ptr(slots), self.code, n, num_heads, num_kv_heads, head_dim, page_size,
-            pages * page_size, partials, stride, self._stream()), "rope_kv_write_q8")
+            pages * page_size, partials, stride, stream), "rope_kv_write_q8")
 
     def kv_read(self, keys, values, slots, k_out, v_out):
         """Reads tokens back from 8-bit pages: row n of `k_out` and `v_out` ([N, kv heads * head size], contiguous, in the engine's
         type) is what `slots[n]` (int32 [N]) holds, codes times scale in 32 bits rounded once; zeros for a slot that is none of
         the pool's (a negative one, say).  A row stored from an infinity or a NaN comes back as NaN."""
-        from .cuda_ops import _check, _dense, _ptr
+        from .cuda_ops import _check
 
         if not quantised(keys, values):
             raise _error("kv_read reads 8-bit pages; a cache in the engine's type is indexed as it is")
-        pages, page_size, heads, dim = self._q8_pages(keys, values)
-        n = slots.numel()
-        self._q8_ints(slots, n, "slots")
-        for x, what in ((k_out, "keys read"), (v_out, "values read")):
-            _dense(x, self.dtype, what)
-            if tuple(x.shape) != (n, heads * dim):
-                raise _error(f"{what} must be [{n}, {heads * dim}], are {list(x.shape)}")
-            if x.data_ptr() % 16:
-                raise _error(f"{what} must begin on 16 bytes")
-        self._q8_here(slots, k_out, v_out)
+        device, stream = self._q8_stream()
+        pages, page_size, heads, dim = keys.codes.shape
+        n, dtype = slots.numel(), self.dtype
+        k_at, v_at = k_out.data_ptr(), v_out.data_ptr()
+        shape = (n, heads * dim)
+        if not (self._q8_pages_fit(device, keys, values) and self._q8_ints_fit(device, slots, n) and k_out.dtype == dtype
+                and v_out.dtype == dtype and k_out.shape == shape and v_out.shape == shape and k_out.get_device() == device
+                and v_out.get_device() == device and k_out.is_contiguous() and v_out.is_contiguous() and not (k_at | v_at) % 16):
+            self._q8_refuse(device, [(k_out, dtype, "keys read"), (v_out, dtype, "values read")], [(slots, n, "slots")],
+                            (keys, values, None, None))
+            raise _error(f"keys and values read must be [{n}, {heads * dim}], are {list(k_out.shape)} and {list(v_out.shape)}")
         if n == 0:
             return
         self.launches += 1
         _check(self.core.shrike_kv_read_q8(
-            _ptr(keys.codes), _ptr(keys.scales), _ptr(values.codes), _ptr(values.scales), _ptr(slots), _ptr(k_out), _ptr(v_out),
-            self.code, n, heads, dim, page_size, pages * page_size, self._stream()), "kv_read_q8")
+            keys.codes.data_ptr(), keys.scales.data_ptr(), values.codes.data_ptr(), values.scales.data_ptr(), slots.data_ptr(),
+            k_at, v_at, self.code, n, heads, dim, page_size, pages * page_size, stream), "kv_read_q8")
 
     # ---- attention
     def q8_plan(self, num_heads, num_kv_heads, head_dim, num_seqs, max_blocks, page_size, max_q_len, min_q_len, window=0) -> QuantisedPlan:
         """How a batch over 8-bit pages is cut: a function of its shape alone, so that a captured launch sequence serves every
         batch of that shape."""
+        key = (num_heads, num_kv_heads, head_dim, num_seqs, max_blocks, page_size, max_q_len > 1, min_q_len <= 1, window, self.q8_splits)
+        held = self._q8_plans.get(key)
+        if held is not None and held[0] == self.generation:   # the scratch has not moved since
+            return held[1]
         lib = self._q8_lib(head_dim)
         has_single, has_portions = min_q_len <= 1, max_q_len > 1
         splits, scratch, arrivals = 1, None, None
@@ -207,7 +238,11 @@ class QuantisedCacheOps:
                     self._q8_arrivals = torch.zeros(max(pairs, 4096), dtype=torch.int32, device=self.device)
                     self.generation += 1
                 scratch, arrivals = self._q8_scratch, self._q8_arrivals
-        return QuantisedPlan(has_single, has_portions, splits, scratch, arrivals)
+        plan = QuantisedPlan(has_single, has_portions, splits, scratch, arrivals)
+        if len(self._q8_plans) >= 4096:
+            self._q8_plans.clear()
+        self._q8_plans[key] = (self.generation, plan)
+        return plan
 
     @staticmethod
     def q8_few_row_splits(keys: int, pairs: int, resident: int) -> int:
@@ -217,31 +252,33 @@ class QuantisedCacheOps:
 
     def _paged_attention_q8(self, q, keys, values, block_table, q_start, ctx_len, seq_of_token, num_heads, num_kv_heads, head_dim,
                             scale, window, out, max_q_len, min_q_len):
-        from .cuda_ops import _check, _dense, _ptr
+        from .cuda_ops import _check, _ptr
 
-        pages, page_size, _heads, _dim = self._q8_pages(keys, values, num_kv_heads, head_dim)
-        _dense(q, self.dtype, "q")
-        _dense(out, self.dtype, "attention output")
-        _dense(block_table, torch.int32, "block table")
-        n = q.shape[0]
-        if num_kv_heads < 1 or num_heads % num_kv_heads:
-            raise _error(f"{num_heads} heads do not share {num_kv_heads} kv heads evenly")
-        if tuple(q.shape) != (n, num_heads * head_dim) or out.shape != q.shape:
-            raise _error(f"q {list(q.shape)} and output {list(out.shape)} must be [tokens, {num_heads * head_dim}]")
+        device, stream = self._q8_stream()
+        pages, page_size, heads, dim = keys.codes.shape
         num_seqs, max_blocks = block_table.shape
-        self._q8_ints(q_start, num_seqs + 1, "query starts")
-        self._q8_ints(ctx_len, num_seqs, "context lengths")
-        self._q8_here(q, out, block_table, q_start, ctx_len)
-        if q.data_ptr() % 16 or out.data_ptr() % 16:
-            raise _error("q and the attention output must begin on 16 bytes")
+        n, dtype = q.shape[0], self.dtype
+        q_at, out_at = q.data_ptr(), out.data_ptr()
+        shape = (n, num_heads * head_dim)
+        if not (self._q8_pages_fit(device, keys, values) and heads == num_kv_heads and dim == head_dim and not num_heads % heads
+                and q.dtype == dtype and out.dtype == dtype and q.shape == shape and out.shape == shape and q.get_device() == device
+                and out.get_device() == device and q.is_contiguous() and out.is_contiguous() and not (q_at | out_at) % 16
+                and self._q8_ints_fit(device, block_table, num_seqs * max_blocks) and self._q8_ints_fit(device, q_start, num_seqs + 1)
+                and self._q8_ints_fit(device, ctx_len, num_seqs) and max_q_len >= 1):
+            self._q8_refuse(device, [(q, dtype, "q"), (out, dtype, "attention output")], [
+                (block_table, num_seqs * max_blocks, "block table"), (q_start, num_seqs + 1, "query starts"),
+                (ctx_len, num_seqs, "context lengths")], (keys, values, num_kv_heads, head_dim))
+            if num_heads % num_kv_heads:
+                raise _error(f"{num_heads} heads do not share {num_kv_heads} kv heads evenly")
+            if max_q_len < 1:
+                raise _error("paged_attention over 8-bit pages needs max_q_len, the longest entry of the batch")
+            raise _error(f"q {list(q.shape)} and output {list(out.shape)} must be [tokens, {num_heads * head_dim}]")
         if n == 0 or num_seqs == 0:
             return
-        if max_q_len < 1:
-            raise _error("paged_attention over 8-bit pages needs max_q_len, the longest entry of the batch")
         plan = self.q8_plan(num_heads, num_kv_heads, head_dim, num_seqs, max_blocks, page_size, max_q_len, min_q_len, window or 0)
         self.launches += plan.has_single + plan.has_portions
-        _check(self._q8_lib(head_dim).shrike_paged_attention_q8(
-            _ptr(q), _ptr(keys.codes), _ptr(keys.scales), _ptr(values.codes), _ptr(values.scales), _ptr(block_table), max_blocks,
-            _ptr(q_start), _ptr(ctx_len), self.code, num_seqs, num_heads, num_kv_heads, page_size, pages, scale, window or 0,
-            _ptr(out), int(plan.has_single), int(plan.has_portions), max_q_len, plan.splits, _ptr(plan.scratch),
-            _ptr(plan.arrivals), self._stream()), "paged_attention_q8")
+        _check(self._q8_libs[head_dim].shrike_paged_attention_q8(
+            q_at, keys.codes.data_ptr(), keys.scales.data_ptr(), values.codes.data_ptr(), values.scales.data_ptr(),
+            block_table.data_ptr(), max_blocks, q_start.data_ptr(), ctx_len.data_ptr(), self.code, num_seqs, num_heads, num_kv_heads,
+            page_size, pages, scale, window or 0, out_at, plan.has_single, plan.has_portions, max_q_len, plan.splits,
+            _ptr(plan.scratch), _ptr(plan.arrivals), stream), "paged_attention_q8")
