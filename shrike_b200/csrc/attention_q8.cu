@@ -2,26 +2,29 @@
 //
 // With codes c and scales s (keys: c^k_j, s^k_j; values: c^v_j, s^v_j) a row q of head h sees
 //   z_j = scale s^k_j (q . c^k_j),   p_j = 2^(log2e z_j - m),   o = sum_j (p_j s^v_j) c^v_j / sum_j p_j
-// Codes are integers up to 127: exact in float16.  Both products run on mma.sync m16n8k16 with float16 operands and float32
+// Codes are integers up to 127: exact in float16.  Both products run on mma.sync m16n8k16 with float16 operands and 32-bit
 // sums, and nothing but the queries and the weights is ever rounded:
 //   queries   scaled by a power of two per row (largest magnitude in [2^14, 2^15)); bfloat16 queries are then exact, float32
 //             ones are split in two float16 parts (22 bits) whose products are added in the accumulator
-//   weights   w_j = p_j s^v_j.  The base m of the exponentials is a row's largest score plus an exponent F that puts the largest
-//             value scale the row has seen at 2^13 ... 2^14 (the sums and the outputs are all in units of 2^m, so F costs
-//             nothing): float16 then keeps 11 bits of a weight down to 2^-27 of the largest possible one (bfloat16 would keep 8
-//             bits), and 22 bits in two parts for float32
-// A warp takes 16 query rows (the heads that share a kv head side by side, token by token) against 32 keys a step.
-//
-// The keys' order inside a product is free as long as scores and values agree on it, and so is the order of a head's elements
-// in q . c: both are chosen so that a lane's operands are consecutive bytes.  Element order: a lane reads 16 codes of a key
-// with one load and they are its operands of four products.  Key order: column n of a group of eight is key n ^ ((n >> 1) & 1),
-// and 16-byte chunks of a row are swizzled with it, so that neither the keys' nor the values' loads meet in a bank.
-// Four codes become two registers of float16 pairs by a byte permutation (1024 + code + 128, exact) and a subtraction.
+//   weights   w_j = p_j s^v_j.  The base m of the exponentials is a row's largest score (it may lag by up to 2^6) plus an
+//             exponent F that puts the largest value scale the row has seen at 2^8 ... 2^9 (the sums and the outputs are all in
+//             units of 2^m, so F costs nothing): float16 then keeps 11 bits of a weight down to 2^-22 of the largest possible
+//             one (bfloat16 would keep 8 bits), and 22 bits in two parts for float32
+// KEYS ARE THE M OF THE PRODUCTS, query rows the N: S^T = K Q^T and O^T = V^T P^T.  The heads that share a kv head lie side by
+// side, token by token, as rows; eight of them make a product's N, so that the usual groups of up to eight heads waste nothing
+// (rows as M would be padded to 16: twice the products, softmax work and registers), and wider tiles (`NT` times eight rows)
+// share the conversion of the codes, which is what the kernel spends most of its instructions on.
+// A warp takes 32 keys a step.  The keys' order inside a product is free as long as scores and values agree on it, and so is
+// the order of a head's elements in q . c: both are chosen so that a lane's operands are consecutive bytes.  Element order: a
+// lane reads 16 codes of a key with one load and they are its operands of four products.  Key order: row n of a group of eight
+// is key n ^ ((n >> 1) & 1), and 16-byte chunks of a row are swizzled with it, so that neither the keys' nor the values' loads
+// meet in a bank.  Four codes become two registers of float16 pairs by a byte permutation (1024 + code + 128, exact) and a
+// subtraction; the weights go from the scores' layout to an operand's through movmatrix.
 //
 // Two forms.  Few rows (single tokens): the rows' keys are dealt to `splits` CTAs and to each CTA's four warps, each with its
 // own ring of cp.async copies (no barrier in the loop); the warps' results meet in shared memory, the CTAs' in global memory,
-// where the last CTA to arrive adds them up in the order of the splits.  Many rows (portions): four warps of 16 rows each share
-// one ring of key tiles.
+// where the last CTA to arrive adds them up in the order of the splits.  Many rows (portions): four warps of 8 NT rows each
+// share one ring of key tiles.
 #include <cuda_fp16.h>
 
 #include "common.cuh"
@@ -35,7 +38,6 @@ namespace attnq8 {
 constexpr int D = SHRIKE_HEAD_DIM;
 static_assert(D % 16 == 0 && D >= 16 && D <= 256, "head sizes are multiples of 16 up to 256");
 constexpr int WARPS = 4, THREADS = WARPS * 32;
-constexpr int ROWS = 16;                 // query rows of a warp
 constexpr int KEYS = 32;                 // keys of a step
 constexpr int CHUNKS = D / 16;           // 16-byte chunks of a key's codes
 constexpr int STEPS_K = D / 16;          // products along the head size, for 8 keys
@@ -43,7 +45,7 @@ constexpr int BLOCKS_V = (D + 31) / 32;  // runs of 32 elements of the output
 constexpr bool WIDE = D % 64 == 0;       // keys are read 16 bytes a lane (else 4)
 constexpr int TILE = KEYS * D;           // bytes of a step's key (or value) codes
 constexpr int STAGE = 2 * TILE + 2 * KEYS * 4;   // keys, values, and their scales
-constexpr int STAGES = 3;
+constexpr int STAGES = 2;                // one lands while the other is used; a third would cost a CTA an SM
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr int MAX_SPLITS = 64;
 
@@ -58,10 +60,11 @@ struct Args {
   const void* q;
   void* out;
   int max_blocks, num_heads, num_kv_heads, page_size, num_pages, window;
+  int page_shift;      // page_size is 2^page_shift, or -1
   int only;            // 1: entries of one token, 2: longer ones, 0: all
   float scale_log2;
   int splits;
-  float* scratch;      // [(entry, kv head, row tile)][split][16][D + 2]: unnormalised rows, then each row's base and sum
+  float* scratch;      // [(entry, kv head, row tile)][split][rows][D + 2]: unnormalised rows, then each row's base and sum
   int* arrivals;       // [(entry, kv head, row tile)]: CTAs that have left their share; zero between launches
 };
 
@@ -109,7 +112,8 @@ __device__ __forceinline__ int swizzle(int row) {
 __device__ __forceinline__ int chunk_at(int row, int chunk) { return row * D + ((chunk ^ swizzle(row)) << 4); }
 
 // F's range: sums of 2^(z - m) stay within float32 for any count of keys, and weights of 2^-20 of the largest above its least.
-constexpr int LEAST_EXPONENT = -93, MOST_EXPONENT = 107;
+constexpr int LEAST_EXPONENT = -93, MOST_EXPONENT = 107, SCALE_BITS = 8;
+constexpr float BASE_LAG = 6.0f;   // float16's largest power of two is 2^15: 2^9 times 2^6
 // A magnitude's bits (which order as the magnitudes do), 0 for infinities and NaN.
 __device__ __forceinline__ unsigned finite_bits(float x) {
   const unsigned bits = __float_as_uint(x) & 0x7fffffffu;
@@ -119,159 +123,155 @@ __device__ __forceinline__ unsigned finite_bits(float x) {
 // 2^e for e in [-126, 127].
 __device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e + 127) << 23); }
 
-// Brings the codes and scales of the 32 keys from `key0` on into a stage; `threads` threads of which this is number `id` share
-// the work, and each of their warps holds in lane l the slot of key key0 + l (-1: no such key).
+// Where a lane's key lies: its row among all codes (-1: no such key), and its place among the scales.
+struct Place {
+  int row;
+  long long scale;
+};
+// The place of a key, nowhere if it lies behind `last_key` or its page is not one of the pool's.
+__device__ __forceinline__ Place place_of(const Args& args, const int* table, int kv_head, int key, int last_key) {
+  Place at{-1, 0};
+  if (key > last_key) return at;
+  const int block = args.page_shift >= 0 ? key >> args.page_shift : key / args.page_size;
+  if (block >= args.max_blocks) return at;
+  const int page = table[block], within = key - block * args.page_size;
+  if (page < 0 || page >= args.num_pages) return at;
+  at.row = page * args.page_size + within;
+  at.scale = (static_cast<long long>(page) * args.num_kv_heads + kv_head) * args.page_size + within;
+  return at;
+}
+
+// Brings the codes and scales of 32 keys into a stage; `COUNT` threads of which this is number `id` share the work, and each of
+// their warps holds in lane l the place of key l.
 template <int COUNT>
-__device__ __forceinline__ void load_step(const Args& args, int kv_head, int slot_of_lane, unsigned stage, int id) {
+__device__ __forceinline__ void load_step(const Args& args, int kv_head, const Place& place, unsigned stage, int id) {
+  const int row_bytes = args.num_kv_heads * D;
 #pragma unroll
   for (int k = 0; k < (KEYS * CHUNKS + COUNT - 1) / COUNT; ++k) {
     const int idx = id + k * COUNT;
     const int key = idx / CHUNKS, chunk = idx - key * CHUNKS;
-    const int slot = __shfl_sync(0xffffffffu, slot_of_lane, key & 31);
+    const int row = __shfl_sync(0xffffffffu, place.row, key & 31);
     if (KEYS * CHUNKS % COUNT == 0 || idx < KEYS * CHUNKS) {
-      const bool there = slot >= 0;
-      const size_t at = (static_cast<size_t>(there ? slot : 0) * args.num_kv_heads + kv_head) * D + chunk * 16;
+      const bool there = row >= 0;
+      const long long at = static_cast<long long>(there ? row : 0) * row_bytes + (kv_head * D + chunk * 16);
       const unsigned to = stage + chunk_at(key, chunk);
       copy16(to, args.k_codes + at, there);
       copy16(to + TILE, args.v_codes + at, there);
     }
   }
   if (id < KEYS) {
-    const bool there = slot_of_lane >= 0;
-    const int page = there ? slot_of_lane / args.page_size : 0, within = there ? slot_of_lane - page * args.page_size : 0;
-    const size_t at = (static_cast<size_t>(page) * args.num_kv_heads + kv_head) * args.page_size + within;
-    copy4(stage + 2 * TILE + id * 4, args.k_scales + at, there);
-    copy4(stage + 2 * TILE + KEYS * 4 + id * 4, args.v_scales + at, there);
+    copy4(stage + 2 * TILE + id * 4, args.k_scales + place.scale, place.row >= 0);
+    copy4(stage + 2 * TILE + KEYS * 4 + id * 4, args.v_scales + place.scale, place.row >= 0);
   }
-}
-
-// The slot of a key, -1 where it lies behind `last_key` or its page is not one of the pool's.
-__device__ __forceinline__ int slot_of(const Args& args, const int* table, int key, int last_key) {
-  if (key > last_key) return -1;
-  const int block = key / args.page_size;
-  if (block >= args.max_blocks) return -1;
-  const int page = table[block];
-  return page < 0 || page >= args.num_pages ? -1 : page * args.page_size + key % args.page_size;
 }
 
 template <typename T> struct Parts { static constexpr int COUNT = 1; };
 template <> struct Parts<float> { static constexpr int COUNT = 2; };
 
-// A warp's 16 rows: queries as operands, running base, sum and output.
-template <typename T>
+// The 8x8 matrix of 16-bit elements whose row g a quad of lanes holds, transposed.
+__device__ __forceinline__ unsigned transpose8(unsigned v) {
+  unsigned d;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(v));
+  return d;
+}
+
+// A warp's rows, NT times eight of them: queries as operands, running bases, sums and outputs.  Lane 4 g + t holds query row g's
+// operands (of each eight), and the scores, sums and outputs of rows 2 t and 2 t + 1.
+template <typename T, int NT>
 struct Rows {
+  static constexpr int ROWS = 8 * NT;
   static constexpr int PARTS = Parts<T>::COUNT;
-  static constexpr bool IN_SHARED = STEPS_K * PARTS > 8;   // query operands in shared memory, else in registers
-  static constexpr int SHARED_BYTES = IN_SHARED ? STEPS_K * PARTS * 512 : 0;   // for one warp's rows
-  unsigned q[IN_SHARED ? 1 : STEPS_K * PARTS][4];
-  float factor[2];      // what a score is multiplied by, for rows g and g + 8
-  int first[2], last[2];   // the keys those rows see
-  float most[2], base[2], sum[2];   // largest score, base m = most + F, sum of 2^(z - m)
-  int exponent[2];      // F
-  float o[BLOCKS_V * 4][4];
+  static constexpr bool IN_SHARED = STEPS_K * PARTS * NT > 16;   // query operands in shared memory, else in registers
+  static constexpr int SHARED_BYTES = IN_SHARED ? STEPS_K * PARTS * NT * 256 : 0;   // for one warp's rows
+  uint2 q[IN_SHARED ? 1 : STEPS_K * PARTS * NT];
+  float factor[NT][2];         // what q . c s^k is multiplied by to be a score
+  int first[NT][2], last[NT][2];   // the keys a row sees
+  float most[NT][2], base[NT][2], sum[NT][2];   // what is taken for the largest score, base m = most + F, sum of 2^(z - m)
+  int exponent[NT][2];         // F
+  float o[NT][BLOCKS_V * 2][4];
 
   __device__ __forceinline__ static int element_of(int step, int t) {   // a lane's first element of four in a product
     return WIDE ? 16 * (t + 4 * (step / 4)) + 4 * (step % 4) : 4 * (t + 4 * step);
   }
+  // The element of the head that o[nt][2 b + m][c] belongs to, and its row.
+  __device__ __forceinline__ static int out_element(int b, int g) { return 32 * b + 4 * g; }   // m = 0, c = 0; then + 2 m + (c >> 1)
 
-  // Rows row0 ... row0 + 15 of an entry whose tokens begin at `start`; `group` heads share kv head `kv_head`.
-  __device__ void begin(const Args& args, int row0, int rows, int start, int group, int kv_head, int pos0, uint4* shared, int lane) {
+  // Rows row0 ... of an entry whose tokens begin at `start`; `group` heads share kv head `kv_head`.
+  __device__ __forceinline__ void begin(const Args& args, int row0, int rows, int start, int group, int kv_head, int pos0, uint2* shared, int lane) {
     const int g = lane >> 2, t = lane & 3;
-    const T* src[2];
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const int row = row0 + g + 8 * r, token = row / group, head = kv_head * group + row - token * group;
+    for (int nt = 0; nt < NT; ++nt) {
+      const int row = row0 + 8 * nt + g, token = row / group, head = kv_head * group + row - token * group;
       const bool there = row < rows;
-      src[r] = there ? static_cast<const T*>(args.q) + (static_cast<size_t>(start + token) * args.num_heads + head) * D : nullptr;
-      last[r] = pos0 + (there ? token : (rows - 1) / group);   // a row that is not there sees what the last one sees: nobody reads it
-      first[r] = first_visible_key(last[r], args.window);
-      most[r] = base[r] = -INFINITY;
-      sum[r] = 0.f;
-      exponent[r] = LEAST_EXPONENT;
-    }
-    float lift[2];
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
+      const T* src = static_cast<const T*>(args.q) + (there ? (static_cast<size_t>(start + token) * args.num_heads + head) * D : 0);
+      float x[STEPS_K][4];
       unsigned top = 0u;   // the largest magnitude's bits, of finite elements
 #pragma unroll
       for (int s = 0; s < STEPS_K; ++s) {
-        float x[4] = {0.f, 0.f, 0.f, 0.f};
-        if (src[r] != nullptr) load4<T>(src[r] + element_of(s, t), x);
+        x[s][0] = x[s][1] = x[s][2] = x[s][3] = 0.f;
+        if (there) load4<T>(src + element_of(s, t), x[s]);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const unsigned bits = __float_as_uint(x[e]) & 0x7fffffffu;
-          top = bits < 0x7f800000u && bits > top ? bits : top;
-        }
+        for (int e = 0; e < 4; ++e) top = max(top, finite_bits(x[s][e]));
       }
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
       const int e = min(max(static_cast<int>(top >> 23) - 127, -100), 126);
-      lift[r] = power_of_two(14 - e);
-      factor[r] = args.scale_log2 * power_of_two(e - 14);
-    }
+      const float lift = args.scale_log2 < 0.f ? -power_of_two(14 - e) : power_of_two(14 - e);
 #pragma unroll
-    for (int s = 0; s < STEPS_K; ++s) {
-      unsigned a[PARTS][4];
+      for (int s = 0; s < STEPS_K; ++s) {
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        float x[4] = {0.f, 0.f, 0.f, 0.f};
-        if (src[r] != nullptr) load4<T>(src[r] + element_of(s, t), x);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] *= lift[r];
+        for (int i = 0; i < 4; ++i) x[s][i] *= lift;
 #pragma unroll
         for (int part = 0; part < PARTS; ++part) {
-          a[part][r] = pack_half(x[0], x[1]);
-          a[part][r + 2] = pack_half(x[2], x[3]);
+          const uint2 b = make_uint2(pack_half(x[s][0], x[s][1]), pack_half(x[s][2], x[s][3]));
+          if (IN_SHARED) shared[((s * PARTS + part) * NT + nt) * 32 + lane] = b;
+          else q[IN_SHARED ? 0 : (s * PARTS + part) * NT + nt] = b;
           if (part + 1 < PARTS) {
-            x[0] -= low_half(a[part][r]);
-            x[1] -= high_half(a[part][r]);
-            x[2] -= low_half(a[part][r + 2]);
-            x[3] -= high_half(a[part][r + 2]);
+            x[s][0] -= low_half(b.x);
+            x[s][1] -= high_half(b.x);
+            x[s][2] -= low_half(b.y);
+            x[s][3] -= high_half(b.y);
           }
         }
       }
 #pragma unroll
-      for (int part = 0; part < PARTS; ++part) {
-        if (IN_SHARED) {
-          shared[(s * PARTS + part) * 32 + lane] = make_uint4(a[part][0], a[part][1], a[part][2], a[part][3]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) q[IN_SHARED ? 0 : s * PARTS + part][i] = a[part][i];
-        }
+      for (int c = 0; c < 2; ++c) {
+        const int mine = row0 + 8 * nt + 2 * t + c;
+        // a scale of zero leaves all scores equal; a hidden key's -inf has to stay one
+        factor[nt][c] = fmaxf(fabsf(args.scale_log2) * power_of_two(__shfl_sync(0xffffffffu, e, 4 * (2 * t + c)) - 14), 1e-38f);
+        // a row that is not there sees what the last one sees: nobody reads it
+        last[nt][c] = pos0 + min(mine, rows - 1) / group;
+        first[nt][c] = first_visible_key(last[nt][c], args.window);
+        most[nt][c] = base[nt][c] = -INFINITY;
+        sum[nt][c] = 0.f;
+        exponent[nt][c] = LEAST_EXPONENT;
       }
-    }
 #pragma unroll
-    for (int i = 0; i < BLOCKS_V * 4; ++i)
+      for (int i = 0; i < BLOCKS_V * 2; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
-  }
-
-  __device__ __forceinline__ void operand(unsigned (&a)[4], int index, const uint4* shared, int lane) const {
-    if (IN_SHARED) {
-      const uint4 v = shared[index * 32 + lane];
-      a[0] = v.x; a[1] = v.y; a[2] = v.z; a[3] = v.w;
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) a[i] = q[IN_SHARED ? 0 : index][i];
+        for (int c = 0; c < 4; ++c) o[nt][i][c] = 0.f;
     }
   }
 
   // The 32 keys from `key0` on, which lie in `stage`.
-  __device__ __forceinline__ void step(const unsigned char* stage, int key0, const uint4* shared, int lane) {
+  __device__ __forceinline__ void step(const unsigned char* stage, int key0, const uint2* shared, int lane) {
     const int g = lane >> 2, t = lane & 3;
     const unsigned char* k_tile = stage;
     const unsigned char* v_tile = stage + TILE;
     const float* k_scales = reinterpret_cast<const float*>(stage + 2 * TILE);
     const float* v_scales = k_scales + KEYS;
-    float s[4][4];
+    float s[NT][2][4];   // [16 keys]: c & 1 the row, c >> 1 the eight keys
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int c = 0; c < 4; ++c) s[j][c] = 0.f;
+      for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) s[nt][kk][c] = 0.f;
     // scores
 #pragma unroll
     for (int i = 0; i < (WIDE ? D / 64 : STEPS_K); ++i) {
-      unsigned words[4][WIDE ? 4 : 1];
+      constexpr int WORDS = WIDE ? 4 : 1;
+      unsigned words[4][WORDS];   // of keys 8 j + key_of(g)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int key = 8 * j + key_of(g);
@@ -286,92 +286,108 @@ struct Rows {
         }
       }
 #pragma unroll
-      for (int w = 0; w < (WIDE ? 4 : 1); ++w) {
-        unsigned a[PARTS][4];
+      for (int w = 0; w < WORDS; ++w) {
+        uint2 b[PARTS][NT];
 #pragma unroll
-        for (int part = 0; part < PARTS; ++part) operand(a[part], ((WIDE ? 4 * i : i) + w) * PARTS + part, shared, lane);
+        for (int part = 0; part < PARTS; ++part)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const unsigned biased = words[j][w] ^ 0x80808080u;
-          const unsigned b0 = codes_to_half<0x4140>(biased), b1 = codes_to_half<0x4342>(biased);
-#pragma unroll
-          for (int part = 0; part < PARTS; ++part) mma(s[j], a[part], b0, b1);
-        }
-      }
-    }
-    // what each row sees, and the largest value scale among that
-    const bool edge = __any_sync(0xffffffffu, key0 < first[0] || key0 < first[1] || key0 + KEYS - 1 > last[0] || key0 + KEYS - 1 > last[1]);
-    unsigned top[2];
-    if (!edge) {
-      top[0] = top[1] = __reduce_max_sync(0xffffffffu, finite_bits(v_scales[lane]));
-    } else {
-#pragma unroll
-      for (int r = 0; r < 2; ++r) top[r] = 0u;
-    }
-    float correction[2];
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const int within = 8 * j + key_of(2 * t + c), key = key0 + within;
-        const float k_scale = k_scales[within];
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          s[j][2 * r + c] *= k_scale * factor[r];
-          if (edge) {
-            if (key >= first[r] && key <= last[r]) top[r] = max(top[r], finite_bits(v_scales[within]));
-            else s[j][2 * r + c] = -INFINITY;
+          for (int nt = 0; nt < NT; ++nt) {
+            const int index = ((i * WORDS + w) * PARTS + part) * NT + nt;
+            b[part][nt] = IN_SHARED ? shared[index * 32 + lane] : q[IN_SHARED ? 0 : index];
           }
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+          const unsigned lo = words[2 * kk][w] ^ 0x80808080u, hi = words[2 * kk + 1][w] ^ 0x80808080u;
+          const unsigned a[4] = {codes_to_half<0x4140>(lo), codes_to_half<0x4140>(hi), codes_to_half<0x4342>(lo), codes_to_half<0x4342>(hi)};
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int part = 0; part < PARTS; ++part) mma(s[nt][kk], a, b[part][nt].x, b[part][nt].y);
         }
       }
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      float largest = -INFINITY;
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int c = 0; c < 2; ++c) largest = fmaxf(largest, s[j][2 * r + c]);
-      largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
-      largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
-      if (edge) {
-        top[r] = max(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
-        top[r] = max(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
-      }
-      exponent[r] = max(exponent[r], min(static_cast<int>(top[r] >> 23) - 127 - 13, MOST_EXPONENT));
-      most[r] = fmaxf(most[r], largest);
-      const float next = most[r] + static_cast<float>(exponent[r]), from = most[r] == -INFINITY ? 0.f : next;
-      correction[r] = base[r] == next ? 1.f : fast_exp2(base[r] - from);
-      base[r] = next;
-      float total = 0.f;
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const float p = fast_exp2(s[j][2 * r + c] - from);
-          s[j][2 * r + c] = p;
-          total += p;
-        }
-      sum[r] = sum[r] * correction[r] + total;
     }
-    if (__any_sync(0xffffffffu, correction[0] != 1.f || correction[1] != 1.f)) {
-#pragma unroll
-      for (int i = 0; i < BLOCKS_V * 4; ++i)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) o[i][c] *= correction[c >> 1];
-    }
-    // weights
-    unsigned w[2][PARTS][4];   // [16 keys][part]
+    // this lane's keys: their scales
+    float k_scale[4], v_scale[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const float lo = v_scales[8 * j + key_of(2 * t)], hi = v_scales[8 * j + key_of(2 * t + 1)];
+      k_scale[j] = k_scales[8 * j + key_of(g)];
+      v_scale[j] = v_scales[8 * j + key_of(g)];
+    }
+    bool inside = true;   // whether every row sees every key
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) inside = inside && key0 >= first[nt][r] && key0 + KEYS - 1 <= last[nt][r];
+    const bool edge = __any_sync(0xffffffffu, !inside);
+    const unsigned all_top = edge ? 0u : __reduce_max_sync(0xffffffffu, max(max(finite_bits(v_scale[0]), finite_bits(v_scale[1])),
+                                                                            max(finite_bits(v_scale[2]), finite_bits(v_scale[3]))));
+    unsigned weights[NT][2][2][PARTS];   // [16 keys][eight of them]: operands of the second product
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      float largest[2] = {-INFINITY, -INFINITY};
+      unsigned top[2] = {all_top, all_top};
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          float& z = s[nt][j >> 1][2 * (j & 1) + r];
+          z *= k_scale[j];
+          if (edge) {
+            const int key = key0 + 8 * j + key_of(g);
+            if (key >= first[nt][r] && key <= last[nt][r]) top[r] = max(top[r], finite_bits(v_scale[j]));
+            else z = -INFINITY;
+          }
+          largest[r] = fmaxf(largest[r], z);
+        }
+      // the base moves only where a score or a value scale has outgrown it
+      bool stays = true;
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        // a key that a row does not see has no part in it, whatever its scale
-        float x = s[j][2 * r] == 0.f ? 0.f : s[j][2 * r] * lo, y = s[j][2 * r + 1] == 0.f ? 0.f : s[j][2 * r + 1] * hi;
+        largest[r] *= factor[nt][r];
+        stays = stays && largest[r] <= most[nt][r] + BASE_LAG && static_cast<int>(top[r] >> 23) - 127 - SCALE_BITS <= exponent[nt][r];
+      }
+      if (__any_sync(0xffffffffu, !stays)) {
+        float correction[2];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+#pragma unroll
+          for (int offset = 4; offset < 32; offset <<= 1) {
+            largest[r] = fmaxf(largest[r], __shfl_xor_sync(0xffffffffu, largest[r], offset));
+            if (edge) top[r] = max(top[r], __shfl_xor_sync(0xffffffffu, top[r], offset));
+          }
+          exponent[nt][r] = max(exponent[nt][r], min(static_cast<int>(top[r] >> 23) - 127 - SCALE_BITS, MOST_EXPONENT));
+          most[nt][r] = fmaxf(most[nt][r], largest[r]);
+          const float next = most[nt][r] + static_cast<float>(exponent[nt][r]);
+          correction[r] = base[nt][r] == next ? 1.f : fast_exp2(base[nt][r] - (next == -INFINITY ? 0.f : next));
+          base[nt][r] = next;
+          sum[nt][r] *= correction[r];
+        }
+#pragma unroll
+        for (int i = 0; i < BLOCKS_V * 2; ++i)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) o[nt][i][c] *= correction[c & 1];
+      }
+      float p[4][2];
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const float from = base[nt][r] == -INFINITY ? 0.f : base[nt][r];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          p[j][r] = fast_exp2(fmaf(s[nt][j >> 1][2 * (j & 1) + r], factor[nt][r], -from));
+          sum[nt][r] += p[j][r];
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float x = p[j][0] * v_scale[j], y = p[j][1] * v_scale[j];
+        if (edge) {   // a key that a row does not see has no part in it, whatever its scale
+          x = p[j][0] == 0.f ? 0.f : x;
+          y = p[j][1] == 0.f ? 0.f : y;
+        }
 #pragma unroll
         for (int part = 0; part < PARTS; ++part) {
           const unsigned packed = pack_half(x, y);
-          w[j >> 1][part][(j & 1) * 2 + r] = packed;
+          weights[nt][j >> 1][j & 1][part] = transpose8(packed);
           if (part + 1 < PARTS) {
             x -= low_half(packed);
             y -= high_half(packed);
@@ -392,14 +408,15 @@ struct Rows {
           rows[i] = D % 32 == 0 || chunk < CHUNKS ? *reinterpret_cast<const unsigned*>(v_tile + chunk_at(key, chunk) + 4 * (g & 3)) : 0u;
           rows[i] ^= 0x80808080u;
         }
-        const unsigned lo01 = __byte_perm(rows[0], rows[1], 0x5140), lo23 = __byte_perm(rows[0], rows[1], 0x7362);
-        const unsigned hi01 = __byte_perm(rows[2], rows[3], 0x5140), hi23 = __byte_perm(rows[2], rows[3], 0x7362);
-        const unsigned b0[4] = {codes_to_half<0x4140>(lo01), codes_to_half<0x4342>(lo01), codes_to_half<0x4140>(lo23), codes_to_half<0x4342>(lo23)};
-        const unsigned b1[4] = {codes_to_half<0x4140>(hi01), codes_to_half<0x4342>(hi01), codes_to_half<0x4140>(hi23), codes_to_half<0x4342>(hi23)};
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int m = 0; m < 2; ++m) {   // elements 4 g + 2 m and + 1 are rows g and g + 8 of the product
+          const unsigned lo = __byte_perm(rows[0], rows[1], m == 0 ? 0x5140 : 0x7362), hi = __byte_perm(rows[2], rows[3], m == 0 ? 0x5140 : 0x7362);
+          const unsigned a[4] = {codes_to_half<0x4140>(lo), codes_to_half<0x4342>(lo), codes_to_half<0x4140>(hi), codes_to_half<0x4342>(hi)};
 #pragma unroll
-          for (int part = 0; part < PARTS; ++part) mma(o[b * 4 + j], w[kk][part], b0[j], b1[j]);
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int part = 0; part < PARTS; ++part) mma(o[nt][2 * b + m], a, weights[nt][kk][0][part], weights[nt][kk][1][part]);
+        }
       }
     }
   }
@@ -407,13 +424,12 @@ struct Rows {
   // Sums of whole rows.
   __device__ __forceinline__ void finish() {
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 1);
-      sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 2);
-    }
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int offset = 4; offset < 32; offset <<= 1) sum[nt][r] += __shfl_xor_sync(0xffffffffu, sum[nt][r], offset);
   }
-  // The element of the head that o[b * 4 + j][c] belongs to (c's low bit: which of a lane's two columns).
-  __device__ __forceinline__ static int out_element(int b, int j, int c, int t) { return 32 * b + 4 * (2 * t + (c & 1)) + j; }
 };
 
 // Which entry this is, and whether it is this launch's.
@@ -424,10 +440,29 @@ __device__ __forceinline__ bool entry_of(const Args& args, int seq, int& start, 
   return q_len > 0 && !(args.only == 1 && q_len > 1) && !(args.only == 2 && q_len == 1);
 }
 
-// Few rows: grid (splits, kv heads * row tiles, entries).
+// Adds up `count` shares of a row's four elements from `element` on (bases and sums `pair_stride` floats apart, rows
+// `row_stride`) and stores the result, or leaves it as a share itself.
+__device__ __forceinline__ void add_share(float m, float l, const float4& v, float base, float& total, float (&acc)[4]) {
+  const float weight = m == -INFINITY ? 0.f : fast_exp2(m - base);
+  if (weight == 0.f) return;
+  total += l * weight;
+  acc[0] += v.x * weight; acc[1] += v.y * weight; acc[2] += v.z * weight; acc[3] += v.w * weight;
+}
 template <typename T>
+__device__ __forceinline__ void store_row(const Args& args, int row, int start, int group, int kv_head, int element, float total, float (&acc)[4]) {
+  const float inv = total == 0.f ? 0.f : 1.f / total;   // a row that sees nothing is zeros
+#pragma unroll
+  for (int e = 0; e < 4; ++e) acc[e] *= inv;
+  const int token = row / group, head = kv_head * group + row - token * group;
+  store4<T>(static_cast<T*>(args.out) + (static_cast<size_t>(start + token) * args.num_heads + head) * D + element, acc);
+}
+
+// Few rows: grid (splits, kv heads * row tiles, entries).
+template <typename T, int NT>
 __global__ void __launch_bounds__(THREADS)
 split_keys_kernel(const Args args) {
+  using R = Rows<T, NT>;
+  constexpr int ROWS = R::ROWS;
   extern __shared__ __align__(128) unsigned char smem[];
   let_dependents_start();
   const int seq = blockIdx.z, split = blockIdx.x;
@@ -446,8 +481,7 @@ split_keys_kernel(const Args args) {
   const int per = (steps + args.splits - 1) / args.splits;
   const int mine_lo = step_lo + min(steps, split * per), mine_hi = step_lo + min(steps, (split + 1) * per);
 
-  using R = Rows<T>;
-  uint4* shared_q = reinterpret_cast<uint4*>(smem + WARPS * STAGES * STAGE);
+  uint2* shared_q = reinterpret_cast<uint2*>(smem + WARPS * STAGES * STAGE);
   unsigned char* ring = smem + warp * STAGES * STAGE;
   const unsigned ring_at = smem_u32(ring);
   const int* table = args.block_table + static_cast<size_t>(seq) * args.max_blocks;
@@ -455,55 +489,55 @@ split_keys_kernel(const Args args) {
   // this warp's steps: mine_lo + warp, + WARPS, ...
   const int begin = mine_lo + warp;
   int loaded = begin;
-  int next_slot = slot_of(args, table, loaded * KEYS + lane, loaded < mine_hi ? last_key : -1);
+  Place next = place_of(args, table, kv_head, loaded * KEYS + lane, loaded < mine_hi ? last_key : -1);
 #pragma unroll
-  for (int i = 0; i < STAGES - 1; ++i) {
-    if (loaded < mine_hi) load_step<32>(args, kv_head, next_slot, ring_at + i * STAGE, lane);
+  for (int i = 0; i < STAGES; ++i) {
+    if (loaded < mine_hi) load_step<32>(args, kv_head, next, ring_at + i * STAGE, lane);
     copies_commit();
     loaded += WARPS;
-    next_slot = slot_of(args, table, loaded * KEYS + lane, loaded < mine_hi ? last_key : -1);
+    next = place_of(args, table, kv_head, loaded * KEYS + lane, loaded < mine_hi ? last_key : -1);
   }
   r.begin(args, row0, rows, start, group, kv_head, pos0, shared_q, lane);   // all warps write the same operands
   __syncwarp();
   int stage = 0;
   for (int step = begin; step < mine_hi; step += WARPS) {
-    copies_wait<STAGES - 2>();
+    copies_wait<STAGES - 1>();
     __syncwarp();
-    const int into = stage + STAGES - 1 >= STAGES ? stage - 1 : stage + STAGES - 1;
-    if (loaded < mine_hi) load_step<32>(args, kv_head, next_slot, ring_at + into * STAGE, lane);
-    copies_commit();
-    loaded += WARPS;
-    next_slot = slot_of(args, table, loaded * KEYS + lane, loaded < mine_hi ? last_key : -1);
     r.step(ring + stage * STAGE, step * KEYS, shared_q, lane);
     __syncwarp();
+    if (loaded < mine_hi) load_step<32>(args, kv_head, next, ring_at + stage * STAGE, lane);
+    copies_commit();
+    loaded += WARPS;
+    next = place_of(args, table, kv_head, loaded * KEYS + lane, loaded < mine_hi ? last_key : -1);
     stage = stage + 1 == STAGES ? 0 : stage + 1;
   }
   copies_wait<0>();
   r.finish();
   __syncthreads();
-  // the warps' rows meet: [warp][16][D] and [warp][16][base, sum]
+  // the warps' rows meet: [warp][ROWS][D + 4] (four more, so that the stores of a quad fall into different banks), and
+  // [warp][ROWS][base, sum]
+  constexpr int ROW_FLOATS = D + 4;
   float* all_o = reinterpret_cast<float*>(smem);
-  float* all_m = all_o + WARPS * ROWS * D;
+  float* all_m = all_o + WARPS * ROWS * ROW_FLOATS;
 #pragma unroll
-  for (int b = 0; b < BLOCKS_V; ++b)
+  for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int c = 0; c < 2; ++c) {
+      const int row = warp * ROWS + 8 * nt + 2 * t + c;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const int element = R::out_element(b, j, c, t);
-        if (D % 32 == 0 || element < D) all_o[(warp * ROWS + g + 8 * (c >> 1)) * D + element] = r.o[b * 4 + j][c];
+      for (int b = 0; b < BLOCKS_V; ++b)
+        if (D % 32 == 0 || R::out_element(b, g) < D)
+          *reinterpret_cast<float4*>(all_o + row * ROW_FLOATS + R::out_element(b, g)) =
+              make_float4(r.o[nt][2 * b][c], r.o[nt][2 * b][2 + c], r.o[nt][2 * b + 1][c], r.o[nt][2 * b + 1][2 + c]);
+      if (g == 0) {
+        all_m[2 * row] = r.base[nt][c];
+        all_m[2 * row + 1] = r.sum[nt][c];
       }
-  if (t == 0) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      all_m[(warp * ROWS + g + 8 * i) * 2] = r.base[i];
-      all_m[(warp * ROWS + g + 8 * i) * 2 + 1] = r.sum[i];
     }
-  }
   __syncthreads();
   const size_t pair = (static_cast<size_t>(seq) * gridDim.y + blockIdx.y);
-  float* share = args.splits > 1 ? args.scratch + (pair * args.splits + split) * ROWS * (D + 2) : nullptr;
-  T* out = static_cast<T*>(args.out);
+  constexpr int SHARE = ROWS * (D + 2);
+  float* share = args.splits > 1 ? args.scratch + (pair * args.splits + split) * SHARE : nullptr;
   for (int i = threadIdx.x; i < tile_rows * (D / 4); i += THREADS) {
     const int row = i / (D / 4), element = (i - row * (D / 4)) * 4;
     float base = -INFINITY;
@@ -511,14 +545,9 @@ split_keys_kernel(const Args args) {
     for (int w = 0; w < WARPS; ++w) base = fmaxf(base, all_m[(w * ROWS + row) * 2]);
     float total = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int w = 0; w < WARPS; ++w) {
-      const float m = all_m[(w * ROWS + row) * 2];
-      const float weight = m == -INFINITY ? 0.f : fast_exp2(m - base);
-      if (weight == 0.f) continue;
-      total += all_m[(w * ROWS + row) * 2 + 1] * weight;
-      const float4 v = *reinterpret_cast<const float4*>(all_o + (w * ROWS + row) * D + element);
-      acc[0] += v.x * weight; acc[1] += v.y * weight; acc[2] += v.z * weight; acc[3] += v.w * weight;
-    }
+    for (int w = 0; w < WARPS; ++w)
+      add_share(all_m[(w * ROWS + row) * 2], all_m[(w * ROWS + row) * 2 + 1],
+                *reinterpret_cast<const float4*>(all_o + (w * ROWS + row) * ROW_FLOATS + element), base, total, acc);
     if (share != nullptr) {
       *reinterpret_cast<float4*>(share + row * D + element) = make_float4(acc[0], acc[1], acc[2], acc[3]);
       if (element == 0) {
@@ -526,11 +555,7 @@ split_keys_kernel(const Args args) {
         share[ROWS * D + 2 * row + 1] = total;
       }
     } else {
-      const float inv = total == 0.f ? 0.f : 1.f / total;   // a row that sees nothing is zeros
-#pragma unroll
-      for (int e = 0; e < 4; ++e) acc[e] *= inv;
-      const int at = row0 + row, token = at / group, head = kv_head * group + at - token * group;
-      store4<T>(out + (static_cast<size_t>(start + token) * args.num_heads + head) * D + element, acc);
+      store_row<T>(args, row0 + row, start, group, kv_head, element, total, acc);
     }
   }
   if (args.splits == 1) return;
@@ -541,34 +566,30 @@ split_keys_kernel(const Args args) {
   __syncthreads();
   if (arrived != args.splits - 1) return;
   __threadfence();
-  const float* shares = args.scratch + pair * args.splits * ROWS * (D + 2);
+  const float* shares = args.scratch + pair * args.splits * SHARE;
   for (int i = threadIdx.x; i < tile_rows * (D / 4); i += THREADS) {
     const int row = i / (D / 4), element = (i - row * (D / 4)) * 4;
     float base = -INFINITY;
-    for (int s = 0; s < args.splits; ++s) base = fmaxf(base, __ldcg(shares + static_cast<size_t>(s) * ROWS * (D + 2) + ROWS * D + 2 * row));
+#pragma unroll 8
+    for (int s = 0; s < args.splits; ++s) base = fmaxf(base, __ldcg(shares + static_cast<size_t>(s) * SHARE + ROWS * D + 2 * row));
     float total = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
     for (int s = 0; s < args.splits; ++s) {
-      const float* share_s = shares + static_cast<size_t>(s) * ROWS * (D + 2);
-      const float m = __ldcg(share_s + ROWS * D + 2 * row);
-      const float weight = m == -INFINITY ? 0.f : fast_exp2(m - base);
-      if (weight == 0.f) continue;
-      total += __ldcg(share_s + ROWS * D + 2 * row + 1) * weight;
-      const float4 v = __ldcg(reinterpret_cast<const float4*>(share_s + row * D + element));
-      acc[0] += v.x * weight; acc[1] += v.y * weight; acc[2] += v.z * weight; acc[3] += v.w * weight;
+      const float* share_s = shares + static_cast<size_t>(s) * SHARE;
+      add_share(__ldcg(share_s + ROWS * D + 2 * row), __ldcg(share_s + ROWS * D + 2 * row + 1),
+                __ldcg(reinterpret_cast<const float4*>(share_s + row * D + element)), base, total, acc);
     }
-    const float inv = total == 0.f ? 0.f : 1.f / total;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) acc[e] *= inv;
-    const int at = row0 + row, token = at / group, head = kv_head * group + at - token * group;
-    store4<T>(out + (static_cast<size_t>(start + token) * args.num_heads + head) * D + element, acc);
+    store_row<T>(args, row0 + row, start, group, kv_head, element, total, acc);
   }
   if (threadIdx.x == 0) args.arrivals[pair] = 0;
 }
 
-// Many rows: grid (row tiles of 64, kv heads, entries); the CTA's warps share the key tiles.
-template <typename T>
+// Many rows: grid (row tiles of 4 * 8 NT, kv heads, entries); the CTA's warps share the key tiles.
+template <typename T, int NT>
 __global__ void __launch_bounds__(THREADS)
 portion_rows_kernel(const Args args) {
+  using R = Rows<T, NT>;
+  constexpr int ROWS = R::ROWS;
   extern __shared__ __align__(128) unsigned char smem[];
   let_dependents_start();
   const int seq = blockIdx.z, kv_head = blockIdx.y;
@@ -590,17 +611,16 @@ portion_rows_kernel(const Args args) {
   const int my_last = row0 < rows ? pos0 + (min(row0 + ROWS, rows) - 1) / group : -1;
   const int my_first = first_visible_key(pos0 + row0 / group, args.window);
 
-  using R = Rows<T>;
-  uint4* shared_q = reinterpret_cast<uint4*>(smem + STAGES * STAGE + warp * R::SHARED_BYTES);
+  uint2* shared_q = reinterpret_cast<uint2*>(smem + STAGES * STAGE + warp * R::SHARED_BYTES);
   const unsigned ring_at = smem_u32(smem);
   const int* table = args.block_table + static_cast<size_t>(seq) * args.max_blocks;
   R r;
-  int next_slot = slot_of(args, table, step_lo * KEYS + lane, last_key);
+  Place next = place_of(args, table, kv_head, step_lo * KEYS + lane, last_key);
 #pragma unroll
   for (int i = 0; i < STAGES - 1; ++i) {
-    if (step_lo + i < step_hi) load_step<THREADS>(args, kv_head, next_slot, ring_at + i * STAGE, threadIdx.x);
+    if (step_lo + i < step_hi) load_step<THREADS>(args, kv_head, next, ring_at + i * STAGE, threadIdx.x);
     copies_commit();
-    next_slot = slot_of(args, table, (step_lo + i + 1) * KEYS + lane, last_key);
+    next = place_of(args, table, kv_head, (step_lo + i + 1) * KEYS + lane, last_key);
   }
   r.begin(args, row0, rows, start, group, kv_head, pos0, shared_q, lane);
   __syncwarp();
@@ -609,49 +629,59 @@ portion_rows_kernel(const Args args) {
     copies_wait<STAGES - 2>();
     __syncthreads();   // this step's copies of all threads have landed; everyone has left the stage that is loaded next
     const int into = stage + STAGES - 1 >= STAGES ? stage - 1 : stage + STAGES - 1;
-    if (step + STAGES - 1 < step_hi) load_step<THREADS>(args, kv_head, next_slot, ring_at + into * STAGE, threadIdx.x);
+    if (step + STAGES - 1 < step_hi) load_step<THREADS>(args, kv_head, next, ring_at + into * STAGE, threadIdx.x);
     copies_commit();
-    next_slot = slot_of(args, table, (step + STAGES) * KEYS + lane, last_key);
+    next = place_of(args, table, kv_head, (step + STAGES) * KEYS + lane, last_key);
     if (step * KEYS <= my_last && step * KEYS + KEYS > my_first) r.step(smem + stage * STAGE, step * KEYS, shared_q, lane);
     stage = stage + 1 == STAGES ? 0 : stage + 1;
   }
   copies_wait<0>();
   r.finish();
-  T* out = static_cast<T*>(args.out);
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int row = row0 + g + 8 * i;
-    if (row >= rows) continue;
-    const int token = row / group, head = kv_head * group + row - token * group;
-    T* dst = out + (static_cast<size_t>(start + token) * args.num_heads + head) * D;
-    const float inv = r.sum[i] == 0.f ? 0.f : 1.f / r.sum[i];
+  for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-    for (int b = 0; b < BLOCKS_V; ++b)
+    for (int c = 0; c < 2; ++c) {
+      const int row = row0 + 8 * nt + 2 * t + c;
+      if (row >= rows) continue;
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {   // a lane's four elements of a run are neighbours
-        const int element = R::out_element(b, 0, c, t);
-        float v[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = r.o[b * 4 + j][2 * i + c] * inv;
-        if (D % 32 == 0 || element < D) store4<T>(dst + element, v);
+      for (int b = 0; b < BLOCKS_V; ++b) {
+        float v[4] = {r.o[nt][2 * b][c], r.o[nt][2 * b][2 + c], r.o[nt][2 * b + 1][c], r.o[nt][2 * b + 1][2 + c]};
+        if (D % 32 == 0 || R::out_element(b, g) < D) store_row<T>(args, row, start, group, kv_head, R::out_element(b, g), r.sum[nt][c], v);
       }
-  }
+    }
 }
 
-template <typename T> constexpr size_t split_keys_smem() {
-  const size_t ring = static_cast<size_t>(WARPS) * STAGES * STAGE + Rows<T>::SHARED_BYTES;
-  const size_t merge = static_cast<size_t>(WARPS) * ROWS * (D + 2) * 4;
+template <typename T, int NT> constexpr size_t split_keys_smem() {
+  const size_t ring = static_cast<size_t>(WARPS) * STAGES * STAGE + Rows<T, NT>::SHARED_BYTES;
+  const size_t merge = static_cast<size_t>(WARPS) * Rows<T, NT>::ROWS * (D + 6) * 4;
   return ring > merge ? ring : merge;
 }
-template <typename T> constexpr size_t portion_rows_smem() { return static_cast<size_t>(STAGES) * STAGE + WARPS * Rows<T>::SHARED_BYTES; }
+template <typename T, int NT> constexpr size_t portion_rows_smem() { return static_cast<size_t>(STAGES) * STAGE + WARPS * Rows<T, NT>::SHARED_BYTES; }
 
-template <typename T>
+constexpr int PORTION_NT = 2;
+// Row tiles of the few-rows form: eights, pairs of them for groups of more than eight heads.
+static int few_rows(int group) { return group <= 8 ? 8 : 16; }
+
+template <typename T, int NT>
 static int resident() {
   static PerDevice raised;
-  if (shrike_raise_smem(raised, split_keys_kernel<T>, split_keys_smem<T>()) != 0) return shrike_device().sm_count;
+  if (shrike_raise_smem(raised, split_keys_kernel<T, NT>, split_keys_smem<T, NT>()) != 0) return shrike_device().sm_count;
   int per_sm = 0;
-  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, split_keys_kernel<T>, THREADS, split_keys_smem<T>()) != cudaSuccess || per_sm < 1) per_sm = 1;
+  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, split_keys_kernel<T, NT>, THREADS, split_keys_smem<T, NT>()) != cudaSuccess || per_sm < 1)
+    per_sm = 1;
   return per_sm * shrike_device().sm_count;
+}
+
+template <typename T, int NT>
+static int launch_few(const Args& args, int num_seqs, int tokens, cudaStream_t stream) {
+  static PerDevice raised;
+  const int rc = shrike_raise_smem(raised, split_keys_kernel<T, NT>, split_keys_smem<T, NT>());
+  if (rc != 0) return rc;
+  const long long tiles = (static_cast<long long>(tokens) * (args.num_heads / args.num_kv_heads) + 8 * NT - 1) / (8 * NT);
+  if (tiles * args.num_kv_heads > 65535) return SHRIKE_BAD_ARGUMENT;
+  return static_cast<int>(launch_dependent(split_keys_kernel<T, NT>,
+                                           dim3(args.splits, static_cast<unsigned>(tiles * args.num_kv_heads), num_seqs), dim3(THREADS),
+                                           split_keys_smem<T, NT>(), stream, args));
 }
 
 template <typename T>
@@ -659,25 +689,21 @@ static int launch(const Args& base, int num_seqs, int max_q_len, int has_single,
   Args args = base;
   const int group = args.num_heads / args.num_kv_heads;
   if (has_single) {
-    static PerDevice raised;
-    const int rc = shrike_raise_smem(raised, split_keys_kernel<T>, split_keys_smem<T>());
-    if (rc != 0) return rc;
     args.only = has_portions ? 1 : 0;
-    const long long tiles = (static_cast<long long>(has_portions ? 1 : max_q_len) * group + ROWS - 1) / ROWS;
-    if (tiles * args.num_kv_heads > 65535) return SHRIKE_BAD_ARGUMENT;
-    const cudaError_t err = launch_dependent(split_keys_kernel<T>, dim3(args.splits, static_cast<unsigned>(tiles * args.num_kv_heads), num_seqs),
-                                             dim3(THREADS), split_keys_smem<T>(), stream, args);
-    if (err != cudaSuccess) return static_cast<int>(err);
+    const int tokens = has_portions ? 1 : max_q_len;
+    const int rc = few_rows(group) == 8 ? launch_few<T, 1>(args, num_seqs, tokens, stream) : launch_few<T, 2>(args, num_seqs, tokens, stream);
+    if (rc != 0) return rc;
   }
   if (has_portions) {
     static PerDevice raised;
-    const int rc = shrike_raise_smem(raised, portion_rows_kernel<T>, portion_rows_smem<T>());
+    const int rc = shrike_raise_smem(raised, portion_rows_kernel<T, PORTION_NT>, portion_rows_smem<T, PORTION_NT>());
     if (rc != 0) return rc;
     args.only = has_single ? 2 : 0;
-    const long long tiles = (static_cast<long long>(max_q_len) * group + WARPS * ROWS - 1) / (WARPS * ROWS);
+    constexpr int ROWS = WARPS * Rows<T, PORTION_NT>::ROWS;
+    const long long tiles = (static_cast<long long>(max_q_len) * group + ROWS - 1) / ROWS;
     if (tiles > 0x7fffffff) return SHRIKE_BAD_ARGUMENT;
-    const cudaError_t err = launch_dependent(portion_rows_kernel<T>, dim3(static_cast<unsigned>(tiles), args.num_kv_heads, num_seqs),
-                                             dim3(THREADS), portion_rows_smem<T>(), stream, args);
+    const cudaError_t err = launch_dependent(portion_rows_kernel<T, PORTION_NT>, dim3(static_cast<unsigned>(tiles), args.num_kv_heads, num_seqs),
+                                             dim3(THREADS), portion_rows_smem<T, PORTION_NT>(), stream, args);
     if (err != cudaSuccess) return static_cast<int>(err);
   }
   return shrike_launch_status();
@@ -685,18 +711,22 @@ static int launch(const Args& base, int num_seqs, int max_q_len, int has_single,
 
 }  // namespace attnq8
 
+// Query rows of a tile of the few-rows form, for groups of `group` heads a kv head.
+SHRIKE_API int shrike_attention_q8_tile_rows(int group) { return attnq8::few_rows(group); }
 // CTAs of the few-rows form that the device holds at once, for queries of `dtype`.
-SHRIKE_API int shrike_attention_q8_resident_ctas(int dtype) {
-  return dtype == SHRIKE_F32 ? attnq8::resident<float>() : attnq8::resident<__nv_bfloat16>();
+SHRIKE_API int shrike_attention_q8_resident_ctas(int dtype, int group) {
+  using namespace attnq8;
+  if (dtype == SHRIKE_F32) return few_rows(group) == 8 ? resident<float, 1>() : resident<float, 2>();
+  return few_rows(group) == 8 ? resident<__nv_bfloat16, 1>() : resident<__nv_bfloat16, 2>();
 }
-// Floats of scratch for a (entry, kv head, row tile) and split, and the most splits.
-SHRIKE_API int shrike_attention_q8_share_floats() { return attnq8::ROWS * (attnq8::D + 2); }
+// Floats of scratch for a row of a (entry, kv head, row tile) and split, and the most splits.
+SHRIKE_API int shrike_attention_q8_row_floats() { return attnq8::D + 2; }
 SHRIKE_API int shrike_attention_q8_max_splits() { return attnq8::MAX_SPLITS; }
 
 // q and out [tokens, heads * D] of `dtype`, 16-byte aligned; codes [pages, page_size, kv heads, D], 16-byte aligned, scales
 // [pages, kv heads, page_size].  `has_single`: entries of one token (every entry, where has_portions is 0: then `max_q_len`
 // tokens at most) run on the few-rows form with `splits` CTAs a row tile; `has_portions`: the longer ones (all of them where
-// has_single is 0) on the other.  splits > 1 needs `scratch` (share_floats() a pair of (entry, kv head, row tile) and split)
+// has_single is 0) on the other.  splits > 1 needs `scratch` (row_floats() for every row of a tile of (entry, kv head, row tile) and split)
 // and `arrivals` (an int a pair, zero before the first launch).
 SHRIKE_API int shrike_paged_attention_q8(const void* q, const void* k_codes, const float* k_scales, const void* v_codes,
                                          const float* v_scales, const int* block_table, int max_blocks, const int* q_start,
@@ -727,6 +757,7 @@ SHRIKE_API int shrike_paged_attention_q8(const void* q, const void* k_codes, con
   args.page_size = page_size;
   args.num_pages = num_pages;
   args.window = window;
+  args.page_shift = (page_size & (page_size - 1)) == 0 ? __builtin_ctz(page_size) : -1;
   args.only = 0;
   args.scale_log2 = scale * attnq8::LOG2E;
   args.splits = splits;

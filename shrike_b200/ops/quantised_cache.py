@@ -69,11 +69,12 @@ class QuantisedCacheOps:
             lib = build.attention_q8_library(head_dim)
             lib.shrike_paged_attention_q8.argtypes = [_P] * 6 + [_I, _P, _P] + [_I] * 6 + [_F, _I, _P] + [_I] * 4 + [_P, _P, _P]
             lib.shrike_paged_attention_q8.restype = _I
-            for name in ("share_floats", "max_splits"):
+            for name in ("row_floats", "max_splits"):
                 getattr(lib, f"shrike_attention_q8_{name}").argtypes = []
                 getattr(lib, f"shrike_attention_q8_{name}").restype = _I
-            lib.shrike_attention_q8_resident_ctas.argtypes = [_I]
-            lib.shrike_attention_q8_resident_ctas.restype = _I
+            lib.shrike_attention_q8_resident_ctas.argtypes = [_I, _I]
+            lib.shrike_attention_q8_tile_rows.argtypes = [_I]
+            lib.shrike_attention_q8_resident_ctas.restype = lib.shrike_attention_q8_tile_rows.restype = _I
             self._q8_libs[head_dim] = lib
         return lib
 
@@ -219,15 +220,16 @@ class QuantisedCacheOps:
         has_single, has_portions = min_q_len <= 1, max_q_len > 1
         splits, scratch, arrivals = 1, None, None
         if has_single:
-            tiles = -(-(num_heads // num_kv_heads) // 16)
-            pairs = num_seqs * num_kv_heads * tiles
+            group = num_heads // num_kv_heads
+            rows = lib.shrike_attention_q8_tile_rows(group)
+            pairs = num_seqs * num_kv_heads * -(-group // rows)
             keys = max_blocks * page_size
             if window > 0:
                 keys = min(keys, window)
             elif window < 0:
                 keys = min(keys, -window)
-            splits = self.q8_splits or self.q8_few_row_splits(keys, pairs, lib.shrike_attention_q8_resident_ctas(self.code))
-            share = lib.shrike_attention_q8_share_floats()
+            splits = self.q8_splits or self.q8_few_row_splits(keys, pairs, lib.shrike_attention_q8_resident_ctas(self.code, group))
+            share = rows * lib.shrike_attention_q8_row_floats()
             splits = max(1, min(splits, lib.shrike_attention_q8_max_splits(), self.Q8_SCRATCH_FLOATS // (share * pairs)))
             if splits > 1:
                 need = pairs * splits * share
@@ -244,11 +246,19 @@ class QuantisedCacheOps:
         self._q8_plans[key] = (self.generation, plan)
         return plan
 
-    @staticmethod
-    def q8_few_row_splits(keys: int, pairs: int, resident: int) -> int:
-        """CTAs that share the `keys` of each of `pairs` (entry, kv head, row tile) where the device holds `resident` at once: as
-        many as fill it, each with at least two steps of 32 keys for its four warps."""
-        return max(1, min(resident // pairs, keys // 256))
+    Q8_SPLIT_KEYS = 160   # what a CTA's start, and its share's way to the others, cost in keys
+
+    @classmethod
+    def q8_few_row_splits(cls, keys: int, pairs: int, resident: int) -> int:
+        """CTAs that share the `keys` of each of `pairs` (entry, kv head, row tile) where the device holds `resident` at once: the
+        count with the least time, rounds of CTAs times what each takes, a CTA having at least a step of 32 keys for each of its
+        four warps."""
+        best, least = 1, None
+        for splits in range(1, max(1, min(64, keys // 128)) + 1):
+            time = -(-pairs * splits // resident) * (-(-keys // splits) + cls.Q8_SPLIT_KEYS)
+            if least is None or time < least:
+                best, least = splits, time
+        return best
 
     def _paged_attention_q8(self, q, keys, values, block_table, q_start, ctx_len, seq_of_token, num_heads, num_kv_heads, head_dim,
                             scale, window, out, max_q_len, min_q_len):

@@ -62,9 +62,9 @@ def attention(q, sequences, q_lens, ctx_lens, heads, kv_heads, dim, scale, windo
       a score: dim / 16 additions of products, their factors and, for 32-bit queries, what two 11-bit parts leave (2^-22), all
                relative to sum |q k|; the subtraction of the base and the exponential, 2^-22 each of the argument's size
       a weight: half a step of float16 (2^-11), or of two parts of it (2^-22) for 32-bit queries, and never less than half of
-                float16's least step, 2^-25, where a weight of one at the largest value scale seen stands at 2^13 or more (so
-                that the exponentials' largest, one, is at least that large in the sums): 2^-38 of that scale a key, times codes
-                of up to 127
+                float16's least step, 2^-25, where a weight of one at the largest value scale seen stands at 2^8 or more (and the
+                sums hold the largest score's exponential, one, or up to 2^6 where the base lags): 2^-33 of that scale a key,
+                times codes of up to 127
       a sum over n keys: n / 16 additions and as many rescalings
     all relative to sum p |v| / sum p, and half a step of the output's type relative to the output."""
     u = 2.0 ** -23
@@ -98,7 +98,7 @@ def attention(q, sequences, q_lens, ctx_lens, heads, kv_heads, dim, scale, windo
             there = torch.where(seen, size, 0.0).amax(-1, keepdim=True)
             score = there * ((dim / 16 + 4) * u + (2.0 ** -22 if wide else 0.0)) + 2.0 ** -21 * (there + 32)
             sums = (context / 8 + 16) * u
-            least = seen.sum(-1, keepdim=True) * 2.0 ** -38 * 127 * torch.where(seen, values[1][:, g].double(), 0.0).amax(-1, keepdim=True)
+            least = seen.sum(-1, keepdim=True) * 2.0 ** -33 * 127 * torch.where(seen, values[1][:, g].double(), 0.0).amax(-1, keepdim=True)
             bound[:, head] = least + (p @ vv.abs()) * (2 * score + (2.0 ** -22 if wide else 2.0 ** -11) + 2 * sums)
         outs.append(out.view(new, -1))
         bounds.append((bound + half_step * out.abs()).view(new, -1))
