@@ -22,8 +22,8 @@
 // subtraction; the weights go from the scores' layout to an operand's through movmatrix.
 //
 // Two forms.  Few rows (single tokens): the rows' keys are dealt to `splits` CTAs and to each CTA's four warps, each with its
-// own ring of cp.async copies (no barrier in the loop); the warps' results meet in shared memory, the CTAs' in global memory,
-// where the last CTA to arrive adds them up in the order of the splits.  Many rows (portions): four warps of 8 NT rows each
+// own ring of cp.async copies (no barrier in the loop); the warps' results meet in shared memory, those of up to eight CTAs in
+// the shared memory of their cluster, and the clusters' in global memory, where the last CTA to arrive adds them up in order.  Many rows (portions): four warps of 8 NT rows each
 // share one ring of key tiles.
 #include <cuda_fp16.h>
 
@@ -63,8 +63,8 @@ struct Args {
   int page_shift;      // page_size is 2^page_shift, or -1
   int only;            // 1: entries of one token, 2: longer ones, 0: all
   float scale_log2;
-  int splits;
-  float* scratch;      // [(entry, kv head, row tile)][split][rows][D + 2]: unnormalised rows, then each row's base and sum
+  int splits, cluster; // CTAs that share a row tile's keys, and how many of them form a cluster
+  float* scratch;      // [(entry, kv head, row tile)][cluster][rows][D + 2]: unnormalised rows, then each row's base and sum
   int* arrivals;       // [(entry, kv head, row tile)]: CTAs that have left their share; zero between launches
 };
 
@@ -118,6 +118,25 @@ constexpr float BASE_LAG = 6.0f;   // float16's largest power of two is 2^15: 2^
 __device__ __forceinline__ unsigned finite_bits(float x) {
   const unsigned bits = __float_as_uint(x) & 0x7fffffffu;
   return bits < 0x7f800000u ? bits : 0u;
+}
+
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ unsigned map_to_rank(unsigned address, int rank) {
+  unsigned there;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(address), "r"(rank));
+  return there;
+}
+__device__ __forceinline__ float2 load_peer2(unsigned address) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(address) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 load_peer4(unsigned address) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(address) : "memory");
+  return v;
 }
 
 // 2^e for e in [-126, 127].
@@ -440,13 +459,17 @@ __device__ __forceinline__ bool entry_of(const Args& args, int seq, int& start, 
   return q_len > 0 && !(args.only == 1 && q_len > 1) && !(args.only == 2 && q_len == 1);
 }
 
-// Adds up `count` shares of a row's four elements from `element` on (bases and sums `pair_stride` floats apart, rows
-// `row_stride`) and stores the result, or leaves it as a share itself.
+// A share of a row is its elements in units of 2^base, the sum of its exponentials likewise, and the base.  Adds one to others
+// whose largest base is `base`.
 __device__ __forceinline__ void add_share(float m, float l, const float4& v, float base, float& total, float (&acc)[4]) {
   const float weight = m == -INFINITY ? 0.f : fast_exp2(m - base);
   if (weight == 0.f) return;
   total += l * weight;
   acc[0] += v.x * weight; acc[1] += v.y * weight; acc[2] += v.z * weight; acc[3] += v.w * weight;
+}
+__device__ __forceinline__ void leave_share(float* share, int rows, int row, int element, float base, float total, const float (&acc)[4]) {
+  *reinterpret_cast<float4*>(share + row * D + element) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+  if (element == 0) *reinterpret_cast<float2*>(share + rows * D + 2 * row) = make_float2(base, total);
 }
 template <typename T>
 __device__ __forceinline__ void store_row(const Args& args, int row, int start, int group, int kv_head, int element, float total, float (&acc)[4]) {
@@ -535,9 +558,12 @@ split_keys_kernel(const Args args) {
       }
     }
   __syncthreads();
+  // What leaves this CTA: a share of the result, in shared memory for the cluster, in global memory beyond it, or the result.
   const size_t pair = (static_cast<size_t>(seq) * gridDim.y + blockIdx.y);
   constexpr int SHARE = ROWS * (D + 2);
-  float* share = args.splits > 1 ? args.scratch + (pair * args.splits + split) * SHARE : nullptr;
+  const int cluster = args.cluster, clusters = args.splits / cluster;
+  float* merged = all_m + WARPS * ROWS * 2;   // [ROWS][D], then [ROWS][base, sum]: for the cluster's other CTAs
+  float* share = clusters > 1 ? args.scratch + (pair * clusters + split / cluster) * SHARE : nullptr;
   for (int i = threadIdx.x; i < tile_rows * (D / 4); i += THREADS) {
     const int row = i / (D / 4), element = (i - row * (D / 4)) * 4;
     float base = -INFINITY;
@@ -548,17 +574,39 @@ split_keys_kernel(const Args args) {
     for (int w = 0; w < WARPS; ++w)
       add_share(all_m[(w * ROWS + row) * 2], all_m[(w * ROWS + row) * 2 + 1],
                 *reinterpret_cast<const float4*>(all_o + (w * ROWS + row) * ROW_FLOATS + element), base, total, acc);
-    if (share != nullptr) {
-      *reinterpret_cast<float4*>(share + row * D + element) = make_float4(acc[0], acc[1], acc[2], acc[3]);
-      if (element == 0) {
-        share[ROWS * D + 2 * row] = base;
-        share[ROWS * D + 2 * row + 1] = total;
-      }
-    } else {
-      store_row<T>(args, row0 + row, start, group, kv_head, element, total, acc);
-    }
+    if (cluster > 1) leave_share(merged, ROWS, row, element, base, total, acc);
+    else if (share != nullptr) leave_share(share, ROWS, row, element, base, total, acc);
+    else store_row<T>(args, row0 + row, start, group, kv_head, element, total, acc);
   }
-  if (args.splits == 1) return;
+  if (cluster > 1) {
+    const int rank = split % cluster;
+    cluster_sync();
+    const unsigned here = smem_u32(merged);
+    for (int i = rank * THREADS + threadIdx.x; i < tile_rows * (D / 4); i += cluster * THREADS) {
+      const int row = i / (D / 4), element = (i - row * (D / 4)) * 4;
+      float2 ml[8];
+      float4 v[8];
+#pragma unroll
+      for (int c = 0; c < 8; ++c)
+        if (c < cluster) {
+          const unsigned peer = map_to_rank(here, c);
+          ml[c] = load_peer2(peer + (ROWS * D + 2 * row) * 4);
+          v[c] = load_peer4(peer + (row * D + element) * 4);
+        }
+      float base = -INFINITY;
+#pragma unroll
+      for (int c = 0; c < 8; ++c)
+        if (c < cluster) base = fmaxf(base, ml[c].x);
+      float total = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < 8; ++c)
+        if (c < cluster) add_share(ml[c].x, ml[c].y, v[c], base, total, acc);
+      if (share != nullptr) leave_share(share, ROWS, row, element, base, total, acc);
+      else store_row<T>(args, row0 + row, start, group, kv_head, element, total, acc);
+    }
+    cluster_sync();   // nobody leaves while another CTA reads its shares
+  }
+  if (clusters == 1) return;
   __threadfence();
   __syncthreads();
   __shared__ int arrived;
@@ -566,18 +614,30 @@ split_keys_kernel(const Args args) {
   __syncthreads();
   if (arrived != args.splits - 1) return;
   __threadfence();
-  const float* shares = args.scratch + pair * args.splits * SHARE;
+  const float* shares = args.scratch + pair * clusters * SHARE;
   for (int i = threadIdx.x; i < tile_rows * (D / 4); i += THREADS) {
     const int row = i / (D / 4), element = (i - row * (D / 4)) * 4;
-    float base = -INFINITY;
-#pragma unroll 8
-    for (int s = 0; s < args.splits; ++s) base = fmaxf(base, __ldcg(shares + static_cast<size_t>(s) * SHARE + ROWS * D + 2 * row));
-    float total = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 8
-    for (int s = 0; s < args.splits; ++s) {
-      const float* share_s = shares + static_cast<size_t>(s) * SHARE;
-      add_share(__ldcg(share_s + ROWS * D + 2 * row), __ldcg(share_s + ROWS * D + 2 * row + 1),
-                __ldcg(reinterpret_cast<const float4*>(share_s + row * D + element)), base, total, acc);
+    float base = -INFINITY, total = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int first = 0; first < clusters; first += 8) {   // eight shares' loads at a time
+      float2 ml[8];
+      float4 v[8];
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        const float* share_c = shares + static_cast<size_t>(min(first + c, clusters - 1)) * SHARE;
+        ml[c] = __ldcg(reinterpret_cast<const float2*>(share_c + ROWS * D + 2 * row));
+        v[c] = __ldcg(reinterpret_cast<const float4*>(share_c + row * D + element));
+      }
+      float next = base;
+#pragma unroll
+      for (int c = 0; c < 8; ++c) next = fmaxf(next, ml[c].x);
+      const float down = base == -INFINITY ? 0.f : fast_exp2(base - next);
+      total *= down;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[e] *= down;
+      base = next;
+#pragma unroll
+      for (int c = 0; c < 8; ++c)
+        if (first + c < clusters) add_share(ml[c].x, ml[c].y, v[c], base, total, acc);
     }
     store_row<T>(args, row0 + row, start, group, kv_head, element, total, acc);
   }
@@ -653,7 +713,7 @@ portion_rows_kernel(const Args args) {
 
 template <typename T, int NT> constexpr size_t split_keys_smem() {
   const size_t ring = static_cast<size_t>(WARPS) * STAGES * STAGE + Rows<T, NT>::SHARED_BYTES;
-  const size_t merge = static_cast<size_t>(WARPS) * Rows<T, NT>::ROWS * (D + 6) * 4;
+  const size_t merge = (static_cast<size_t>(WARPS) * Rows<T, NT>::ROWS * (D + 6) + Rows<T, NT>::ROWS * (D + 2)) * 4;
   return ring > merge ? ring : merge;
 }
 template <typename T, int NT> constexpr size_t portion_rows_smem() { return static_cast<size_t>(STAGES) * STAGE + WARPS * Rows<T, NT>::SHARED_BYTES; }
@@ -679,9 +739,11 @@ static int launch_few(const Args& args, int num_seqs, int tokens, cudaStream_t s
   if (rc != 0) return rc;
   const long long tiles = (static_cast<long long>(tokens) * (args.num_heads / args.num_kv_heads) + 8 * NT - 1) / (8 * NT);
   if (tiles * args.num_kv_heads > 65535) return SHRIKE_BAD_ARGUMENT;
-  return static_cast<int>(launch_dependent(split_keys_kernel<T, NT>,
-                                           dim3(args.splits, static_cast<unsigned>(tiles * args.num_kv_heads), num_seqs), dim3(THREADS),
-                                           split_keys_smem<T, NT>(), stream, args));
+  const dim3 grid(args.splits, static_cast<unsigned>(tiles * args.num_kv_heads), num_seqs);
+  if (args.cluster == 1)
+    return static_cast<int>(launch_dependent(split_keys_kernel<T, NT>, grid, dim3(THREADS), split_keys_smem<T, NT>(), stream, args));
+  return static_cast<int>(launch_dependent_clusters(split_keys_kernel<T, NT>, grid, dim3(THREADS), split_keys_smem<T, NT>(), stream,
+                                                    static_cast<unsigned>(args.cluster), args));
 }
 
 template <typename T>
@@ -732,12 +794,13 @@ SHRIKE_API int shrike_paged_attention_q8(const void* q, const void* k_codes, con
                                          const float* v_scales, const int* block_table, int max_blocks, const int* q_start,
                                          const int* ctx_len, int dtype, int num_seqs, int num_heads, int num_kv_heads, int page_size,
                                          int num_pages, float scale, int window, void* out, int has_single, int has_portions,
-                                         int max_q_len, int splits, float* scratch, int* arrivals, cudaStream_t stream) {
+                                         int max_q_len, int splits, int cluster, float* scratch, int* arrivals, cudaStream_t stream) {
   if (num_seqs <= 0) return SHRIKE_OK;
   if (num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads || num_kv_heads > 65535 || max_blocks <= 0 || page_size <= 0 ||
       num_pages <= 0 || static_cast<long long>(num_pages) * page_size > 0x7fffffff ||
       static_cast<long long>(max_blocks) * page_size > 0x7fffffff - 4096 || max_q_len < 1 || num_seqs > 65535 || splits < 1 ||
-      splits > attnq8::MAX_SPLITS || (splits > 1 && (scratch == nullptr || arrivals == nullptr)) ||
+      cluster < 1 || cluster > 8 || splits % cluster || splits > attnq8::MAX_SPLITS ||
+      (splits > cluster && (scratch == nullptr || arrivals == nullptr)) ||
       (reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(k_codes) |
        reinterpret_cast<uintptr_t>(v_codes) | reinterpret_cast<uintptr_t>(scratch)) % 16)
     return SHRIKE_BAD_ARGUMENT;
@@ -761,6 +824,7 @@ SHRIKE_API int shrike_paged_attention_q8(const void* q, const void* k_codes, con
   args.only = 0;
   args.scale_log2 = scale * attnq8::LOG2E;
   args.splits = splits;
+  args.cluster = cluster;
   args.scratch = scratch;
   args.arrivals = arrivals;
   if (dtype == SHRIKE_F32) return attnq8::launch<float>(args, num_seqs, max_q_len, has_single, has_portions, stream);

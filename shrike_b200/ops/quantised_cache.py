@@ -28,6 +28,7 @@ class QuantisedPlan:
     has_single: bool      # entries of one token run on the form for few rows
     has_portions: bool    # longer ones on the form for many
     splits: int           # CTAs that share the keys of a row tile of the former
+    cluster: int          # how many of them form a thread-block cluster
     scratch: torch.Tensor | None
     arrivals: torch.Tensor | None
 
@@ -59,7 +60,7 @@ class QuantisedCacheOps:
             getattr(lib, name).restype = _I
         self._q8_libs, self._q8_plans = {}, {}
         self._q8_scratch = self._q8_arrivals = None
-        self.q8_splits = 0   # 0: the rule of `q8_plan`; n: that many splits for few rows (tests)
+        self.q8_splits = None   # None: the rule of `q8_few_row_splits`; (splits, cluster) for few rows (tests)
 
     def _q8_lib(self, head_dim: int):
         lib = self._q8_libs.get(head_dim)
@@ -67,7 +68,7 @@ class QuantisedCacheOps:
             if head_dim % 16 or not 16 <= head_dim <= MOST_HEAD_DIM:
                 raise _error(f"head size {head_dim} is not served: 8-bit pages take multiples of 16 from 16 to {MOST_HEAD_DIM}")
             lib = build.attention_q8_library(head_dim)
-            lib.shrike_paged_attention_q8.argtypes = [_P] * 6 + [_I, _P, _P] + [_I] * 6 + [_F, _I, _P] + [_I] * 4 + [_P, _P, _P]
+            lib.shrike_paged_attention_q8.argtypes = [_P] * 6 + [_I, _P, _P] + [_I] * 6 + [_F, _I, _P] + [_I] * 5 + [_P, _P, _P]
             lib.shrike_paged_attention_q8.restype = _I
             for name in ("row_floats", "max_splits"):
                 getattr(lib, f"shrike_attention_q8_{name}").argtypes = []
@@ -218,7 +219,7 @@ class QuantisedCacheOps:
             return held[1]
         lib = self._q8_lib(head_dim)
         has_single, has_portions = min_q_len <= 1, max_q_len > 1
-        splits, scratch, arrivals = 1, None, None
+        splits, cluster, scratch, arrivals = 1, 1, None, None
         if has_single:
             group = num_heads // num_kv_heads
             rows = lib.shrike_attention_q8_tile_rows(group)
@@ -228,11 +229,13 @@ class QuantisedCacheOps:
                 keys = min(keys, window)
             elif window < 0:
                 keys = min(keys, -window)
-            splits = self.q8_splits or self.q8_few_row_splits(keys, pairs, lib.shrike_attention_q8_resident_ctas(self.code, group))
-            share = rows * lib.shrike_attention_q8_row_floats()
-            splits = max(1, min(splits, lib.shrike_attention_q8_max_splits(), self.Q8_SCRATCH_FLOATS // (share * pairs)))
-            if splits > 1:
-                need = pairs * splits * share
+            most = lib.shrike_attention_q8_max_splits()
+            splits, cluster = self.q8_splits or self.q8_few_row_splits(keys, pairs, lib.shrike_attention_q8_resident_ctas(self.code, group))
+            share = rows * lib.shrike_attention_q8_row_floats() * pairs
+            if splits > most or splits // cluster * share > self.Q8_SCRATCH_FLOATS:
+                splits = cluster * max(1, min(most // cluster, self.Q8_SCRATCH_FLOATS // share))
+            if splits > cluster:
+                need = splits // cluster * share
                 if self._q8_scratch is None or self._q8_scratch.numel() < need:
                     self._q8_scratch = torch.empty(max(need, 1 << 20), dtype=torch.float32, device=self.device)
                     self.generation += 1
@@ -240,7 +243,7 @@ class QuantisedCacheOps:
                     self._q8_arrivals = torch.zeros(max(pairs, 4096), dtype=torch.int32, device=self.device)
                     self.generation += 1
                 scratch, arrivals = self._q8_scratch, self._q8_arrivals
-        plan = QuantisedPlan(has_single, has_portions, splits, scratch, arrivals)
+        plan = QuantisedPlan(has_single, has_portions, splits, cluster, scratch, arrivals)
         if len(self._q8_plans) >= 4096:
             self._q8_plans.clear()
         self._q8_plans[key] = (self.generation, plan)
@@ -249,16 +252,20 @@ class QuantisedCacheOps:
     Q8_SPLIT_KEYS = 160   # what a CTA's start, and its share's way to the others, cost in keys
 
     @classmethod
-    def q8_few_row_splits(cls, keys: int, pairs: int, resident: int) -> int:
-        """CTAs that share the `keys` of each of `pairs` (entry, kv head, row tile) where the device holds `resident` at once: the
-        count with the least time, rounds of CTAs times what each takes, a CTA having at least a step of 32 keys for each of its
-        four warps."""
+    def q8_few_row_splits(cls, keys: int, pairs: int, resident: int):
+        """(splits, cluster): CTAs that share the `keys` of each of `pairs` (entry, kv head, row tile) where the device holds
+        `resident` at once, and how many of them form a cluster.  The count with the least time, rounds of CTAs times what each
+        takes, a CTA having at least a step of 32 keys for each of its four warps."""
         best, least = 1, None
-        for splits in range(1, max(1, min(64, keys // 128)) + 1):
+        for splits in (1, 2, 3, 4, 5, 6, 7, 8, 16, 24, 32, 40, 48, 56, 64):
+            if splits > max(1, -(-keys // 128)):
+                break
             time = -(-pairs * splits // resident) * (-(-keys // splits) + cls.Q8_SPLIT_KEYS)
             if least is None or time < least:
                 best, least = splits, time
-        return best
+        # clusters while they fill no more than two thirds of the device: a fuller grid of them starts late
+        cluster = best & -best if pairs * best * 3 <= resident * 2 else 1
+        return best, min(cluster, 8)
 
     def _paged_attention_q8(self, q, keys, values, block_table, q_start, ctx_len, seq_of_token, num_heads, num_kv_heads, head_dim,
                             scale, window, out, max_q_len, min_q_len):
@@ -290,5 +297,5 @@ class QuantisedCacheOps:
         _check(self._q8_libs[head_dim].shrike_paged_attention_q8(
             q_at, keys.codes.data_ptr(), keys.scales.data_ptr(), values.codes.data_ptr(), values.scales.data_ptr(),
             block_table.data_ptr(), max_blocks, q_start.data_ptr(), ctx_len.data_ptr(), self.code, num_seqs, num_heads, num_kv_heads,
-            page_size, pages, scale, window or 0, out_at, plan.has_single, plan.has_portions, max_q_len, plan.splits,
+            page_size, pages, scale, window or 0, out_at, plan.has_single, plan.has_portions, max_q_len, plan.splits, plan.cluster,
             _ptr(plan.scratch), _ptr(plan.arrivals), stream), "paged_attention_q8")

@@ -139,7 +139,7 @@ def attend(ops, case, heads, kv_heads, dim, q_lens, ctx_lens, window=None, chunk
     return out
 
 
-def check_attention(dtype, heads, kv_heads, dim, page, q_lens, ctx_lens, seed=0, q_scale=1.0, splits=0, known=True, **options):
+def check_attention(dtype, heads, kv_heads, dim, page, q_lens, ctx_lens, seed=0, q_scale=1.0, splits=None, known=True, **options):
     ops = cuda_ops(dtype)
     ops.q8_splits = splits
     case = oracle.pages_case(heads, kv_heads, dim, page, q_lens, ctx_lens, dtype, seed, DEV, q_scale)
@@ -165,7 +165,7 @@ def test_single_tokens(dtype, heads, kv_heads, dim, page):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("splits", [1, 2, 3, 16, 64])
+@pytest.mark.parametrize("splits", [(1, 1), (2, 1), (2, 2), (3, 1), (8, 8), (16, 8), (12, 4), (64, 1), (64, 8)])
 @pytest.mark.parametrize("options", [{}, {"window": 40}, {"chunk": 48}])
 def test_single_tokens_in_any_number_of_splits(dtype, splits, options):
     ctx_lens = [1, 33, 700, 1900]
