@@ -44,8 +44,8 @@ constexpr int STEPS_K = D / 16;          // products along the head size, for 8 
 constexpr int BLOCKS_V = (D + 31) / 32;  // runs of 32 elements of the output
 constexpr bool WIDE = D % 64 == 0;       // keys are read 16 bytes a lane (else 4)
 constexpr int TILE = KEYS * D;           // bytes of a step's key (or value) codes
-constexpr int STAGE = 2 * TILE + 2 * KEYS * 4;   // keys, values, and their scales
-constexpr int STAGES = 2;                // one lands while the other is used; a third would cost a CTA an SM
+constexpr int RING = 3 * (KEYS * D) + 4 * KEYS * 4;   // a warp's share of the few-rows form: two steps' keys, one step's values
+constexpr int K_STAGE = TILE + 2 * KEYS * 4;   // a step's keys and both kinds of scales; its values are TILE bytes
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr int MAX_SPLITS = 64;
 
@@ -160,27 +160,25 @@ __device__ __forceinline__ Place place_of(const Args& args, const int* table, in
   return at;
 }
 
-// Brings the codes and scales of 32 keys into a stage; `COUNT` threads of which this is number `id` share the work, and each of
-// their warps holds in lane l the place of key l.
+// Brings the codes of 32 keys (or of their values) into shared memory; `COUNT` threads of which this is number `id` share the
+// work, and each of their warps holds in lane l the row of key l (`Place::row`).
 template <int COUNT>
-__device__ __forceinline__ void load_step(const Args& args, int kv_head, const Place& place, unsigned stage, int id) {
-  const int row_bytes = args.num_kv_heads * D;
+__device__ __forceinline__ void load_codes(const signed char* codes, int row_bytes, int head_at, int row_of_lane, unsigned tile, int id) {
 #pragma unroll
   for (int k = 0; k < (KEYS * CHUNKS + COUNT - 1) / COUNT; ++k) {
     const int idx = id + k * COUNT;
     const int key = idx / CHUNKS, chunk = idx - key * CHUNKS;
-    const int row = __shfl_sync(0xffffffffu, place.row, key & 31);
+    const int row = __shfl_sync(0xffffffffu, row_of_lane, key & 31);
     if (KEYS * CHUNKS % COUNT == 0 || idx < KEYS * CHUNKS) {
       const bool there = row >= 0;
-      const long long at = static_cast<long long>(there ? row : 0) * row_bytes + (kv_head * D + chunk * 16);
-      const unsigned to = stage + chunk_at(key, chunk);
-      copy16(to, args.k_codes + at, there);
-      copy16(to + TILE, args.v_codes + at, there);
+      copy16(tile + chunk_at(key, chunk), codes + (static_cast<long long>(there ? row : 0) * row_bytes + (head_at + chunk * 16)), there);
     }
   }
+}
+__device__ __forceinline__ void load_scales(const Args& args, const Place& place, unsigned k_stage, int id) {
   if (id < KEYS) {
-    copy4(stage + 2 * TILE + id * 4, args.k_scales + place.scale, place.row >= 0);
-    copy4(stage + 2 * TILE + KEYS * 4 + id * 4, args.v_scales + place.scale, place.row >= 0);
+    copy4(k_stage + TILE + id * 4, args.k_scales + place.scale, place.row >= 0);
+    copy4(k_stage + TILE + KEYS * 4 + id * 4, args.v_scales + place.scale, place.row >= 0);
   }
 }
 
@@ -212,8 +210,8 @@ struct Rows {
   __device__ __forceinline__ static int element_of(int step, int t) {   // a lane's first element of four in a product
     return WIDE ? 16 * (t + 4 * (step / 4)) + 4 * (step % 4) : 4 * (t + 4 * step);
   }
-  // The element of the head that o[nt][2 b + m][c] belongs to, and its row.
-  __device__ __forceinline__ static int out_element(int b, int g) { return 32 * b + 4 * g; }   // m = 0, c = 0; then + 2 m + (c >> 1)
+  // The element of the head that o[nt][2 b][0] belongs to; o[nt][2 b + m][c] is 2 m + (c >> 1) further.
+  __device__ __forceinline__ static int out_element(int b, int g) { return WIDE ? 64 * (b / 2) + 8 * g + 4 * (b % 2) : 32 * b + 4 * g; }
 
   // Rows row0 ... of an entry whose tokens begin at `start`; `group` heads share kv head `kv_head`.
   __device__ __forceinline__ void begin(const Args& args, int row0, int rows, int start, int group, int kv_head, int pos0, uint2* shared, int lane) {
@@ -272,12 +270,13 @@ struct Rows {
     }
   }
 
-  // The 32 keys from `key0` on, which lie in `stage`.
-  __device__ __forceinline__ void step(const unsigned char* stage, int key0, const uint2* shared, int lane) {
+  using Weights = unsigned[NT][2][2][PARTS];   // [16 keys][eight of them]: operands of the second product
+
+  // The weights of the 32 keys from `key0` on, whose codes and scales lie in `k_stage`.
+  __device__ __forceinline__ void weigh(const unsigned char* k_stage, int key0, const uint2* shared, int lane, Weights& weights) {
     const int g = lane >> 2, t = lane & 3;
-    const unsigned char* k_tile = stage;
-    const unsigned char* v_tile = stage + TILE;
-    const float* k_scales = reinterpret_cast<const float*>(stage + 2 * TILE);
+    const unsigned char* k_tile = k_stage;
+    const float* k_scales = reinterpret_cast<const float*>(k_stage + TILE);
     const float* v_scales = k_scales + KEYS;
     float s[NT][2][4];   // [16 keys]: c & 1 the row, c >> 1 the eight keys
 #pragma unroll
@@ -340,7 +339,6 @@ struct Rows {
     const bool edge = __any_sync(0xffffffffu, !inside);
     const unsigned all_top = edge ? 0u : __reduce_max_sync(0xffffffffu, max(max(finite_bits(v_scale[0]), finite_bits(v_scale[1])),
                                                                             max(finite_bits(v_scale[2]), finite_bits(v_scale[3]))));
-    unsigned weights[NT][2][2][PARTS];   // [16 keys][eight of them]: operands of the second product
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       float largest[2] = {-INFINITY, -INFINITY};
@@ -414,28 +412,41 @@ struct Rows {
         }
       }
     }
-    // output
+  }
+
+  // Adds the same keys' values, in `v_tile`.
+  __device__ __forceinline__ void add(const unsigned char* v_tile, int lane, const Weights& weights) {
+    const int g = lane >> 2, t = lane & 3;
+    constexpr int RUN = WIDE ? 2 : 1;   // words a lane reads of a value row at a time
 #pragma unroll
-    for (int b = 0; b < BLOCKS_V; ++b) {
-      const int chunk = 2 * b + (g >> 2);
+    for (int b = 0; b < BLOCKS_V; b += RUN) {
 #pragma unroll
       for (int kk = 0; kk < 2; ++kk) {
-        unsigned rows[4];
+        unsigned rows[4][RUN];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {   // keys 2 t, 2 t + 1 of the first eight, then of the second
           const int key = 16 * kk + 8 * (i >> 1) + key_of(2 * t + (i & 1));
-          rows[i] = D % 32 == 0 || chunk < CHUNKS ? *reinterpret_cast<const unsigned*>(v_tile + chunk_at(key, chunk) + 4 * (g & 3)) : 0u;
-          rows[i] ^= 0x80808080u;
+          const int at = WIDE ? 4 * (b / 2) + (g >> 1) : 2 * b + (g >> 2);
+          if (WIDE) {
+            const uint2 v = *reinterpret_cast<const uint2*>(v_tile + chunk_at(key, at) + 8 * (g & 1));
+            rows[i][0] = v.x ^ 0x80808080u;
+            rows[i][RUN - 1] = WIDE ? v.y ^ 0x80808080u : v.x ^ 0x80808080u;
+          } else {
+            rows[i][0] = D % 32 == 0 || at < CHUNKS ? *reinterpret_cast<const unsigned*>(v_tile + chunk_at(key, at) + 4 * (g & 3)) : 0u;
+            rows[i][0] ^= 0x80808080u;
+          }
         }
 #pragma unroll
-        for (int m = 0; m < 2; ++m) {   // elements 4 g + 2 m and + 1 are rows g and g + 8 of the product
-          const unsigned lo = __byte_perm(rows[0], rows[1], m == 0 ? 0x5140 : 0x7362), hi = __byte_perm(rows[2], rows[3], m == 0 ? 0x5140 : 0x7362);
-          const unsigned a[4] = {codes_to_half<0x4140>(lo), codes_to_half<0x4342>(lo), codes_to_half<0x4140>(hi), codes_to_half<0x4342>(hi)};
+        for (int w = 0; w < RUN; ++w)
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
+          for (int m = 0; m < 2; ++m) {   // of a word's four elements the pair 2 m, 2 m + 1: rows g and g + 8 of the product
+            const unsigned lo = __byte_perm(rows[0][w], rows[1][w], m == 0 ? 0x5140 : 0x7362), hi = __byte_perm(rows[2][w], rows[3][w], m == 0 ? 0x5140 : 0x7362);
+            const unsigned a[4] = {codes_to_half<0x4140>(lo), codes_to_half<0x4342>(lo), codes_to_half<0x4140>(hi), codes_to_half<0x4342>(hi)};
 #pragma unroll
-            for (int part = 0; part < PARTS; ++part) mma(o[nt][2 * b + m], a, weights[nt][kk][0][part], weights[nt][kk][1][part]);
-        }
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int part = 0; part < PARTS; ++part) mma(o[nt][2 * (b + w) + m], a, weights[nt][kk][0][part], weights[nt][kk][1][part]);
+          }
       }
     }
   }
@@ -482,7 +493,7 @@ __device__ __forceinline__ void store_row(const Args& args, int row, int start, 
 
 // Few rows: grid (splits, kv heads * row tiles, entries).
 template <typename T, int NT>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(THREADS, Parts<T>::COUNT * NT * D <= 128 ? 4 : 1)
 split_keys_kernel(const Args args) {
   using R = Rows<T, NT>;
   constexpr int ROWS = R::ROWS;
@@ -504,35 +515,49 @@ split_keys_kernel(const Args args) {
   const int per = (steps + args.splits - 1) / args.splits;
   const int mine_lo = step_lo + min(steps, split * per), mine_hi = step_lo + min(steps, (split + 1) * per);
 
-  uint2* shared_q = reinterpret_cast<uint2*>(smem + WARPS * STAGES * STAGE);
-  unsigned char* ring = smem + warp * STAGES * STAGE;
-  const unsigned ring_at = smem_u32(ring);
+  uint2* shared_q = reinterpret_cast<uint2*>(smem + WARPS * RING);
+  unsigned char* ring = smem + warp * RING;   // two steps' keys, one step's values
+  unsigned char* v_tile = ring + 2 * K_STAGE;
+  const unsigned ring_at = smem_u32(ring), v_at = ring_at + 2 * K_STAGE;
   const int* table = args.block_table + static_cast<size_t>(seq) * args.max_blocks;
+  const int row_bytes = args.num_kv_heads * D, head_at = kv_head * D;
+  auto load_keys = [&](const Place& place, unsigned to) {
+    load_codes<32>(args.k_codes, row_bytes, head_at, place.row, to, lane);
+    load_scales(args, place, to, lane);
+  };
   R r;
-  // this warp's steps: mine_lo + warp, + WARPS, ...
+  // This warp's steps: mine_lo + warp, + WARPS, ...  The keys of the step after next are asked for as soon as this step's are
+  // used, the values of the next step as soon as this step's are: keys have a step and a half to come, values most of one.
   const int begin = mine_lo + warp;
-  int loaded = begin;
-  Place next = place_of(args, table, kv_head, loaded * KEYS + lane, loaded < mine_hi ? last_key : -1);
-#pragma unroll
-  for (int i = 0; i < STAGES; ++i) {
-    if (loaded < mine_hi) load_step<32>(args, kv_head, next, ring_at + i * STAGE, lane);
-    copies_commit();
-    loaded += WARPS;
-    next = place_of(args, table, kv_head, loaded * KEYS + lane, loaded < mine_hi ? last_key : -1);
-  }
+  Place place = place_of(args, table, kv_head, begin * KEYS + lane, begin < mine_hi ? last_key : -1);
+  Place next = place_of(args, table, kv_head, (begin + WARPS) * KEYS + lane, begin + WARPS < mine_hi ? last_key : -1);
+  if (begin < mine_hi) load_keys(place, ring_at);
+  copies_commit();
+  if (begin + WARPS < mine_hi) load_keys(next, ring_at + K_STAGE);
+  copies_commit();
+  if (begin < mine_hi) load_codes<32>(args.v_codes, row_bytes, head_at, place.row, v_at, lane);
+  copies_commit();
+  place = place_of(args, table, kv_head, (begin + 2 * WARPS) * KEYS + lane, begin + 2 * WARPS < mine_hi ? last_key : -1);
   r.begin(args, row0, rows, start, group, kv_head, pos0, shared_q, lane);   // all warps write the same operands
   __syncwarp();
-  int stage = 0;
+  int stage = 0;   // `next`: the place of the step after this one, `place`: of the one after that
   for (int step = begin; step < mine_hi; step += WARPS) {
-    copies_wait<STAGES - 1>();
+    typename R::Weights weights;
+    copies_wait<2>();   // outstanding: the next step's keys, this step's values
     __syncwarp();
-    r.step(ring + stage * STAGE, step * KEYS, shared_q, lane);
+    r.weigh(ring + stage * K_STAGE, step * KEYS, shared_q, lane, weights);
     __syncwarp();
-    if (loaded < mine_hi) load_step<32>(args, kv_head, next, ring_at + stage * STAGE, lane);
+    if (step + 2 * WARPS < mine_hi) load_keys(place, ring_at + stage * K_STAGE);
     copies_commit();
-    loaded += WARPS;
-    next = place_of(args, table, kv_head, loaded * KEYS + lane, loaded < mine_hi ? last_key : -1);
-    stage = stage + 1 == STAGES ? 0 : stage + 1;
+    copies_wait<1>();
+    __syncwarp();
+    r.add(v_tile, lane, weights);
+    __syncwarp();
+    if (step + WARPS < mine_hi) load_codes<32>(args.v_codes, row_bytes, head_at, next.row, v_at, lane);
+    copies_commit();
+    next = place;
+    place = place_of(args, table, kv_head, (step + 3 * WARPS) * KEYS + lane, step + 3 * WARPS < mine_hi ? last_key : -1);
+    stage ^= 1;
   }
   copies_wait<0>();
   r.finish();
@@ -671,29 +696,36 @@ portion_rows_kernel(const Args args) {
   const int my_last = row0 < rows ? pos0 + (min(row0 + ROWS, rows) - 1) / group : -1;
   const int my_first = first_visible_key(pos0 + row0 / group, args.window);
 
-  uint2* shared_q = reinterpret_cast<uint2*>(smem + STAGES * STAGE + warp * R::SHARED_BYTES);
+  uint2* shared_q = reinterpret_cast<uint2*>(smem + 2 * (K_STAGE + TILE) + warp * R::SHARED_BYTES);
   const unsigned ring_at = smem_u32(smem);
   const int* table = args.block_table + static_cast<size_t>(seq) * args.max_blocks;
+  const int row_bytes = args.num_kv_heads * D, head_at = kv_head * D;
+  auto load_step = [&](const Place& place, unsigned to) {
+    load_codes<THREADS>(args.k_codes, row_bytes, head_at, place.row, to, threadIdx.x);
+    load_scales(args, place, to, threadIdx.x);
+    load_codes<THREADS>(args.v_codes, row_bytes, head_at, place.row, to + K_STAGE, threadIdx.x);
+  };
   R r;
   Place next = place_of(args, table, kv_head, step_lo * KEYS + lane, last_key);
-#pragma unroll
-  for (int i = 0; i < STAGES - 1; ++i) {
-    if (step_lo + i < step_hi) load_step<THREADS>(args, kv_head, next, ring_at + i * STAGE, threadIdx.x);
-    copies_commit();
-    next = place_of(args, table, kv_head, (step_lo + i + 1) * KEYS + lane, last_key);
-  }
+  if (step_lo < step_hi) load_step(next, ring_at);
+  copies_commit();
+  next = place_of(args, table, kv_head, (step_lo + 1) * KEYS + lane, last_key);
   r.begin(args, row0, rows, start, group, kv_head, pos0, shared_q, lane);
   __syncwarp();
   int stage = 0;
   for (int step = step_lo; step < step_hi; ++step) {
-    copies_wait<STAGES - 2>();
+    copies_wait<0>();
     __syncthreads();   // this step's copies of all threads have landed; everyone has left the stage that is loaded next
-    const int into = stage + STAGES - 1 >= STAGES ? stage - 1 : stage + STAGES - 1;
-    if (step + STAGES - 1 < step_hi) load_step<THREADS>(args, kv_head, next, ring_at + into * STAGE, threadIdx.x);
+    if (step + 1 < step_hi) load_step(next, ring_at + (stage ^ 1) * (K_STAGE + TILE));
     copies_commit();
-    next = place_of(args, table, kv_head, (step + STAGES) * KEYS + lane, last_key);
-    if (step * KEYS <= my_last && step * KEYS + KEYS > my_first) r.step(smem + stage * STAGE, step * KEYS, shared_q, lane);
-    stage = stage + 1 == STAGES ? 0 : stage + 1;
+    next = place_of(args, table, kv_head, (step + 2) * KEYS + lane, last_key);
+    if (step * KEYS <= my_last && step * KEYS + KEYS > my_first) {
+      typename R::Weights weights;
+      const unsigned char* at = smem + stage * (K_STAGE + TILE);
+      r.weigh(at, step * KEYS, shared_q, lane, weights);
+      r.add(at + K_STAGE, lane, weights);
+    }
+    stage ^= 1;
   }
   copies_wait<0>();
   r.finish();
@@ -712,11 +744,11 @@ portion_rows_kernel(const Args args) {
 }
 
 template <typename T, int NT> constexpr size_t split_keys_smem() {
-  const size_t ring = static_cast<size_t>(WARPS) * STAGES * STAGE + Rows<T, NT>::SHARED_BYTES;
+  const size_t ring = static_cast<size_t>(WARPS) * RING + Rows<T, NT>::SHARED_BYTES;
   const size_t merge = (static_cast<size_t>(WARPS) * Rows<T, NT>::ROWS * (D + 6) + Rows<T, NT>::ROWS * (D + 2)) * 4;
   return ring > merge ? ring : merge;
 }
-template <typename T, int NT> constexpr size_t portion_rows_smem() { return static_cast<size_t>(STAGES) * STAGE + WARPS * Rows<T, NT>::SHARED_BYTES; }
+template <typename T, int NT> constexpr size_t portion_rows_smem() { return 2 * static_cast<size_t>(K_STAGE + TILE) + WARPS * Rows<T, NT>::SHARED_BYTES; }
 
 constexpr int PORTION_NT = 2;
 // Row tiles of the few-rows form: eights, pairs of them for groups of more than eight heads.

@@ -257,15 +257,13 @@ class QuantisedCacheOps:
         `resident` at once, and how many of them form a cluster.  The count with the least time, rounds of CTAs times what each
         takes, a CTA having at least a step of 32 keys for each of its four warps."""
         best, least = 1, None
-        for splits in (1, 2, 3, 4, 5, 6, 7, 8, 16, 24, 32, 40, 48, 56, 64):
+        for splits in (1, 2, 4, 8, 16, 24, 32, 40, 48, 56, 64):
             if splits > max(1, -(-keys // 128)):
                 break
             time = -(-pairs * splits // resident) * (-(-keys // splits) + cls.Q8_SPLIT_KEYS)
             if least is None or time < least:
                 best, least = splits, time
-        # clusters while they fill no more than two thirds of the device: a fuller grid of them starts late
-        cluster = best & -best if pairs * best * 3 <= resident * 2 else 1
-        return best, min(cluster, 8)
+        return best, min(best, 8)
 
     def _paged_attention_q8(self, q, keys, values, block_table, q_start, ctx_len, seq_of_token, num_heads, num_kv_heads, head_dim,
                             scale, window, out, max_q_len, min_q_len):
