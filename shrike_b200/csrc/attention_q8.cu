@@ -142,20 +142,23 @@ __device__ __forceinline__ float4 load_peer4(unsigned address) {
 // 2^e for e in [-126, 127].
 __device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e + 127) << 23); }
 
-// Where a lane's key lies: its row among all codes (-1: no such key), and its place among the scales.
+// Where a lane's key lies: its row among all codes, its place among the scales, and whether it exists.  A key that does not
+// has scales of zero and whatever codes the pool's first row holds: codes are finite whatever they are, so it counts as zeros.
 struct Place {
   int row;
+  bool there;
   long long scale;
 };
 // The place of a key, nowhere if it lies behind `last_key` or its page is not one of the pool's.
 __device__ __forceinline__ Place place_of(const Args& args, const int* table, int kv_head, int key, int last_key) {
-  Place at{-1, 0};
+  Place at{0, false, 0};
   if (key > last_key) return at;
   const int block = args.page_shift >= 0 ? key >> args.page_shift : key / args.page_size;
   if (block >= args.max_blocks) return at;
   const int page = table[block], within = key - block * args.page_size;
   if (page < 0 || page >= args.num_pages) return at;
   at.row = page * args.page_size + within;
+  at.there = true;
   at.scale = (static_cast<long long>(page) * args.num_kv_heads + kv_head) * args.page_size + within;
   return at;
 }
@@ -164,21 +167,35 @@ __device__ __forceinline__ Place place_of(const Args& args, const int* table, in
 // work, and each of their warps holds in lane l the row of key l (`Place::row`).
 template <int COUNT>
 __device__ __forceinline__ void load_codes(const signed char* codes, int row_bytes, int head_at, int row_of_lane, unsigned tile, int id) {
+  if constexpr (COUNT % CHUNKS == 0) {
+    // COUNT / CHUNKS keys a turn.  Where these are few, a turn's number and a thread's own key are different bits of the key's
+    // number, and since a swizzle is made of exclusive ors, the thread's part of it is formed once.
+    constexpr int AT_ONCE = COUNT / CHUNKS;
+    const int chunk = id % CHUNKS, own = id / CHUNKS;
+    const signed char* src = codes + (head_at + chunk * 16);
+    const int own_at = own * D;
+    const int own_chunk = chunk ^ swizzle(own);
 #pragma unroll
-  for (int k = 0; k < (KEYS * CHUNKS + COUNT - 1) / COUNT; ++k) {
-    const int idx = id + k * COUNT;
-    const int key = idx / CHUNKS, chunk = idx - key * CHUNKS;
-    const int row = __shfl_sync(0xffffffffu, row_of_lane, key & 31);
-    if (KEYS * CHUNKS % COUNT == 0 || idx < KEYS * CHUNKS) {
-      const bool there = row >= 0;
-      copy16(tile + chunk_at(key, chunk), codes + (static_cast<long long>(there ? row : 0) * row_bytes + (head_at + chunk * 16)), there);
+    for (int k = 0; k < (KEYS + AT_ONCE - 1) / AT_ONCE; ++k) {
+      const int row = __shfl_sync(0xffffffffu, row_of_lane, (k * AT_ONCE + own) & 31);
+      if (AT_ONCE <= KEYS || own < KEYS)
+        copy16(tile + (k * AT_ONCE * D + own_at + ((own_chunk ^ swizzle(k * AT_ONCE)) << 4)), src + static_cast<long long>(row) * row_bytes, true);
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < (KEYS * CHUNKS + COUNT - 1) / COUNT; ++k) {
+      const int idx = id + k * COUNT;
+      const int key = idx / CHUNKS, chunk = idx - key * CHUNKS;
+      const int row = __shfl_sync(0xffffffffu, row_of_lane, key & 31);
+      if (KEYS * CHUNKS % COUNT == 0 || idx < KEYS * CHUNKS)
+        copy16(tile + chunk_at(key, chunk), codes + (static_cast<long long>(row) * row_bytes + (head_at + chunk * 16)), true);
     }
   }
 }
 __device__ __forceinline__ void load_scales(const Args& args, const Place& place, unsigned k_stage, int id) {
   if (id < KEYS) {
-    copy4(k_stage + TILE + id * 4, args.k_scales + place.scale, place.row >= 0);
-    copy4(k_stage + TILE + KEYS * 4 + id * 4, args.v_scales + place.scale, place.row >= 0);
+    copy4(k_stage + TILE + id * 4, args.k_scales + place.scale, place.there);
+    copy4(k_stage + TILE + KEYS * 4 + id * 4, args.v_scales + place.scale, place.there);
   }
 }
 
@@ -337,8 +354,11 @@ struct Rows {
 #pragma unroll
       for (int r = 0; r < 2; ++r) inside = inside && key0 >= first[nt][r] && key0 + KEYS - 1 <= last[nt][r];
     const bool edge = __any_sync(0xffffffffu, !inside);
-    const unsigned all_top = edge ? 0u : __reduce_max_sync(0xffffffffu, max(max(finite_bits(v_scale[0]), finite_bits(v_scale[1])),
-                                                                            max(finite_bits(v_scale[2]), finite_bits(v_scale[3]))));
+    // the largest of this lane's value scales (negative ones, infinities and NaN, none of which a store leaves but the last,
+    // order above all finite bits)
+    unsigned all_top = max(max(__float_as_uint(v_scale[0]), __float_as_uint(v_scale[1])), max(__float_as_uint(v_scale[2]), __float_as_uint(v_scale[3])));
+    if (edge) all_top = 0u;
+    else if (all_top >= 0x7f800000u) all_top = max(max(finite_bits(v_scale[0]), finite_bits(v_scale[1])), max(finite_bits(v_scale[2]), finite_bits(v_scale[3])));
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       float largest[2] = {-INFINITY, -INFINITY};
@@ -370,7 +390,7 @@ struct Rows {
 #pragma unroll
           for (int offset = 4; offset < 32; offset <<= 1) {
             largest[r] = fmaxf(largest[r], __shfl_xor_sync(0xffffffffu, largest[r], offset));
-            if (edge) top[r] = max(top[r], __shfl_xor_sync(0xffffffffu, top[r], offset));
+            top[r] = max(top[r], __shfl_xor_sync(0xffffffffu, top[r], offset));
           }
           exponent[nt][r] = max(exponent[nt][r], min(static_cast<int>(top[r] >> 23) - 127 - SCALE_BITS, MOST_EXPONENT));
           most[nt][r] = fmaxf(most[nt][r], largest[r]);
