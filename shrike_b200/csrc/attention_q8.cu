@@ -799,12 +799,12 @@ static int launch_few(const Args& args, int num_seqs, int tokens, cudaStream_t s
 }
 
 template <typename T>
-static int launch(const Args& base, int num_seqs, int max_q_len, int has_single, int has_portions, cudaStream_t stream) {
+static int launch(const Args& base, int num_seqs, int max_q_len, int has_single, int has_portions, int others, cudaStream_t stream) {
   Args args = base;
   const int group = args.num_heads / args.num_kv_heads;
   if (has_single) {
-    args.only = has_portions ? 1 : 0;
-    const int tokens = has_portions ? 1 : max_q_len;
+    args.only = has_portions || others ? 1 : 0;
+    const int tokens = args.only ? 1 : max_q_len;
     const int rc = few_rows(group) == 8 ? launch_few<T, 1>(args, num_seqs, tokens, stream) : launch_few<T, 2>(args, num_seqs, tokens, stream);
     if (rc != 0) return rc;
   }
@@ -840,13 +840,13 @@ SHRIKE_API int shrike_attention_q8_max_splits() { return attnq8::MAX_SPLITS; }
 // q and out [tokens, heads * D] of `dtype`, 16-byte aligned; codes [pages, page_size, kv heads, D], 16-byte aligned, scales
 // [pages, kv heads, page_size].  `has_single`: entries of one token (every entry, where has_portions is 0: then `max_q_len`
 // tokens at most) run on the few-rows form with `splits` CTAs a row tile; `has_portions`: the longer ones (all of them where
-// has_single is 0) on the other.  splits > 1 needs `scratch` (row_floats() for every row of a tile of (entry, kv head, row tile) and split)
+// has_single is 0) on the other, or on another kernel where `others` is set.  splits > 1 needs `scratch` (row_floats() for every row of a tile of (entry, kv head, row tile) and split)
 // and `arrivals` (an int a pair, zero before the first launch).
 SHRIKE_API int shrike_paged_attention_q8(const void* q, const void* k_codes, const float* k_scales, const void* v_codes,
                                          const float* v_scales, const int* block_table, int max_blocks, const int* q_start,
                                          const int* ctx_len, int dtype, int num_seqs, int num_heads, int num_kv_heads, int page_size,
                                          int num_pages, float scale, int window, void* out, int has_single, int has_portions,
-                                         int max_q_len, int splits, int cluster, float* scratch, int* arrivals, cudaStream_t stream) {
+                                         int max_q_len, int others, int splits, int cluster, float* scratch, int* arrivals, cudaStream_t stream) {
   if (num_seqs <= 0) return SHRIKE_OK;
   if (num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads || num_kv_heads > 65535 || max_blocks <= 0 || page_size <= 0 ||
       num_pages <= 0 || static_cast<long long>(num_pages) * page_size > 0x7fffffff ||
@@ -879,7 +879,7 @@ SHRIKE_API int shrike_paged_attention_q8(const void* q, const void* k_codes, con
   args.cluster = cluster;
   args.scratch = scratch;
   args.arrivals = arrivals;
-  if (dtype == SHRIKE_F32) return attnq8::launch<float>(args, num_seqs, max_q_len, has_single, has_portions, stream);
-  if (dtype == SHRIKE_BF16) return attnq8::launch<__nv_bfloat16>(args, num_seqs, max_q_len, has_single, has_portions, stream);
+  if (dtype == SHRIKE_F32) return attnq8::launch<float>(args, num_seqs, max_q_len, has_single, has_portions, others, stream);
+  if (dtype == SHRIKE_BF16) return attnq8::launch<__nv_bfloat16>(args, num_seqs, max_q_len, has_single, has_portions, others, stream);
   return SHRIKE_BAD_ARGUMENT;
 }

@@ -1,0 +1,867 @@
+// Paged causal attention for portions (q_len > 1) over keys and values in 8 bits, queries in bfloat16, on the fifth-generation
+// tensor cores.  The mathematics is that of attention_q8.cu: codes are exact in float16, queries are scaled by a power of two
+// per row so that they are too, weights p s^v are rounded to float16 under a base that keeps the row's largest value scale at
+// 2^8 ... 2^9, everything else is in 32 bits.
+//
+// One CTA owns two chains of up to 128 query rows.  The rows of a chain are 128 / group tokens of ALL the heads that share a kv
+// head, token by token: a key tile is turned into float16 once for every head that reads it, a portion of a few dozen tokens
+// fills the rows, and a chain's tokens lie close together, so that little is computed behind the causal border.  A chain walks
+// the keys 64 at a time, as the kernel over bfloat16 pages does (attention_tcgen05.cu): scores by tcgen05.mma into tensor
+// memory, a thread a row for the softmax, weights back into tensor memory as the operand of the second product, outputs there.
+//
+// What is new is the way of the keys and values: TMA brings a tile's codes (one box a page, in the swizzle of their row
+// length), four warps turn them into float16 tiles in the 128-byte swizzle (a thread owns a key: its codes, its page, its two
+// scales), and those are what the products read.  Eight codes take 10 instructions (a byte permutation and a subtraction a
+// pair, an exclusive or for four).  A tile of 128 keys x 128 elements costs each of the four warps about 370 issue slots for the
+// keys and as many for the values, against about 2,050 clocks that the two chains' products and exponentials take.
+//
+// Roles: warp 0 brings key codes (and the queries), warp 3 value codes (and owns tensor memory), warps 1 and 2 issue the products
+// of a chain each, warps 4..7 and 8..11 are the softmax and epilogue of a chain each, warps 12..15 convert.  The softmax
+// warpgroups take 168 registers a thread, the other two 88 (together the 128 a thread that the CTA is launched with).
+// Barriers: raw_k / raw_v full (TMA) and free (converters); k_full / v_full[stage] (converters; v_full also says that the
+// tile's scales lie in shared memory), k_free / v_free[stage] (commits of both chains); q_ready[chain] once the softmax warps
+// have turned the queries into float16; the others as in attention_tcgen05.cu.
+// Every wait is bounded (status word, CTA-wide abort flag); no TMA load uses multicast.
+// Built once per head size; serves head sizes 64 and 128, page sizes 8, 16, 32, 64, and groups of up to 64 heads.
+#include <cuda_fp16.h>
+
+#include "blackwell.cuh"
+
+#ifndef SHRIKE_HEAD_DIM
+#error "compile with -DSHRIKE_HEAD_DIM=<head size>"
+#endif
+
+#if SHRIKE_HEAD_DIM == 64 || SHRIKE_HEAD_DIM == 128
+
+namespace tcq8 {
+using namespace bw;
+
+constexpr int D = SHRIKE_HEAD_DIM;
+constexpr int BM = 128;                         // query rows of one chain
+constexpr int HALVES = D / 64;                 // 64-element groups of the head size
+constexpr int Q_HALF = BM * 128;               // bytes of one 64-element-wide sub-tile of a query tile
+constexpr int Q_BYTES = HALVES * Q_HALF;
+constexpr int KEYS = 128;                      // keys of a tile
+constexpr int HALF_KEYS = KEYS / 2;            // keys of a softmax step
+constexpr int STAGES = 2;
+constexpr int KV_HALF = KEYS * 128;            // bytes of one 64-element-wide sub-tile of a float16 key (or value) tile
+constexpr int KV_TILE = HALVES * KV_HALF;
+constexpr int RAW_TILE = KEYS * D;             // a tile's codes
+constexpr int THREADS = 512;
+constexpr unsigned CHAIN_COLS = 256, P_COL = 64, O_COL = 128, TMEM_COLS = 512;   // as in attention_tcgen05.cu
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr int LEAST_EXPONENT = -93, MOST_EXPONENT = 107, SCALE_BITS = 8;   // as in attention_q8.cu
+constexpr float BASE_LAG = 6.0f;
+
+enum : int { ERR_PRODUCER = 61, ERR_CONVERT = 62, ERR_MMA = 63, ERR_SOFTMAX = 64, ERR_DRAIN = 65, ERR_ALIGNMENT = 66 };
+
+__device__ __forceinline__ float fast_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ unsigned long long pair_of(float lo, float hi) {
+  unsigned long long d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
+  return d;
+}
+__device__ __forceinline__ void halves_of(unsigned long long v, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ unsigned long long fma_pair(unsigned long long a, unsigned long long b, unsigned long long c) {
+  unsigned long long d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ unsigned long long add_pair(unsigned long long a, unsigned long long b) {
+  unsigned long long d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ unsigned long long mul_pair(unsigned long long a, unsigned long long b) {
+  unsigned long long d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ unsigned pack_half(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const unsigned*>(&h);
+}
+__device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e + 127) << 23); }
+__device__ __forceinline__ unsigned finite_bits(float x) {
+  const unsigned bits = __float_as_uint(x) & 0x7fffffffu;
+  return bits < 0x7f800000u ? bits : 0u;
+}
+// Two codes, biased by 128 in bytes 0, 1 (or 2, 3) of `biased`, as float16: byte b under 0x64 is 1024 + b.
+template <int SELECT> __device__ __forceinline__ unsigned codes_to_half(unsigned biased) {
+  const unsigned raw = __byte_perm(biased, 0x64646464u, SELECT), offset = 0x64806480u;   // 1152 twice
+  const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&raw), *reinterpret_cast<const __half2*>(&offset));
+  return *reinterpret_cast<const unsigned*>(&h);
+}
+// kind::f16 instruction descriptor: D float32, A and B float16, A K-major; B K-major or MN-major.
+__device__ __forceinline__ unsigned half_descriptor(int m, int n, bool b_mn_major) {
+  return (1u << 4) | ((b_mn_major ? 1u : 0u) << 16) | (static_cast<unsigned>(n >> 3) << 17) | (static_cast<unsigned>(m >> 4) << 24);
+}
+__device__ __forceinline__ void tma_load_3d(void* smem, const CUtensorMap* map, unsigned long long* bar, int x, int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+      ::"r"(smem_u32(smem)), "l"(reinterpret_cast<unsigned long long>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+// D[tmem] (+)= A[tmem] * B[smem]: the A operand (weights, float16 packed two to a column, one row per lane) from tensor memory.
+__device__ __forceinline__ void umma_a_in_tmem(unsigned leader, unsigned tmem_d, unsigned tmem_a, unsigned long long b, unsigned idesc,
+                                               unsigned accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 e, %5, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(tmem_d), "r"(tmem_a), "l"(b), "r"(idesc), "r"(accumulate), "r"(leader) : "memory");
+}
+template <int REGISTERS> __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGISTERS)); }
+template <int REGISTERS> __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGISTERS)); }
+
+struct Args {
+  const float* k_scales;
+  const float* v_scales;
+  const int* block_table;
+  const int* q_start;
+  const int* ctx_len;
+  __nv_bfloat16* out;
+  int* status;
+  int max_blocks, num_heads, num_kv_heads, page_size, page_shift, num_pages, window, skip_single;
+  int group, tokens;   // heads of a kv head, tokens of a chain (128 / group)
+  float scale_log2;
+  int splits;          // CTAs that share a query tile's keys; > 1: results go to the scratch below
+  float* partial_o;    // [splits][tokens][heads][D] unnormalised output rows
+  float* partial_ml;   // [splits][tokens][heads][2] their base (log2 domain) and sum
+  int num_tokens, num_seqs;
+  const int* seq_of_token;   // [tokens], for the second kernel
+};
+
+// Which (sequence, query tile) a CTA with work index `work` owns: sequences in order, each with its query tiles of `rows`
+// tokens, the last (longest to walk) first; sequences of one token own none when skip_single.  Every lane of the calling warp
+// gets the answer; tile_start < 0: no such work.
+__device__ __forceinline__ void find_work(const Args& args, int work, int rows, int& seq_out, int& tile_start_out) {
+  const int lane = threadIdx.x & 31;
+  int before = 0;
+  seq_out = -1;
+  tile_start_out = -1;
+  for (int base = 0; base < args.num_seqs; base += 32) {
+    const int s = base + lane;
+    int tiles = 0;
+    if (s < args.num_seqs) {
+      const int q_len = args.q_start[s + 1] - args.q_start[s];
+      tiles = q_len <= 0 || (q_len == 1 && args.skip_single) ? 0 : (q_len + rows - 1) / rows;
+    }
+    int inclusive = tiles;
+#pragma unroll
+    for (int offset = 1; offset < 32; offset <<= 1) {
+      const int other = __shfl_up_sync(0xffffffffu, inclusive, offset);
+      if (lane >= offset) inclusive += other;
+    }
+    const int first = before + inclusive - tiles;            // work index of this sequence's first tile
+    const unsigned owner = __ballot_sync(0xffffffffu, tiles > 0 && work >= first && work < first + tiles);
+    if (owner != 0) {
+      const int src = __ffs(owner) - 1;
+      const int first_of_owner = __shfl_sync(0xffffffffu, first, src);
+      const int tiles_of_owner = __shfl_sync(0xffffffffu, tiles, src);
+      seq_out = base + src;
+      tile_start_out = (tiles_of_owner - 1 - (work - first_of_owner)) * rows;
+      return;
+    }
+    before += __shfl_sync(0xffffffffu, inclusive, 31);
+  }
+}
+
+struct Shared {
+  float k_scale[STAGES][KEYS], v_scale[STAGES][KEYS];
+  int v_top[STAGES][4];   // per 32 keys: the exponent of the largest value scale
+  unsigned long long q_full, q_ready[2], s_full[2], s_read[2], p_full[2][2], pv_done[2][2], pv_last[2], stagger;
+  unsigned long long raw_k_full, raw_k_free, raw_v_full, raw_v_free;
+  unsigned long long k_full[STAGES], k_free[STAGES], v_full[STAGES], v_free[STAGES];
+  unsigned tmem_base;
+  volatile int abort;
+};
+constexpr size_t SMEM = 2 * Q_BYTES + 2 * STAGES * KV_TILE + 2 * RAW_TILE + sizeof(Shared);
+static_assert(SMEM <= 232448, "more than an SM's shared memory");
+
+__device__ __noinline__ void rescale_output_row(unsigned tmem_o, float correction) {
+#pragma unroll
+  for (int c = 0; c < D / 32; ++c) {
+    unsigned o[32];
+    tmem_load32(tmem_o + c * 32, o);
+    tmem_wait_load();
+#pragma unroll
+    for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * correction);
+    tmem_store32(tmem_o + c * 32, o);
+  }
+}
+
+// The converters' share: thread `row` turns its key's codes into a row of float16 in the 128-byte swizzle.
+constexpr int RAW_CHUNKS = D / 16;
+__device__ __forceinline__ void read_codes(const unsigned char* raw, int row, uint4 (&codes)[RAW_CHUNKS]) {
+  // rows of 128 bytes in the 128-byte swizzle, rows of 64 bytes in the 64-byte one
+  const int exchanged = D == 128 ? row & 7 : (row >> 1) & 3;
+#pragma unroll
+  for (int c = 0; c < RAW_CHUNKS; ++c) codes[c] = *reinterpret_cast<const uint4*>(raw + row * D + ((c ^ exchanged) << 4));
+}
+__device__ __forceinline__ void write_halves(unsigned char* tile, int row, const uint4 (&codes)[RAW_CHUNKS]) {
+#pragma unroll
+  for (int c = 0; c < RAW_CHUNKS; ++c) {
+    unsigned char* half = tile + (c / 4) * KV_HALF + row * 128;
+    const unsigned w[4] = {codes[c].x ^ 0x80808080u, codes[c].y ^ 0x80808080u, codes[c].z ^ 0x80808080u, codes[c].w ^ 0x80808080u};
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      *reinterpret_cast<uint4*>(half + (((2 * (c % 4) + i) ^ (row & 7)) << 4)) =
+          make_uint4(codes_to_half<0x4140>(w[2 * i]), codes_to_half<0x4342>(w[2 * i]), codes_to_half<0x4140>(w[2 * i + 1]), codes_to_half<0x4342>(w[2 * i + 1]));
+  }
+}
+
+__global__ void __launch_bounds__(THREADS, 1)
+portions_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                const __grid_constant__ CUtensorMap map_v, const Args args) {
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  const int kv_head = blockIdx.x, split = blockIdx.z;
+  int seq, tile_start;
+  find_work(args, blockIdx.y, 2 * args.tokens, seq, tile_start);           // metadata: written before the step's kernels
+  if (tile_start < 0 || (smem_u32(smem_raw) & 1023u)) {
+    if (tile_start >= 0 && threadIdx.x == 0 && args.status != nullptr) *args.status = ERR_ALIGNMENT;
+    let_dependents_start();
+    wait_for_previous();
+    return;
+  }
+  const int start = args.q_start[seq];
+  const int q_len = args.q_start[seq + 1] - start;
+  unsigned char* q_tiles = smem_raw;                             // [2 chains][Q_BYTES]
+  unsigned char* k_tiles = q_tiles + 2 * Q_BYTES;                // [STAGES][KV_TILE]
+  unsigned char* v_tiles = k_tiles + STAGES * KV_TILE;           // [STAGES][KV_TILE]
+  unsigned char* raw_k = v_tiles + STAGES * KV_TILE;
+  unsigned char* raw_v = raw_k + RAW_TILE;
+  Shared* sh = reinterpret_cast<Shared*>(raw_v + RAW_TILE);
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+
+  const int pos0 = args.ctx_len[seq] - q_len;                   // position of the first new token
+  // chain c owns tokens tile_start + c * tokens ...; tokens_1 <= 0: the later chain has none
+  const int tokens_0 = min(args.tokens, q_len - tile_start), tokens_1 = min(args.tokens, q_len - tile_start - args.tokens);
+  const int lo = first_visible_key(max(pos0 + tile_start, 0), args.window);   // first key any row sees
+  const int hi_0 = pos0 + tile_start + tokens_0 - 1;            // last key chain 0 sees (below 0: none)
+  const int hi_1 = tokens_1 > 0 ? hi_0 + tokens_1 : -1;
+  const int hi = max(hi_0, hi_1);
+  const int tile_hi = hi >= 0 ? hi / KEYS : -1;
+  const int all_tiles = hi >= 0 ? tile_hi - lo / KEYS + 1 : 0;
+  const int per = (all_tiles + args.splits - 1) / args.splits;
+  // this CTA's share: tiles tile_lo ... last_tile (none: an empty split)
+  const int tile_lo = lo / KEYS + split * per;
+  const int last_tile = min(tile_hi, tile_lo + per - 1);
+  const int count_0 = hi_0 >= 0 ? max(0, min(last_tile, hi_0 / KEYS) - tile_lo + 1) : 0;
+  const int count_1 = hi_1 >= 0 ? max(0, min(last_tile, hi_1 / KEYS) - tile_lo + 1) : 0;
+  const int num_tiles = max(count_0, count_1);
+  // the same in steps of 64 keys: a chain's last tile may need its first half only
+  const int steps_0 = count_0 > 0 ? min(2 * count_0, hi_0 / HALF_KEYS - 2 * tile_lo + 1) : 0;
+  const int steps_1 = count_1 > 0 ? min(2 * count_1, hi_1 / HALF_KEYS - 2 * tile_lo + 1) : 0;
+
+  const unsigned users = (steps_0 > 0 ? 1u : 0u) + (steps_1 > 0 ? 1u : 0u);   // chains that read the key and value stages
+  if (threadIdx.x == 0) {
+    mbar_init(&sh->q_full, 1);
+    for (int c = 0; c < 2; ++c) {
+      mbar_init(&sh->q_ready[c], 128);
+      mbar_init(&sh->s_full[c], 1);
+      mbar_init(&sh->s_read[c], 128);
+      for (int b = 0; b < 2; ++b) {
+        mbar_init(&sh->p_full[c][b], 128);
+        mbar_init(&sh->pv_done[c][b], 1);
+      }
+      mbar_init(&sh->pv_last[c], 1);
+    }
+    mbar_init(&sh->raw_k_full, 1);
+    mbar_init(&sh->raw_v_full, 1);
+    mbar_init(&sh->raw_k_free, 128);
+    mbar_init(&sh->raw_v_free, 128);
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&sh->k_full[s], 128);
+      mbar_init(&sh->k_free[s], users > 0 ? users : 1u);
+      mbar_init(&sh->v_full[s], 128);
+      mbar_init(&sh->v_free[s], users > 0 ? users : 1u);
+    }
+    mbar_init(&sh->stagger, 1);
+    sh->abort = 0;
+    mbar_init_fence();
+  }
+  if (warp == 3) tmem_alloc(&sh->tmem_base, TMEM_COLS);
+  fence_before_sync();
+  __syncthreads();
+  fence_after_sync();
+  let_dependents_start();
+  wait_for_previous();   // the query and the newest keys come from the kernel before this one
+
+  if (warp < 4) {
+    fewer_registers<88>();
+    if (warp == 0 || warp == 3) {
+      // Key (warp 0) and value codes (warp 3): lane 0 waits for the buffer and arms its barrier, then lane pg issues the box of
+      // page pg of the tile.  Page ids come a chunk of 32 at a time (lane l: page l of the chunk, several tiles' worth), the next
+      // chunk while this one is used.
+      const bool for_keys = warp == 0;
+      const int* table = args.block_table + static_cast<size_t>(seq) * args.max_blocks;
+      const int pages_per_tile = KEYS / args.page_size;
+      const int nowhere = args.num_pages * args.page_size;      // a row coordinate outside the cache: reads zeros
+      if (for_keys && lane == 0 && num_tiles > 0) {
+        mbar_expect_tx(&sh->q_full, 2 * HALVES * args.tokens * args.group * 128);
+        for (int c = 0; c < 2; ++c)
+          for (int h = 0; h < HALVES; ++h)
+            tma_load_3d(q_tiles + c * Q_BYTES + h * Q_HALF, &map_q, &sh->q_full, h * 64, kv_head * args.group, start + tile_start + c * args.tokens);
+      }
+      const int tiles_per_chunk = 32 / pages_per_tile;
+      auto load_chunk = [&](int chunk) -> int {
+        const int key0 = tile_lo * KEYS + (chunk * 32 + lane) * args.page_size;
+        const int block = key0 / args.page_size;
+        return (chunk * tiles_per_chunk < num_tiles && key0 <= hi && block < args.max_blocks) ? table[block] : -1;
+      };
+      unsigned char* const raw = for_keys ? raw_k : raw_v;
+      unsigned long long* const full = for_keys ? &sh->raw_k_full : &sh->raw_v_full;
+      unsigned long long* const free_again = for_keys ? &sh->raw_k_free : &sh->raw_v_free;
+      const CUtensorMap* const map = for_keys ? &map_k : &map_v;
+      int chunk_pages = load_chunk(0), next_pages = load_chunk(1);
+      int issued = 0;
+      for (int i = 0; i < num_tiles; ++i) {
+        const int within = i % tiles_per_chunk;
+        if (within == 0 && i > 0) {
+          chunk_pages = next_pages;
+          next_pages = load_chunk(i / tiles_per_chunk + 1);
+        }
+        int page = __shfl_sync(0xffffffffu, chunk_pages, within * pages_per_tile + (lane % pages_per_tile));
+        if (page >= args.num_pages) page = -1;
+        const int y = page < 0 ? nowhere : page * args.page_size;
+        int ok = 1;
+        if (lane == 0) {
+          ok = mbar_wait(free_again, (i & 1) ^ 1, &sh->abort, args.status, ERR_PRODUCER) ? 1 : 0;
+          if (ok) mbar_expect_tx(full, RAW_TILE);
+        }
+        ok = __shfl_sync(0xffffffffu, ok, 0);
+        if (!ok) break;
+        if (lane < pages_per_tile) tma_load_2d(raw + lane * args.page_size * D, map, full, kv_head * D, y);
+        issued = i + 1;
+      }
+      if (lane == 0 && sh->abort) {   // copies may still be in flight: wait for what was armed last
+        bool landed = issued == 0;
+        for (unsigned tries = 0; tries < WAIT_LIMIT && !landed; ++tries) landed = mbar_try_wait(full, (issued - 1) & 1);
+        if (!landed && args.status != nullptr) *args.status = ERR_DRAIN;
+        landed = !for_keys || num_tiles <= 0;
+        for (unsigned tries = 0; tries < WAIT_LIMIT && !landed; ++tries) landed = mbar_try_wait(&sh->q_full, 0);
+      }
+    } else {
+      // One issuing warp per chain, as in attention_tcgen05.cu: s_read(h) -> S(h + 1), p_full(h) -> PV(h).
+      const int c = warp - 1;
+      const int steps = c == 0 ? steps_0 : steps_1;
+      if (steps > 0) {
+        const unsigned leader = elect_one();
+        auto wait_for = [&](unsigned long long* bar, unsigned parity) {
+          return __all_sync(0xffffffffu, mbar_wait(bar, parity, &sh->abort, args.status, ERR_MMA)) != 0;
+        };
+        const unsigned idesc_s = half_descriptor(BM, HALF_KEYS, false);
+        const unsigned idesc_o = half_descriptor(BM, D, true);
+        const unsigned tmem_chain = __shfl_sync(0xffffffffu, sh->tmem_base, 0) + c * CHAIN_COLS, tmem_o = tmem_chain + O_COL;
+        const unsigned long long q_base = smem_descriptor(smem_u32(q_tiles + c * Q_BYTES));
+        const unsigned long long k_desc0 = smem_descriptor(smem_u32(k_tiles));
+        const unsigned long long v_desc0 = smem_descriptor(smem_u32(v_tiles), KV_HALF, 1024);
+        bool ok = wait_for(&sh->q_ready[c], 0);
+        int keys_ready = -1, values_ready = -1;   // the newest tile whose keys (values) are known to be there
+        auto issue_scores = [&](int h) {
+          const int i = h >> 1, st = i % STAGES;
+          if (keys_ready < i) {
+            ok = wait_for(&sh->k_full[st], (i / STAGES) & 1);
+            if (!ok) return;
+            keys_ready = i;
+          }
+          fence_after_sync();
+          const unsigned long long k_base = k_desc0 + static_cast<unsigned>((st * KV_TILE + (h & 1) * HALF_KEYS * 128) >> 4);
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk)
+            umma(leader, tmem_chain, q_base + (((kk / 4) * Q_HALF + (kk % 4) * 32) >> 4), k_base + (((kk / 4) * KV_HALF + (kk % 4) * 32) >> 4), idesc_s,
+                 kk > 0 ? 1u : 0u);
+          umma_commit(leader, &sh->s_full[c]);
+          if ((h & 1) || h + 1 == steps) umma_commit(leader, &sh->k_free[st]);
+        };
+        // the later chain starts most of a step behind the earlier one
+        if (ok && c == 1 && steps_0 > 0) ok = wait_for(&sh->stagger, 0);
+        if (ok) issue_scores(0);
+        for (int h = 0; h < steps && ok; ++h) {
+          if (h + 1 < steps) {
+            ok = wait_for(&sh->s_read[c], h & 1);
+            if (!ok) break;
+            issue_scores(h + 1);
+            if (!ok) break;
+          }
+          const int i = h >> 1, st = i % STAGES;
+          if (values_ready < i) {
+            ok = wait_for(&sh->v_full[st], (i / STAGES) & 1);
+            values_ready = i;
+          }
+          if (ok) ok = wait_for(&sh->p_full[c][h & 1], (h >> 1) & 1);
+          if (!ok) break;
+          if (c == 0 && h == 0 && leader) mbar_arrive(&sh->stagger);   // on every path: the other issuer waits for it
+          fence_after_sync();
+          const unsigned long long v_base = v_desc0 + static_cast<unsigned>((st * KV_TILE + (h & 1) * HALF_KEYS * 128) >> 4);
+          const unsigned tmem_p = tmem_chain + P_COL + (h & 1) * 32;
+#pragma unroll
+          for (int kk = 0; kk < HALF_KEYS / 16; ++kk)
+            umma_a_in_tmem(leader, tmem_o, tmem_p + kk * 8, v_base + ((kk * 16 * 128) >> 4), idesc_o, (h > 0 || kk > 0) ? 1u : 0u);
+          umma_commit(leader, &sh->pv_done[c][h & 1]);
+          if (h + 1 == steps) umma_commit(leader, &sh->pv_last[c]);
+          if ((h & 1) || h + 1 == steps) umma_commit(leader, &sh->v_free[st]);
+        }
+      }
+    }
+  } else if (warp >= 12) {
+    // ---- converters: thread `row` owns key `row` of every tile
+    fewer_registers<88>();
+    const int row = threadIdx.x - 384;
+    const int* table = args.block_table + static_cast<size_t>(seq) * args.max_blocks;
+    // the place of this thread's key of tile i among the scales; -1: no such key
+    auto scale_place = [&](int i) -> long long {
+      const int key = (tile_lo + i) * KEYS + row, block = key >> args.page_shift;
+      if (i >= num_tiles || key > hi || block >= args.max_blocks) return -1;
+      const int page = table[block];
+      if (page < 0 || page >= args.num_pages) return -1;
+      return (static_cast<long long>(page) * args.num_kv_heads + kv_head) * args.page_size + (key & (args.page_size - 1));
+    };
+    long long place = scale_place(0);
+    float k_scale = place >= 0 ? args.k_scales[place] : 0.f, v_scale = place >= 0 ? args.v_scales[place] : 0.f;
+    place = scale_place(1);
+    for (int i = 0; i < num_tiles; ++i) {
+      const int st = i % STAGES;
+      const unsigned reuse = ((i / STAGES) & 1) ^ 1;
+      const float next_k = place >= 0 ? args.k_scales[place] : 0.f, next_v = place >= 0 ? args.v_scales[place] : 0.f;
+      place = scale_place(i + 2);
+      uint4 codes[RAW_CHUNKS];
+      bool ok = mbar_wait(&sh->raw_k_full, i & 1, &sh->abort, args.status, ERR_CONVERT);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      read_codes(raw_k, row, codes);
+      mbar_arrive(&sh->raw_k_free);
+      ok = mbar_wait(&sh->k_free[st], reuse, &sh->abort, args.status, ERR_CONVERT);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      write_halves(k_tiles + st * KV_TILE, row, codes);
+      fence_async_shared();
+      mbar_arrive(&sh->k_full[st]);
+      ok = mbar_wait(&sh->raw_v_full, i & 1, &sh->abort, args.status, ERR_CONVERT);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      read_codes(raw_v, row, codes);
+      mbar_arrive(&sh->raw_v_free);
+      ok = mbar_wait(&sh->v_free[st], reuse, &sh->abort, args.status, ERR_CONVERT);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      // the softmax threads have read the scales of the tile that was here: its products are done
+      sh->k_scale[st][row] = k_scale;
+      sh->v_scale[st][row] = v_scale;
+      const unsigned top = __reduce_max_sync(0xffffffffu, finite_bits(v_scale));
+      if (lane == 0) sh->v_top[st][row >> 5] = static_cast<int>(top >> 23) - 127;
+      write_halves(v_tiles + st * KV_TILE, row, codes);
+      fence_async_shared();
+      mbar_arrive(&sh->v_full[st]);
+      k_scale = next_k;
+      v_scale = next_v;
+    }
+  } else {
+    // ---- softmax and epilogue: a thread a row
+    more_registers<168>();
+    const int chain = (warp - 4) >> 2, quarter = warp & 3;
+    const int row = quarter * 32 + lane;
+    const int token = tile_start + chain * args.tokens + row / args.group, head = kv_head * args.group + row % args.group;
+    const bool there = row < args.tokens * args.group && token < q_len;
+    const int my_steps = chain == 0 ? steps_0 : steps_1;
+    // a row that is not there (128 is no multiple of the group, or the portion ends) has zeros for a query and sees what the
+    // chain's last token sees, so that it takes the same turns; nobody reads it
+    const int last = pos0 + min(token, tile_start + chain * args.tokens + (chain == 0 ? tokens_0 : tokens_1) - 1);
+    const int first = first_visible_key(max(last, 0), args.window);
+    const unsigned lane_base = static_cast<unsigned>(quarter * 32) << 16;
+    const unsigned tmem_chain = sh->tmem_base + chain * CHAIN_COLS + lane_base, tmem_o = tmem_chain + O_COL;
+    float most = -INFINITY, base = -INFINITY, row_sum = 0.f, factor = 0.f;
+    int exponent = LEAST_EXPONENT;
+    bool ok = true;
+    if (my_steps > 0) {
+      // the query's row: scaled so that its largest element lies in [2^14, 2^15), then float16
+      ok = mbar_wait(&sh->q_full, 0, &sh->abort, args.status, ERR_SOFTMAX);
+      ok = __all_sync(0xffffffffu, ok);
+      if (ok) {
+        unsigned char* q_row = q_tiles + chain * Q_BYTES + row * 128;
+        unsigned top = 0u;
+#pragma unroll
+        for (int c = 0; c < HALVES * 8; ++c) {
+          const uint4 v = *reinterpret_cast<const uint4*>(q_row + (c / 8) * Q_HALF + (((c % 8) ^ (row & 7)) << 4));
+          const unsigned w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) top = max(top, max(finite_bits(__uint_as_float(w[i] << 16)), finite_bits(__uint_as_float(w[i] & 0xffff0000u))));
+        }
+        const int e = min(max(static_cast<int>(top >> 23) - 127, -100), 126);
+        const float lift = args.scale_log2 < 0.f ? -power_of_two(14 - e) : power_of_two(14 - e);
+        factor = fmaxf(fabsf(args.scale_log2) * power_of_two(e - 14), 1e-38f);   // a hidden key's -inf has to stay one
+#pragma unroll
+        for (int c = 0; c < HALVES * 8; ++c) {
+          uint4* at = reinterpret_cast<uint4*>(q_row + (c / 8) * Q_HALF + (((c % 8) ^ (row & 7)) << 4));
+          const uint4 v = *at;
+          const unsigned w[4] = {v.x, v.y, v.z, v.w};
+          unsigned h[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) h[i] = there ? pack_half(__uint_as_float(w[i] << 16) * lift, __uint_as_float(w[i] & 0xffff0000u) * lift) : 0u;
+          *at = make_uint4(h[0], h[1], h[2], h[3]);
+        }
+        fence_async_shared();
+        mbar_arrive(&sh->q_ready[chain]);
+      }
+    }
+    for (int h = 0; h < my_steps && ok; ++h) {
+      const int st = (h >> 1) % STAGES;
+      if ((h & 1) == 0) {   // the tile's scales
+        ok = mbar_wait(&sh->v_full[st], ((h >> 1) / STAGES) & 1, &sh->abort, args.status, ERR_SOFTMAX);
+      }
+      if (ok) ok = mbar_wait(&sh->s_full[chain], h & 1, &sh->abort, args.status, ERR_SOFTMAX);
+      ok = __all_sync(0xffffffffu, ok);   // the warp stays together: the tensor-memory accesses below are warp-wide
+      if (!ok) break;
+      fence_after_sync();
+      unsigned v[2][32];
+      tmem_load32(tmem_chain, v[0]);
+      tmem_load32(tmem_chain + 32, v[1]);
+      const float* k_scale = sh->k_scale[st] + (h & 1) * HALF_KEYS;
+      const float* v_scale = sh->v_scale[st] + (h & 1) * HALF_KEYS;
+      int top = max(sh->v_top[st][2 * (h & 1)], sh->v_top[st][2 * (h & 1) + 1]);
+      tmem_wait_load();
+      fence_before_sync();
+      mbar_arrive(&sh->s_read[chain]);    // the scores are in registers: their columns may take the next step
+      const int key_base = (tile_lo * 2 + h) * HALF_KEYS;
+      float part_max[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};   // four chains of dependent instructions, not one
+      const bool edge = key_base < first || key_base + HALF_KEYS - 1 > last;   // only steps at the edge of the row's range pay for masking
+#pragma unroll
+      for (int g = 0; g < 2; ++g)
+#pragma unroll
+        for (int j = 0; j < 32; j += 4) {
+          const float4 s = *reinterpret_cast<const float4*>(k_scale + g * 32 + j);
+          float x[4];
+          halves_of(mul_pair(pair_of(__uint_as_float(v[g][j]), __uint_as_float(v[g][j + 1])), pair_of(s.x, s.y)), x[0], x[1]);
+          halves_of(mul_pair(pair_of(__uint_as_float(v[g][j + 2]), __uint_as_float(v[g][j + 3])), pair_of(s.z, s.w)), x[2], x[3]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) v[g][j + i] = __float_as_uint(x[i]);
+        }
+      if (edge) {
+        unsigned top_bits = 0u;
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            const int key = key_base + g * 32 + j;
+            if (key < first || key > last) v[g][j] = 0xff800000u;   // -inf
+            else top_bits = max(top_bits, finite_bits(v_scale[g * 32 + j]));
+          }
+        top = static_cast<int>(top_bits >> 23) - 127;
+      }
+#pragma unroll
+      for (int g = 0; g < 2; ++g)
+#pragma unroll
+        for (int j = 0; j < 32; j += 8)
+#pragma unroll
+          for (int a = 0; a < 4; ++a) part_max[a] = max3(part_max[a], __uint_as_float(v[g][j + 2 * a]), __uint_as_float(v[g][j + 2 * a + 1]));
+      const float step_max = fmaxf(max3(part_max[0], part_max[1], part_max[2]), part_max[3]) * factor;
+      // The base follows the largest score lazily (2^6), and the largest value scale at once: the weights stay below 2^15.
+      float correction = 1.0f;
+      top = min(top - SCALE_BITS, MOST_EXPONENT);
+      if (step_max > most + BASE_LAG || top > exponent || most == -INFINITY) {
+        most = fmaxf(most, step_max);
+        exponent = max(exponent, top);
+        const float next = most + static_cast<float>(exponent);
+        // a row that has seen no key yet has O = 0 and a sum of 0: nothing to rescale
+        correction = base == -INFINITY ? 1.0f : fast_exp2(base - next);
+        base = next;
+      }
+      const float from = base == -INFINITY ? 0.f : base;
+      const unsigned long long factor_pair = pair_of(factor, factor), base_pair = pair_of(-from, -from);
+      unsigned long long sum_pair[2] = {pair_of(0.f, 0.f), pair_of(0.f, 0.f)};
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+#pragma unroll
+        for (int j = 0; j < 32; j += 4) {
+          const float4 s = *reinterpret_cast<const float4*>(v_scale + g * 32 + j);
+#pragma unroll
+          for (int i = 0; i < 4; i += 2) {
+            float x0, x1, w0, w1;
+            halves_of(fma_pair(pair_of(__uint_as_float(v[g][j + i]), __uint_as_float(v[g][j + i + 1])), factor_pair, base_pair), x0, x1);
+            x0 = fast_exp2(x0);
+            x1 = fast_exp2(x1);
+            const unsigned long long p = pair_of(x0, x1);
+            sum_pair[i >> 1] = add_pair(sum_pair[i >> 1], p);
+            halves_of(mul_pair(p, i == 0 ? pair_of(s.x, s.y) : pair_of(s.z, s.w)), w0, w1);
+            if (edge) {   // a key that the row does not see has no part in it, whatever its scale
+              w0 = x0 == 0.f ? 0.f : w0;
+              w1 = x1 == 0.f ? 0.f : w1;
+            }
+            v[0][g * 16 + (j + i) / 2] = pack_half(w0, w1);   // over the scores already used
+          }
+        }
+      }
+      float sum_lo, sum_hi;
+      halves_of(add_pair(sum_pair[0], sum_pair[1]), sum_lo, sum_hi);
+      row_sum = row_sum * correction + (sum_lo + sum_hi);
+      // P(h) goes where P(h - 2) was: the PV of step h - 2 must have read it
+      if (h >= 2) {
+        ok = mbar_wait(&sh->pv_done[chain][h & 1], ((h >> 1) & 1) ^ 1, &sh->abort, args.status, ERR_SOFTMAX);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        fence_after_sync();
+      }
+      tmem_store32(tmem_chain + P_COL + (h & 1) * 32, v[0]);   // keys 2 j and 2 j + 1 of the step in column j
+      if (h > 0 && __any_sync(0xffffffffu, correction != 1.0f)) {
+        // O still takes the step before: wait for its PV, then rescale
+        ok = mbar_wait(&sh->pv_done[chain][(h - 1) & 1], ((h - 1) >> 1) & 1, &sh->abort, args.status, ERR_SOFTMAX);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        fence_after_sync();
+        rescale_output_row(tmem_o, correction);
+      }
+      tmem_wait_store();
+      fence_before_sync();
+      mbar_arrive(&sh->p_full[chain][h & 1]);
+    }
+    if (ok && my_steps > 0) ok = mbar_wait(&sh->pv_last[chain], 0, &sh->abort, args.status, ERR_SOFTMAX);
+    ok = __all_sync(0xffffffffu, ok);
+    fence_after_sync();
+    if (ok) {
+      const size_t token_head = static_cast<size_t>(start + token) * args.num_heads + head;
+      const size_t at = static_cast<size_t>(split) * args.num_tokens * args.num_heads + token_head;
+      if (args.splits > 1 && there) {
+        args.partial_ml[2 * at] = my_steps > 0 ? base : -INFINITY;
+        args.partial_ml[2 * at + 1] = my_steps > 0 ? row_sum : 0.f;
+      }
+      const float inv = row_sum == 0.f ? 0.f : 1.0f / row_sum;   // a row that sees nothing is zeros
+      if (my_steps > 0 || args.splits == 1) {
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+          unsigned o[32];
+          if (my_steps > 0) {
+            tmem_load32(tmem_o + c * 32, o);
+            tmem_wait_load();
+          } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) o[j] = 0u;
+          }
+          if (there && args.splits > 1) {
+            float* dst = args.partial_o + at * D + c * 32;
+#pragma unroll
+            for (int j = 0; j < 32; j += 4) *reinterpret_cast<uint4*>(dst + j) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+          } else if (there) {
+            __nv_bfloat16* dst = args.out + token_head * D + c * 32;
+#pragma unroll
+            for (int j = 0; j < 32; j += 8) {
+              unsigned packed[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                // a row without weight is zeros even where the products left none
+                const float x = row_sum == 0.f ? 0.f : __uint_as_float(o[j + 2 * i]) * inv, y = row_sum == 0.f ? 0.f : __uint_as_float(o[j + 2 * i + 1]) * inv;
+                const __nv_bfloat162 two = __floats2bfloat162_rn(x, y);
+                packed[i] = *reinterpret_cast<const unsigned*>(&two);
+              }
+              *reinterpret_cast<uint4*>(dst + j) = make_uint4(packed[0], packed[1], packed[2], packed[3]);
+            }
+          }
+        }
+      }
+    }
+  }
+  fence_before_sync();
+  __syncthreads();
+  if (warp == 3) {
+    fence_after_sync();
+    tmem_free(sh->tmem_base, TMEM_COLS);
+  }
+}
+
+// Adds up the splits of every query row of the portions: out = sum_s O_s 2^(base_s - M) / sum_s l_s 2^(base_s - M) with M the
+// largest base.  One warp per (token, head), lanes over the splits first (bases and sums), then over the head size.  Tokens of
+// one-token sequences belong to the other kernel and are left alone.
+__global__ void __launch_bounds__(256)
+combine_portions_kernel(const Args args) {
+  let_dependents_start();
+  wait_for_previous();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int token = blockIdx.y * 8 + warp, head = blockIdx.x;
+  if (token >= args.num_tokens) return;
+  const int seq = args.seq_of_token[token];
+  if (args.skip_single && args.q_start[seq + 1] - args.q_start[seq] == 1) return;
+  const size_t token_head = static_cast<size_t>(token) * args.num_heads + head;
+  const size_t slice = static_cast<size_t>(args.num_tokens) * args.num_heads;
+  float m = -INFINITY, l = 0.f;                       // lane s holds split s (at most 32 splits)
+  if (lane < args.splits) {
+    m = args.partial_ml[2 * (lane * slice + token_head)];
+    l = args.partial_ml[2 * (lane * slice + token_head) + 1];
+  }
+  float base = m;
+#pragma unroll
+  for (int offset = 16; offset > 0; offset >>= 1) base = fmaxf(base, __shfl_xor_sync(0xffffffffu, base, offset));
+  const float weight = m == -INFINITY ? 0.f : fast_exp2(m - base);   // a split that saw no key of this row has base -inf
+  float total = weight == 0.f ? 0.f : l * weight;
+#pragma unroll
+  for (int offset = 16; offset > 0; offset >>= 1) total += __shfl_xor_sync(0xffffffffu, total, offset);
+  float acc[D / 32];
+#pragma unroll
+  for (int c = 0; c < D / 32; ++c) acc[c] = 0.f;
+  for (int s = 0; s < args.splits; ++s) {
+    const float w = __shfl_sync(0xffffffffu, weight, s);
+    if (w == 0.f) continue;                           // its output row may never have been written
+    const float* src = args.partial_o + (s * slice + token_head) * D;
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) acc[c] += src[c * 32 + lane] * w;
+  }
+  const float inv = total == 0.f ? 0.f : 1.0f / total;
+  __nv_bfloat16* dst = args.out + token_head * D;
+#pragma unroll
+  for (int c = 0; c < D / 32; ++c) dst[c * 32 + lane] = __float2bfloat16_rn(acc[c] * inv);
+}
+
+// Tensor maps, kept by what they describe (host only).
+struct Key {
+  const void* base;
+  long long rows;
+  int a, b, c;
+  bool operator==(const Key& o) const { return base == o.base && rows == o.rows && a == o.a && b == o.b && c == o.c; }
+};
+struct KeyHash {
+  size_t operator()(const Key& k) const {
+    size_t h = reinterpret_cast<size_t>(k.base);
+    for (const long long v : {k.rows, static_cast<long long>(k.a), static_cast<long long>(k.b), static_cast<long long>(k.c)}) h = h * 1000003u ^ static_cast<size_t>(v);
+    return h;
+  }
+};
+template <typename Encode>
+static int kept_map(const Key& key, CUtensorMap* out, Encode&& encode) {
+  static std::mutex mutex;
+  static std::unordered_map<Key, CUtensorMap, KeyHash> cache;
+  std::lock_guard<std::mutex> guard(mutex);
+  const auto found = cache.find(key);
+  if (found != cache.end()) {
+    *out = found->second;
+    return SHRIKE_OK;
+  }
+  EncodeTiled fn = encode_tiled();
+  if (fn == nullptr) return SHRIKE_BAD_ARGUMENT;
+  const CUresult rc = encode(fn, out);
+  if (rc != CUDA_SUCCESS) return 1000 + static_cast<int>(rc);
+  if (cache.size() > 4096) cache.clear();
+  cache.emplace(key, *out);
+  return SHRIKE_OK;
+}
+// Codes [rows, cols bytes] as boxes of `box_rows` rows of D bytes, in the swizzle of that row length.
+static int map_codes(const void* base, long long rows, int cols, int box_rows, CUtensorMap* out) {
+  return kept_map(Key{base, rows, cols, box_rows, 1}, out, [&](EncodeTiled fn, CUtensorMap* map) {
+    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)}, strides[1] = {static_cast<cuuint64_t>(cols)};
+    const cuuint32_t box[2] = {D, static_cast<cuuint32_t>(box_rows)}, steps[2] = {1, 1};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  });
+}
+// Queries [tokens, heads, D] as boxes of `box_tokens` tokens, `group` heads and 64 elements in the 128-byte swizzle.
+static int map_queries(const void* base, long long tokens, int heads, int group, int box_tokens, CUtensorMap* out) {
+  return kept_map(Key{base, tokens, heads, group, 2}, out, [&](EncodeTiled fn, CUtensorMap* map) {
+    const cuuint64_t dims[3] = {D, static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(tokens)};
+    const cuuint64_t strides[2] = {D * 2, static_cast<cuuint64_t>(heads) * D * 2};
+    const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(group), static_cast<cuuint32_t>(box_tokens)}, steps[3] = {1, 1, 1};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  });
+}
+
+}  // namespace tcq8
+
+// Tokens of a query tile for groups of `group` heads a kv head: what the caller counts the portions' tiles in; 0: not served.
+SHRIKE_API int shrike_attention_q8_tc_tokens(int group) { return group >= 1 && group <= 64 ? 2 * (tcq8::BM / group) : 0; }
+
+// How many CTAs should share the keys of a query tile, for a batch whose portions make `tiles` query tiles over block tables of
+// `keys` keys: the GPU holds one CTA per SM, and splitting pays while every CTA still starts at once.  Among the counts that
+// keep the launch to one round, with at least two key tiles a split and at most 32, the one with the fewest tiles a CTA,
+// counting two tiles' worth for a CTA's start and two more for the second kernel that adds the splits up.
+SHRIKE_API int shrike_attention_q8_tc_splits(int tiles, int num_kv_heads, long long keys) {
+  const long long ctas = static_cast<long long>(num_kv_heads) * tiles, capacity = shrike_device().sm_count;
+  const long long key_tiles = (keys + tcq8::KEYS - 1) / tcq8::KEYS;
+  int best = 1;
+  long long best_cost = -1;
+  for (int s = 1; s <= 32 && (s == 1 || (key_tiles / s >= 2 && ctas * s <= capacity)); ++s) {
+    const long long cost = (key_tiles + s - 1) / s + 2 + (s > 1 ? 2 : 0);
+    if (best_cost < 0 || cost < best_cost) {
+      best_cost = cost;
+      best = s;
+    }
+  }
+  return best;
+}
+
+// Portions (q_len > 1) of a batch; entries with q_len == 1 are skipped when skip_single.  `tiles`: the query tiles of
+// shrike_attention_q8_tc_tokens(group) tokens that they make.  splits > 1 needs `scratch`, splits * num_tokens * num_heads *
+// (D + 2) floats, and `seq_of_token`.
+SHRIKE_API int shrike_paged_attention_q8_tc(const void* q, const void* k_codes, const float* k_scales, const void* v_codes,
+                                            const float* v_scales, const int* block_table, int max_blocks, const int* q_start,
+                                            const int* ctx_len, const int* seq_of_token, int num_tokens, int num_seqs, int num_heads,
+                                            int num_kv_heads, int page_size, int num_pages, float scale, int window, void* out,
+                                            int skip_single, int tiles, int splits, float* scratch, int* status, cudaStream_t stream) {
+  using namespace tcq8;
+  if (num_seqs <= 0 || num_tokens <= 0 || tiles <= 0) return SHRIKE_OK;
+  if (num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads || num_heads / num_kv_heads > 64 || max_blocks <= 0 || num_pages <= 0 ||
+      tiles > 65535 || !(page_size == 8 || page_size == 16 || page_size == 32 || page_size == 64) || splits < 1 || splits > 32 ||
+      static_cast<long long>(num_pages) * page_size > 0x7fffffff || static_cast<long long>(max_blocks) * page_size > 0x7fffffff - 4096 ||
+      (splits > 1 && (scratch == nullptr || seq_of_token == nullptr)) ||
+      (reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(k_codes) |
+       reinterpret_cast<uintptr_t>(v_codes) | reinterpret_cast<uintptr_t>(scratch)) % 16)
+    return SHRIKE_BAD_ARGUMENT;
+  static PerDevice raised;
+  const int raise_rc = shrike_raise_smem(raised, portions_kernel, SMEM);
+  if (raise_rc != 0) return raise_rc;
+  const int group = num_heads / num_kv_heads;
+  CUtensorMap map_q, map_k, map_v;
+  int rc = map_queries(q, num_tokens, num_heads, group, BM / group, &map_q);
+  if (rc != SHRIKE_OK) return rc;
+  rc = map_codes(k_codes, static_cast<long long>(num_pages) * page_size, num_kv_heads * D, page_size, &map_k);
+  if (rc != SHRIKE_OK) return rc;
+  rc = map_codes(v_codes, static_cast<long long>(num_pages) * page_size, num_kv_heads * D, page_size, &map_v);
+  if (rc != SHRIKE_OK) return rc;
+  Args args;
+  args.k_scales = k_scales;
+  args.v_scales = v_scales;
+  args.block_table = block_table;
+  args.q_start = q_start;
+  args.ctx_len = ctx_len;
+  args.out = static_cast<__nv_bfloat16*>(out);
+  args.status = status;
+  args.max_blocks = max_blocks;
+  args.num_heads = num_heads;
+  args.num_kv_heads = num_kv_heads;
+  args.page_size = page_size;
+  args.page_shift = __builtin_ctz(page_size);
+  args.num_pages = num_pages;
+  args.window = window;
+  args.skip_single = skip_single;
+  args.group = group;
+  args.tokens = BM / group;
+  args.scale_log2 = scale * LOG2E;
+  args.splits = splits;
+  args.num_tokens = num_tokens;
+  args.num_seqs = num_seqs;
+  args.seq_of_token = seq_of_token;
+  args.partial_o = splits > 1 ? scratch : nullptr;   // rows first (16-byte stores), then the (base, sum) pairs
+  args.partial_ml = splits > 1 ? scratch + static_cast<long long>(splits) * num_tokens * num_heads * D : nullptr;
+  cudaError_t err = launch_dependent(portions_kernel, dim3(num_kv_heads, tiles, splits), dim3(THREADS), SMEM, stream, map_q, map_k, map_v, args);
+  if (err != cudaSuccess) return static_cast<int>(err);
+  if (splits > 1) {
+    err = launch_dependent(combine_portions_kernel, dim3(num_heads, (num_tokens + 7) / 8), dim3(256), 0, stream, args);
+    if (err != cudaSuccess) return static_cast<int>(err);
+  }
+  return shrike_launch_status();
+}
+
+#else  // other head sizes: the mma.sync kernel serves them
+
+SHRIKE_API int shrike_attention_q8_tc_tokens(int) { return 0; }
+SHRIKE_API int shrike_attention_q8_tc_splits(int, int, long long) { return 1; }
+SHRIKE_API int shrike_paged_attention_q8_tc(const void*, const void*, const float*, const void*, const float*, const int*, int, const int*,
+                                            const int*, const int*, int, int, int, int, int, int, float, int, void*, int, int, int,
+                                            float*, int*, cudaStream_t) {
+  return SHRIKE_BAD_ARGUMENT;
+}
+
+#endif

@@ -165,7 +165,7 @@ def load_library(name: str, sources, defines=None, extra_flags=()) -> ctypes.CDL
 # The libraries of this package.
 CORE_SOURCES = ["elementwise.cu", "branch_ops.cu", "parallel_ops.cu", "decay_ops.cu", "stream_ops.cu", "delta_ops.cu", "gemm_fp32.cu", "sampling.cu", "cache_q8.cu"]
 ATTENTION_SOURCES = ["attention_fp32.cu", "attention_bf16.cu", "attention_tcgen05.cu"]
-ATTENTION_Q8_SOURCES = ["attention_q8.cu"]
+ATTENTION_Q8_SOURCES = ["attention_q8.cu", "attention_q8_tcgen05.cu"]
 
 
 def core_library() -> ctypes.CDLL:

@@ -75,6 +75,7 @@ _LIMITS = {
     "kv_write_q8": "heads of 16 to 256 elements in sixteens, codes on 16-byte borders",
     "rope_kv_write_q8": "heads of 16 to 256 elements in sixteens, codes on 16-byte borders",
     "kv_read_q8": "heads in sixteens, codes and outputs on 16-byte borders",
+    "paged_attention_q8_tc": "at most 65535 query tiles, groups of at most 64 heads, everything on 16-byte borders",
     "paged_attention_q8": "at most 65535 sequences and kv heads, heads a multiple of kv heads, everything on 16-byte borders",
     "paged_attention_bf16": "at most 65535 sequences and heads, heads a multiple of kv heads, at most 32 splits",
 }
@@ -652,6 +653,12 @@ class CudaOps(QuantisedCacheOps):
             51: "decode_step: the weight stream's wait for a free stage ran out",
             52: "decode_step: a warp's wait for a loaded stage ran out",
             53: "decode_step: the wait for another CTA's values ran out",
+            61: "attention_q8_tcgen05: the loader's wait for a free buffer of codes ran out",
+            62: "attention_q8_tcgen05: a converting thread's wait ran out",
+            63: "attention_q8_tcgen05: the MMA issuer's wait ran out",
+            64: "attention_q8_tcgen05: a softmax thread's wait ran out",
+            65: "attention_q8_tcgen05: copies still in flight after an aborted wait",
+            66: "attention_q8_tcgen05: shared memory was not aligned as the tiles need",
             54: "decode_step: copies still in flight after an aborted wait",
             31: "sampling: a row of logits had no finite element (NaN logits); token 0 was returned for it",
         }
@@ -738,7 +745,7 @@ class CudaOps(QuantisedCacheOps):
             if chunk and window:
                 raise KernelError("attention takes a window or a chunk, not both")
             self._paged_attention_q8(q, keys, values, block_table, q_start, ctx_len, seq_of_token, num_heads, num_kv_heads, head_dim,
-                                     scale, -int(chunk) if chunk else window, out, max_q_len, min_q_len)
+                                     scale, -int(chunk) if chunk else window, out, max_q_len, min_q_len, q_lens)
             return
         _dense(q, self.dtype, "q")
         if sinks is not None:

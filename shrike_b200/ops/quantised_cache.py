@@ -27,10 +27,14 @@ class QuantisedPlan:
 
     has_single: bool      # entries of one token run on the form for few rows
     has_portions: bool    # longer ones on the form for many
+    tc_portions: bool     # which is the tcgen05 kernel, else the mma.sync one
     splits: int           # CTAs that share the keys of a row tile of the former
     cluster: int          # how many of them form a thread-block cluster
     scratch: torch.Tensor | None
     arrivals: torch.Tensor | None
+    tiles: int = 0        # query tiles that the tcgen05 kernel's portions make
+    portion_splits: int = 1   # CTAs that share the keys of one
+    portion_scratch: torch.Tensor | None = None
 
 
 def _error(text):
@@ -59,7 +63,7 @@ class QuantisedCacheOps:
         for name in ("shrike_kv_write_q8", "shrike_rope_kv_write_q8", "shrike_kv_read_q8"):
             getattr(lib, name).restype = _I
         self._q8_libs, self._q8_plans = {}, {}
-        self._q8_scratch = self._q8_arrivals = None
+        self._q8_scratch = self._q8_arrivals = self._q8_portion_scratch = None
         self.q8_splits = None   # None: the rule of `q8_few_row_splits`; (splits, cluster) for few rows (tests)
 
     def _q8_lib(self, head_dim: int):
@@ -68,8 +72,13 @@ class QuantisedCacheOps:
             if head_dim % 16 or not 16 <= head_dim <= MOST_HEAD_DIM:
                 raise _error(f"head size {head_dim} is not served: 8-bit pages take multiples of 16 from 16 to {MOST_HEAD_DIM}")
             lib = build.attention_q8_library(head_dim)
-            lib.shrike_paged_attention_q8.argtypes = [_P] * 6 + [_I, _P, _P] + [_I] * 6 + [_F, _I, _P] + [_I] * 5 + [_P, _P, _P]
+            lib.shrike_paged_attention_q8.argtypes = [_P] * 6 + [_I, _P, _P] + [_I] * 6 + [_F, _I, _P] + [_I] * 6 + [_P, _P, _P]
             lib.shrike_paged_attention_q8.restype = _I
+            lib.shrike_paged_attention_q8_tc.argtypes = [_P] * 6 + [_I] + [_P] * 3 + [_I] * 6 + [_F, _I, _P] + [_I] * 3 + [_P] * 3
+            lib.shrike_attention_q8_tc_tokens.argtypes = [_I]
+            lib.shrike_attention_q8_tc_splits.argtypes = [_I, _I, _LL]
+            for name in ("shrike_paged_attention_q8_tc", "shrike_attention_q8_tc_tokens", "shrike_attention_q8_tc_splits"):
+                getattr(lib, name).restype = _I
             for name in ("row_floats", "max_splits"):
                 getattr(lib, f"shrike_attention_q8_{name}").argtypes = []
                 getattr(lib, f"shrike_attention_q8_{name}").restype = _I
@@ -210,10 +219,13 @@ class QuantisedCacheOps:
             k_at, v_at, self.code, n, heads, dim, page_size, pages * page_size, stream), "kv_read_q8")
 
     # ---- attention
-    def q8_plan(self, num_heads, num_kv_heads, head_dim, num_seqs, max_blocks, page_size, max_q_len, min_q_len, window=0) -> QuantisedPlan:
+    def q8_plan(self, num_heads, num_kv_heads, head_dim, num_seqs, max_blocks, page_size, max_q_len, min_q_len, window=0, num_tokens=0,
+                q_lens=None) -> QuantisedPlan:
         """How a batch over 8-bit pages is cut: a function of its shape alone, so that a captured launch sequence serves every
-        batch of that shape."""
-        key = (num_heads, num_kv_heads, head_dim, num_seqs, max_blocks, page_size, max_q_len > 1, min_q_len <= 1, window, self.q8_splits)
+        batch of that shape.  `q_lens`: every entry's length, if they are known."""
+        shape = (num_tokens, tuple(q_lens) if q_lens is not None else None) if max_q_len > 1 else None
+        key = (num_heads, num_kv_heads, head_dim, num_seqs, max_blocks, page_size, min_q_len <= 1, window, shape, self.q8_splits,
+               self.tensor_core_attention, self.portion_splits)
         held = self._q8_plans.get(key)
         if held is not None and held[0] == self.generation:   # the scratch has not moved since
             return held[1]
@@ -243,7 +255,25 @@ class QuantisedCacheOps:
                     self._q8_arrivals = torch.zeros(max(pairs, 4096), dtype=torch.int32, device=self.device)
                     self.generation += 1
                 scratch, arrivals = self._q8_scratch, self._q8_arrivals
-        plan = QuantisedPlan(has_single, has_portions, splits, cluster, scratch, arrivals)
+        tc_portions, tiles, portion_splits, portion_scratch = False, 0, 1, None
+        rows = lib.shrike_attention_q8_tc_tokens(num_heads // num_kv_heads)
+        if (has_portions and rows and self.tensor_core_attention and self.dtype == torch.bfloat16 and page_size in (8, 16, 32, 64)
+                and num_tokens > 0):
+            tc_portions = True
+            if q_lens is not None:
+                tiles = sum(-(-q // rows) for q in q_lens if q > 1 or not has_single)
+            else:   # lengths that are not known: what the tokens can make at most
+                tiles = num_tokens // rows + num_seqs
+            portion_splits = self.portion_splits or lib.shrike_attention_q8_tc_splits(tiles, num_kv_heads, max_blocks * page_size)
+            each = num_tokens * num_heads * (head_dim + 2)
+            portion_splits = max(1, min(portion_splits, 32, self.PORTION_SCRATCH_FLOATS // each))
+            if portion_splits > 1:
+                need = portion_splits * each
+                if self._q8_portion_scratch is None or self._q8_portion_scratch.numel() < need:
+                    self._q8_portion_scratch = torch.empty(max(need, 1 << 22), dtype=torch.float32, device=self.device)
+                    self.generation += 1
+                portion_scratch = self._q8_portion_scratch
+        plan = QuantisedPlan(has_single, has_portions, tc_portions, splits, cluster, scratch, arrivals, tiles, portion_splits, portion_scratch)
         if len(self._q8_plans) >= 4096:
             self._q8_plans.clear()
         self._q8_plans[key] = (self.generation, plan)
@@ -266,7 +296,7 @@ class QuantisedCacheOps:
         return best, min(best, 8)
 
     def _paged_attention_q8(self, q, keys, values, block_table, q_start, ctx_len, seq_of_token, num_heads, num_kv_heads, head_dim,
-                            scale, window, out, max_q_len, min_q_len):
+                            scale, window, out, max_q_len, min_q_len, q_lens):
         from .cuda_ops import _check, _ptr
 
         device, stream = self._q8_stream()
@@ -290,10 +320,22 @@ class QuantisedCacheOps:
             raise _error(f"q {list(q.shape)} and output {list(out.shape)} must be [tokens, {num_heads * head_dim}]")
         if n == 0 or num_seqs == 0:
             return
-        plan = self.q8_plan(num_heads, num_kv_heads, head_dim, num_seqs, max_blocks, page_size, max_q_len, min_q_len, window or 0)
-        self.launches += plan.has_single + plan.has_portions
-        _check(self._q8_libs[head_dim].shrike_paged_attention_q8(
-            q_at, keys.codes.data_ptr(), keys.scales.data_ptr(), values.codes.data_ptr(), values.scales.data_ptr(),
-            block_table.data_ptr(), max_blocks, q_start.data_ptr(), ctx_len.data_ptr(), self.code, num_seqs, num_heads, num_kv_heads,
-            page_size, pages, scale, window or 0, out_at, plan.has_single, plan.has_portions, max_q_len, plan.splits, plan.cluster,
-            _ptr(plan.scratch), _ptr(plan.arrivals), stream), "paged_attention_q8")
+        plan = self.q8_plan(num_heads, num_kv_heads, head_dim, num_seqs, max_blocks, page_size, max_q_len, min_q_len, window or 0, n, q_lens)
+        lib, has_portions = self._q8_libs[head_dim], plan.has_portions
+        pages_at = (keys.codes.data_ptr(), keys.scales.data_ptr(), values.codes.data_ptr(), values.scales.data_ptr(), block_table.data_ptr(),
+                    max_blocks, q_start.data_ptr(), ctx_len.data_ptr())
+        self.launches += plan.has_single + has_portions + (plan.portion_splits > 1)
+        if plan.tc_portions:
+            if not self._q8_ints_fit(device, seq_of_token, n):
+                self._q8_refuse(device, (), [(seq_of_token, n, "sequences of tokens")])
+            _check(lib.shrike_paged_attention_q8_tc(
+                q_at, *pages_at, seq_of_token.data_ptr(), n, num_seqs, num_heads, num_kv_heads, page_size, pages, scale, window or 0,
+                out_at, plan.has_single, plan.tiles, plan.portion_splits, _ptr(plan.portion_scratch), self.status.data_ptr(), stream),
+                "paged_attention_q8_tc")
+            has_portions = False
+            if not plan.has_single:
+                return
+        _check(lib.shrike_paged_attention_q8(
+            q_at, *pages_at, self.code, num_seqs, num_heads, num_kv_heads, page_size, pages, scale, window or 0, out_at, plan.has_single,
+            has_portions, max_q_len, 1 if plan.tc_portions else 0, plan.splits, plan.cluster, _ptr(plan.scratch), _ptr(plan.arrivals), stream),
+            "paged_attention_q8")

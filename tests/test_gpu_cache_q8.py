@@ -139,9 +139,10 @@ def attend(ops, case, heads, kv_heads, dim, q_lens, ctx_lens, window=None, chunk
     return out
 
 
-def check_attention(dtype, heads, kv_heads, dim, page, q_lens, ctx_lens, seed=0, q_scale=1.0, splits=None, known=True, **options):
+def check_attention(dtype, heads, kv_heads, dim, page, q_lens, ctx_lens, seed=0, q_scale=1.0, splits=None, known=True, tensor_cores=True,
+                    portion_splits=0, **options):
     ops = cuda_ops(dtype)
-    ops.q8_splits = splits
+    ops.q8_splits, ops.tensor_core_attention, ops.portion_splits = splits, tensor_cores, portion_splits
     case = oracle.pages_case(heads, kv_heads, dim, page, q_lens, ctx_lens, dtype, seed, DEV, q_scale)
     got = attend(ops, case, heads, kv_heads, dim, q_lens, ctx_lens, known=known, **options)
     scale = options.pop("scale", None)
@@ -152,6 +153,7 @@ def check_attention(dtype, heads, kv_heads, dim, page, q_lens, ctx_lens, seed=0,
     assert excess.max().item() <= 0, f"off by {excess.max().item():.3e} more than the bound at {divmod(int(excess.argmax()), heads * dim)}"
     again = attend(ops, case, heads, kv_heads, dim, q_lens, ctx_lens, known=known, scale=scale, **options)
     assert torch.equal(got, again)   # no result depends on who comes first
+    ops.check_status()
 
 
 HEADS = [(7, 1, 128, 16), (14, 2, 64, 16), (6, 3, 32, 8), (4, 2, 16, 5), (40, 8, 128, 64), (17, 1, 48, 7), (2, 2, 256, 16), (33, 1, 80, 1)]
@@ -177,7 +179,15 @@ def test_single_tokens_in_any_number_of_splits(dtype, splits, options):
 @pytest.mark.parametrize("options", [{}, {"window": 40}, {"chunk": 48}])
 def test_portions(dtype, heads, kv_heads, dim, page, options):
     q_lens, ctx_lens = [2, 5, 33, 64, 70, 130, 3], [2, 40, 33, 129, 300, 130, 517]
-    check_attention(dtype, heads, kv_heads, dim, page, q_lens, ctx_lens, seed=dim, **options)
+    check_attention(dtype, heads, kv_heads, dim, page, q_lens, ctx_lens, seed=dim, tensor_cores=False, **options)
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,page", [(7, 1, 128, 16), (14, 2, 64, 8), (40, 8, 128, 64), (2, 2, 64, 32), (64, 1, 128, 16), (25, 1, 64, 16)])
+@pytest.mark.parametrize("splits", [1, 2, 5])
+@pytest.mark.parametrize("options", [{}, {"window": 40}, {"window": 300}, {"chunk": 48}])
+def test_portions_on_tcgen05_in_any_number_of_splits(heads, kv_heads, dim, page, splits, options):
+    q_lens, ctx_lens = [2, 40, 129, 300, 64, 17], [2, 600, 129, 420, 1111, 128]
+    check_attention(torch.bfloat16, heads, kv_heads, dim, page, q_lens, ctx_lens, seed=dim, portion_splits=splits, **options)
 
 
 @pytest.mark.parametrize("dtype", TYPES)
