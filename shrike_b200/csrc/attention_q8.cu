@@ -287,6 +287,19 @@ struct Rows {
     }
   }
 
+  // Hides from two rows the keys that they do not see, and finds the largest value scale of the others.
+  static __device__ __forceinline__ void hide(float (&s)[2][4], int key0, int g, const int (&first)[2], const int (&last)[2], const float (&v_scale)[4],
+                                           unsigned (&top)[2]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const int key = key0 + 8 * j + key_of(g);
+        if (key >= first[r] && key <= last[r]) top[r] = max(top[r], finite_bits(v_scale[j]));
+        else s[j >> 1][2 * (j & 1) + r] = -INFINITY;
+      }
+  }
+
   using Weights = unsigned[NT][2][2][PARTS];   // [16 keys][eight of them]: operands of the second product
 
   // The weights of the 32 keys from `key0` on, whose codes and scales lie in `k_stage`.
@@ -357,8 +370,9 @@ struct Rows {
     // the largest of this lane's value scales (negative ones, infinities and NaN, none of which a store leaves but the last,
     // order above all finite bits)
     unsigned all_top = max(max(__float_as_uint(v_scale[0]), __float_as_uint(v_scale[1])), max(__float_as_uint(v_scale[2]), __float_as_uint(v_scale[3])));
+    const bool odd_scale = all_top >= 0x7f800000u, careful = edge && __any_sync(0xffffffffu, odd_scale);
     if (edge) all_top = 0u;
-    else if (all_top >= 0x7f800000u) all_top = max(max(finite_bits(v_scale[0]), finite_bits(v_scale[1])), max(finite_bits(v_scale[2]), finite_bits(v_scale[3])));
+    else if (odd_scale) all_top = max(max(finite_bits(v_scale[0]), finite_bits(v_scale[1])), max(finite_bits(v_scale[2]), finite_bits(v_scale[3])));
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       float largest[2] = {-INFINITY, -INFINITY};
@@ -366,16 +380,12 @@ struct Rows {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          float& z = s[nt][j >> 1][2 * (j & 1) + r];
-          z *= k_scale[j];
-          if (edge) {
-            const int key = key0 + 8 * j + key_of(g);
-            if (key >= first[nt][r] && key <= last[nt][r]) top[r] = max(top[r], finite_bits(v_scale[j]));
-            else z = -INFINITY;
-          }
-          largest[r] = fmaxf(largest[r], z);
-        }
+        for (int r = 0; r < 2; ++r) s[nt][j >> 1][2 * (j & 1) + r] *= k_scale[j];
+      if (edge) hide(s[nt], key0, g, first[nt], last[nt], v_scale, top);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) largest[r] = fmaxf(largest[r], s[nt][j >> 1][2 * (j & 1) + r]);
       // the base moves only where a score or a value scale has outgrown it
       bool stays = true;
 #pragma unroll
@@ -417,7 +427,7 @@ struct Rows {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         float x = p[j][0] * v_scale[j], y = p[j][1] * v_scale[j];
-        if (edge) {   // a key that a row does not see has no part in it, whatever its scale
+        if (careful) {   // a key that a row does not see has no part in it, not even a scale of NaN
           x = p[j][0] == 0.f ? 0.f : x;
           y = p[j][1] == 0.f ? 0.f : y;
         }

@@ -180,6 +180,7 @@ __device__ __forceinline__ void find_work(const Args& args, int work, int rows, 
 struct Shared {
   float k_scale[STAGES][KEYS], v_scale[STAGES][KEYS];
   int v_top[STAGES][4];   // per 32 keys: the exponent of the largest value scale
+  int v_bad[STAGES][4];   // whether one of them is no finite number
   unsigned long long q_full, q_ready[2], s_full[2], s_read[2], p_full[2][2], pv_done[2][2], pv_last[2], stagger;
   unsigned long long raw_k_full, raw_k_free, raw_v_full, raw_v_free;
   unsigned long long k_full[STAGES], k_free[STAGES], v_full[STAGES], v_free[STAGES];
@@ -456,7 +457,11 @@ portions_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       sh->k_scale[st][row] = k_scale;
       sh->v_scale[st][row] = v_scale;
       const unsigned top = __reduce_max_sync(0xffffffffu, finite_bits(v_scale));
-      if (lane == 0) sh->v_top[st][row >> 5] = static_cast<int>(top >> 23) - 127;
+      const bool bad = __any_sync(0xffffffffu, !(fabsf(v_scale) < INFINITY));
+      if (lane == 0) {
+        sh->v_top[st][row >> 5] = static_cast<int>(top >> 23) - 127;
+        sh->v_bad[st][row >> 5] = bad ? 1 : 0;
+      }
       write_halves(v_tiles + st * KV_TILE, row, codes);
       fence_async_shared();
       mbar_arrive(&sh->v_full[st]);
@@ -590,12 +595,16 @@ portions_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
             const unsigned long long p = pair_of(x0, x1);
             sum_pair[i >> 1] = add_pair(sum_pair[i >> 1], p);
             halves_of(mul_pair(p, i == 0 ? pair_of(s.x, s.y) : pair_of(s.z, s.w)), w0, w1);
-            if (edge) {   // a key that the row does not see has no part in it, whatever its scale
-              w0 = x0 == 0.f ? 0.f : w0;
-              w1 = x1 == 0.f ? 0.f : w1;
-            }
             v[0][g * 16 + (j + i) / 2] = pack_half(w0, w1);   // over the scores already used
           }
+        }
+      }
+      if (edge && (sh->v_bad[st][2 * (h & 1)] | sh->v_bad[st][2 * (h & 1) + 1])) {   // rare: a key that the row does not see has no part in it, not even a scale of NaN
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+          const int key = key_base + 2 * j;
+          if (key < first || key > last) v[0][j] &= 0xffff0000u;
+          if (key + 1 < first || key + 1 > last) v[0][j] &= 0x0000ffffu;
         }
       }
       float sum_lo, sum_hi;
