@@ -50,6 +50,21 @@ __device__ __forceinline__ float largest(float a, float b) {
   return m;
 }
 
+// Eight elements with 16-byte stores.
+__device__ __forceinline__ void store8(float* p, const float (&x)[8]) {
+  reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
+  reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
+}
+__device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&x)[8]) {
+  unsigned w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __nv_bfloat162 two = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+    w[i] = *reinterpret_cast<const unsigned*>(&two);
+  }
+  *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
 struct Pages {
   signed char* codes;
   float* scales;
@@ -192,32 +207,51 @@ rope_kv_write_q8_kernel(const float* __restrict__ qkv, const float* __restrict__
 }
 
 // ---- reading back
-// Four elements a thread and turn: 4 bytes of codes, 8 or 16 bytes out.
+// A thread takes 16 codes of a key and the 16 of its value: two 16-byte loads that do not wait for one another, two to four
+// 16-byte stores each.  Bound by memory.
+template <typename T> __device__ __forceinline__ void read_chunk(const Pages& from, long long row, long long scale_at, int within, T* out) {
+  uint4 words = make_uint4(0u, 0u, 0u, 0u);
+  float scale = 0.f;
+  if (row >= 0) {
+    words = __ldg(reinterpret_cast<const uint4*>(from.codes + row + within));
+    scale = __ldg(from.scales + scale_at);
+  }
+  const unsigned w[4] = {words.x, words.y, words.z, words.w};
+#pragma unroll
+  for (int i = 0; i < 4; i += 2) {
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = __fmul_rn(static_cast<float>(static_cast<signed char>(w[i + e / 4] >> (8 * (e % 4)))), scale);
+    store8(out + 4 * i, x);
+  }
+}
 template <typename T>
 __global__ void __launch_bounds__(256)
 kv_read_q8_kernel(const Pages keys, const Pages values, const int* __restrict__ slots, T* __restrict__ k_out, T* __restrict__ v_out,
-                  long long quads, int kv_heads, int dim, int page_size, long long num_slots) {
+                  long long chunks, unsigned per_row, int kv_heads, int dim, int page_size, long long num_slots) {
   let_dependents_start();
   wait_for_previous();
-  const int per_head = dim / 4;
-  for (long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; i < 2 * quads;
-       i += static_cast<long long>(gridDim.x) * blockDim.x) {
-    const bool is_value = i >= quads;
-    const long long at = is_value ? i - quads : i;
-    const int within = static_cast<int>(at % per_head);
-    const long long row = at / per_head, token = row / kv_heads;
-    const int head = static_cast<int>(row % kv_heads);
-    const long long slot = slots[token];
-    float x[4] = {0.f, 0.f, 0.f, 0.f};
-    if (slot >= 0 && slot < num_slots) {
-      const Pages& from = is_value ? values : keys;
-      const unsigned word = *reinterpret_cast<const unsigned*>(from.codes + (slot * kv_heads + head) * dim + within * 4);
-      const float scale = from.scales[(slot / page_size * kv_heads + head) * page_size + slot % page_size];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = __fmul_rn(static_cast<float>(static_cast<signed char>(word >> (8 * e))), scale);
-    }
-    store4<T>((is_value ? v_out : k_out) + at * 4, x);
+  const long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x;
+  if (i >= chunks) return;
+  long long token;
+  unsigned chunk;
+  if (chunks <= 0xffffffffll) {   // a 32-bit division wherever it will do
+    token = static_cast<unsigned>(i) / per_row;
+    chunk = static_cast<unsigned>(i) - static_cast<unsigned>(token) * per_row;
+  } else {
+    token = i / per_row;
+    chunk = static_cast<unsigned>(i - token * per_row);
   }
+  const int per_head = dim / 16, head = static_cast<int>(chunk) / per_head, within = (static_cast<int>(chunk) - head * per_head) * 16;
+  const int slot = slots[token];
+  long long row = -1, scale_at = 0;
+  if (slot >= 0 && slot < num_slots) {
+    const int page = slot / page_size;
+    row = (static_cast<long long>(slot) * kv_heads + head) * dim;
+    scale_at = (static_cast<long long>(page) * kv_heads + head) * page_size + (slot - page * page_size);
+  }
+  read_chunk(keys, row, scale_at, within, k_out + i * 16);
+  read_chunk(values, row, scale_at, within, v_out + i * 16);
 }
 
 static bool good_pages(const void* codes, const void* scales) {
@@ -293,17 +327,17 @@ SHRIKE_API int shrike_kv_read_q8(const void* k_codes, const float* k_scales, con
     return SHRIKE_BAD_ARGUMENT;
   const Pages keys{static_cast<signed char*>(const_cast<void*>(k_codes)), const_cast<float*>(k_scales)};
   const Pages values{static_cast<signed char*>(const_cast<void*>(v_codes)), const_cast<float*>(v_scales)};
-  const long long quads = static_cast<long long>(n) * kv_heads * (dim / 4);
-  const long long want = (2 * quads + 255) / 256, most = 16ll * shrike_device().sm_count;
-  const unsigned blocks = static_cast<unsigned>(want < most ? want : most);
+  const unsigned per_row = static_cast<unsigned>(kv_heads) * static_cast<unsigned>(dim / 16);
+  const long long chunks = static_cast<long long>(n) * per_row, blocks = (chunks + 255) / 256;
+  if (blocks > 0x7fffffff || num_slots > 0x7fffffff) return SHRIKE_BAD_ARGUMENT;
   cudaError_t err;
   if (dtype == SHRIKE_F32)
-    err = launch_dependent(kv_read_q8_kernel<float>, dim3(blocks), dim3(256), 0, stream, keys, values, slots,
-                           static_cast<float*>(k_out), static_cast<float*>(v_out), quads, kv_heads, dim, page_size, num_slots);
+    err = launch_dependent(kv_read_q8_kernel<float>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, keys, values, slots,
+                           static_cast<float*>(k_out), static_cast<float*>(v_out), chunks, per_row, kv_heads, dim, page_size, num_slots);
   else if (dtype == SHRIKE_BF16)
-    err = launch_dependent(kv_read_q8_kernel<__nv_bfloat16>, dim3(blocks), dim3(256), 0, stream, keys, values, slots,
-                           static_cast<__nv_bfloat16*>(k_out), static_cast<__nv_bfloat16*>(v_out), quads, kv_heads, dim, page_size,
-                           num_slots);
+    err = launch_dependent(kv_read_q8_kernel<__nv_bfloat16>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, keys, values, slots,
+                           static_cast<__nv_bfloat16*>(k_out), static_cast<__nv_bfloat16*>(v_out), chunks, per_row, kv_heads, dim,
+                           page_size, num_slots);
   else
     return SHRIKE_BAD_ARGUMENT;
   return err == cudaSuccess ? shrike_launch_status() : static_cast<int>(err);

@@ -288,9 +288,9 @@ class QuantisedCacheOps:
         takes, a CTA having at least a step of 32 keys for each of its four warps."""
         best, least = 1, None
         for splits in (1, 2, 4, 8, 16, 24, 32, 40, 48, 56, 64):
-            if splits > max(1, -(-keys // 128)):
+            if splits > max(1, -(-keys // 64)):
                 break
-            time = -(-pairs * splits // resident) * (-(-keys // splits) + cls.Q8_SPLIT_KEYS)
+            time = max(1.0, pairs * splits / (0.87 * resident)) * (-(-keys // (128 * splits)) * 128 + cls.Q8_SPLIT_KEYS * (1 + (splits > 8)))
             if least is None or time < least:
                 best, least = splits, time
         return best, min(best, 8)
