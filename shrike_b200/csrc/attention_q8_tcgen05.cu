@@ -7,20 +7,24 @@
 // head, token by token: a key tile is turned into float16 once for every head that reads it, a portion of a few dozen tokens
 // fills the rows, and a chain's tokens lie close together, so that little is computed behind the causal border.  A chain walks
 // the keys 64 at a time, as the kernel over bfloat16 pages does (attention_tcgen05.cu): scores by tcgen05.mma into tensor
-// memory, a thread a row for the softmax, weights back into tensor memory as the operand of the second product, outputs there.
+// memory, softmax, weights back into tensor memory as the operand of the second product, outputs there.
 //
-// What is new is the way of the keys and values: TMA brings a tile's codes (one box a page, in the swizzle of their row
-// length), four warps turn them into float16 tiles in the 128-byte swizzle (a thread owns a key: its codes, its page, its two
-// scales), and those are what the products read.  Eight codes take 10 instructions (a byte permutation and a subtraction a
-// pair, an exclusive or for four).  A tile of 128 keys x 128 elements costs each of the four warps about 370 issue slots for the
-// keys and as many for the values, against about 2,050 clocks that the two chains' products and exponentials take.
+// The way of the keys and values: TMA brings a tile's codes (one box a page, in the swizzle of their row length), eight warps
+// turn them into float16 tiles in the 128-byte swizzle (four the keys', four the values'; two threads a key), and those are
+// what the products read.  Eight codes take 10 instructions (a byte permutation and a subtraction a pair, an exclusive or for
+// four).
+// The softmax is bound by the latency of its instructions, not by their number: with a thread a row (eight warps, as the kernel
+// over bfloat16 pages has) a step of 64 keys takes 2,700 clocks, and leaving out the exponentials, the scales' products or the
+// conversion saves 8 to 10 % each.  So two threads share a row, each with 32 of a step's keys: twice the warps to hide latency
+// with, half the unrolled code.  They agree on the row's base through a barrier of their two warps that says whether anyone's
+// has to move (rarely), and only then exchange their maxima.
 //
 // Roles: warp 0 brings key codes (and the queries), warp 3 value codes (and owns tensor memory), warps 1 and 2 issue the products
-// of a chain each, warps 4..7 and 8..11 are the softmax and epilogue of a chain each, warps 12..15 convert.  The softmax
-// warpgroups take 168 registers a thread, the other two 88 (together the 128 a thread that the CTA is launched with).
-// Barriers: raw_k / raw_v full (TMA) and free (converters); k_full / v_full[stage] (converters; v_full also says that the
-// tile's scales lie in shared memory), k_free / v_free[stage] (commits of both chains); q_ready[chain] once the softmax warps
-// have turned the queries into float16; the others as in attention_tcgen05.cu.
+// of a chain each, warps 4..11 and 12..19 are the softmax and epilogue of a chain each, warps 20..23 convert keys, 24..27 values.
+// Registers a thread: 72 at launch, 96 in the softmax warpgroups, 40 in the others (16 x 96 + 12 x 40 = 28 x 72).
+// Barriers: raw_k / raw_v full[raw stage] (TMA) and free (converters, an arrival a warp); k_full / v_full[stage] (converters;
+// v_full also says that the tile's scales lie in shared memory), k_free / v_free[stage] (commits of both chains); q_ready[chain]
+// once the softmax warps have turned the queries into float16; the others as in attention_tcgen05.cu.
 // Every wait is bounded (status word, CTA-wide abort flag); no TMA load uses multicast.
 // Built once per head size; serves head sizes 64 and 128, page sizes 8, 16, 32, 64, and groups of up to 64 heads.
 #include <cuda_fp16.h>
@@ -41,13 +45,12 @@ constexpr int BM = 128;                         // query rows of one chain
 constexpr int HALVES = D / 64;                 // 64-element groups of the head size
 constexpr int Q_HALF = BM * 128;               // bytes of one 64-element-wide sub-tile of a query tile
 constexpr int Q_BYTES = HALVES * Q_HALF;
-constexpr int KEYS = 128;                      // keys of a tile
-constexpr int HALF_KEYS = KEYS / 2;            // keys of a softmax step
-constexpr int STAGES = 2;
+constexpr int KEYS = 64;                       // keys of a tile, and of a softmax step
+constexpr int STAGES = 3, RAW_STAGES = 3;
 constexpr int KV_HALF = KEYS * 128;            // bytes of one 64-element-wide sub-tile of a float16 key (or value) tile
 constexpr int KV_TILE = HALVES * KV_HALF;
 constexpr int RAW_TILE = KEYS * D;             // a tile's codes
-constexpr int THREADS = 512;
+constexpr int WARPS = 28, THREADS = WARPS * 32;
 constexpr unsigned CHAIN_COLS = 256, P_COL = 64, O_COL = 128, TMEM_COLS = 512;   // as in attention_tcgen05.cu
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr int LEAST_EXPONENT = -93, MOST_EXPONENT = 107, SCALE_BITS = 8;   // as in attention_q8.cu
@@ -179,20 +182,30 @@ __device__ __forceinline__ void find_work(const Args& args, int work, int rows, 
 
 struct Shared {
   float k_scale[STAGES][KEYS], v_scale[STAGES][KEYS];
-  int v_top[STAGES][4];   // per 32 keys: the exponent of the largest value scale
-  int v_bad[STAGES][4];   // whether one of them is no finite number
+  int v_top[STAGES][2];   // per 32 keys: the exponent of the largest value scale
+  int v_bad[STAGES][2];   // whether one of them is no finite number
+  float row_max[2][2][BM], row_sum[2][2][BM];   // [chain][key half]: what the two threads of a row tell each other
+  int row_top[2][2][BM];
   unsigned long long q_full, q_ready[2], s_full[2], s_read[2], p_full[2][2], pv_done[2][2], pv_last[2], stagger;
-  unsigned long long raw_k_full, raw_k_free, raw_v_full, raw_v_free;
+  unsigned long long raw_k_full[RAW_STAGES], raw_k_free[RAW_STAGES], raw_v_full[RAW_STAGES], raw_v_free[RAW_STAGES];
   unsigned long long k_full[STAGES], k_free[STAGES], v_full[STAGES], v_free[STAGES];
   unsigned tmem_base;
   volatile int abort;
 };
-constexpr size_t SMEM = 2 * Q_BYTES + 2 * STAGES * KV_TILE + 2 * RAW_TILE + sizeof(Shared);
+constexpr size_t SMEM = 2 * Q_BYTES + 2 * STAGES * KV_TILE + 2 * RAW_STAGES * RAW_TILE + sizeof(Shared);
 static_assert(SMEM <= 232448, "more than an SM's shared memory");
 
-__device__ __noinline__ void rescale_output_row(unsigned tmem_o, float correction) {
-#pragma unroll
-  for (int c = 0; c < D / 32; ++c) {
+// 32 lanes x 16 columns of 32-bit.
+__device__ __forceinline__ void tmem_store16(unsigned taddr, const unsigned (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+        "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+// This thread's share (every other run of 32 columns) of its output row.
+__device__ __noinline__ void rescale_output_row(unsigned tmem_o, int half, float correction) {
+  for (int c = half; c < D / 32; c += 2) {
     unsigned o[32];
     tmem_load32(tmem_o + c * 32, o);
     tmem_wait_load();
@@ -201,23 +214,35 @@ __device__ __noinline__ void rescale_output_row(unsigned tmem_o, float correctio
     tmem_store32(tmem_o + c * 32, o);
   }
 }
+// The barriers of the two warps that share 32 rows.
+__device__ __forceinline__ bool pair_any(int id, bool mine) {
+  unsigned any;
+  __syncwarp();
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %2, 0;\n\tbarrier.cta.red.or.pred.aligned q, %1, 64, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+               : "=r"(any) : "r"(id), "r"(mine ? 1u : 0u) : "memory");
+  return any != 0;
+}
+__device__ __forceinline__ void pair_sync(int id) {
+  __syncwarp();
+  asm volatile("barrier.cta.sync.aligned %0, 64;" ::"r"(id) : "memory");
+}
 
-// The converters' share: thread `row` turns its key's codes into a row of float16 in the 128-byte swizzle.
-constexpr int RAW_CHUNKS = D / 16;
-__device__ __forceinline__ void read_codes(const unsigned char* raw, int row, uint4 (&codes)[RAW_CHUNKS]) {
+// A converting thread's share: 16-byte chunks first ... first + COUNT - 1 of its key's codes, and the float16 they become.
+constexpr int RAW_CHUNKS = D / 16, MY_CHUNKS = RAW_CHUNKS / 2;
+__device__ __forceinline__ void read_codes(const unsigned char* raw, int row, int first, uint4 (&codes)[MY_CHUNKS]) {
   // rows of 128 bytes in the 128-byte swizzle, rows of 64 bytes in the 64-byte one
   const int exchanged = D == 128 ? row & 7 : (row >> 1) & 3;
 #pragma unroll
-  for (int c = 0; c < RAW_CHUNKS; ++c) codes[c] = *reinterpret_cast<const uint4*>(raw + row * D + ((c ^ exchanged) << 4));
+  for (int c = 0; c < MY_CHUNKS; ++c) codes[c] = *reinterpret_cast<const uint4*>(raw + row * D + (((first + c) ^ exchanged) << 4));
 }
-__device__ __forceinline__ void write_halves(unsigned char* tile, int row, const uint4 (&codes)[RAW_CHUNKS]) {
+__device__ __forceinline__ void write_halves(unsigned char* tile, int row, int first, const uint4 (&codes)[MY_CHUNKS]) {
 #pragma unroll
-  for (int c = 0; c < RAW_CHUNKS; ++c) {
-    unsigned char* half = tile + (c / 4) * KV_HALF + row * 128;
+  for (int c = 0; c < MY_CHUNKS; ++c) {
+    unsigned char* half = tile + ((first + c) / 4) * KV_HALF + row * 128;
     const unsigned w[4] = {codes[c].x ^ 0x80808080u, codes[c].y ^ 0x80808080u, codes[c].z ^ 0x80808080u, codes[c].w ^ 0x80808080u};
 #pragma unroll
     for (int i = 0; i < 2; ++i)
-      *reinterpret_cast<uint4*>(half + (((2 * (c % 4) + i) ^ (row & 7)) << 4)) =
+      *reinterpret_cast<uint4*>(half + (((2 * ((first + c) % 4) + i) ^ (row & 7)) << 4)) =
           make_uint4(codes_to_half<0x4140>(w[2 * i]), codes_to_half<0x4342>(w[2 * i]), codes_to_half<0x4140>(w[2 * i + 1]), codes_to_half<0x4342>(w[2 * i + 1]));
   }
 }
@@ -240,9 +265,9 @@ portions_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
   unsigned char* q_tiles = smem_raw;                             // [2 chains][Q_BYTES]
   unsigned char* k_tiles = q_tiles + 2 * Q_BYTES;                // [STAGES][KV_TILE]
   unsigned char* v_tiles = k_tiles + STAGES * KV_TILE;           // [STAGES][KV_TILE]
-  unsigned char* raw_k = v_tiles + STAGES * KV_TILE;
-  unsigned char* raw_v = raw_k + RAW_TILE;
-  Shared* sh = reinterpret_cast<Shared*>(raw_v + RAW_TILE);
+  unsigned char* raw_k = v_tiles + STAGES * KV_TILE;             // [RAW_STAGES][RAW_TILE]
+  unsigned char* raw_v = raw_k + RAW_STAGES * RAW_TILE;          // [RAW_STAGES][RAW_TILE]
+  Shared* sh = reinterpret_cast<Shared*>(raw_v + RAW_STAGES * RAW_TILE);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
   const int pos0 = args.ctx_len[seq] - q_len;                   // position of the first new token
@@ -255,37 +280,37 @@ portions_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
   const int tile_hi = hi >= 0 ? hi / KEYS : -1;
   const int all_tiles = hi >= 0 ? tile_hi - lo / KEYS + 1 : 0;
   const int per = (all_tiles + args.splits - 1) / args.splits;
-  // this CTA's share: tiles tile_lo ... last_tile (none: an empty split)
+  // this CTA's share: tiles tile_lo ... last_tile (none: an empty split).  The later chain takes up to two tiles (its 128
+  // tokens at most) that the earlier one does not, the last ones: nobody waits for a stage to be free that such a tile was in.
   const int tile_lo = lo / KEYS + split * per;
   const int last_tile = min(tile_hi, tile_lo + per - 1);
-  const int count_0 = hi_0 >= 0 ? max(0, min(last_tile, hi_0 / KEYS) - tile_lo + 1) : 0;
-  const int count_1 = hi_1 >= 0 ? max(0, min(last_tile, hi_1 / KEYS) - tile_lo + 1) : 0;
-  const int num_tiles = max(count_0, count_1);
-  // the same in steps of 64 keys: a chain's last tile may need its first half only
-  const int steps_0 = count_0 > 0 ? min(2 * count_0, hi_0 / HALF_KEYS - 2 * tile_lo + 1) : 0;
-  const int steps_1 = count_1 > 0 ? min(2 * count_1, hi_1 / HALF_KEYS - 2 * tile_lo + 1) : 0;
+  const int steps_0 = hi_0 >= 0 ? max(0, min(last_tile, hi_0 / KEYS) - tile_lo + 1) : 0;
+  const int steps_1 = hi_1 >= 0 ? max(0, min(last_tile, hi_1 / KEYS) - tile_lo + 1) : 0;
+  const int num_tiles = max(steps_0, steps_1);
 
   const unsigned users = (steps_0 > 0 ? 1u : 0u) + (steps_1 > 0 ? 1u : 0u);   // chains that read the key and value stages
   if (threadIdx.x == 0) {
     mbar_init(&sh->q_full, 1);
     for (int c = 0; c < 2; ++c) {
-      mbar_init(&sh->q_ready[c], 128);
+      mbar_init(&sh->q_ready[c], 8);
       mbar_init(&sh->s_full[c], 1);
-      mbar_init(&sh->s_read[c], 128);
+      mbar_init(&sh->s_read[c], 8);
       for (int b = 0; b < 2; ++b) {
-        mbar_init(&sh->p_full[c][b], 128);
+        mbar_init(&sh->p_full[c][b], 8);
         mbar_init(&sh->pv_done[c][b], 1);
       }
       mbar_init(&sh->pv_last[c], 1);
     }
-    mbar_init(&sh->raw_k_full, 1);
-    mbar_init(&sh->raw_v_full, 1);
-    mbar_init(&sh->raw_k_free, 128);
-    mbar_init(&sh->raw_v_free, 128);
+    for (int s = 0; s < RAW_STAGES; ++s) {
+      mbar_init(&sh->raw_k_full[s], 1);
+      mbar_init(&sh->raw_v_full[s], 1);
+      mbar_init(&sh->raw_k_free[s], 4);
+      mbar_init(&sh->raw_v_free[s], 4);
+    }
     for (int s = 0; s < STAGES; ++s) {
-      mbar_init(&sh->k_full[s], 128);
+      mbar_init(&sh->k_full[s], 4);
       mbar_init(&sh->k_free[s], users > 0 ? users : 1u);
-      mbar_init(&sh->v_full[s], 128);
+      mbar_init(&sh->v_full[s], 4);
       mbar_init(&sh->v_free[s], users > 0 ? users : 1u);
     }
     mbar_init(&sh->stagger, 1);
@@ -300,14 +325,14 @@ portions_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
   wait_for_previous();   // the query and the newest keys come from the kernel before this one
 
   if (warp < 4) {
-    fewer_registers<88>();
+    fewer_registers<40>();
     if (warp == 0 || warp == 3) {
       // Key (warp 0) and value codes (warp 3): lane 0 waits for the buffer and arms its barrier, then lane pg issues the box of
       // page pg of the tile.  Page ids come a chunk of 32 at a time (lane l: page l of the chunk, several tiles' worth), the next
       // chunk while this one is used.
       const bool for_keys = warp == 0;
       const int* table = args.block_table + static_cast<size_t>(seq) * args.max_blocks;
-      const int pages_per_tile = KEYS / args.page_size;
+      const int pages_per_tile = KEYS >> args.page_shift;
       const int nowhere = args.num_pages * args.page_size;      // a row coordinate outside the cache: reads zeros
       if (for_keys && lane == 0 && num_tiles > 0) {
         mbar_expect_tx(&sh->q_full, 2 * HALVES * args.tokens * args.group * 128);
@@ -317,40 +342,44 @@ portions_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       }
       const int tiles_per_chunk = 32 / pages_per_tile;
       auto load_chunk = [&](int chunk) -> int {
-        const int key0 = tile_lo * KEYS + (chunk * 32 + lane) * args.page_size;
-        const int block = key0 / args.page_size;
+        const int key0 = tile_lo * KEYS + ((chunk * 32 + lane) << args.page_shift);
+        const int block = key0 >> args.page_shift;
         return (chunk * tiles_per_chunk < num_tiles && key0 <= hi && block < args.max_blocks) ? table[block] : -1;
       };
       unsigned char* const raw = for_keys ? raw_k : raw_v;
-      unsigned long long* const full = for_keys ? &sh->raw_k_full : &sh->raw_v_full;
-      unsigned long long* const free_again = for_keys ? &sh->raw_k_free : &sh->raw_v_free;
+      unsigned long long* const full = for_keys ? sh->raw_k_full : sh->raw_v_full;
+      unsigned long long* const free_again = for_keys ? sh->raw_k_free : sh->raw_v_free;
       const CUtensorMap* const map = for_keys ? &map_k : &map_v;
       int chunk_pages = load_chunk(0), next_pages = load_chunk(1);
-      int issued = 0;
+      int issued = 0, within = 0, chunk = 0;
       for (int i = 0; i < num_tiles; ++i) {
-        const int within = i % tiles_per_chunk;
-        if (within == 0 && i > 0) {
+        const int s = i % RAW_STAGES;
+        if (within == tiles_per_chunk) {
+          within = 0;
           chunk_pages = next_pages;
-          next_pages = load_chunk(i / tiles_per_chunk + 1);
+          next_pages = load_chunk(++chunk + 1);
         }
-        int page = __shfl_sync(0xffffffffu, chunk_pages, within * pages_per_tile + (lane % pages_per_tile));
+        int page = __shfl_sync(0xffffffffu, chunk_pages, within * pages_per_tile + (lane & (pages_per_tile - 1)));
+        ++within;
         if (page >= args.num_pages) page = -1;
-        const int y = page < 0 ? nowhere : page * args.page_size;
+        const int y = page < 0 ? nowhere : page << args.page_shift;
         int ok = 1;
         if (lane == 0) {
-          ok = mbar_wait(free_again, (i & 1) ^ 1, &sh->abort, args.status, ERR_PRODUCER) ? 1 : 0;
-          if (ok) mbar_expect_tx(full, RAW_TILE);
+          ok = mbar_wait(&free_again[s], ((i / RAW_STAGES) & 1) ^ 1, &sh->abort, args.status, ERR_PRODUCER) ? 1 : 0;
+          if (ok) mbar_expect_tx(&full[s], RAW_TILE);
         }
         ok = __shfl_sync(0xffffffffu, ok, 0);
         if (!ok) break;
-        if (lane < pages_per_tile) tma_load_2d(raw + lane * args.page_size * D, map, full, kv_head * D, y);
+        if (lane < pages_per_tile) tma_load_2d(raw + s * RAW_TILE + ((lane << args.page_shift) * D), map, &full[s], kv_head * D, y);
         issued = i + 1;
       }
-      if (lane == 0 && sh->abort) {   // copies may still be in flight: wait for what was armed last
-        bool landed = issued == 0;
-        for (unsigned tries = 0; tries < WAIT_LIMIT && !landed; ++tries) landed = mbar_try_wait(full, (issued - 1) & 1);
-        if (!landed && args.status != nullptr) *args.status = ERR_DRAIN;
-        landed = !for_keys || num_tiles <= 0;
+      if (lane == 0 && sh->abort) {   // copies may still be in flight: wait for the buffers armed last
+        for (int i = max(0, issued - RAW_STAGES); i < issued; ++i) {
+          bool landed = false;
+          for (unsigned tries = 0; tries < WAIT_LIMIT && !landed; ++tries) landed = mbar_try_wait(&full[i % RAW_STAGES], (i / RAW_STAGES) & 1);
+          if (!landed && args.status != nullptr) *args.status = ERR_DRAIN;
+        }
+        bool landed = !for_keys || num_tiles <= 0;
         for (unsigned tries = 0; tries < WAIT_LIMIT && !landed; ++tries) landed = mbar_try_wait(&sh->q_full, 0);
       }
     } else {
@@ -362,29 +391,25 @@ portions_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         auto wait_for = [&](unsigned long long* bar, unsigned parity) {
           return __all_sync(0xffffffffu, mbar_wait(bar, parity, &sh->abort, args.status, ERR_MMA)) != 0;
         };
-        const unsigned idesc_s = half_descriptor(BM, HALF_KEYS, false);
+        const unsigned idesc_s = half_descriptor(BM, KEYS, false);
         const unsigned idesc_o = half_descriptor(BM, D, true);
         const unsigned tmem_chain = __shfl_sync(0xffffffffu, sh->tmem_base, 0) + c * CHAIN_COLS, tmem_o = tmem_chain + O_COL;
         const unsigned long long q_base = smem_descriptor(smem_u32(q_tiles + c * Q_BYTES));
         const unsigned long long k_desc0 = smem_descriptor(smem_u32(k_tiles));
         const unsigned long long v_desc0 = smem_descriptor(smem_u32(v_tiles), KV_HALF, 1024);
         bool ok = wait_for(&sh->q_ready[c], 0);
-        int keys_ready = -1, values_ready = -1;   // the newest tile whose keys (values) are known to be there
         auto issue_scores = [&](int h) {
-          const int i = h >> 1, st = i % STAGES;
-          if (keys_ready < i) {
-            ok = wait_for(&sh->k_full[st], (i / STAGES) & 1);
-            if (!ok) return;
-            keys_ready = i;
-          }
+          const int st = h % STAGES;
+          ok = wait_for(&sh->k_full[st], (h / STAGES) & 1);
+          if (!ok) return;
           fence_after_sync();
-          const unsigned long long k_base = k_desc0 + static_cast<unsigned>((st * KV_TILE + (h & 1) * HALF_KEYS * 128) >> 4);
+          const unsigned long long k_base = k_desc0 + static_cast<unsigned>((st * KV_TILE) >> 4);
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk)
             umma(leader, tmem_chain, q_base + (((kk / 4) * Q_HALF + (kk % 4) * 32) >> 4), k_base + (((kk / 4) * KV_HALF + (kk % 4) * 32) >> 4), idesc_s,
                  kk > 0 ? 1u : 0u);
           umma_commit(leader, &sh->s_full[c]);
-          if ((h & 1) || h + 1 == steps) umma_commit(leader, &sh->k_free[st]);
+          umma_commit(leader, &sh->k_free[st]);
         };
         // the later chain starts most of a step behind the earlier one
         if (ok && c == 1 && steps_0 > 0) ok = wait_for(&sh->stagger, 0);
@@ -396,30 +421,35 @@ portions_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
             issue_scores(h + 1);
             if (!ok) break;
           }
-          const int i = h >> 1, st = i % STAGES;
-          if (values_ready < i) {
-            ok = wait_for(&sh->v_full[st], (i / STAGES) & 1);
-            values_ready = i;
-          }
+          const int st = h % STAGES;
+          ok = wait_for(&sh->v_full[st], (h / STAGES) & 1);
           if (ok) ok = wait_for(&sh->p_full[c][h & 1], (h >> 1) & 1);
           if (!ok) break;
           if (c == 0 && h == 0 && leader) mbar_arrive(&sh->stagger);   // on every path: the other issuer waits for it
           fence_after_sync();
-          const unsigned long long v_base = v_desc0 + static_cast<unsigned>((st * KV_TILE + (h & 1) * HALF_KEYS * 128) >> 4);
+          const unsigned long long v_base = v_desc0 + static_cast<unsigned>((st * KV_TILE) >> 4);
           const unsigned tmem_p = tmem_chain + P_COL + (h & 1) * 32;
 #pragma unroll
-          for (int kk = 0; kk < HALF_KEYS / 16; ++kk)
+          for (int kk = 0; kk < KEYS / 16; ++kk)
             umma_a_in_tmem(leader, tmem_o, tmem_p + kk * 8, v_base + ((kk * 16 * 128) >> 4), idesc_o, (h > 0 || kk > 0) ? 1u : 0u);
           umma_commit(leader, &sh->pv_done[c][h & 1]);
           if (h + 1 == steps) umma_commit(leader, &sh->pv_last[c]);
-          if ((h & 1) || h + 1 == steps) umma_commit(leader, &sh->v_free[st]);
+          umma_commit(leader, &sh->v_free[st]);
         }
       }
     }
-  } else if (warp >= 12) {
-    // ---- converters: thread `row` owns key `row` of every tile
-    fewer_registers<88>();
-    const int row = threadIdx.x - 384;
+  } else if (warp >= 20) {
+    // ---- converters: two threads a key, each half of its codes
+    fewer_registers<40>();
+    const bool for_keys = warp < 24;
+    const int row = threadIdx.x & 63, half = (threadIdx.x >> 6) & 1, first = half * MY_CHUNKS;
+    const unsigned char* const raw = for_keys ? raw_k : raw_v;
+    unsigned char* const tiles = for_keys ? k_tiles : v_tiles;
+    unsigned long long* const raw_full = for_keys ? sh->raw_k_full : sh->raw_v_full;
+    unsigned long long* const raw_free = for_keys ? sh->raw_k_free : sh->raw_v_free;
+    unsigned long long* const full = for_keys ? sh->k_full : sh->v_full;
+    unsigned long long* const free_again = for_keys ? sh->k_free : sh->v_free;
+    const bool scales = !for_keys && half == 0;   // these bring the tile's scales too (whole warps)
     const int* table = args.block_table + static_cast<size_t>(seq) * args.max_blocks;
     // the place of this thread's key of tile i among the scales; -1: no such key
     auto scale_place = [&](int i) -> long long {
@@ -427,51 +457,58 @@ portions_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       if (i >= num_tiles || key > hi || block >= args.max_blocks) return -1;
       const int page = table[block];
       if (page < 0 || page >= args.num_pages) return -1;
-      return (static_cast<long long>(page) * args.num_kv_heads + kv_head) * args.page_size + (key & (args.page_size - 1));
+      return ((static_cast<long long>(page) * args.num_kv_heads + kv_head) << args.page_shift) + (key & (args.page_size - 1));
     };
-    long long place = scale_place(0);
-    float k_scale = place >= 0 ? args.k_scales[place] : 0.f, v_scale = place >= 0 ? args.v_scales[place] : 0.f;
-    place = scale_place(1);
-    for (int i = 0; i < num_tiles; ++i) {
-      const int st = i % STAGES;
-      const unsigned reuse = ((i / STAGES) & 1) ^ 1;
-      const float next_k = place >= 0 ? args.k_scales[place] : 0.f, next_v = place >= 0 ? args.v_scales[place] : 0.f;
-      place = scale_place(i + 2);
-      uint4 codes[RAW_CHUNKS];
-      bool ok = mbar_wait(&sh->raw_k_full, i & 1, &sh->abort, args.status, ERR_CONVERT);
-      if (!__all_sync(0xffffffffu, ok)) break;
-      read_codes(raw_k, row, codes);
-      mbar_arrive(&sh->raw_k_free);
-      ok = mbar_wait(&sh->k_free[st], reuse, &sh->abort, args.status, ERR_CONVERT);
-      if (!__all_sync(0xffffffffu, ok)) break;
-      write_halves(k_tiles + st * KV_TILE, row, codes);
-      fence_async_shared();
-      mbar_arrive(&sh->k_full[st]);
-      ok = mbar_wait(&sh->raw_v_full, i & 1, &sh->abort, args.status, ERR_CONVERT);
-      if (!__all_sync(0xffffffffu, ok)) break;
-      read_codes(raw_v, row, codes);
-      mbar_arrive(&sh->raw_v_free);
-      ok = mbar_wait(&sh->v_free[st], reuse, &sh->abort, args.status, ERR_CONVERT);
-      if (!__all_sync(0xffffffffu, ok)) break;
-      // the softmax threads have read the scales of the tile that was here: its products are done
-      sh->k_scale[st][row] = k_scale;
-      sh->v_scale[st][row] = v_scale;
-      const unsigned top = __reduce_max_sync(0xffffffffu, finite_bits(v_scale));
-      const bool bad = __any_sync(0xffffffffu, !(fabsf(v_scale) < INFINITY));
-      if (lane == 0) {
-        sh->v_top[st][row >> 5] = static_cast<int>(top >> 23) - 127;
-        sh->v_bad[st][row >> 5] = bad ? 1 : 0;
+    long long place = -1;
+    float k_scale = 0.f, v_scale = 0.f;
+    if (scales) {
+      place = scale_place(0);
+      if (place >= 0) {
+        k_scale = args.k_scales[place];
+        v_scale = args.v_scales[place];
       }
-      write_halves(v_tiles + st * KV_TILE, row, codes);
+      place = scale_place(1);
+    }
+    for (int i = 0; i < num_tiles; ++i) {
+      const int st = i % STAGES, rs = i % RAW_STAGES;
+      float next_k = 0.f, next_v = 0.f;
+      if (scales) {
+        if (place >= 0) {
+          next_k = args.k_scales[place];
+          next_v = args.v_scales[place];
+        }
+        place = scale_place(i + 2);
+      }
+      uint4 codes[MY_CHUNKS];
+      bool ok = mbar_wait(&raw_full[rs], (i / RAW_STAGES) & 1, &sh->abort, args.status, ERR_CONVERT);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      read_codes(raw + rs * RAW_TILE, row, first, codes);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&raw_free[rs]);
+      ok = mbar_wait(&free_again[st], ((i / STAGES) & 1) ^ 1, &sh->abort, args.status, ERR_CONVERT);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      if (scales) {   // the softmax threads have read the scales of the tile that was here: its products are done
+        sh->k_scale[st][row] = k_scale;
+        sh->v_scale[st][row] = v_scale;
+        const unsigned top = __reduce_max_sync(0xffffffffu, finite_bits(v_scale));
+        const bool bad = __any_sync(0xffffffffu, !(fabsf(v_scale) < INFINITY));
+        if (lane == 0) {
+          sh->v_top[st][row >> 5] = static_cast<int>(top >> 23) - 127;
+          sh->v_bad[st][row >> 5] = bad ? 1 : 0;
+        }
+        k_scale = next_k;
+        v_scale = next_v;
+      }
+      write_halves(tiles + st * KV_TILE, row, first, codes);
       fence_async_shared();
-      mbar_arrive(&sh->v_full[st]);
-      k_scale = next_k;
-      v_scale = next_v;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&full[st]);
     }
   } else {
-    // ---- softmax and epilogue: a thread a row
-    more_registers<168>();
-    const int chain = (warp - 4) >> 2, quarter = warp & 3;
+    // ---- softmax and epilogue: two threads a row, each with 32 of a step's 64 keys
+    more_registers<96>();
+    const int chain = (warp - 4) >> 3, sub = ((warp - 4) >> 2) & 1, quarter = warp & 3;
+    const int pair = 1 + chain * 4 + quarter;   // the barrier of the two warps that share these rows
     const int row = quarter * 32 + lane;
     const int token = tile_start + chain * args.tokens + row / args.group, head = kv_head * args.group + row % args.group;
     const bool there = row < args.tokens * args.group && token < q_len;
@@ -486,25 +523,32 @@ portions_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     int exponent = LEAST_EXPONENT;
     bool ok = true;
     if (my_steps > 0) {
-      // the query's row: scaled so that its largest element lies in [2^14, 2^15), then float16
+      // the query's row, half of it each: scaled so that its largest element lies in [2^14, 2^15), then float16
       ok = mbar_wait(&sh->q_full, 0, &sh->abort, args.status, ERR_SOFTMAX);
       ok = __all_sync(0xffffffffu, ok);
+      constexpr int MINE = HALVES * 4;   // 16-byte chunks of this thread
+      unsigned char* q_row = q_tiles + chain * Q_BYTES + row * 128;
+      auto chunk_of = [&](int c) { return reinterpret_cast<uint4*>(q_row + ((sub * MINE + c) / 8) * Q_HALF + ((((sub * MINE + c) % 8) ^ (row & 7)) << 4)); };
+      unsigned top = 0u;
       if (ok) {
-        unsigned char* q_row = q_tiles + chain * Q_BYTES + row * 128;
-        unsigned top = 0u;
 #pragma unroll
-        for (int c = 0; c < HALVES * 8; ++c) {
-          const uint4 v = *reinterpret_cast<const uint4*>(q_row + (c / 8) * Q_HALF + (((c % 8) ^ (row & 7)) << 4));
+        for (int c = 0; c < MINE; ++c) {
+          const uint4 v = *chunk_of(c);
           const unsigned w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
           for (int i = 0; i < 4; ++i) top = max(top, max(finite_bits(__uint_as_float(w[i] << 16)), finite_bits(__uint_as_float(w[i] & 0xffff0000u))));
         }
+        sh->row_top[chain][sub][row] = static_cast<int>(top);
+      }
+      pair_sync(pair);   // on every path: the partner waits for it
+      if (ok) {
+        top = max(top, static_cast<unsigned>(sh->row_top[chain][sub ^ 1][row]));
         const int e = min(max(static_cast<int>(top >> 23) - 127, -100), 126);
         const float lift = args.scale_log2 < 0.f ? -power_of_two(14 - e) : power_of_two(14 - e);
         factor = fmaxf(fabsf(args.scale_log2) * power_of_two(e - 14), 1e-38f);   // a hidden key's -inf has to stay one
 #pragma unroll
-        for (int c = 0; c < HALVES * 8; ++c) {
-          uint4* at = reinterpret_cast<uint4*>(q_row + (c / 8) * Q_HALF + (((c % 8) ^ (row & 7)) << 4));
+        for (int c = 0; c < MINE; ++c) {
+          uint4* at = chunk_of(c);
           const uint4 v = *at;
           const unsigned w[4] = {v.x, v.y, v.z, v.w};
           unsigned h[4];
@@ -513,98 +557,101 @@ portions_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
           *at = make_uint4(h[0], h[1], h[2], h[3]);
         }
         fence_async_shared();
-        mbar_arrive(&sh->q_ready[chain]);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh->q_ready[chain]);
       }
     }
-    for (int h = 0; h < my_steps && ok; ++h) {
-      const int st = (h >> 1) % STAGES;
-      if ((h & 1) == 0) {   // the tile's scales
-        ok = mbar_wait(&sh->v_full[st], ((h >> 1) / STAGES) & 1, &sh->abort, args.status, ERR_SOFTMAX);
-      }
+    for (int h = 0; h < my_steps; ++h) {
+      const int st = h % STAGES;
+      if (ok) ok = mbar_wait(&sh->v_full[st], (h / STAGES) & 1, &sh->abort, args.status, ERR_SOFTMAX);   // the tile's scales
       if (ok) ok = mbar_wait(&sh->s_full[chain], h & 1, &sh->abort, args.status, ERR_SOFTMAX);
       ok = __all_sync(0xffffffffu, ok);   // the warp stays together: the tensor-memory accesses below are warp-wide
-      if (!ok) break;
-      fence_after_sync();
-      unsigned v[2][32];
-      tmem_load32(tmem_chain, v[0]);
-      tmem_load32(tmem_chain + 32, v[1]);
-      const float* k_scale = sh->k_scale[st] + (h & 1) * HALF_KEYS;
-      const float* v_scale = sh->v_scale[st] + (h & 1) * HALF_KEYS;
-      int top = max(sh->v_top[st][2 * (h & 1)], sh->v_top[st][2 * (h & 1) + 1]);
-      tmem_wait_load();
-      fence_before_sync();
-      mbar_arrive(&sh->s_read[chain]);    // the scores are in registers: their columns may take the next step
-      const int key_base = (tile_lo * 2 + h) * HALF_KEYS;
-      float part_max[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};   // four chains of dependent instructions, not one
-      const bool edge = key_base < first || key_base + HALF_KEYS - 1 > last;   // only steps at the edge of the row's range pay for masking
-#pragma unroll
-      for (int g = 0; g < 2; ++g)
+      unsigned v[32];
+      const int key_base = (tile_lo + h) * KEYS + sub * 32;
+      const bool edge = key_base < first || key_base + 31 > last;   // only steps at the edge of the row's range pay for masking
+      float step_max = -INFINITY;
+      int top = LEAST_EXPONENT;
+      if (ok) {
+        fence_after_sync();
+        tmem_load32(tmem_chain + sub * 32, v);
+        const float* k_scale = sh->k_scale[st] + sub * 32;
+        top = sh->v_top[st][sub];
+        tmem_wait_load();
+        fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh->s_read[chain]);    // the scores are in registers: their columns may take the next step
 #pragma unroll
         for (int j = 0; j < 32; j += 4) {
-          const float4 s = *reinterpret_cast<const float4*>(k_scale + g * 32 + j);
+          const float4 s = *reinterpret_cast<const float4*>(k_scale + j);
           float x[4];
-          halves_of(mul_pair(pair_of(__uint_as_float(v[g][j]), __uint_as_float(v[g][j + 1])), pair_of(s.x, s.y)), x[0], x[1]);
-          halves_of(mul_pair(pair_of(__uint_as_float(v[g][j + 2]), __uint_as_float(v[g][j + 3])), pair_of(s.z, s.w)), x[2], x[3]);
+          halves_of(mul_pair(pair_of(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), pair_of(s.x, s.y)), x[0], x[1]);
+          halves_of(mul_pair(pair_of(__uint_as_float(v[j + 2]), __uint_as_float(v[j + 3])), pair_of(s.z, s.w)), x[2], x[3]);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) v[g][j + i] = __float_as_uint(x[i]);
+          for (int i = 0; i < 4; ++i) v[j + i] = __float_as_uint(x[i]);
         }
-      if (edge) {
-        unsigned top_bits = 0u;
-#pragma unroll
-        for (int g = 0; g < 2; ++g)
+        if (edge) {
+          const float* v_scale = sh->v_scale[st] + sub * 32;
+          unsigned top_bits = 0u;
 #pragma unroll
           for (int j = 0; j < 32; ++j) {
-            const int key = key_base + g * 32 + j;
-            if (key < first || key > last) v[g][j] = 0xff800000u;   // -inf
-            else top_bits = max(top_bits, finite_bits(v_scale[g * 32 + j]));
+            const int key = key_base + j;
+            if (key < first || key > last) v[j] = 0xff800000u;   // -inf
+            else top_bits = max(top_bits, finite_bits(v_scale[j]));
           }
-        top = static_cast<int>(top_bits >> 23) - 127;
+          top = static_cast<int>(top_bits >> 23) - 127;
+        }
+        float part_max[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int j = 0; j < 32; j += 4)
+#pragma unroll
+          for (int a = 0; a < 2; ++a) part_max[a] = max3(part_max[a], __uint_as_float(v[j + 2 * a]), __uint_as_float(v[j + 2 * a + 1]));
+        step_max = fmaxf(part_max[0], part_max[1]) * factor;
+        top = min(top - SCALE_BITS, MOST_EXPONENT);
       }
-#pragma unroll
-      for (int g = 0; g < 2; ++g)
-#pragma unroll
-        for (int j = 0; j < 32; j += 8)
-#pragma unroll
-          for (int a = 0; a < 4; ++a) part_max[a] = max3(part_max[a], __uint_as_float(v[g][j + 2 * a]), __uint_as_float(v[g][j + 2 * a + 1]));
-      const float step_max = fmaxf(max3(part_max[0], part_max[1], part_max[2]), part_max[3]) * factor;
       // The base follows the largest score lazily (2^6), and the largest value scale at once: the weights stay below 2^15.
+      // Both threads of a row have the same; the warps that share the rows ask each other whether any row's has to move (on
+      // every path: the partner waits).
       float correction = 1.0f;
-      top = min(top - SCALE_BITS, MOST_EXPONENT);
-      if (step_max > most + BASE_LAG || top > exponent || most == -INFINITY) {
-        most = fmaxf(most, step_max);
-        exponent = max(exponent, top);
+      const bool moves = !ok || step_max > most + BASE_LAG || top > exponent || most == -INFINITY;
+      if (pair_any(pair, moves)) {
+        sh->row_max[chain][sub][row] = ok ? step_max : -INFINITY;
+        sh->row_top[chain][sub][row] = top;
+        pair_sync(pair);
+        most = fmaxf(most, fmaxf(step_max, sh->row_max[chain][sub ^ 1][row]));
+        exponent = max(exponent, max(top, sh->row_top[chain][sub ^ 1][row]));
         const float next = most + static_cast<float>(exponent);
         // a row that has seen no key yet has O = 0 and a sum of 0: nothing to rescale
         correction = base == -INFINITY ? 1.0f : fast_exp2(base - next);
         base = next;
       }
+      if (!ok) {   // given up: the partner may still be a step behind, and must not wait for this warp's barriers
+        continue;
+      }
+      const float* v_scale = sh->v_scale[st] + sub * 32;
       const float from = base == -INFINITY ? 0.f : base;
       const unsigned long long factor_pair = pair_of(factor, factor), base_pair = pair_of(-from, -from);
       unsigned long long sum_pair[2] = {pair_of(0.f, 0.f), pair_of(0.f, 0.f)};
 #pragma unroll
-      for (int g = 0; g < 2; ++g) {
+      for (int j = 0; j < 32; j += 4) {
+        const float4 s = *reinterpret_cast<const float4*>(v_scale + j);
 #pragma unroll
-        for (int j = 0; j < 32; j += 4) {
-          const float4 s = *reinterpret_cast<const float4*>(v_scale + g * 32 + j);
-#pragma unroll
-          for (int i = 0; i < 4; i += 2) {
-            float x0, x1, w0, w1;
-            halves_of(fma_pair(pair_of(__uint_as_float(v[g][j + i]), __uint_as_float(v[g][j + i + 1])), factor_pair, base_pair), x0, x1);
-            x0 = fast_exp2(x0);
-            x1 = fast_exp2(x1);
-            const unsigned long long p = pair_of(x0, x1);
-            sum_pair[i >> 1] = add_pair(sum_pair[i >> 1], p);
-            halves_of(mul_pair(p, i == 0 ? pair_of(s.x, s.y) : pair_of(s.z, s.w)), w0, w1);
-            v[0][g * 16 + (j + i) / 2] = pack_half(w0, w1);   // over the scores already used
-          }
+        for (int i = 0; i < 4; i += 2) {
+          float x0, x1, w0, w1;
+          halves_of(fma_pair(pair_of(__uint_as_float(v[j + i]), __uint_as_float(v[j + i + 1])), factor_pair, base_pair), x0, x1);
+          x0 = fast_exp2(x0);
+          x1 = fast_exp2(x1);
+          const unsigned long long p = pair_of(x0, x1);
+          sum_pair[i >> 1] = add_pair(sum_pair[i >> 1], p);
+          halves_of(mul_pair(p, i == 0 ? pair_of(s.x, s.y) : pair_of(s.z, s.w)), w0, w1);
+          v[(j + i) / 2] = pack_half(w0, w1);   // over the scores already used
         }
       }
-      if (edge && (sh->v_bad[st][2 * (h & 1)] | sh->v_bad[st][2 * (h & 1) + 1])) {   // rare: a key that the row does not see has no part in it, not even a scale of NaN
+      if (edge && sh->v_bad[st][sub]) {   // rare: a key that the row does not see has no part in it, not even a scale of NaN
 #pragma unroll
-        for (int j = 0; j < 32; ++j) {
+        for (int j = 0; j < 16; ++j) {
           const int key = key_base + 2 * j;
-          if (key < first || key > last) v[0][j] &= 0xffff0000u;
-          if (key + 1 < first || key + 1 > last) v[0][j] &= 0x0000ffffu;
+          if (key < first || key > last) v[j] &= 0xffff0000u;
+          if (key + 1 < first || key + 1 > last) v[j] &= 0x0000ffffu;
         }
       }
       float sum_lo, sum_hi;
@@ -614,36 +661,42 @@ portions_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       if (h >= 2) {
         ok = mbar_wait(&sh->pv_done[chain][h & 1], ((h >> 1) & 1) ^ 1, &sh->abort, args.status, ERR_SOFTMAX);
         ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
+        if (!ok) continue;
         fence_after_sync();
       }
-      tmem_store32(tmem_chain + P_COL + (h & 1) * 32, v[0]);   // keys 2 j and 2 j + 1 of the step in column j
+      tmem_store16(tmem_chain + P_COL + (h & 1) * 32 + sub * 16, v);   // keys 2 j and 2 j + 1 of the step in column j
       if (h > 0 && __any_sync(0xffffffffu, correction != 1.0f)) {
         // O still takes the step before: wait for its PV, then rescale
         ok = mbar_wait(&sh->pv_done[chain][(h - 1) & 1], ((h - 1) >> 1) & 1, &sh->abort, args.status, ERR_SOFTMAX);
         ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
+        if (!ok) continue;
         fence_after_sync();
-        rescale_output_row(tmem_o, correction);
+        rescale_output_row(tmem_o, sub, correction);
       }
       tmem_wait_store();
       fence_before_sync();
-      mbar_arrive(&sh->p_full[chain][h & 1]);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh->p_full[chain][h & 1]);
     }
     if (ok && my_steps > 0) ok = mbar_wait(&sh->pv_last[chain], 0, &sh->abort, args.status, ERR_SOFTMAX);
     ok = __all_sync(0xffffffffu, ok);
     fence_after_sync();
+    if (my_steps > 0) {
+      sh->row_sum[chain][sub][row] = row_sum;
+      pair_sync(pair);   // on every path
+      row_sum += sh->row_sum[chain][sub ^ 1][row];
+    }
     if (ok) {
       const size_t token_head = static_cast<size_t>(start + token) * args.num_heads + head;
       const size_t at = static_cast<size_t>(split) * args.num_tokens * args.num_heads + token_head;
-      if (args.splits > 1 && there) {
+      if (args.splits > 1 && there && sub == 0) {
         args.partial_ml[2 * at] = my_steps > 0 ? base : -INFINITY;
         args.partial_ml[2 * at + 1] = my_steps > 0 ? row_sum : 0.f;
       }
-      const float inv = row_sum == 0.f ? 0.f : 1.0f / row_sum;   // a row that sees nothing is zeros
+      const bool nothing = row_sum == 0.f;   // a row that sees nothing is zeros
+      const float inv = nothing ? 0.f : 1.0f / row_sum;
       if (my_steps > 0 || args.splits == 1) {
-#pragma unroll
-        for (int c = 0; c < D / 32; ++c) {
+        for (int c = sub; c < D / 32; c += 2) {
           unsigned o[32];
           if (my_steps > 0) {
             tmem_load32(tmem_o + c * 32, o);
@@ -663,8 +716,7 @@ portions_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
               unsigned packed[4];
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
-                // a row without weight is zeros even where the products left none
-                const float x = row_sum == 0.f ? 0.f : __uint_as_float(o[j + 2 * i]) * inv, y = row_sum == 0.f ? 0.f : __uint_as_float(o[j + 2 * i + 1]) * inv;
+                const float x = nothing ? 0.f : __uint_as_float(o[j + 2 * i]) * inv, y = nothing ? 0.f : __uint_as_float(o[j + 2 * i + 1]) * inv;
                 const __nv_bfloat162 two = __floats2bfloat162_rn(x, y);
                 packed[i] = *reinterpret_cast<const unsigned*>(&two);
               }
