@@ -14,18 +14,25 @@ import torch
 class QuantisedPages:
     """`codes` int8 [pages, page_size, kv heads, head size], `scales` float32 [pages, kv heads, page_size], on one device."""
 
-    __slots__ = ("codes", "scales")
+    __slots__ = ("codes", "scales", "dims", "device_index")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor):
+        dims = tuple(codes.shape)
+        if not (codes.dtype is torch.int8 and len(dims) == 4 and codes.is_contiguous() and scales.dtype is torch.float32
+                and scales.shape == (dims[0], dims[2], dims[1]) and scales.is_contiguous() and codes.get_device() == scales.get_device()):
+            self._refuse(codes, scales)
+        self.codes, self.scales = codes, scales
+        self.dims, self.device_index = dims, codes.get_device()   # (pages, page_size, kv heads, head size); -1: not on a GPU
+
+    @staticmethod
+    def _refuse(codes, scales):
         if codes.dtype != torch.int8 or codes.dim() != 4 or not codes.is_contiguous():
             raise ValueError("codes must be a contiguous int8 [pages, page_size, kv heads, head size]")
         pages, page_size, heads, _dim = codes.shape
         if scales.dtype != torch.float32 or tuple(scales.shape) != (pages, heads, page_size) or not scales.is_contiguous():
             raise ValueError(f"scales must be a contiguous float32 [{pages}, {heads}, {page_size}], are "
                              f"{scales.dtype} {list(scales.shape)}")
-        if codes.device != scales.device:
-            raise ValueError(f"codes are on {codes.device}, scales on {scales.device}")
-        self.codes, self.scales = codes, scales
+        raise ValueError(f"codes are on {codes.device}, scales on {scales.device}")
 
     @classmethod
     def zeros(cls, pages: int, page_size: int, kv_heads: int, head_dim: int, device) -> "QuantisedPages":

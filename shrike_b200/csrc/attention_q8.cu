@@ -27,6 +27,7 @@
 // share one ring of key tiles.
 #include <cuda_fp16.h>
 
+#include "attention_q8.cuh"
 #include "common.cuh"
 
 #ifndef SHRIKE_HEAD_DIM
@@ -852,11 +853,10 @@ SHRIKE_API int shrike_attention_q8_max_splits() { return attnq8::MAX_SPLITS; }
 // tokens at most) run on the few-rows form with `splits` CTAs a row tile; `has_portions`: the longer ones (all of them where
 // has_single is 0) on the other, or on another kernel where `others` is set.  splits > 1 needs `scratch` (row_floats() for every row of a tile of (entry, kv head, row tile) and split)
 // and `arrivals` (an int a pair, zero before the first launch).
-SHRIKE_API int shrike_paged_attention_q8(const void* q, const void* k_codes, const float* k_scales, const void* v_codes,
-                                         const float* v_scales, const int* block_table, int max_blocks, const int* q_start,
-                                         const int* ctx_len, int dtype, int num_seqs, int num_heads, int num_kv_heads, int page_size,
-                                         int num_pages, float scale, int window, void* out, int has_single, int has_portions,
-                                         int max_q_len, int others, int splits, int cluster, float* scratch, int* arrivals, cudaStream_t stream) {
+SHRIKE_API int shrike_paged_attention_q8(const ShrikeAttentionQ8* call) {
+  const auto& [q, k_codes, k_scales, v_codes, v_scales, block_table, q_start, ctx_len, seq_of_token, out, scratch, arrivals, status, stream, max_blocks,
+               dtype, num_tokens, num_seqs, num_heads, num_kv_heads, page_size, num_pages, window, has_single, has_portions, max_q_len, others, splits,
+               cluster, tiles, scale] = *call;
   if (num_seqs <= 0) return SHRIKE_OK;
   if (num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads || num_kv_heads > 65535 || max_blocks <= 0 || page_size <= 0 ||
       num_pages <= 0 || static_cast<long long>(num_pages) * page_size > 0x7fffffff ||

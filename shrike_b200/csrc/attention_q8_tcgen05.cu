@@ -29,6 +29,7 @@
 // Built once per head size; serves head sizes 64 and 128, page sizes 8, 16, 32, 64, and groups of up to 64 heads.
 #include <cuda_fp16.h>
 
+#include "attention_q8.cuh"
 #include "blackwell.cuh"
 
 #ifndef SHRIKE_HEAD_DIM
@@ -856,11 +857,10 @@ SHRIKE_API int shrike_attention_q8_tc_splits(int tiles, int num_kv_heads, long l
 // Portions (q_len > 1) of a batch; entries with q_len == 1 are skipped when skip_single.  `tiles`: the query tiles of
 // shrike_attention_q8_tc_tokens(group) tokens that they make.  splits > 1 needs `scratch`, splits * num_tokens * num_heads *
 // (D + 2) floats, and `seq_of_token`.
-SHRIKE_API int shrike_paged_attention_q8_tc(const void* q, const void* k_codes, const float* k_scales, const void* v_codes,
-                                            const float* v_scales, const int* block_table, int max_blocks, const int* q_start,
-                                            const int* ctx_len, const int* seq_of_token, int num_tokens, int num_seqs, int num_heads,
-                                            int num_kv_heads, int page_size, int num_pages, float scale, int window, void* out,
-                                            int skip_single, int tiles, int splits, float* scratch, int* status, cudaStream_t stream) {
+SHRIKE_API int shrike_paged_attention_q8_tc(const ShrikeAttentionQ8* call) {
+  const auto& [q, k_codes, k_scales, v_codes, v_scales, block_table, q_start, ctx_len, seq_of_token, out, scratch, arrivals, status, stream, max_blocks,
+               dtype, num_tokens, num_seqs, num_heads, num_kv_heads, page_size, num_pages, window, skip_single, has_portions, max_q_len, others, splits,
+               cluster, tiles, scale] = *call;
   using namespace tcq8;
   if (num_seqs <= 0 || num_tokens <= 0 || tiles <= 0) return SHRIKE_OK;
   if (num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads || num_heads / num_kv_heads > 64 || max_blocks <= 0 || num_pages <= 0 ||
@@ -919,10 +919,6 @@ SHRIKE_API int shrike_paged_attention_q8_tc(const void* q, const void* k_codes, 
 
 SHRIKE_API int shrike_attention_q8_tc_tokens(int) { return 0; }
 SHRIKE_API int shrike_attention_q8_tc_splits(int, int, long long) { return 1; }
-SHRIKE_API int shrike_paged_attention_q8_tc(const void*, const void*, const float*, const void*, const float*, const int*, int, const int*,
-                                            const int*, const int*, int, int, int, int, int, int, float, int, void*, int, int, int,
-                                            float*, int*, cudaStream_t) {
-  return SHRIKE_BAD_ARGUMENT;
-}
+SHRIKE_API int shrike_paged_attention_q8_tc(const ShrikeAttentionQ8*) { return SHRIKE_BAD_ARGUMENT; }
 
 #endif

@@ -262,11 +262,22 @@ static bool good_pages(const void* codes, const void* scales) {
 
 using namespace cacheq8;
 
-// k_new and v_new: n rows of kv_heads * dim elements of `dtype`, `k_stride` / `v_stride` elements apart.  Rows whose slot is
-// not one of the pool's are left out; the others' slots have to differ from one another.
-SHRIKE_API int shrike_kv_write_q8(const void* k_new, const void* v_new, long long k_stride, long long v_stride, void* k_codes,
-                                  float* k_scales, void* v_codes, float* v_scales, const int* slots, int dtype, int n, int kv_heads,
-                                  int dim, int page_size, long long num_slots, cudaStream_t stream) {
+// The arguments of a store or a reading back, packed by the caller (a call with a dozen arguments costs more to make than the
+// kernel takes for a token): rows k and v, `k_stride` / `v_stride` elements apart where they are stored, dense where they are read.
+struct ShrikeCacheQ8 {
+  void *k, *v, *k_codes, *v_codes;
+  float *k_scales, *v_scales;
+  const int* slots;
+  cudaStream_t stream;
+  long long k_stride, v_stride;
+  int dtype, n, kv_heads, dim, pages, page_size;
+};
+
+// Stores n rows of kv_heads * dim elements of `dtype`.  Rows whose slot is not one of the pool's are left out; the others' slots
+// have to differ from one another.
+SHRIKE_API int shrike_kv_write_q8(const ShrikeCacheQ8* call) {
+  const auto [k_new, v_new, k_codes, v_codes, k_scales, v_scales, slots, stream, k_stride, v_stride, dtype, n, kv_heads, dim, pages, page_size] = *call;
+  const long long num_slots = static_cast<long long>(pages) * page_size;
   if (n <= 0) return SHRIKE_OK;
   if (kv_heads <= 0 || dim <= 0 || dim % 16 || dim > 256 || page_size <= 0 || !good_pages(k_codes, k_scales) ||
       !good_pages(v_codes, v_scales) || (dtype != SHRIKE_F32 && dtype != SHRIKE_BF16))
@@ -316,17 +327,16 @@ SHRIKE_API int shrike_rope_kv_write_q8(const float* qkv, const float* bias, cons
   return err == cudaSuccess ? shrike_launch_status() : static_cast<int>(err);
 }
 
-// k_out and v_out: n rows of kv_heads * dim elements of `dtype`, 16-byte aligned; rows whose slot is not one of the pool's
-// become zeros.
-SHRIKE_API int shrike_kv_read_q8(const void* k_codes, const float* k_scales, const void* v_codes, const float* v_scales,
-                                 const int* slots, void* k_out, void* v_out, int dtype, int n, int kv_heads, int dim, int page_size,
-                                 long long num_slots, cudaStream_t stream) {
+// Reads n rows of kv_heads * dim elements of `dtype` back to k and v, 16-byte aligned and dense; rows whose slot is not one of
+// the pool's become zeros.
+SHRIKE_API int shrike_kv_read_q8(const ShrikeCacheQ8* call) {
+  const auto [k_out, v_out, k_codes, v_codes, k_scales, v_scales, slots, stream, k_stride, v_stride, dtype, n, kv_heads, dim, pages, page_size] = *call;
+  const long long num_slots = static_cast<long long>(pages) * page_size;
   if (n <= 0) return SHRIKE_OK;
   if (kv_heads <= 0 || dim <= 0 || dim % 16 || page_size <= 0 || !good_pages(k_codes, k_scales) || !good_pages(v_codes, v_scales) ||
       (reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out)) % 16)
     return SHRIKE_BAD_ARGUMENT;
-  const Pages keys{static_cast<signed char*>(const_cast<void*>(k_codes)), const_cast<float*>(k_scales)};
-  const Pages values{static_cast<signed char*>(const_cast<void*>(v_codes)), const_cast<float*>(v_scales)};
+  const Pages keys{static_cast<signed char*>(k_codes), k_scales}, values{static_cast<signed char*>(v_codes), v_scales};
   const unsigned per_row = static_cast<unsigned>(kv_heads) * static_cast<unsigned>(dim / 16);
   const long long chunks = static_cast<long long>(n) * per_row, blocks = (chunks + 255) / 256;
   if (blocks > 0x7fffffff || num_slots > 0x7fffffff) return SHRIKE_BAD_ARGUMENT;

@@ -8,6 +8,7 @@ belong on one stream at a time, captured launch sequences included.
 from __future__ import annotations
 
 import ctypes
+import struct
 from dataclasses import dataclass
 
 import torch
@@ -19,6 +20,12 @@ _c = ctypes
 _P, _I, _F, _LL = _c.c_void_p, _c.c_int, _c.c_float, _c.c_longlong
 DTYPE_CODE = {torch.float32: 0, torch.bfloat16: 1}
 MOST_HEAD_DIM = 256   # of the kernels over 8-bit pages
+# The launchers take their arguments as one packed structure (ShrikeCacheQ8, ShrikeAttentionQ8): a call of thirty arguments takes
+# ctypes two microseconds, this a third of one.
+_CACHE_CALL = struct.Struct("=8Q2q6i")
+_ATTENTION_CALL = struct.Struct("=14Q16if")
+_device = getattr(torch._C, "_cuda_getDevice", None)          # the current device's number, and its current stream's handle:
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)   # asking torch for the objects costs more than a launch
 
 
 @dataclass(frozen=True, slots=True)
@@ -35,6 +42,11 @@ class QuantisedPlan:
     tiles: int = 0        # query tiles that the tcgen05 kernel's portions make
     portion_splits: int = 1   # CTAs that share the keys of one
     portion_scratch: torch.Tensor | None = None
+    lib: object = None
+
+    @property
+    def launches(self) -> int:
+        return int(self.has_single) + int(self.has_portions) + (self.portion_splits > 1)
 
 
 def _error(text):
@@ -43,12 +55,17 @@ def _error(text):
     return KernelError(text)
 
 
+def _failed(code: int, what: str):
+    from .cuda_ops import _check
+
+    _check(code, what)
+
+
 def quantised(keys, values) -> bool:
     """Whether a layer's cache is of 8-bit pages; both tensors of a layer have to be of one form."""
-    forms = (isinstance(keys, QuantisedPages), isinstance(values, QuantisedPages))
-    if forms[0] != forms[1]:
+    if (type(keys) is QuantisedPages) != (type(values) is QuantisedPages):
         raise _error("keys and values must both be 8-bit pages, or neither")
-    return forms[0]
+    return type(keys) is QuantisedPages
 
 
 class QuantisedCacheOps:
@@ -57,9 +74,8 @@ class QuantisedCacheOps:
     Q8_SCRATCH_FLOATS = 64 << 20   # at most 256 MiB for the shares of split rows: fewer splits beyond that
 
     def _declare_q8_core(self, lib):
-        lib.shrike_kv_write_q8.argtypes = [_P, _P, _LL, _LL, _P, _P, _P, _P, _P] + [_I] * 5 + [_LL, _P]
+        lib.shrike_kv_write_q8.argtypes = lib.shrike_kv_read_q8.argtypes = [_c.c_char_p]
         lib.shrike_rope_kv_write_q8.argtypes = [_P] * 10 + [_I] * 6 + [_LL, _I, _LL, _P]
-        lib.shrike_kv_read_q8.argtypes = [_P] * 7 + [_I] * 5 + [_LL, _P]
         for name in ("shrike_kv_write_q8", "shrike_rope_kv_write_q8", "shrike_kv_read_q8"):
             getattr(lib, name).restype = _I
         self._q8_libs, self._q8_plans = {}, {}
@@ -72,9 +88,8 @@ class QuantisedCacheOps:
             if head_dim % 16 or not 16 <= head_dim <= MOST_HEAD_DIM:
                 raise _error(f"head size {head_dim} is not served: 8-bit pages take multiples of 16 from 16 to {MOST_HEAD_DIM}")
             lib = build.attention_q8_library(head_dim)
-            lib.shrike_paged_attention_q8.argtypes = [_P] * 6 + [_I, _P, _P] + [_I] * 6 + [_F, _I, _P] + [_I] * 6 + [_P, _P, _P]
+            lib.shrike_paged_attention_q8.argtypes = lib.shrike_paged_attention_q8_tc.argtypes = [_c.c_char_p]
             lib.shrike_paged_attention_q8.restype = _I
-            lib.shrike_paged_attention_q8_tc.argtypes = [_P] * 6 + [_I] + [_P] * 3 + [_I] * 6 + [_F, _I, _P] + [_I] * 3 + [_P] * 3
             lib.shrike_attention_q8_tc_tokens.argtypes = [_I]
             lib.shrike_attention_q8_tc_splits.argtypes = [_I, _I, _LL]
             for name in ("shrike_paged_attention_q8_tc", "shrike_attention_q8_tc_tokens", "shrike_attention_q8_tc_splits"):
@@ -92,9 +107,9 @@ class QuantisedCacheOps:
     # A call of the engine's takes longer on the host than its kernel takes for few tokens, so what is right is seen in one
     # expression of cheap questions; which of them failed is looked up only then.
     def _q8_stream(self):
-        """The current stream's handle and device (asking torch for the stream object costs more than a launch)."""
-        device = torch._C._cuda_getDevice()
-        return device, self._held_stream if self._held_stream is not None else torch._C._cuda_getCurrentRawStream(device)
+        """The current device and the handle of its current stream (or of the one that is held)."""
+        device = _device()
+        return device, _raw_stream(device) if self._held_stream is None else self._held_stream
 
     @staticmethod
     def _q8_refuse(device, named, ints=(), pages=None):
@@ -129,18 +144,18 @@ class QuantisedCacheOps:
 
     @staticmethod
     def _q8_pages_fit(device, keys, values) -> bool:
-        codes, others = keys.codes, values.codes
-        count, page_size, _heads, dim = codes.shape
-        return (codes.shape == others.shape and codes.get_device() == device and others.get_device() == device
-                and not dim % 16 and 16 <= dim <= MOST_HEAD_DIM and count * page_size <= 0x7FFFFFFF)
+        dims = keys.dims
+        return (dims == values.dims and keys.device_index == device and values.device_index == device and not dims[3] % 16
+                and 16 <= dims[3] <= MOST_HEAD_DIM and dims[0] * dims[1] <= 0x7FFFFFFF and not keys.codes.data_ptr() % 16
+                and not values.codes.data_ptr() % 16)
 
     @staticmethod
     def _q8_ints_fit(device, tensor, count) -> bool:
-        return tensor.get_device() == device and tensor.dtype == torch.int32 and tensor.numel() == count and tensor.is_contiguous()
+        return tensor.get_device() == device and tensor.dtype is torch.int32 and tensor.numel() == count and tensor.is_contiguous()
 
     def _q8_rows(self, device, x, n, width, what):
         """The distance of x's rows in elements; a row's elements lie side by side."""
-        if (x.get_device() != device or x.dtype != self.dtype or tuple(x.shape) != (n, width) or (width > 1 and x.stride(1) != 1)
+        if (x.get_device() != device or x.dtype is not self.dtype or x.shape != (n, width) or (width > 1 and x.stride(1) != 1)
                 or (n > 1 and x.stride(0) < 0)):
             raise _error(f"{what} must be {self.dtype} [{n}, {width}] with adjacent columns on cuda:{device}, is {x.dtype} "
                          f"{list(x.shape)} on {x.device}")
@@ -148,10 +163,8 @@ class QuantisedCacheOps:
 
     # ---- the cache
     def _kv_write_q8(self, k_new, v_new, keys, values, slots):
-        from .cuda_ops import _check
-
         device, stream = self._q8_stream()
-        pages, page_size, heads, dim = keys.codes.shape
+        pages, page_size, heads, dim = keys.dims
         n = k_new.shape[0]
         if not (self._q8_pages_fit(device, keys, values) and self._q8_ints_fit(device, slots, n)):
             self._q8_refuse(device, (), [(slots, n, "slots")], (keys, values, None, None))
@@ -160,16 +173,17 @@ class QuantisedCacheOps:
         if n == 0:
             return
         self.launches += 1
-        _check(self.core.shrike_kv_write_q8(
-            k_new.data_ptr(), v_new.data_ptr(), k_stride, v_stride, keys.codes.data_ptr(), keys.scales.data_ptr(),
-            values.codes.data_ptr(), values.scales.data_ptr(), slots.data_ptr(), self.code, n, heads, dim, page_size,
-            pages * page_size, stream), "kv_write_q8")
+        code = self.core.shrike_kv_write_q8(_CACHE_CALL.pack(
+            k_new.data_ptr(), v_new.data_ptr(), keys.codes.data_ptr(), values.codes.data_ptr(), keys.scales.data_ptr(),
+            values.scales.data_ptr(), slots.data_ptr(), stream, k_stride, v_stride, self.code, n, heads, dim, pages, page_size))
+        if code:
+            _failed(code, "kv_write_q8")
 
     def _rope_kv_write_q8(self, qkv, bias, positions, inv_freq, q_out, keys, values, slots, num_heads, num_kv_heads, head_dim):
         from .cuda_ops import _check, _ptr
 
         device, stream = self._q8_stream()
-        pages, page_size, _heads, _dim = keys.codes.shape
+        pages, page_size, _heads, _dim = keys.dims
         partials, stride = self._stack(qkv)
         n, width = qkv.shape[-2], (num_heads + 2 * num_kv_heads) * head_dim
         self._q8_refuse(device, [(q_out, self.dtype, "q")] + [(x, torch.float32, what) for x, what in (
@@ -196,17 +210,15 @@ class QuantisedCacheOps:
         """Reads tokens back from 8-bit pages: row n of `k_out` and `v_out` ([N, kv heads * head size], contiguous, in the engine's
         type) is what `slots[n]` (int32 [N]) holds, codes times scale in 32 bits rounded once; zeros for a slot that is none of
         the pool's (a negative one, say).  A row stored from an infinity or a NaN comes back as NaN."""
-        from .cuda_ops import _check
-
         if not quantised(keys, values):
             raise _error("kv_read reads 8-bit pages; a cache in the engine's type is indexed as it is")
         device, stream = self._q8_stream()
-        pages, page_size, heads, dim = keys.codes.shape
+        pages, page_size, heads, dim = keys.dims
         n, dtype = slots.numel(), self.dtype
         k_at, v_at = k_out.data_ptr(), v_out.data_ptr()
         shape = (n, heads * dim)
-        if not (self._q8_pages_fit(device, keys, values) and self._q8_ints_fit(device, slots, n) and k_out.dtype == dtype
-                and v_out.dtype == dtype and k_out.shape == shape and v_out.shape == shape and k_out.get_device() == device
+        if not (self._q8_pages_fit(device, keys, values) and self._q8_ints_fit(device, slots, n) and k_out.dtype is dtype
+                and v_out.dtype is dtype and k_out.shape == shape and v_out.shape == shape and k_out.get_device() == device
                 and v_out.get_device() == device and k_out.is_contiguous() and v_out.is_contiguous() and not (k_at | v_at) % 16):
             self._q8_refuse(device, [(k_out, dtype, "keys read"), (v_out, dtype, "values read")], [(slots, n, "slots")],
                             (keys, values, None, None))
@@ -214,9 +226,11 @@ class QuantisedCacheOps:
         if n == 0:
             return
         self.launches += 1
-        _check(self.core.shrike_kv_read_q8(
-            keys.codes.data_ptr(), keys.scales.data_ptr(), values.codes.data_ptr(), values.scales.data_ptr(), slots.data_ptr(),
-            k_at, v_at, self.code, n, heads, dim, page_size, pages * page_size, stream), "kv_read_q8")
+        code = self.core.shrike_kv_read_q8(_CACHE_CALL.pack(
+            k_at, v_at, keys.codes.data_ptr(), values.codes.data_ptr(), keys.scales.data_ptr(), values.scales.data_ptr(),
+            slots.data_ptr(), stream, 0, 0, self.code, n, heads, dim, pages, page_size))
+        if code:
+            _failed(code, "kv_read_q8")
 
     # ---- attention
     def q8_plan(self, num_heads, num_kv_heads, head_dim, num_seqs, max_blocks, page_size, max_q_len, min_q_len, window=0, num_tokens=0,
@@ -273,7 +287,7 @@ class QuantisedCacheOps:
                     self._q8_portion_scratch = torch.empty(max(need, 1 << 22), dtype=torch.float32, device=self.device)
                     self.generation += 1
                 portion_scratch = self._q8_portion_scratch
-        plan = QuantisedPlan(has_single, has_portions, tc_portions, splits, cluster, scratch, arrivals, tiles, portion_splits, portion_scratch)
+        plan = QuantisedPlan(has_single, has_portions, tc_portions, splits, cluster, scratch, arrivals, tiles, portion_splits, portion_scratch, lib)
         if len(self._q8_plans) >= 4096:
             self._q8_plans.clear()
         self._q8_plans[key] = (self.generation, plan)
@@ -297,16 +311,14 @@ class QuantisedCacheOps:
 
     def _paged_attention_q8(self, q, keys, values, block_table, q_start, ctx_len, seq_of_token, num_heads, num_kv_heads, head_dim,
                             scale, window, out, max_q_len, min_q_len, q_lens):
-        from .cuda_ops import _check, _ptr
-
         device, stream = self._q8_stream()
-        pages, page_size, heads, dim = keys.codes.shape
+        pages, page_size, heads, dim = keys.dims
         num_seqs, max_blocks = block_table.shape
         n, dtype = q.shape[0], self.dtype
         q_at, out_at = q.data_ptr(), out.data_ptr()
         shape = (n, num_heads * head_dim)
         if not (self._q8_pages_fit(device, keys, values) and heads == num_kv_heads and dim == head_dim and not num_heads % heads
-                and q.dtype == dtype and out.dtype == dtype and q.shape == shape and out.shape == shape and q.get_device() == device
+                and q.dtype is dtype and out.dtype is dtype and q.shape == shape and out.shape == shape and q.get_device() == device
                 and out.get_device() == device and q.is_contiguous() and out.is_contiguous() and not (q_at | out_at) % 16
                 and self._q8_ints_fit(device, block_table, num_seqs * max_blocks) and self._q8_ints_fit(device, q_start, num_seqs + 1)
                 and self._q8_ints_fit(device, ctx_len, num_seqs) and max_q_len >= 1):
@@ -320,22 +332,28 @@ class QuantisedCacheOps:
             raise _error(f"q {list(q.shape)} and output {list(out.shape)} must be [tokens, {num_heads * head_dim}]")
         if n == 0 or num_seqs == 0:
             return
-        plan = self.q8_plan(num_heads, num_kv_heads, head_dim, num_seqs, max_blocks, page_size, max_q_len, min_q_len, window or 0, n, q_lens)
-        lib, has_portions = self._q8_libs[head_dim], plan.has_portions
-        pages_at = (keys.codes.data_ptr(), keys.scales.data_ptr(), values.codes.data_ptr(), values.scales.data_ptr(), block_table.data_ptr(),
-                    max_blocks, q_start.data_ptr(), ctx_len.data_ptr())
-        self.launches += plan.has_single + has_portions + (plan.portion_splits > 1)
-        if plan.tc_portions:
-            if not self._q8_ints_fit(device, seq_of_token, n):
-                self._q8_refuse(device, (), [(seq_of_token, n, "sequences of tokens")])
-            _check(lib.shrike_paged_attention_q8_tc(
-                q_at, *pages_at, seq_of_token.data_ptr(), n, num_seqs, num_heads, num_kv_heads, page_size, pages, scale, window or 0,
-                out_at, plan.has_single, plan.tiles, plan.portion_splits, _ptr(plan.portion_scratch), self.status.data_ptr(), stream),
-                "paged_attention_q8_tc")
+        window = window or 0
+        plan = self.q8_plan(num_heads, num_kv_heads, head_dim, num_seqs, max_blocks, page_size, max_q_len, min_q_len, window, n, q_lens)
+        tc, has_portions = plan.tc_portions, plan.has_portions
+        if tc and not self._q8_ints_fit(device, seq_of_token, n):
+            self._q8_refuse(device, (), [(seq_of_token, n, "sequences of tokens")])
+        at = (q_at, keys.codes.data_ptr(), keys.scales.data_ptr(), values.codes.data_ptr(), values.scales.data_ptr(),
+              block_table.data_ptr(), q_start.data_ptr(), ctx_len.data_ptr())
+        sizes = (max_blocks, self.code, n, num_seqs, num_heads, num_kv_heads, page_size, pages, window, plan.has_single)
+        self.launches += plan.launches
+        if tc:
+            scratch = plan.portion_scratch
+            code = plan.lib.shrike_paged_attention_q8_tc(_ATTENTION_CALL.pack(
+                *at, seq_of_token.data_ptr(), out_at, 0 if scratch is None else scratch.data_ptr(), 0, self.status.data_ptr(), stream,
+                *sizes, 1, max_q_len, 0, plan.portion_splits, 1, plan.tiles, scale))
+            if code:
+                _failed(code, "paged_attention_q8_tc")
             has_portions = False
             if not plan.has_single:
                 return
-        _check(lib.shrike_paged_attention_q8(
-            q_at, *pages_at, self.code, num_seqs, num_heads, num_kv_heads, page_size, pages, scale, window or 0, out_at, plan.has_single,
-            has_portions, max_q_len, 1 if plan.tc_portions else 0, plan.splits, plan.cluster, _ptr(plan.scratch), _ptr(plan.arrivals), stream),
-            "paged_attention_q8")
+        scratch, arrivals = plan.scratch, plan.arrivals
+        code = plan.lib.shrike_paged_attention_q8(_ATTENTION_CALL.pack(
+            *at, 0, out_at, 0 if scratch is None else scratch.data_ptr(), 0 if arrivals is None else arrivals.data_ptr(), 0, stream,
+            *sizes, has_portions, max_q_len, tc, plan.splits, plan.cluster, 0, scale))
+        if code:
+            _failed(code, "paged_attention_q8")
