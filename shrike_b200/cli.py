@@ -12,7 +12,7 @@ conversation.  A model folder without tokenizer files is served too: a line of
 space-separated token ids is the prompt then, and ids are printed back.
 
     python -m shrike_b200.cli --model DIR | --random SHAPE [--seed 0]
-        [--dtype bfloat16|float32] [--block-size 16] [--num-blocks N] [--gpu-mem-util 0.85]
+        [--dtype bfloat16|float32] [--kv-cache int8] [--block-size 16] [--num-blocks N] [--gpu-mem-util 0.85]
         [--max-tokens-per-step 512] [--max-running 256]
 
 `--random SHAPE` starts without a checkpoint: SHAPE names one of the package's shape
@@ -43,6 +43,8 @@ def add_engine_options(parser: argparse.ArgumentParser) -> None:
                         help="no checkpoint: a named shape or a config.json, filled with random weights")
     parser.add_argument("--seed", type=int, default=0, help="seed of random weights and of sampling")
     parser.add_argument("--dtype", default=None, choices=["bfloat16", "float32"])
+    parser.add_argument("--kv-cache", default=None, choices=["int8"],
+                        help="keep keys and values as 8-bit codes with a scale per token and head (default: in the engine's dtype)")
     parser.add_argument("--block-size", type=int, default=16)
     parser.add_argument("--num-blocks", type=int, default=None)
     parser.add_argument("--gpu-mem-util", type=float, default=0.85)
@@ -61,6 +63,8 @@ def open_engine(args):
     options = dict(block_size=args.block_size, gpu_mem_util=args.gpu_mem_util,
                    max_tokens_per_step=args.max_tokens_per_step, max_running=args.max_running,
                    num_blocks=args.num_blocks, dtype=args.dtype, seed=args.seed)
+    if getattr(args, "kv_cache", None) is not None:
+        options["kv_cache"] = args.kv_cache
     if args.random is not None:
         engine, name = llm_engine.LLMEngine.from_random(args.random, **options), f"random weights, shape {args.random}"
     else:

@@ -6,7 +6,8 @@ constructor's `block_size`, `gpu_mem_util`, `max_tokens_per_step`, `max_running`
 `step() -> [StepOutput(req_id, token_id, finished, finish_reason)]`,
 `generate(prompts, sampling) -> [[token ids]]`, `metrics()`, and the attributes
 `requests`, `scheduler`, `block_manager`, `tokenizer`, `stats`.  Added: `num_blocks`
-(an explicit pool size), `dtype` ("bfloat16" or "float32"), `seed`.  Left out:
+(an explicit pool size), `dtype` ("bfloat16" or "float32"), `seed`, `kv_cache`
+(None or "int8").  Left out:
 prefix caching and speculation.  step() = schedule -> one batched forward -> sample
 -> append / finish (engine.py:109-164); the sampled token of a request whose step
 reached the end of its known tokens comes from that entry's last row
@@ -28,7 +29,7 @@ from ..sampling.rng import step_seed
 from ..weights.loader import load_weights
 from .batch import StepEntry
 from .request import Request, SamplingParams
-from .runner import TORCH_DTYPES, ModelRunner
+from .runner import TORCH_DTYPES, ModelRunner, check_kv_cache
 from .scheduler import Scheduler
 
 
@@ -77,15 +78,20 @@ class LLMEngine:
         config=None,
         tensors=None,
         ops=None,
+        kv_cache: str | None = None,
     ) -> None:
         """`model_dir` holds config.json and *.safetensors; or pass `config` and
-        `tensors` (name -> tensor on `device`) to serve weights made in memory."""
+        `tensors` (name -> tensor on `device`) to serve weights made in memory.
+        `kv_cache="int8"` keeps keys and values as 8-bit codes with a scale per token and
+        kv head (`cache/quantised.py`): twice the blocks in the same memory, half the cache
+        bytes a decode step reads, and logits that differ by what 8 bits leave out."""
         if config is None:
             config = load_config(model_dir)
         self.config = config
         self.dtype = dtype or config.dtype
         if self.dtype not in TORCH_DTYPES:
             raise ValueError(f"dtype {self.dtype!r}: choose bfloat16 or float32")
+        check_kv_cache(kv_cache, config)   # before weights are read
         self.device = torch.device(device)
         self.ops = ops if ops is not None else make_ops(self.dtype, self.device)
         if tensors is None:
@@ -94,7 +100,7 @@ class LLMEngine:
         self.runner = ModelRunner(
             config, tensors, self.ops, self.device, self.dtype, page_size=block_size,
             num_pages=num_blocks, gpu_mem_util=gpu_mem_util, max_slots=max_running,
-            max_portion=max_tokens_per_step,
+            max_portion=max_tokens_per_step, kv_cache=kv_cache,
         )
         self.block_manager = self.runner.cache
         self.scheduler = Scheduler(self.block_manager, max_tokens_per_step, max_running)

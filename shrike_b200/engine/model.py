@@ -22,9 +22,10 @@ class Runtime:
     A named buffer keeps its address while its capacity suffices, so captured
     launch sequences stay valid; the same name is reused by every layer."""
 
-    def __init__(self, device, act_dtype: torch.dtype):
+    def __init__(self, device, act_dtype: torch.dtype, quantised_cache: bool = False):
         self.device = torch.device(device)
         self.act_dtype = act_dtype
+        self.quantised_cache = quantised_cache   # keys and values lie in 8-bit pages: layers run part by part
         self._buffers: dict[str, torch.Tensor] = {}
         self._views: dict = {}   # (name, shape, dtype) -> view, while the buffer has not moved
         self.generation = 0  # grows when a buffer moves
@@ -118,7 +119,7 @@ class DecoderModel:
         self.capture_safe = all(getattr(part, "capture_safe", False) for part in parts)
         # decode steps of few sequences may run as one kernel where the kernels offer that for these layers
         offer = getattr(ops, "decode_step", None)
-        plain = self.pass_entry is None and self.side_table is None and self.residual is None
+        plain = self.pass_entry is None and self.side_table is None and self.residual is None and not runtime.quantised_cache
         self._whole_step = offer(runtime, self.blocks, config.order) if offer is not None and plain else None
 
     def cache_needs(self):

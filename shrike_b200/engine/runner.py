@@ -19,6 +19,24 @@ from .batch import BatchBuilder, StepEntry
 from .model import DecoderModel, Runtime
 
 TORCH_DTYPES = {"bfloat16": torch.bfloat16, "float32": torch.float32}
+KV_CACHES = (None, "int8")   # keys and values in the engine's type, or as 8-bit codes with a scale per token and kv head
+
+
+def check_kv_cache(kv_cache, config) -> None:
+    """Raises ValueError when the model's layers do not keep their keys and values in that form."""
+    from ..parts.base import KVNeed, part_class
+
+    if kv_cache not in KV_CACHES:
+        raise ValueError(f"kv_cache {kv_cache!r}: choose None (the engine's dtype) or 'int8'")
+    if kv_cache is None:
+        return
+    for index, layer in enumerate(config.layers):
+        cls = part_class("mixer", layer.mixer.kind)
+        for need in cls.cache_needs(layer.mixer):
+            if isinstance(need, KVNeed) and not getattr(cls, "quantised_cache", False):
+                raise ValueError(f"kv_cache 'int8': layer {index} ({layer.mixer.kind}) keeps its cache in the engine's dtype only")
+            if isinstance(need, KVNeed) and (need.head_dim % 16 or not 16 <= need.head_dim <= 256):
+                raise ValueError(f"kv_cache 'int8': layer {index} has heads of {need.head_dim}; multiples of 16 from 16 to 256 are served")
 
 
 class Prepared:
@@ -48,8 +66,11 @@ class ModelRunner:
         gpu_mem_util: float = 0.85,
         max_slots: int = 256,
         max_portion: int | None = None,
+        kv_cache: str | None = None,
     ):
-        """`num_pages`: pages of every group (an int) or of each group (a list); None sizes the pools
+        """`kv_cache`: None keeps keys and values in `dtype`, "int8" as 8-bit codes with a float32 scale per token and kv head
+        (about half, or a quarter, of the memory, and of the bytes a decode step reads).
+        `num_pages`: pages of every group (an int) or of each group (a list); None sizes the pools
         from free device memory: `gpu_mem_util` of it, less the per-request state of `max_slots`
         requests, shared out by `pages_per_group` (groups that keep every key get equal counts, a
         group with a window what `max_slots` requests fed `max_portion` tokens a step can hold)."""
@@ -57,13 +78,15 @@ class ModelRunner:
         self.device = torch.device(device)
         self.dtype = TORCH_DTYPES[dtype]
         self.ops = ops
-        self.runtime = Runtime(self.device, self.dtype)
+        check_kv_cache(kv_cache, config)
+        self.kv_cache = kv_cache
+        self.runtime = Runtime(self.device, self.dtype, quantised_cache=kv_cache is not None)
         self.model = DecoderModel(config, tensors, ops, self.runtime)
         kv_needs, state_needs = self.model.cache_needs()
         self.groups = group_caches(kv_needs)
         self.page_size = page_size
         element = torch.empty((), dtype=self.dtype).element_size()
-        per_group = [page_bytes(g, page_size, element) for g in self.groups]
+        per_group = [page_bytes(g, page_size, element, kv_cache is not None) for g in self.groups]
         self.bytes_per_page = sum(per_group)
         self.state_bytes = state_bytes(state_needs, max_slots)
         if num_pages is None:
@@ -83,7 +106,7 @@ class ModelRunner:
         self.num_pages = list(num_pages)
         self.cache = CacheManager(self.groups, page_size, num_pages, max_slots)
         self.storage = CacheStorage(
-            self.groups, page_size, num_pages, state_needs, max_slots, self.dtype, self.device
+            self.groups, page_size, num_pages, state_needs, max_slots, self.dtype, self.device, kv_cache is not None
         )
         self.builder = BatchBuilder(page_size, len(self.groups), self.device, self.storage)
         self.builder.watches_pages = self.model.has_one_kernel

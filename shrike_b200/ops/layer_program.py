@@ -101,6 +101,8 @@ class LayerProgram:
             return False
         if type(mixer) is not PagedAttention or type(feed_forward) is not GatedMLP:
             return False
+        if mixer.runtime.quantised_cache:   # the native issue takes a cache in the engine's type
+            return False
         if type(mixer_norm) is not RMSNorm or type(feed_forward_norm) is not RMSNorm:
             return False
         if mixer.position is not None and mixer.position.rotary_table() is None:

@@ -34,6 +34,7 @@ from .rotary import PairRotation
 
 class PagedAttention:
     capture_safe = True   # forward() launches the same kernels for the same batch shape, whatever the positions
+    quantised_cache = True   # its keys and values may lie in 8-bit pages: the kernels take either form of pages
 
     @staticmethod
     def parameters(spec) -> dict[str, ParamSpec]:

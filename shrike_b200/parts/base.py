@@ -56,6 +56,9 @@ be checked and the cache sized before anything is put on the device):
       forward(hidden[R,W]) -> float32 logits [R, vocab]   (hidden: the final norm's output on the
           wanted rows); built with tensors {"weight": ...}, the embedding's table when tied
 
+A mixer that keeps keys and values may declare `quantised_cache = True`: `ctx.storage.keys_values` may then hand it
+`QuantisedPages` in place of tensors, which it passes on to kernels that take both.
+
 A part may declare the class attribute `capture_safe = True`.  It then promises that forward()
 launches the same kernels with the same sizes for the same batch shape, whatever the positions,
 slots and pages of the step (so a recorded launch sequence can be replayed), and that it leaves
