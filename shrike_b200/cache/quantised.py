@@ -19,7 +19,7 @@ class QuantisedPages:
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor):
         dims = tuple(codes.shape)
         if not (codes.dtype is torch.int8 and len(dims) == 4 and codes.is_contiguous() and scales.dtype is torch.float32
-                and scales.shape == (dims[0], dims[2], dims[1]) and scales.is_contiguous() and codes.get_device() == scales.get_device()):
+                and scales.shape == (dims[0], dims[2], dims[1]) and scales.is_contiguous() and codes.device == scales.device):
             self._refuse(codes, scales)
         self.codes, self.scales = codes, scales
         self.dims, self.device_index = dims, codes.get_device()   # (pages, page_size, kv heads, head size); -1: not on a GPU
