@@ -13,10 +13,13 @@
 // turn them into float16 tiles in the 128-byte swizzle (four the keys', four the values'; two threads a key), and those are
 // what the products read.  Eight codes take 10 instructions (a byte permutation and a subtraction a pair, an exclusive or for
 // four).
-// The softmax is bound by the latency of its instructions, not by their number: with a thread a row (eight warps, as the kernel
-// over bfloat16 pages has) a step of 64 keys takes 2,700 clocks, and leaving out the exponentials, the scales' products or the
-// conversion saves 8 to 10 % each.  So two threads share a row, each with 32 of a step's keys: twice the warps to hide latency
-// with, half the unrolled code.  They agree on the row's base through a barrier of their two warps that says whether anyone's
+// The softmax is bound by the latency of its instructions more than by their number: with a thread a row (eight warps, as the
+// kernel over bfloat16 pages has) leaving out the exponentials, the scales' products or the conversion saved 8 to 10 % each.
+// So two threads share a row, each with 32 of a step's keys: twice the warps to hide latency with, half the unrolled code (a
+// prompt of 2,048 tokens, 28 heads: 66 us and 58).  Now issue slots and shared memory's bandwidth bound it together: a step of
+// 64 keys takes about 2,800 clocks of two chains, in which an SM issues 64 % of what it could, and 190 KB go to and from
+// shared memory (queries and keys of the first product 96, values 32, codes 16, conversion 48), 1,500 clocks of its bandwidth,
+// beside 1,024 each of the tensor pipe and of the special-function units.  They agree on the row's base through a barrier of their two warps that says whether anyone's
 // has to move (rarely), and only then exchange their maxima.
 //
 // Roles: warp 0 brings key codes (and the queries), warp 3 value codes (and owns tensor memory), warps 1 and 2 issue the products
@@ -45,7 +48,8 @@ constexpr int D = SHRIKE_HEAD_DIM;
 constexpr int BM = 128;                         // query rows of one chain
 constexpr int HALVES = D / 64;                 // 64-element groups of the head size
 constexpr int Q_HALF = BM * 128;               // bytes of one 64-element-wide sub-tile of a query tile
-constexpr int Q_BYTES = HALVES * Q_HALF;
+constexpr int Q_BYTES = 2 * Q_HALF;              // room for a query tile, and for 64 elements of 128 rows of 32-bit output
+static_assert(HALVES * Q_HALF <= Q_BYTES && BM * 256 <= Q_BYTES, "the output's pieces leave by way of the query tile");
 constexpr int KEYS = 64;                       // keys of a tile, and of a softmax step
 constexpr int STAGES = 3, RAW_STAGES = 3;
 constexpr int KV_HALF = KEYS * 128;            // bytes of one 64-element-wide sub-tile of a float16 key (or value) tile
@@ -412,8 +416,8 @@ portions_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
           umma_commit(leader, &sh->s_full[c]);
           umma_commit(leader, &sh->k_free[st]);
         };
-        // the later chain starts most of a step behind the earlier one
-        if (ok && c == 1 && steps_0 > 0) ok = wait_for(&sh->stagger, 0);
+        // the later chain starts most of a step behind the earlier one, where that is not most of its time
+        if (ok && c == 1 && steps_0 > 4) ok = wait_for(&sh->stagger, 0);
         if (ok) issue_scores(0);
         for (int h = 0; h < steps && ok; ++h) {
           if (h + 1 < steps) {
@@ -530,32 +534,39 @@ portions_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       constexpr int MINE = HALVES * 4;   // 16-byte chunks of this thread
       unsigned char* q_row = q_tiles + chain * Q_BYTES + row * 128;
       auto chunk_of = [&](int c) { return reinterpret_cast<uint4*>(q_row + ((sub * MINE + c) / 8) * Q_HALF + ((((sub * MINE + c) % 8) ^ (row & 7)) << 4)); };
-      unsigned top = 0u;
+      uint4 x[MINE];
+      unsigned top = 0u;   // the largest magnitude's upper sixteen bits
       if (ok) {
 #pragma unroll
         for (int c = 0; c < MINE; ++c) {
-          const uint4 v = *chunk_of(c);
-          const unsigned w[4] = {v.x, v.y, v.z, v.w};
+          x[c] = *chunk_of(c);
+          top = __vmaxu2(top, __vmaxu2(__vmaxu2(x[c].x & 0x7fff7fffu, x[c].y & 0x7fff7fffu), __vmaxu2(x[c].z & 0x7fff7fffu, x[c].w & 0x7fff7fffu)));
+        }
+        top = max(top & 0xffffu, top >> 16);
+        if (top >= 0x7f80u) {   // an infinity or a NaN: of the finite elements, then
+          top = 0u;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) top = max(top, max(finite_bits(__uint_as_float(w[i] << 16)), finite_bits(__uint_as_float(w[i] & 0xffff0000u))));
+          for (int c = 0; c < MINE; ++c) {
+            const unsigned w[4] = {x[c].x, x[c].y, x[c].z, x[c].w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) top = max(top, max(finite_bits(__uint_as_float(w[i] << 16)), finite_bits(__uint_as_float(w[i] & 0xffff0000u))) >> 16);
+          }
         }
         sh->row_top[chain][sub][row] = static_cast<int>(top);
       }
       pair_sync(pair);   // on every path: the partner waits for it
       if (ok) {
         top = max(top, static_cast<unsigned>(sh->row_top[chain][sub ^ 1][row]));
-        const int e = min(max(static_cast<int>(top >> 23) - 127, -100), 126);
+        const int e = min(max(static_cast<int>(top >> 7) - 127, -100), 126);
         const float lift = args.scale_log2 < 0.f ? -power_of_two(14 - e) : power_of_two(14 - e);
         factor = fmaxf(fabsf(args.scale_log2) * power_of_two(e - 14), 1e-38f);   // a hidden key's -inf has to stay one
 #pragma unroll
         for (int c = 0; c < MINE; ++c) {
-          uint4* at = chunk_of(c);
-          const uint4 v = *at;
-          const unsigned w[4] = {v.x, v.y, v.z, v.w};
+          const unsigned w[4] = {x[c].x, x[c].y, x[c].z, x[c].w};
           unsigned h[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) h[i] = there ? pack_half(__uint_as_float(w[i] << 16) * lift, __uint_as_float(w[i] & 0xffff0000u) * lift) : 0u;
-          *at = make_uint4(h[0], h[1], h[2], h[3]);
+          for (int i = 0; i < 4; ++i) h[i] = there ? pack_half(__uint_as_float(w[i] << 16) * lift, __uint_as_float(w[i] & 0xffff0000u) * lift) : 0u;   // whatever lay there
+          *chunk_of(c) = make_uint4(h[0], h[1], h[2], h[3]);
         }
         fence_async_shared();
         __syncwarp();
@@ -575,15 +586,17 @@ portions_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       if (ok) {
         fence_after_sync();
         tmem_load32(tmem_chain + sub * 32, v);
-        const float* k_scale = sh->k_scale[st] + sub * 32;
         top = sh->v_top[st][sub];
+        float4 scale[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) scale[j] = *reinterpret_cast<const float4*>(sh->k_scale[st] + sub * 32 + 4 * j);   // while the scores come
         tmem_wait_load();
         fence_before_sync();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh->s_read[chain]);    // the scores are in registers: their columns may take the next step
 #pragma unroll
         for (int j = 0; j < 32; j += 4) {
-          const float4 s = *reinterpret_cast<const float4*>(k_scale + j);
+          const float4 s = scale[j / 4];
           float x[4];
           halves_of(mul_pair(pair_of(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), pair_of(s.x, s.y)), x[0], x[1]);
           halves_of(mul_pair(pair_of(__uint_as_float(v[j + 2]), __uint_as_float(v[j + 3])), pair_of(s.z, s.w)), x[2], x[3]);
@@ -631,20 +644,28 @@ portions_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       const float* v_scale = sh->v_scale[st] + sub * 32;
       const float from = base == -INFINITY ? 0.f : base;
       const unsigned long long factor_pair = pair_of(factor, factor), base_pair = pair_of(-from, -from);
-      unsigned long long sum_pair[2] = {pair_of(0.f, 0.f), pair_of(0.f, 0.f)};
+      unsigned long long sum_pair[4] = {pair_of(0.f, 0.f), pair_of(0.f, 0.f), pair_of(0.f, 0.f), pair_of(0.f, 0.f)};
+      // one kind of instruction after the other over all elements: in the order of the elements each would wait for the one before
+#pragma unroll
+      for (int j = 0; j < 32; j += 2) {
+        float x0, x1;
+        halves_of(fma_pair(pair_of(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), factor_pair, base_pair), x0, x1);
+        v[j] = __float_as_uint(x0);
+        v[j + 1] = __float_as_uint(x1);
+      }
+#pragma unroll
+      for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(fast_exp2(__uint_as_float(v[j])));
+#pragma unroll
+      for (int j = 0; j < 32; j += 2)
+        sum_pair[(j >> 1) & 3] = add_pair(sum_pair[(j >> 1) & 3], pair_of(__uint_as_float(v[j]), __uint_as_float(v[j + 1])));
 #pragma unroll
       for (int j = 0; j < 32; j += 4) {
         const float4 s = *reinterpret_cast<const float4*>(v_scale + j);
 #pragma unroll
         for (int i = 0; i < 4; i += 2) {
-          float x0, x1, w0, w1;
-          halves_of(fma_pair(pair_of(__uint_as_float(v[j + i]), __uint_as_float(v[j + i + 1])), factor_pair, base_pair), x0, x1);
-          x0 = fast_exp2(x0);
-          x1 = fast_exp2(x1);
-          const unsigned long long p = pair_of(x0, x1);
-          sum_pair[i >> 1] = add_pair(sum_pair[i >> 1], p);
-          halves_of(mul_pair(p, i == 0 ? pair_of(s.x, s.y) : pair_of(s.z, s.w)), w0, w1);
-          v[(j + i) / 2] = pack_half(w0, w1);   // over the scores already used
+          float w0, w1;
+          halves_of(mul_pair(pair_of(__uint_as_float(v[j + i]), __uint_as_float(v[j + i + 1])), i == 0 ? pair_of(s.x, s.y) : pair_of(s.z, s.w)), w0, w1);
+          v[(j + i) / 2] = pack_half(w0, w1);   // over the weights already used
         }
       }
       if (edge && sh->v_bad[st][sub]) {   // rare: a key that the row does not see has no part in it, not even a scale of NaN
@@ -656,7 +677,7 @@ portions_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         }
       }
       float sum_lo, sum_hi;
-      halves_of(add_pair(sum_pair[0], sum_pair[1]), sum_lo, sum_hi);
+      halves_of(add_pair(add_pair(sum_pair[0], sum_pair[1]), add_pair(sum_pair[2], sum_pair[3])), sum_lo, sum_hi);
       row_sum = row_sum * correction + (sum_lo + sum_hi);
       // P(h) goes where P(h - 2) was: the PV of step h - 2 must have read it
       if (h >= 2) {
@@ -687,44 +708,61 @@ portions_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       pair_sync(pair);   // on every path
       row_sum += sh->row_sum[chain][sub ^ 1][row];
     }
-    if (ok) {
-      const size_t token_head = static_cast<size_t>(start + token) * args.num_heads + head;
-      const size_t at = static_cast<size_t>(split) * args.num_tokens * args.num_heads + token_head;
-      if (args.splits > 1 && there && sub == 0) {
-        args.partial_ml[2 * at] = my_steps > 0 ? base : -INFINITY;
-        args.partial_ml[2 * at + 1] = my_steps > 0 ? row_sum : 0.f;
-      }
-      const bool nothing = row_sum == 0.f;   // a row that sees nothing is zeros
-      const float inv = nothing ? 0.f : 1.0f / row_sum;
-      if (my_steps > 0 || args.splits == 1) {
-        for (int c = sub; c < D / 32; c += 2) {
-          unsigned o[32];
-          if (my_steps > 0) {
-            tmem_load32(tmem_o + c * 32, o);
-            tmem_wait_load();
-          } else {
+    // Outputs leave by way of the chain's query tile, which no product reads any more: a thread has a row, but 32 rows' pieces
+    // of 16 bytes would be 32 lines a store.  64 elements of a row a turn, 32 of each of its two threads.
+    const int token_head = there && ok ? (start + token) * args.num_heads + head : -1;
+    if (ok && args.splits > 1 && there && sub == 0) {
+      float* ml = args.partial_ml + 2 * (static_cast<size_t>(split) * args.num_tokens * args.num_heads + token_head);
+      ml[0] = my_steps > 0 ? base : -INFINITY;
+      ml[1] = my_steps > 0 ? row_sum : 0.f;
+    }
+    const bool nothing = row_sum == 0.f;   // a row that sees nothing is zeros
+    const float inv = nothing ? 0.f : 1.0f / row_sum;
+    const bool partial = args.splits > 1;
+    if (my_steps > 0 || !partial) {
+      const int row_bytes = partial ? 256 : 128, lanes = row_bytes / 16;   // of 64 elements: lanes a row
+      unsigned char* stage = q_tiles + chain * Q_BYTES;
+      for (int turn = 0; turn < D / 64; ++turn) {
+        unsigned o[32];
+        if (my_steps > 0 && ok) {
+          tmem_load32(tmem_o + turn * 64 + sub * 32, o);
+          tmem_wait_load();
+        } else {
 #pragma unroll
-            for (int j = 0; j < 32; ++j) o[j] = 0u;
-          }
-          if (there && args.splits > 1) {
-            float* dst = args.partial_o + at * D + c * 32;
+          for (int j = 0; j < 32; ++j) o[j] = 0u;
+        }
+        unsigned char* mine = stage + row * row_bytes;
+        if (partial) {
 #pragma unroll
-            for (int j = 0; j < 32; j += 4) *reinterpret_cast<uint4*>(dst + j) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
-          } else if (there) {
-            __nv_bfloat16* dst = args.out + token_head * D + c * 32;
+          for (int j = 0; j < 8; ++j)
+            *reinterpret_cast<uint4*>(mine + (((sub * 8 + j) ^ (row & 7)) << 4)) = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+        } else {
 #pragma unroll
-            for (int j = 0; j < 32; j += 8) {
-              unsigned packed[4];
+          for (int j = 0; j < 4; ++j) {
+            unsigned packed[4];
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const float x = nothing ? 0.f : __uint_as_float(o[j + 2 * i]) * inv, y = nothing ? 0.f : __uint_as_float(o[j + 2 * i + 1]) * inv;
-                const __nv_bfloat162 two = __floats2bfloat162_rn(x, y);
-                packed[i] = *reinterpret_cast<const unsigned*>(&two);
-              }
-              *reinterpret_cast<uint4*>(dst + j) = make_uint4(packed[0], packed[1], packed[2], packed[3]);
+            for (int i = 0; i < 4; ++i) {
+              const float x = nothing ? 0.f : __uint_as_float(o[8 * j + 2 * i]) * inv, y = nothing ? 0.f : __uint_as_float(o[8 * j + 2 * i + 1]) * inv;
+              const __nv_bfloat162 two = __floats2bfloat162_rn(x, y);
+              packed[i] = *reinterpret_cast<const unsigned*>(&two);
             }
+            *reinterpret_cast<uint4*>(mine + (((sub * 4 + j) ^ (row & 7)) << 4)) = make_uint4(packed[0], packed[1], packed[2], packed[3]);
           }
         }
+        pair_sync(pair);
+        const int piece = lane & (lanes - 1), rows_at_once = 32 / lanes;   // of this warp's 16 of the 32 rows
+        for (int i = 0; i < 16 / rows_at_once; ++i) {
+          const int within = sub * 16 + i * rows_at_once + lane / lanes, from = quarter * 32 + within;
+          const int at = __shfl_sync(0xffffffffu, token_head, within);
+          const uint4 v = *reinterpret_cast<const uint4*>(stage + from * row_bytes + ((piece ^ (from & 7)) << 4));
+          if (at >= 0) {
+            if (partial)
+              *reinterpret_cast<uint4*>(args.partial_o + (static_cast<size_t>(split) * args.num_tokens * args.num_heads + at) * D + turn * 64 + piece * 4) = v;
+            else
+              *reinterpret_cast<uint4*>(args.out + static_cast<size_t>(at) * D + turn * 64 + piece * 8) = v;
+          }
+        }
+        pair_sync(pair);   // the tile is written again in the next turn
       }
     }
   }
@@ -836,16 +874,18 @@ static int map_queries(const void* base, long long tokens, int heads, int group,
 SHRIKE_API int shrike_attention_q8_tc_tokens(int group) { return group >= 1 && group <= 64 ? 2 * (tcq8::BM / group) : 0; }
 
 // How many CTAs should share the keys of a query tile, for a batch whose portions make `tiles` query tiles over block tables of
-// `keys` keys: the GPU holds one CTA per SM, and splitting pays while every CTA still starts at once.  Among the counts that
-// keep the launch to one round, with at least two key tiles a split and at most 32, the one with the fewest tiles a CTA,
-// counting two tiles' worth for a CTA's start and two more for the second kernel that adds the splits up.
+// `keys` keys: the GPU holds one CTA per SM, so the time is that of the rounds of CTAs, each its key tiles and about CTA_START
+// of their time for a CTA's start and end, and a split launch pays COMBINE more for the second kernel.  Measured (40 heads, 512
+// tokens over 8,192 keys, 88 CTAs' worth of query tiles): unsplit 205 us, two splits 210, three 156, five 156, eight 186.
 SHRIKE_API int shrike_attention_q8_tc_splits(int tiles, int num_kv_heads, long long keys) {
+  constexpr long long CTA_START = 6, COMBINE = 4;
   const long long ctas = static_cast<long long>(num_kv_heads) * tiles, capacity = shrike_device().sm_count;
   const long long key_tiles = (keys + tcq8::KEYS - 1) / tcq8::KEYS;
   int best = 1;
   long long best_cost = -1;
-  for (int s = 1; s <= 32 && (s == 1 || (key_tiles / s >= 2 && ctas * s <= capacity)); ++s) {
-    const long long cost = (key_tiles + s - 1) / s + 2 + (s > 1 ? 2 : 0);
+  for (int s = 1; s <= 32 && (s == 1 || key_tiles / s >= 2); ++s) {
+    const long long rounds = (ctas * s + capacity - 1) / capacity;
+    const long long cost = rounds * ((key_tiles + s - 1) / s + CTA_START) + (s > 1 ? COMBINE : 0);
     if (best_cost < 0 || cost < best_cost) {
       best_cost = cost;
       best = s;

@@ -745,7 +745,7 @@ class CudaOps(QuantisedCacheOps):
             if chunk and window:
                 raise KernelError("attention takes a window or a chunk, not both")
             self._paged_attention_q8(q, keys, values, block_table, q_start, ctx_len, seq_of_token, num_heads, num_kv_heads, head_dim,
-                                     scale, -int(chunk) if chunk else window, out, max_q_len, min_q_len, q_lens)
+                                     scale, -int(chunk) if chunk else window, out, max_q_len, min_q_len, q_lens, max_ctx_len)
             return
         _dense(q, self.dtype, "q")
         if sinks is not None:

@@ -234,10 +234,12 @@ class QuantisedCacheOps:
 
     # ---- attention
     def q8_plan(self, num_heads, num_kv_heads, head_dim, num_seqs, max_blocks, page_size, max_q_len, min_q_len, window=0, num_tokens=0,
-                q_lens=None) -> QuantisedPlan:
+                q_lens=None, max_ctx_len=0) -> QuantisedPlan:
         """How a batch over 8-bit pages is cut: a function of its shape alone, so that a captured launch sequence serves every
-        batch of that shape.  `q_lens`: every entry's length, if they are known."""
-        shape = (num_tokens, tuple(q_lens) if q_lens is not None else None) if max_q_len > 1 else None
+        batch of that shape (and of its `context_class`).  `q_lens`: every entry's length, if they are known; `max_ctx_len`: the
+        longest context, or 0."""
+        short = 0 < max_ctx_len <= self.SHORT_CONTEXT
+        shape = (num_tokens, short, tuple(q_lens) if q_lens is not None else None) if max_q_len > 1 else None
         key = (num_heads, num_kv_heads, head_dim, num_seqs, max_blocks, page_size, min_q_len <= 1, window, shape, self.q8_splits,
                self.tensor_core_attention, self.portion_splits)
         held = self._q8_plans.get(key)
@@ -271,8 +273,11 @@ class QuantisedCacheOps:
                 scratch, arrivals = self._q8_scratch, self._q8_arrivals
         tc_portions, tiles, portion_splits, portion_scratch = False, 0, 1, None
         rows = lib.shrike_attention_q8_tc_tokens(num_heads // num_kv_heads)
+        # Up to 64 keys the mma.sync kernel is done before the other has set up (us, 28 heads of 128, mma.sync and tcgen05: one
+        # portion of 16 tokens 5.6 and 7.4, of 64 7.3 and 9.1, four of 64 7.8 and 9.2; one of 5 tokens over 100 keys 8.9 and 8.3,
+        # of 256 over 256 17.1 and 13.8, of 16 over 600 27.9 and 12.5).
         if (has_portions and rows and self.tensor_core_attention and self.dtype == torch.bfloat16 and page_size in (8, 16, 32, 64)
-                and num_tokens > 0):
+                and num_tokens > 0 and not short and max_blocks * page_size > self.SHORT_CONTEXT):
             tc_portions = True
             if q_lens is not None:
                 tiles = sum(-(-q // rows) for q in q_lens if q > 1 or not has_single)
@@ -310,7 +315,7 @@ class QuantisedCacheOps:
         return best, min(best, 8)
 
     def _paged_attention_q8(self, q, keys, values, block_table, q_start, ctx_len, seq_of_token, num_heads, num_kv_heads, head_dim,
-                            scale, window, out, max_q_len, min_q_len, q_lens):
+                            scale, window, out, max_q_len, min_q_len, q_lens, max_ctx_len):
         device, stream = self._q8_stream()
         pages, page_size, heads, dim = keys.dims
         num_seqs, max_blocks = block_table.shape
@@ -333,7 +338,7 @@ class QuantisedCacheOps:
         if n == 0 or num_seqs == 0:
             return
         window = window or 0
-        plan = self.q8_plan(num_heads, num_kv_heads, head_dim, num_seqs, max_blocks, page_size, max_q_len, min_q_len, window, n, q_lens)
+        plan = self.q8_plan(num_heads, num_kv_heads, head_dim, num_seqs, max_blocks, page_size, max_q_len, min_q_len, window, n, q_lens, max_ctx_len)
         tc, has_portions = plan.tc_portions, plan.has_portions
         if tc and not self._q8_ints_fit(device, seq_of_token, n):
             self._q8_refuse(device, (), [(seq_of_token, n, "sequences of tokens")])
