@@ -298,18 +298,25 @@ class QuantisedCacheOps:
         self._q8_plans[key] = (self.generation, plan)
         return plan
 
-    Q8_SPLIT_KEYS = 160   # what a CTA's start, and its share's way to the others, cost in keys
+    # What a CTA costs beside its keys, in keys: its start alone, with its share's way through a cluster's shared memory, and
+    # with the clusters' way through global memory.
+    Q8_START_KEYS, Q8_CLUSTER_KEYS, Q8_GLOBAL_KEYS = 160, 320, 640
 
     @classmethod
     def q8_few_row_splits(cls, keys: int, pairs: int, resident: int):
         """(splits, cluster): CTAs that share the `keys` of each of `pairs` (entry, kv head, row tile) where the device holds
-        `resident` at once, and how many of them form a cluster.  The count with the least time, rounds of CTAs times what each
-        takes, a CTA having at least a step of 32 keys for each of its four warps."""
+        `resident` at once, and how many of them form a cluster (all up to eight: a cluster adds up in shared memory, 2 us
+        sooner than through global memory).  The count with the least time: no less than a CTA's own, and about that of all
+        CTAs' work, whose contexts are of uneven lengths (three quarters of the longest, say), with half a CTA's at the end.
+        Measured, us: 64 sequences of up to 4,096 keys, 8 kv heads: 94 unsplit, 87 with 2, 92 with 4, 106 with 8; one of 65,521
+        keys: 65 with 16, 51 with 32, 42 with 48, 36 with 64; 8 of 1,024 keys, 4 kv heads: 9.7 with 2, 9.3 with 4, 8.9 with 8."""
         best, least = 1, None
         for splits in (1, 2, 4, 8, 16, 24, 32, 40, 48, 56, 64):
             if splits > max(1, -(-keys // 64)):
                 break
-            time = max(1.0, pairs * splits / (0.87 * resident)) * (-(-keys // (128 * splits)) * 128 + cls.Q8_SPLIT_KEYS * (1 + (splits > 8)))
+            extra = cls.Q8_START_KEYS if splits == 1 else cls.Q8_CLUSTER_KEYS if splits <= 8 else cls.Q8_GLOBAL_KEYS
+            each = -(-keys // (128 * splits)) * 128 + extra   # a CTA's four warps take 32 keys each at a time
+            time = max(each, 0.75 * pairs * splits * each / resident + 0.5 * each)
             if least is None or time < least:
                 best, least = splits, time
         return best, min(best, 8)

@@ -264,7 +264,7 @@ def test_rotation_and_store_refuses_what_does_not_fit(calls):
 def test_attention_refuses_what_does_not_fit(calls):
     ops, lib = calls
     (keys, values), _rows, q, out, index = arguments()
-    table, ctx = torch.zeros(3, 2, dtype=torch.int32), index[1:]
+    table, ctx = torch.zeros(3, 8, dtype=torch.int32), index[1:]
 
     def attend(q=q, keys=keys, values=values, table=table, starts=index, ctx=ctx, owner=index[:3], heads=4, kv_heads=2, dim=64, out=out,
                max_q_len=1, min_q_len=1, **options):
@@ -278,6 +278,8 @@ def test_attention_refuses_what_does_not_fit(calls):
     assert launched == 3
     attend(max_q_len=2, q_lens=[2, 1, 0])   # longer entries beside single tokens: both kernels
     assert lib.calls.count("shrike_paged_attention_q8_tc") == 1 and lib.calls.count("shrike_paged_attention_q8") == 4
+    attend(max_q_len=2, q_lens=[2, 1, 0], max_ctx_len=64)   # few keys: one launcher for both
+    assert lib.calls.count("shrike_paged_attention_q8_tc") == 1 and lib.calls.count("shrike_paged_attention_q8") == 5
     shifted = torch.zeros(3 * 256 + 1, dtype=torch.bfloat16)[1:].view(3, 256)
     for options in (dict(softcap=3.0), dict(slopes=torch.zeros(4)), dict(sinks=torch.zeros(4)), dict(window=4, keep_first=2),
                     dict(window=4, chunk=4), dict(max_q_len=0), dict(heads=5), dict(heads=2), dict(kv_heads=4), dict(dim=32),
@@ -286,7 +288,7 @@ def test_attention_refuses_what_does_not_fit(calls):
                     dict(values=torch.zeros(4, 16, 2, 64, dtype=torch.bfloat16)), dict(max_q_len=2, owner=index)):
         with pytest.raises(KernelError):
             attend(**options)
-    assert lib.calls.count("shrike_paged_attention_q8") == 4
+    assert lib.calls.count("shrike_paged_attention_q8") == 5
 
 
 @pytest.mark.parametrize("resident", [148, 592])
