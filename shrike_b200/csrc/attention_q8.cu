@@ -509,6 +509,7 @@ __device__ __forceinline__ bool entry_of(const Args& args, int seq, int& start, 
 // whose largest base is `base`.
 __device__ __forceinline__ void add_share(float m, float l, const float4& v, float base, float& total, float (&acc)[4]) {
   const float weight = m == -INFINITY ? 0.f : fast_exp2(m - base);
+  if (l != l) total = l;   // a score that is no number: the row is none either, whatever the others hold
   if (weight == 0.f) return;
   total += l * weight;
   acc[0] += v.x * weight; acc[1] += v.y * weight; acc[2] += v.z * weight; acc[3] += v.w * weight;

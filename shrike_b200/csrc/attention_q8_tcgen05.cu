@@ -783,8 +783,9 @@ combine_portions_kernel(const Args args) {
   wait_for_previous();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int token = blockIdx.y * 8 + warp, head = blockIdx.x;
-  if (token >= args.num_tokens) return;
+  if (token >= args.num_tokens || token >= args.q_start[args.num_seqs]) return;   // rows behind the last sequence stay as they are
   const int seq = args.seq_of_token[token];
+  if (seq < 0 || seq >= args.num_seqs) return;
   if (args.skip_single && args.q_start[seq + 1] - args.q_start[seq] == 1) return;
   const size_t token_head = static_cast<size_t>(token) * args.num_heads + head;
   const size_t slice = static_cast<size_t>(args.num_tokens) * args.num_heads;
@@ -797,7 +798,7 @@ combine_portions_kernel(const Args args) {
 #pragma unroll
   for (int offset = 16; offset > 0; offset >>= 1) base = fmaxf(base, __shfl_xor_sync(0xffffffffu, base, offset));
   const float weight = m == -INFINITY ? 0.f : fast_exp2(m - base);   // a split that saw no key of this row has base -inf
-  float total = weight == 0.f ? 0.f : l * weight;
+  float total = l != l ? l : weight == 0.f ? 0.f : l * weight;   // a score that is no number makes the row none
 #pragma unroll
   for (int offset = 16; offset > 0; offset >>= 1) total += __shfl_xor_sync(0xffffffffu, total, offset);
   float acc[D / 32];
@@ -834,19 +835,23 @@ template <typename Encode>
 static int kept_map(const Key& key, CUtensorMap* out, Encode&& encode) {
   static std::mutex mutex;
   static std::unordered_map<Key, CUtensorMap, KeyHash> cache;
-  std::lock_guard<std::mutex> guard(mutex);
-  const auto found = cache.find(key);
-  if (found != cache.end()) {
-    *out = found->second;
-    return SHRIKE_OK;
-  }
   EncodeTiled fn = encode_tiled();
   if (fn == nullptr) return SHRIKE_BAD_ARGUMENT;
-  const CUresult rc = encode(fn, out);
-  if (rc != CUDA_SUCCESS) return 1000 + static_cast<int>(rc);
-  if (cache.size() > 4096) cache.clear();
-  cache.emplace(key, *out);
-  return SHRIKE_OK;
+  try {
+    std::lock_guard<std::mutex> guard(mutex);
+    const auto found = cache.find(key);
+    if (found != cache.end()) {
+      *out = found->second;
+      return SHRIKE_OK;
+    }
+    const CUresult rc = encode(fn, out);
+    if (rc != CUDA_SUCCESS) return 1000 + static_cast<int>(rc);
+    if (cache.size() > 4096) cache.clear();
+    cache.emplace(key, *out);
+    return SHRIKE_OK;
+  } catch (...) {   // out of memory for the table: the map itself is made
+    return encode(fn, out) == CUDA_SUCCESS ? SHRIKE_OK : SHRIKE_BAD_ARGUMENT;
+  }
 }
 // Codes [rows, cols bytes] as boxes of `box_rows` rows of D bytes, in the swizzle of that row length.
 static int map_codes(const void* base, long long rows, int cols, int box_rows, CUtensorMap* out) {
@@ -904,7 +909,7 @@ SHRIKE_API int shrike_paged_attention_q8_tc(const ShrikeAttentionQ8* call) {
   using namespace tcq8;
   if (num_seqs <= 0 || num_tokens <= 0 || tiles <= 0) return SHRIKE_OK;
   if (num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads || num_heads / num_kv_heads > 64 || max_blocks <= 0 || num_pages <= 0 ||
-      tiles > 65535 || !(page_size == 8 || page_size == 16 || page_size == 32 || page_size == 64) || splits < 1 || splits > 32 ||
+      tiles > 65535 || static_cast<long long>(num_tokens) * num_heads > 0x7fffffff || (splits > 1 && num_tokens > 8 * 65535) || !(page_size == 8 || page_size == 16 || page_size == 32 || page_size == 64) || splits < 1 || splits > 32 ||
       static_cast<long long>(num_pages) * page_size > 0x7fffffff || static_cast<long long>(max_blocks) * page_size > 0x7fffffff - 4096 ||
       (splits > 1 && (scratch == nullptr || seq_of_token == nullptr)) ||
       (reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(k_codes) |

@@ -285,7 +285,7 @@ class QuantisedCacheOps:
                 tiles = num_tokens // rows + num_seqs
             portion_splits = self.portion_splits or lib.shrike_attention_q8_tc_splits(tiles, num_kv_heads, max_blocks * page_size)
             each = num_tokens * num_heads * (head_dim + 2)
-            portion_splits = max(1, min(portion_splits, 32, self.PORTION_SCRATCH_FLOATS // each))
+            portion_splits = max(1, min(portion_splits, 32, self.PORTION_SCRATCH_FLOATS // each)) if num_tokens <= 8 * 65535 else 1
             if portion_splits > 1:
                 need = portion_splits * each
                 if self._q8_portion_scratch is None or self._q8_portion_scratch.numel() < need:

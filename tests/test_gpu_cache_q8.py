@@ -203,3 +203,195 @@ def test_portions_beside_single_tokens(dtype, dim, known, options):
 def test_large_scores(dtype):
     """Scores of some hundreds: one key takes all the weight."""
     check_attention(dtype, 4, 2, 64, 16, [1, 20, 1], [300, 90, 5], q_scale=60.0)
+
+
+def pages_of(case):
+    return QuantisedPages(case["codes_k"], case["scales_k"]), QuantisedPages(case["codes_v"], case["scales_v"])
+
+
+FORMS = [(torch.bfloat16, 128, True), (torch.bfloat16, 64, True), (torch.bfloat16, 64, False), (torch.float32, 32, False)]
+
+
+@pytest.mark.parametrize("dtype,dim,tensor_cores", FORMS)
+@pytest.mark.parametrize("splits", [0, 3])
+def test_rows_that_see_nothing_are_zeros(dtype, dim, tensor_cores, splits):
+    """A context shorter than the new tokens: the first of them lie before position 0.  An entry without tokens is left out, and
+    rows behind the last sequence stay as they are."""
+    heads, kv_heads, page = 6, 2, 16
+    q_lens, ctx_lens = [5, 90, 0, 1, 1, 40], [3, 70, 9, 0, 4, 400]
+    ops = cuda_ops(dtype)
+    ops.tensor_core_attention, ops.portion_splits, ops.q8_splits = tensor_cores, splits, (2, 2) if splits else None
+    case = oracle.pages_case(heads, kv_heads, dim, page, q_lens, ctx_lens, dtype, 3, DEV)
+    more = 3
+    q = torch.cat([case["q"], rnd(more, heads * dim, dtype=dtype)])
+    out = torch.full_like(q, 9.0)
+    owner = torch.cat([case["seq_of"], torch.full((more,), 5, dtype=torch.int32, device=DEV)])
+    ops.paged_attention(q, *pages_of(case), case["table"], case["q_start"], case["ctx_len"], owner, heads, kv_heads, dim, dim ** -0.5, None, out,
+                        max_q_len=90, min_q_len=0, q_lens=q_lens)
+    want, bound = oracle.attention(case["q"], case["sequences"], q_lens, ctx_lens, heads, kv_heads, dim, dim ** -0.5)
+    assert (out[-more:] == 9.0).all()
+    got = out[:-more].double()
+    assert ((got - want).abs() <= bound).all()
+    assert (got[:2] == 0).all() and (got[5: 25] == 0).all() and (got[95] == 0).all()
+    ops.check_status()
+
+
+@pytest.mark.parametrize("dtype,dim,tensor_cores", FORMS)
+@pytest.mark.parametrize("options", [{}, {"window": 30}])
+def test_what_a_row_does_not_see_has_no_part_in_it(dtype, dim, tensor_cores, options):
+    """Keys and values stored from infinities, NaN and the largest numbers: rows before them are what they would be without,
+    rows that see them are NaN, or large."""
+    heads, kv_heads, page = 4, 2, 16
+    q_lens, ctx_lens = [100, 1, 33], [150, 140, 33]
+    ops = cuda_ops(dtype)
+    ops.tensor_core_attention = tensor_cores
+    case = oracle.pages_case(heads, kv_heads, dim, page, q_lens, ctx_lens, dtype, 7, DEV)
+    bad = {0: 120, 2: 20}   # sequence -> the position that is spoilt
+    for value in (math.nan, 3e38):
+        for kind in ("scales_k", "scales_v"):
+            spoilt = dict(case, **{kind: case[kind].clone()})
+            for s, position in bad.items():
+                page_id = int(case["table"][s, position // page])
+                spoilt[kind][page_id, :, position % page] = value if math.isnan(value) or kind == "scales_v" else 0.0
+            got = attend(ops, spoilt, heads, kv_heads, dim, q_lens, ctx_lens, **options)
+            for s, position in bad.items():
+                first = int(case["q_start"][s])
+                at = position - (ctx_lens[s] - q_lens[s])   # rows before this one do not see it
+                rows = got[first: first + at]
+                # a base that takes the spoilt key's place into account may round a weight otherwise, by no more than the bound says
+                want, bound = oracle.attention(case["q"], case["sequences"], q_lens, ctx_lens, heads, kv_heads, dim, dim ** -0.5, **options)
+                assert torch.isfinite(rows).all()
+                assert ((rows.double() - want[first: first + at]).abs() <= bound[first: first + at]).all()
+                after = got[first + at: first + min(q_lens[s], at + options.get("window", 1 << 30))]
+                if math.isnan(value):
+                    assert torch.isnan(after).all()
+            assert torch.isfinite(got[100]).all()   # the sequence between them
+    ops.check_status()
+
+
+def test_values_of_uneven_sizes():
+    """Value rows between 1e-6 and 1e6 of one another: every row's output is good to its own keys' sizes."""
+    heads, kv_heads, dim, page = 4, 1, 64, 16
+    q_lens, ctx_lens = [200, 1, 1], [300, 900, 40]
+    for dtype in TYPES:
+        ops = cuda_ops(dtype)
+        case = oracle.pages_case(heads, kv_heads, dim, page, q_lens, ctx_lens, dtype, 11, DEV)
+        factor = 10.0 ** torch.randint(-6, 7, case["scales_v"].shape, generator=torch.Generator().manual_seed(1)).float().to(DEV)
+        case["scales_v"] = case["scales_v"] * factor
+        for s, (keys, values) in enumerate(case["sequences"]):
+            for j in range(ctx_lens[s]):
+                values[1][j] = case["scales_v"][case["table"][s, j // page], :, j % page]
+        got = attend(ops, case, heads, kv_heads, dim, q_lens, ctx_lens)
+        want, bound = oracle.attention(case["q"], case["sequences"], q_lens, ctx_lens, heads, kv_heads, dim, dim ** -0.5)
+        assert ((got.double() - want).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.2, 3.0])
+def test_scales_of_any_sign(scale):
+    for dtype, dim, tensor_cores in FORMS:
+        check_attention(dtype, 4, 2, dim, 16, [1, 70], [200, 180], scale=scale, tensor_cores=tensor_cores)
+
+
+@pytest.mark.parametrize("dtype,dim", [(torch.bfloat16, 128), (torch.bfloat16, 64), (torch.float32, 64)])
+def test_pools_beyond_32_bit_offsets(dtype, dim):
+    """Pages whose codes lie more than 2^31 and 2^32 bytes into the pool: stored, read back and attended over."""
+    heads, kv_heads, page = 16, 8, 64
+    pages = (1 << 32) // (page * kv_heads * dim) + 40
+    ops = cuda_ops(dtype)
+    keys, values = (QuantisedPages(torch.empty(pages, page, kv_heads, dim, dtype=torch.int8, device=DEV),
+                                   torch.full((pages, kv_heads, page), math.nan, device=DEV)) for _ in range(2))
+    ctx_lens, q_lens = [200, 333, 130], [1, 120, 1]
+    ids = [[pages - 1 - 7 * s - b for b in range(-(-c // page))] for s, c in enumerate(ctx_lens)]
+    ids[1][0], ids[1][2] = 3, pages // 2 + 1
+    table = torch.full((3, 6), -1, dtype=torch.int32)
+    for s, mine in enumerate(ids):
+        table[s, : len(mine)] = torch.tensor(mine, dtype=torch.int32)
+    table = table.to(DEV)
+    sequences = []
+    for s, context in enumerate(ctx_lens):
+        pair = []
+        x = [rnd(context, kv_heads * dim, seed=10 * s + i, dtype=dtype) for i in range(2)]
+        slots = torch.tensor([ids[s][j // page] * page + j % page for j in range(context)], dtype=torch.int32, device=DEV)
+        ops.kv_write(*x, keys, values, slots)
+        back = [torch.empty_like(y) for y in x]
+        ops.kv_read(keys, values, slots, *back)
+        for y, z in zip(x, back):
+            codes, scales = oracle.quantise(y.view(context, kv_heads, dim))
+            assert torch.equal(z.view(context, kv_heads, dim), (codes.float() * scales[..., None]).to(dtype))
+            pair.append((codes, scales))
+        sequences.append(pair)
+    q = rnd(sum(q_lens), heads * dim, seed=5, dtype=dtype)
+    starts = torch.tensor([0, 1, 121, 122], dtype=torch.int32, device=DEV)
+    owner = torch.repeat_interleave(torch.arange(3), torch.tensor(q_lens)).to(torch.int32).to(DEV)
+    out = torch.empty_like(q)
+    ops.paged_attention(q, keys, values, table, starts, torch.tensor(ctx_lens, dtype=torch.int32, device=DEV), owner, heads, kv_heads, dim,
+                        dim ** -0.5, None, out, max_q_len=120, min_q_len=1, q_lens=q_lens)
+    want, bound = oracle.attention(q, sequences, q_lens, ctx_lens, heads, kv_heads, dim, dim ** -0.5)
+    assert ((out.double() - want).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("dtype,dim,tensor_cores", FORMS)
+def test_a_layer_captured_and_replayed_and_on_another_stream(dtype, dim, tensor_cores):
+    """Rotation and store, then attention, as a layer has them: captured once, replayed with other positions, contexts and pages."""
+    heads, kv_heads, page = 4, 2, 16
+    q_lens, first = [40, 1, 1], [30, 200, 5]
+    ops = cuda_ops(dtype)
+    ops.tensor_core_attention = tensor_cores
+    n, width = sum(q_lens), (heads + 2 * kv_heads) * dim
+    inv_freq = (10000.0 ** (-torch.arange(0, dim, 2).double() / dim)).float().to(DEV)
+    keys, values = (QuantisedPages.zeros(80, page, kv_heads, dim, DEV) for _ in range(2))
+    owner = torch.repeat_interleave(torch.arange(3), torch.tensor(q_lens)).to(torch.int32).to(DEV)
+    starts = torch.tensor([0, 40, 41, 42], dtype=torch.int32, device=DEV)
+    table = torch.randperm(80, generator=torch.Generator().manual_seed(0))[:48].view(3, 16).to(torch.int32).to(DEV)
+    qkv, bias = rnd(n, width, seed=1), rnd(width, seed=2)
+    positions, slots, ctx = (torch.zeros(k, dtype=torch.int32, device=DEV) for k in (n, n, 3))
+    q, out = (torch.empty(n, heads * dim, dtype=dtype, device=DEV) for _ in range(2))
+
+    def fill(before, seed):
+        qkv.copy_(rnd(n, width, seed=seed))
+        at = torch.cat([torch.arange(b, b + k) for b, k in zip(before, q_lens)])
+        positions.copy_(at.to(torch.int32))
+        ctx.copy_(torch.tensor([b + k for b, k in zip(before, q_lens)], dtype=torch.int32))
+        rows = owner.cpu().long()
+        slots.copy_(table.cpu()[rows, at // page] * page + at % page)
+
+    def layer():
+        ops.rope_kv_write(qkv, bias, positions, inv_freq, q, keys, values, slots, heads, kv_heads, dim)
+        ops.paged_attention(q, keys, values, table, starts, ctx, owner, heads, kv_heads, dim, dim ** -0.5, None, out, max_q_len=40, min_q_len=1,
+                            max_ctx_len=256, q_lens=q_lens)
+
+    def expected():
+        sequences, lens = [], ctx.tolist()
+        for s, context in enumerate(lens):
+            where = [(int(table[s, j // page]), j % page) for j in range(context)]
+            pages_at, within = (torch.tensor(x, device=DEV) for x in zip(*where))
+            sequences.append([(p.codes[pages_at, within], p.scales[pages_at, :, within]) for p in (keys, values)])
+        return oracle.attention(q, sequences, q_lens, lens, heads, kv_heads, dim, dim ** -0.5)
+
+    fill(first, 1)
+    for p in (keys, values):   # what earlier steps stored
+        codes, scales = oracle.quantise(rnd(80, page, kv_heads, dim, seed=3))
+        p.codes.copy_(codes)
+        p.scales.copy_(scales.transpose(1, 2))
+    layer()
+    torch.cuda.synchronize()
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        graph.capture_begin()
+        layer()
+        graph.capture_end()
+    torch.cuda.current_stream().wait_stream(side)
+    for seed, before in ((2, [30, 200, 5]), (3, [0, 0, 0]), (4, [100, 255, 17])):
+        fill(before, seed)
+        graph.replay()
+        want, bound = expected()
+        assert ((out.double() - want).abs() <= bound).all()
+        replayed = out.clone()
+        out.zero_()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            layer()
+        torch.cuda.synchronize()
+        assert torch.equal(out, replayed)
+    ops.check_status()
