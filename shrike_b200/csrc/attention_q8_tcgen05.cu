@@ -150,19 +150,22 @@ struct Args {
   const int* seq_of_token;   // [tokens], for the second kernel
 };
 
-// Which (sequence, query tile) a CTA with work index `work` owns: sequences in order, each with its query tiles of `rows`
-// tokens, the last (longest to walk) first; sequences of one token own none when skip_single.  Every lane of the calling warp
-// gets the answer; tile_start < 0: no such work.
-__device__ __forceinline__ void find_work(const Args& args, int work, int rows, int& seq_out, int& tile_start_out) {
+// What a CTA with work index `work` owns: sequences in order, each with its query tiles of `rows` tokens, the last (longest to
+// walk) first; sequences of one token own none when skip_single.  Every lane of the calling warp gets the answer; tile_start
+// < 0: no such work.
+struct Work {
+  int seq, tile_start, start, q_len, context;
+};
+__device__ __forceinline__ Work find_work(const Args& args, int work, int rows) {
   const int lane = threadIdx.x & 31;
   int before = 0;
-  seq_out = -1;
-  tile_start_out = -1;
   for (int base = 0; base < args.num_seqs; base += 32) {
     const int s = base + lane;
-    int tiles = 0;
+    int tiles = 0, start = 0, q_len = 0, context = 0;
     if (s < args.num_seqs) {
-      const int q_len = args.q_start[s + 1] - args.q_start[s];
+      start = args.q_start[s];
+      q_len = args.q_start[s + 1] - start;
+      context = args.ctx_len[s];
       tiles = q_len <= 0 || (q_len == 1 && args.skip_single) ? 0 : (q_len + rows - 1) / rows;
     }
     int inclusive = tiles;
@@ -175,14 +178,13 @@ __device__ __forceinline__ void find_work(const Args& args, int work, int rows, 
     const unsigned owner = __ballot_sync(0xffffffffu, tiles > 0 && work >= first && work < first + tiles);
     if (owner != 0) {
       const int src = __ffs(owner) - 1;
-      const int first_of_owner = __shfl_sync(0xffffffffu, first, src);
-      const int tiles_of_owner = __shfl_sync(0xffffffffu, tiles, src);
-      seq_out = base + src;
-      tile_start_out = (tiles_of_owner - 1 - (work - first_of_owner)) * rows;
-      return;
+      const int from = __shfl_sync(0xffffffffu, first, src), count = __shfl_sync(0xffffffffu, tiles, src);
+      return Work{base + src, (count - 1 - (work - from)) * rows, __shfl_sync(0xffffffffu, start, src),
+                  __shfl_sync(0xffffffffu, q_len, src), __shfl_sync(0xffffffffu, context, src)};
     }
     before += __shfl_sync(0xffffffffu, inclusive, 31);
   }
+  return Work{-1, -1, 0, 0, 0};
 }
 
 struct Shared {
@@ -257,16 +259,14 @@ portions_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                 const __grid_constant__ CUtensorMap map_v, const Args args) {
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   const int kv_head = blockIdx.x, split = blockIdx.z;
-  int seq, tile_start;
-  find_work(args, blockIdx.y, 2 * args.tokens, seq, tile_start);           // metadata: written before the step's kernels
+  const Work own = find_work(args, blockIdx.y, 2 * args.tokens);           // metadata: written before the step's kernels
+  const int seq = own.seq, tile_start = own.tile_start, start = own.start, q_len = own.q_len;
   if (tile_start < 0 || (smem_u32(smem_raw) & 1023u)) {
     if (tile_start >= 0 && threadIdx.x == 0 && args.status != nullptr) *args.status = ERR_ALIGNMENT;
     let_dependents_start();
     wait_for_previous();
     return;
   }
-  const int start = args.q_start[seq];
-  const int q_len = args.q_start[seq + 1] - start;
   unsigned char* q_tiles = smem_raw;                             // [2 chains][Q_BYTES]
   unsigned char* k_tiles = q_tiles + 2 * Q_BYTES;                // [STAGES][KV_TILE]
   unsigned char* v_tiles = k_tiles + STAGES * KV_TILE;           // [STAGES][KV_TILE]
@@ -275,7 +275,7 @@ portions_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
   Shared* sh = reinterpret_cast<Shared*>(raw_v + RAW_STAGES * RAW_TILE);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
-  const int pos0 = args.ctx_len[seq] - q_len;                   // position of the first new token
+  const int pos0 = own.context - q_len;                         // position of the first new token
   // chain c owns tokens tile_start + c * tokens ...; tokens_1 <= 0: the later chain has none
   const int tokens_0 = min(args.tokens, q_len - tile_start), tokens_1 = min(args.tokens, q_len - tile_start - args.tokens);
   const int lo = first_visible_key(max(pos0 + tile_start, 0), args.window);   // first key any row sees
@@ -293,6 +293,7 @@ portions_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
   const int steps_1 = hi_1 >= 0 ? max(0, min(last_tile, hi_1 / KEYS) - tile_lo + 1) : 0;
   const int num_tiles = max(steps_0, steps_1);
 
+  if (warp == 3) tmem_alloc(&sh->tmem_base, TMEM_COLS);
   const unsigned users = (steps_0 > 0 ? 1u : 0u) + (steps_1 > 0 ? 1u : 0u);   // chains that read the key and value stages
   if (threadIdx.x == 0) {
     mbar_init(&sh->q_full, 1);
@@ -322,7 +323,27 @@ portions_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     sh->abort = 0;
     mbar_init_fence();
   }
-  if (warp == 3) tmem_alloc(&sh->tmem_base, TMEM_COLS);
+  // The first page ids (metadata): the loaders' a chunk of 32 at a time (lane l: page l of the chunk, several tiles' worth), the
+  // converting threads' their own key's.
+  const int* table = args.block_table + static_cast<size_t>(seq) * args.max_blocks;
+  auto page_of = [&](int key) -> int {   // of a key that some row sees; -1 for one that none does
+    const int block = key >> args.page_shift;
+    return key <= hi && block < args.max_blocks ? table[block] : -1;
+  };
+  const int pages_per_tile = KEYS >> args.page_shift, tiles_per_chunk = 32 / pages_per_tile;
+  auto load_chunk = [&](int chunk) -> int {
+    return chunk * tiles_per_chunk < num_tiles ? page_of(tile_lo * KEYS + ((chunk * 32 + lane) << args.page_shift)) : -1;
+  };
+  auto load_page = [&](int i, int row) -> int { return i < num_tiles ? page_of((tile_lo + i) * KEYS + row) : -1; };
+  const bool scales = warp == 24 || warp == 25;   // the converting warps that bring the tiles' scales
+  int chunk_pages = -1, next_pages = -1;          // chunks 0 and 1, or this thread's pages of tiles 0 and 1
+  if (warp == 0 || warp == 3) {
+    chunk_pages = load_chunk(0);
+    next_pages = load_chunk(1);
+  } else if (scales) {
+    chunk_pages = load_page(0, threadIdx.x & 63);
+    next_pages = load_page(1, threadIdx.x & 63);
+  }
   fence_before_sync();
   __syncthreads();
   fence_after_sync();
@@ -333,11 +354,8 @@ portions_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     fewer_registers<40>();
     if (warp == 0 || warp == 3) {
       // Key (warp 0) and value codes (warp 3): lane 0 waits for the buffer and arms its barrier, then lane pg issues the box of
-      // page pg of the tile.  Page ids come a chunk of 32 at a time (lane l: page l of the chunk, several tiles' worth), the next
-      // chunk while this one is used.
+      // page pg of the tile.
       const bool for_keys = warp == 0;
-      const int* table = args.block_table + static_cast<size_t>(seq) * args.max_blocks;
-      const int pages_per_tile = KEYS >> args.page_shift;
       const int nowhere = args.num_pages * args.page_size;      // a row coordinate outside the cache: reads zeros
       if (for_keys && lane == 0 && num_tiles > 0) {
         mbar_expect_tx(&sh->q_full, 2 * HALVES * args.tokens * args.group * 128);
@@ -345,17 +363,10 @@ portions_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
           for (int h = 0; h < HALVES; ++h)
             tma_load_3d(q_tiles + c * Q_BYTES + h * Q_HALF, &map_q, &sh->q_full, h * 64, kv_head * args.group, start + tile_start + c * args.tokens);
       }
-      const int tiles_per_chunk = 32 / pages_per_tile;
-      auto load_chunk = [&](int chunk) -> int {
-        const int key0 = tile_lo * KEYS + ((chunk * 32 + lane) << args.page_shift);
-        const int block = key0 >> args.page_shift;
-        return (chunk * tiles_per_chunk < num_tiles && key0 <= hi && block < args.max_blocks) ? table[block] : -1;
-      };
       unsigned char* const raw = for_keys ? raw_k : raw_v;
       unsigned long long* const full = for_keys ? sh->raw_k_full : sh->raw_v_full;
       unsigned long long* const free_again = for_keys ? sh->raw_k_free : sh->raw_v_free;
       const CUtensorMap* const map = for_keys ? &map_k : &map_v;
-      int chunk_pages = load_chunk(0), next_pages = load_chunk(1);
       int issued = 0, within = 0, chunk = 0;
       for (int i = 0; i < num_tiles; ++i) {
         const int s = i % RAW_STAGES;
@@ -454,25 +465,21 @@ portions_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     unsigned long long* const raw_free = for_keys ? sh->raw_k_free : sh->raw_v_free;
     unsigned long long* const full = for_keys ? sh->k_full : sh->v_full;
     unsigned long long* const free_again = for_keys ? sh->k_free : sh->v_free;
-    const bool scales = !for_keys && half == 0;   // these bring the tile's scales too (whole warps)
-    const int* table = args.block_table + static_cast<size_t>(seq) * args.max_blocks;
-    // the place of this thread's key of tile i among the scales; -1: no such key
-    auto scale_place = [&](int i) -> long long {
-      const int key = (tile_lo + i) * KEYS + row, block = key >> args.page_shift;
-      if (i >= num_tiles || key > hi || block >= args.max_blocks) return -1;
-      const int page = table[block];
+    auto scale_at = [&](int page, int i) -> long long {   // the place of this thread's key among the scales; -1: no such key
       if (page < 0 || page >= args.num_pages) return -1;
-      return ((static_cast<long long>(page) * args.num_kv_heads + kv_head) << args.page_shift) + (key & (args.page_size - 1));
+      return ((static_cast<long long>(page) * args.num_kv_heads + kv_head) << args.page_shift) + (((tile_lo + i) * KEYS + row) & (args.page_size - 1));
     };
-    long long place = -1;
     float k_scale = 0.f, v_scale = 0.f;
+    int ahead = -1;   // this thread's page, two tiles ahead
+    long long place = -1;
     if (scales) {
-      place = scale_place(0);
+      place = scale_at(chunk_pages, 0);
       if (place >= 0) {
         k_scale = args.k_scales[place];
         v_scale = args.v_scales[place];
       }
-      place = scale_place(1);
+      place = scale_at(next_pages, 1);
+      ahead = load_page(2, row);
     }
     for (int i = 0; i < num_tiles; ++i) {
       const int st = i % STAGES, rs = i % RAW_STAGES;
@@ -482,7 +489,8 @@ portions_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
           next_k = args.k_scales[place];
           next_v = args.v_scales[place];
         }
-        place = scale_place(i + 2);
+        place = scale_at(ahead, i + 2);
+        ahead = load_page(i + 3, row);
       }
       uint4 codes[MY_CHUNKS];
       bool ok = mbar_wait(&raw_full[rs], (i / RAW_STAGES) & 1, &sh->abort, args.status, ERR_CONVERT);

@@ -21,6 +21,15 @@ __device__ __forceinline__ int code_of(float x, float a, float inv) {
   return code;
 }
 
+// The same for bfloat16 elements.  With X and A the eight-bit significands of x and a, and x smaller by 2^s, 127 x / a lies at
+// least 1 / (510 2^s) from a border it does not lie on, and the product below is off by 2^-23 of up to 127 / 2^s: it decides
+// rightly.  127 x / a lies on a border where 254 X is an odd multiple of A: where A is 254 (the product is exact then, and
+// rounds to the even code) or x = a / 2.
+__device__ __forceinline__ int code_of_bf16(float x, float a, float inv) {
+  const int code = __float2int_rn(__fmul_rn(x, inv));
+  return fabsf(x) * 2.f == a ? (x > 0.f ? 64 : -64) : code;
+}
+
 // What a row's codes are formed with: rows of very small or very large elements are scaled by a power of two first, so that
 // neither 127 / a nor the products leave float32's range (elements that lose bits by it lie far below half a step).
 struct RowScale {
@@ -36,12 +45,14 @@ __device__ __forceinline__ RowScale row_scale(float a) {
   r.inv = __fdiv_rn(127.f, r.a);
   return r;
 }
-__device__ __forceinline__ unsigned pack_codes(const float (&x)[4], const RowScale& r) {
+template <typename T> __device__ __forceinline__ unsigned pack_codes(const float (&x)[4], const RowScale& r) {
   if (!r.good) return 0u;
-  unsigned word = 0u;
+  int code[4];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) word |= (static_cast<unsigned>(code_of(x[e] * r.lift, r.a, r.inv)) & 255u) << (8 * e);
-  return word;
+  for (int e = 0; e < 4; ++e)
+    code[e] = sizeof(T) == 2 ? code_of_bf16(x[e] * r.lift, r.a, r.inv) : code_of(x[e] * r.lift, r.a, r.inv);
+  const unsigned lo = __byte_perm(code[0], code[1], 0x0040), hi = __byte_perm(code[2], code[3], 0x0040);
+  return __byte_perm(lo, hi, 0x5410);
 }
 // The larger magnitude, NaN if either is NaN (fmaxf would drop it).
 __device__ __forceinline__ float largest(float a, float b) {
@@ -76,20 +87,20 @@ struct Pages {
 template <typename T, int LANES>
 __global__ void __launch_bounds__(256)
 kv_write_q8_kernel(const T* __restrict__ k_new, const T* __restrict__ v_new, long long k_stride, long long v_stride, const Pages keys,
-                   const Pages values, const int* __restrict__ slots, long long rows, int kv_heads, int dim, int page_size,
-                   long long num_slots, int aligned) {
+                   const Pages values, const int* __restrict__ slots, unsigned rows, unsigned kv_heads, int dim, unsigned page_size,
+                   unsigned num_slots, int aligned) {
   constexpr int TURNS = LANES == 32 ? 2 : 1;   // heads of up to 256 elements
   let_dependents_start();
   wait_for_previous();
-  const long long row = (static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x) / LANES;
+  const unsigned row = blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
   const int lane = threadIdx.x % LANES;
   // rows in the order token, keys | values, head; a row behind the last takes part in the shuffles with nothing
-  const long long at = row < rows ? row : rows - 1;
-  const int head = static_cast<int>(at % kv_heads);
-  const bool is_value = (at / kv_heads) & 1;
-  const long long token = at / (2 * kv_heads);
-  const long long slot = slots[token];
-  const T* src = (is_value ? v_new + token * v_stride : k_new + token * k_stride) + static_cast<long long>(head) * dim;
+  const unsigned at = row < rows ? row : rows - 1;
+  const unsigned token = at / (2 * kv_heads), within = at - token * 2 * kv_heads;
+  const bool is_value = within >= kv_heads;
+  const unsigned head = is_value ? within - kv_heads : within;
+  const int slot = slots[token];
+  const T* src = (is_value ? v_new + token * v_stride : k_new + token * k_stride) + head * static_cast<unsigned>(dim);
   float x[TURNS][4], a = 0.f;
 #pragma unroll
   for (int i = 0; i < TURNS; ++i) {
@@ -109,16 +120,19 @@ kv_write_q8_kernel(const T* __restrict__ k_new, const T* __restrict__ v_new, lon
   }
 #pragma unroll
   for (int offset = LANES / 2; offset > 0; offset >>= 1) a = largest(a, __shfl_xor_sync(0xffffffffu, a, offset));
-  if (row >= rows || slot < 0 || slot >= num_slots) return;
+  if (row >= rows || static_cast<unsigned>(slot) >= num_slots) return;   // a negative one is none of the pool's either
   const RowScale r = row_scale(a);
   const Pages& to = is_value ? values : keys;
-  signed char* dst = to.codes + (slot * kv_heads + head) * dim;
+  signed char* dst = to.codes + (static_cast<size_t>(slot) * kv_heads + head) * dim;
 #pragma unroll
   for (int i = 0; i < TURNS; ++i) {
     const int first = (lane + i * LANES) * 4;
-    if (first < dim) *reinterpret_cast<unsigned*>(dst + first) = pack_codes(x[i], r);
+    if (first < dim) *reinterpret_cast<unsigned*>(dst + first) = pack_codes<T>(x[i], r);
   }
-  if (lane == 0) to.scales[(slot / page_size * kv_heads + head) * page_size + slot % page_size] = r.scale;
+  if (lane == 0) {
+    const unsigned page = static_cast<unsigned>(slot) / page_size;
+    to.scales[(static_cast<size_t>(page) * kv_heads + head) * page_size + (slot - page * page_size)] = r.scale;
+  }
 }
 
 // ---- bias, rotation and store of a fused q/k/v projection
@@ -289,11 +303,11 @@ SHRIKE_API int shrike_kv_write_q8(const ShrikeCacheQ8* call) {
   const long long rows = 2ll * n * kv_heads;
   const int lanes = dim <= 32 ? 8 : dim <= 64 ? 16 : 32;
   const long long blocks = (rows * lanes + 255) / 256;
-  if (blocks > 0x7fffffff) return SHRIKE_BAD_ARGUMENT;
+  if (rows > 0x7fffffff || num_slots > 0x7fffffff) return SHRIKE_BAD_ARGUMENT;
 #define SHRIKE_WRITE_Q8(T, LANES)                                                                                              \
   launch_dependent(kv_write_q8_kernel<T, LANES>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream,                    \
-                   static_cast<const T*>(k_new), static_cast<const T*>(v_new), k_stride, v_stride, keys, values, slots, rows, \
-                   kv_heads, dim, page_size, num_slots, aligned)
+                   static_cast<const T*>(k_new), static_cast<const T*>(v_new), k_stride, v_stride, keys, values, slots, static_cast<unsigned>(rows), \
+                   static_cast<unsigned>(kv_heads), dim, static_cast<unsigned>(page_size), static_cast<unsigned>(num_slots), aligned)
   cudaError_t err;
   if (dtype == SHRIKE_F32) err = lanes == 8 ? SHRIKE_WRITE_Q8(float, 8) : lanes == 16 ? SHRIKE_WRITE_Q8(float, 16) : SHRIKE_WRITE_Q8(float, 32);
   else err = lanes == 8 ? SHRIKE_WRITE_Q8(__nv_bfloat16, 8) : lanes == 16 ? SHRIKE_WRITE_Q8(__nv_bfloat16, 16) : SHRIKE_WRITE_Q8(__nv_bfloat16, 32);

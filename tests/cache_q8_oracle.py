@@ -100,6 +100,6 @@ def attention(q, sequences, q_lens, ctx_lens, heads, kv_heads, dim, scale, windo
             sums = (context / 8 + 16) * u
             least = seen.sum(-1, keepdim=True) * 2.0 ** -33 * 127 * torch.where(seen, values[1][:, g].double(), 0.0).amax(-1, keepdim=True)
             bound[:, head] = least + (p @ vv.abs()) * (2 * score + (2.0 ** -22 if wide else 2.0 ** -11) + 2 * sums)
-        outs.append(out.view(new, -1))
-        bounds.append((bound + half_step * out.abs()).view(new, -1))
+        outs.append(out.view(new, heads * dim))
+        bounds.append((bound + half_step * out.abs()).view(new, heads * dim))
     return torch.cat(outs), torch.cat(bounds)

@@ -315,3 +315,18 @@ def test_plans_are_kept_by_shape_until_the_scratch_moves(calls):
     assert unknown.tiles == 42 // 32 + 3   # at most
     assert ops.q8_plan(4, 2, 64, 3, 64, 16, 1, 1) is not first   # the scratch has moved: a plan of its own
     assert not ops.q8_plan(4, 2, 64, 3, 64, 5, 40, 1, 0, 42, [40, 1, 1]).tc_portions   # pages of five tokens: the other kernel
+
+
+def test_codes_of_bfloat16_elements_fall_on_the_right_side_of_every_border():
+    """The store's shorter form for bfloat16 (a 32-bit product, and halves of the largest element apart), for every pair of
+    significands, against integers: 127 x / a to the nearest, halves to even."""
+    significands = np.arange(128, 256, dtype=np.int64)
+    for shift in range(10):
+        for a in significands:
+            x = significands if shift else significands[significands <= a]
+            in_32 = x.astype(np.float32) / np.float32(2 ** shift)
+            code = np.rint(in_32 * (np.float32(127) / np.float32(a))).astype(np.int64)
+            code = np.where(2 * in_32 == np.float32(a), 64, code)
+            whole, left = np.divmod(127 * x, a << shift)
+            exact = whole + (2 * left > (a << shift)) + ((2 * left == (a << shift)) & (whole % 2 == 1))
+            assert (code == exact).all()
