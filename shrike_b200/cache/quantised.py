@@ -10,19 +10,25 @@ from __future__ import annotations
 
 import torch
 
+MOST_HEAD_DIM = 256   # of the kernels over 8-bit pages
+_INT8, _FLOAT32 = torch.int8, torch.float32
+
 
 class QuantisedPages:
     """`codes` int8 [pages, page_size, kv heads, head size], `scales` float32 [pages, kv heads, page_size], on one device."""
 
-    __slots__ = ("codes", "scales", "dims", "device_index")
+    __slots__ = ("codes", "scales", "dims", "device_index", "served")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor):
-        dims = tuple(codes.shape)
-        if not (codes.dtype is torch.int8 and len(dims) == 4 and codes.is_contiguous() and scales.dtype is torch.float32
-                and scales.shape == (dims[0], dims[2], dims[1]) and scales.is_contiguous() and codes.device == scales.device):
+        dims = codes.shape
+        if not (len(dims) == 4 and codes.dtype is _INT8 and scales.dtype is _FLOAT32 and scales.shape == (dims[0], dims[2], dims[1])
+                and codes.is_contiguous() and scales.is_contiguous() and codes.device == scales.device):
             self._refuse(codes, scales)
-        self.codes, self.scales = codes, scales
-        self.dims, self.device_index = dims, codes.get_device()   # (pages, page_size, kv heads, head size); -1: not on a GPU
+        self.codes, self.scales, self.dims = codes, scales, dims   # (pages, page_size, kv heads, head size)
+        self.device_index = codes.get_device()   # -1: not on a GPU
+        pages, page_size, _heads, dim = dims
+        # whether the kernels take them: their head sizes, and slots that are 32-bit numbers
+        self.served = not dim % 16 and 16 <= dim <= MOST_HEAD_DIM and pages * page_size <= 0x7FFFFFFF
 
     @staticmethod
     def _refuse(codes, scales):

@@ -13,17 +13,18 @@ from dataclasses import dataclass
 
 import torch
 
-from ..cache.quantised import QuantisedPages
+from ..cache.quantised import MOST_HEAD_DIM, QuantisedPages
 from . import build
 
 _c = ctypes
 _P, _I, _F, _LL = _c.c_void_p, _c.c_int, _c.c_float, _c.c_longlong
 DTYPE_CODE = {torch.float32: 0, torch.bfloat16: 1}
-MOST_HEAD_DIM = 256   # of the kernels over 8-bit pages
 # The launchers take their arguments as one packed structure (ShrikeCacheQ8, ShrikeAttentionQ8): a call of thirty arguments takes
 # ctypes two microseconds, this a third of one.
 _CACHE_CALL = struct.Struct("=8Q2q6i")
 _ATTENTION_CALL = struct.Struct("=14Q16if")
+_pack_cache, _pack_attention = _CACHE_CALL.pack, _ATTENTION_CALL.pack
+_INT32 = torch.int32
 _device = getattr(torch._C, "_cuda_getDevice", None)          # the current device's number, and its current stream's handle:
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)   # asking torch for the objects costs more than a launch
 
@@ -43,10 +44,7 @@ class QuantisedPlan:
     portion_splits: int = 1   # CTAs that share the keys of one
     portion_scratch: torch.Tensor | None = None
     lib: object = None
-
-    @property
-    def launches(self) -> int:
-        return int(self.has_single) + int(self.has_portions) + (self.portion_splits > 1)
+    launches: int = 0
 
 
 def _error(text):
@@ -143,15 +141,8 @@ class QuantisedCacheOps:
                 raise _error(f"{what} must be {count} contiguous int32, is {tensor.dtype} {list(tensor.shape)}")
 
     @staticmethod
-    def _q8_pages_fit(device, keys, values) -> bool:
-        dims = keys.dims
-        return (dims == values.dims and keys.device_index == device and values.device_index == device and not dims[3] % 16
-                and 16 <= dims[3] <= MOST_HEAD_DIM and dims[0] * dims[1] <= 0x7FFFFFFF and not keys.codes.data_ptr() % 16
-                and not values.codes.data_ptr() % 16)
-
-    @staticmethod
     def _q8_ints_fit(device, tensor, count) -> bool:
-        return tensor.get_device() == device and tensor.dtype is torch.int32 and tensor.numel() == count and tensor.is_contiguous()
+        return tensor.get_device() == device and tensor.dtype is _INT32 and tensor.numel() == count and tensor.is_contiguous()
 
     def _q8_rows(self, device, x, n, width, what):
         """The distance of x's rows in elements; a row's elements lie side by side."""
@@ -163,19 +154,28 @@ class QuantisedCacheOps:
 
     # ---- the cache
     def _kv_write_q8(self, k_new, v_new, keys, values, slots):
-        device, stream = self._q8_stream()
-        pages, page_size, heads, dim = keys.dims
+        device = _device()
+        stream = _raw_stream(device) if self._held_stream is None else self._held_stream
+        pages, page_size, heads, dim = dims = keys.dims
+        codes, value_codes, dtype = keys.codes.data_ptr(), values.codes.data_ptr(), self.dtype
         n = k_new.shape[0]
-        if not (self._q8_pages_fit(device, keys, values) and self._q8_ints_fit(device, slots, n)):
+        width = heads * dim
+        if not (keys.served and dims == values.dims and keys.device_index == device and values.device_index == device
+                and not (codes | value_codes) % 16 and slots.get_device() == device and slots.dtype is _INT32 and slots.numel() == n
+                and slots.is_contiguous()):
             self._q8_refuse(device, (), [(slots, n, "slots")], (keys, values, None, None))
-        k_stride = self._q8_rows(device, k_new, n, heads * dim, "new keys")
-        v_stride = self._q8_rows(device, v_new, n, heads * dim, "new values")
+        if (k_new.dtype is dtype and v_new.dtype is dtype and k_new.get_device() == device and v_new.get_device() == device
+                and k_new.shape == v_new.shape == (n, width) and k_new.is_contiguous() and v_new.is_contiguous()):
+            k_stride = v_stride = width
+        else:
+            k_stride = self._q8_rows(device, k_new, n, width, "new keys")
+            v_stride = self._q8_rows(device, v_new, n, width, "new values")
         if n == 0:
             return
         self.launches += 1
-        code = self.core.shrike_kv_write_q8(_CACHE_CALL.pack(
-            k_new.data_ptr(), v_new.data_ptr(), keys.codes.data_ptr(), values.codes.data_ptr(), keys.scales.data_ptr(),
-            values.scales.data_ptr(), slots.data_ptr(), stream, k_stride, v_stride, self.code, n, heads, dim, pages, page_size))
+        code = self.core.shrike_kv_write_q8(_pack_cache(
+            k_new.data_ptr(), v_new.data_ptr(), codes, value_codes, keys.scales.data_ptr(), values.scales.data_ptr(), slots.data_ptr(),
+            stream, k_stride, v_stride, self.code, n, heads, dim, pages, page_size))
         if code:
             _failed(code, "kv_write_q8")
 
@@ -212,23 +212,26 @@ class QuantisedCacheOps:
         the pool's (a negative one, say).  A row stored from an infinity or a NaN comes back as NaN."""
         if not quantised(keys, values):
             raise _error("kv_read reads 8-bit pages; a cache in the engine's type is indexed as it is")
-        device, stream = self._q8_stream()
-        pages, page_size, heads, dim = keys.dims
+        device = _device()
+        stream = _raw_stream(device) if self._held_stream is None else self._held_stream
+        pages, page_size, heads, dim = dims = keys.dims
+        codes, value_codes = keys.codes.data_ptr(), values.codes.data_ptr()
         n, dtype = slots.numel(), self.dtype
         k_at, v_at = k_out.data_ptr(), v_out.data_ptr()
-        shape = (n, heads * dim)
-        if not (self._q8_pages_fit(device, keys, values) and self._q8_ints_fit(device, slots, n) and k_out.dtype is dtype
-                and v_out.dtype is dtype and k_out.shape == shape and v_out.shape == shape and k_out.get_device() == device
-                and v_out.get_device() == device and k_out.is_contiguous() and v_out.is_contiguous() and not (k_at | v_at) % 16):
+        if not (keys.served and dims == values.dims and keys.device_index == device and values.device_index == device
+                and slots.get_device() == device and slots.dtype is _INT32 and slots.is_contiguous() and k_out.dtype is dtype
+                and v_out.dtype is dtype and k_out.shape == v_out.shape == (n, heads * dim) and k_out.get_device() == device
+                and v_out.get_device() == device and k_out.is_contiguous() and v_out.is_contiguous()
+                and not (k_at | v_at | codes | value_codes) % 16):
             self._q8_refuse(device, [(k_out, dtype, "keys read"), (v_out, dtype, "values read")], [(slots, n, "slots")],
                             (keys, values, None, None))
             raise _error(f"keys and values read must be [{n}, {heads * dim}], are {list(k_out.shape)} and {list(v_out.shape)}")
         if n == 0:
             return
         self.launches += 1
-        code = self.core.shrike_kv_read_q8(_CACHE_CALL.pack(
-            k_at, v_at, keys.codes.data_ptr(), values.codes.data_ptr(), keys.scales.data_ptr(), values.scales.data_ptr(),
-            slots.data_ptr(), stream, 0, 0, self.code, n, heads, dim, pages, page_size))
+        code = self.core.shrike_kv_read_q8(_pack_cache(
+            k_at, v_at, codes, value_codes, keys.scales.data_ptr(), values.scales.data_ptr(), slots.data_ptr(), stream, 0, 0, self.code,
+            n, heads, dim, pages, page_size))
         if code:
             _failed(code, "kv_read_q8")
 
@@ -292,7 +295,8 @@ class QuantisedCacheOps:
                     self._q8_portion_scratch = torch.empty(max(need, 1 << 22), dtype=torch.float32, device=self.device)
                     self.generation += 1
                 portion_scratch = self._q8_portion_scratch
-        plan = QuantisedPlan(has_single, has_portions, tc_portions, splits, cluster, scratch, arrivals, tiles, portion_splits, portion_scratch, lib)
+        plan = QuantisedPlan(has_single, has_portions, tc_portions, splits, cluster, scratch, arrivals, tiles, portion_splits, portion_scratch, lib,
+                             int(has_single) + int(has_portions) + (portion_splits > 1))
         if len(self._q8_plans) >= 4096:
             self._q8_plans.clear()
         self._q8_plans[key] = (self.generation, plan)
@@ -323,17 +327,21 @@ class QuantisedCacheOps:
 
     def _paged_attention_q8(self, q, keys, values, block_table, q_start, ctx_len, seq_of_token, num_heads, num_kv_heads, head_dim,
                             scale, window, out, max_q_len, min_q_len, q_lens, max_ctx_len):
-        device, stream = self._q8_stream()
-        pages, page_size, heads, dim = keys.dims
+        device = _device()
+        stream = _raw_stream(device) if self._held_stream is None else self._held_stream
+        pages, page_size, heads, dim = dims = keys.dims
+        codes, value_codes = keys.codes.data_ptr(), values.codes.data_ptr()
         num_seqs, max_blocks = block_table.shape
         n, dtype = q.shape[0], self.dtype
         q_at, out_at = q.data_ptr(), out.data_ptr()
-        shape = (n, num_heads * head_dim)
-        if not (self._q8_pages_fit(device, keys, values) and heads == num_kv_heads and dim == head_dim and not num_heads % heads
-                and q.dtype is dtype and out.dtype is dtype and q.shape == shape and out.shape == shape and q.get_device() == device
-                and out.get_device() == device and q.is_contiguous() and out.is_contiguous() and not (q_at | out_at) % 16
-                and self._q8_ints_fit(device, block_table, num_seqs * max_blocks) and self._q8_ints_fit(device, q_start, num_seqs + 1)
-                and self._q8_ints_fit(device, ctx_len, num_seqs) and max_q_len >= 1):
+        if not (keys.served and dims == values.dims and keys.device_index == device and values.device_index == device
+                and heads == num_kv_heads and dim == head_dim and not num_heads % heads and q.dtype is dtype and out.dtype is dtype
+                and q.shape == out.shape == (n, num_heads * head_dim) and q.get_device() == device and out.get_device() == device
+                and q.is_contiguous() and out.is_contiguous() and not (q_at | out_at | codes | value_codes) % 16
+                and block_table.dtype is _INT32 and block_table.get_device() == device and block_table.is_contiguous()
+                and q_start.dtype is _INT32 and q_start.get_device() == device and q_start.numel() == num_seqs + 1
+                and q_start.is_contiguous() and ctx_len.dtype is _INT32 and ctx_len.get_device() == device
+                and ctx_len.numel() == num_seqs and ctx_len.is_contiguous() and max_q_len >= 1):
             self._q8_refuse(device, [(q, dtype, "q"), (out, dtype, "attention output")], [
                 (block_table, num_seqs * max_blocks, "block table"), (q_start, num_seqs + 1, "query starts"),
                 (ctx_len, num_seqs, "context lengths")], (keys, values, num_kv_heads, head_dim))
@@ -349,13 +357,13 @@ class QuantisedCacheOps:
         tc, has_portions = plan.tc_portions, plan.has_portions
         if tc and not self._q8_ints_fit(device, seq_of_token, n):
             self._q8_refuse(device, (), [(seq_of_token, n, "sequences of tokens")])
-        at = (q_at, keys.codes.data_ptr(), keys.scales.data_ptr(), values.codes.data_ptr(), values.scales.data_ptr(),
-              block_table.data_ptr(), q_start.data_ptr(), ctx_len.data_ptr())
+        at = (q_at, codes, keys.scales.data_ptr(), value_codes, values.scales.data_ptr(), block_table.data_ptr(), q_start.data_ptr(),
+              ctx_len.data_ptr())
         sizes = (max_blocks, self.code, n, num_seqs, num_heads, num_kv_heads, page_size, pages, window, plan.has_single)
         self.launches += plan.launches
         if tc:
             scratch = plan.portion_scratch
-            code = plan.lib.shrike_paged_attention_q8_tc(_ATTENTION_CALL.pack(
+            code = plan.lib.shrike_paged_attention_q8_tc(_pack_attention(
                 *at, seq_of_token.data_ptr(), out_at, 0 if scratch is None else scratch.data_ptr(), 0, self.status.data_ptr(), stream,
                 *sizes, 1, max_q_len, 0, plan.portion_splits, 1, plan.tiles, scale))
             if code:
@@ -364,7 +372,7 @@ class QuantisedCacheOps:
             if not plan.has_single:
                 return
         scratch, arrivals = plan.scratch, plan.arrivals
-        code = plan.lib.shrike_paged_attention_q8(_ATTENTION_CALL.pack(
+        code = plan.lib.shrike_paged_attention_q8(_pack_attention(
             *at, 0, out_at, 0 if scratch is None else scratch.data_ptr(), 0 if arrivals is None else arrivals.data_ptr(), 0, stream,
             *sizes, has_portions, max_q_len, tc, plan.splits, plan.cluster, 0, scale))
         if code:
