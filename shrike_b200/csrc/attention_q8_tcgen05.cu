@@ -581,9 +581,9 @@ portions_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         if (lane == 0) mbar_arrive(&sh->q_ready[chain]);
       }
     }
-    for (int h = 0; h < my_steps; ++h) {
-      const int st = h % STAGES;
-      if (ok) ok = mbar_wait(&sh->v_full[st], (h / STAGES) & 1, &sh->abort, args.status, ERR_SOFTMAX);   // the tile's scales
+    unsigned phase = 0;   // of the stage
+    for (int h = 0, st = 0; h < my_steps; ++h, st = st + 1 == STAGES ? 0 : st + 1, phase ^= st == 0 ? 1u : 0u) {
+      if (ok) ok = mbar_wait(&sh->v_full[st], phase, &sh->abort, args.status, ERR_SOFTMAX);   // the tile's scales
       if (ok) ok = mbar_wait(&sh->s_full[chain], h & 1, &sh->abort, args.status, ERR_SOFTMAX);
       ok = __all_sync(0xffffffffu, ok);   // the warp stays together: the tensor-memory accesses below are warp-wide
       unsigned v[32];
@@ -687,13 +687,8 @@ portions_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       float sum_lo, sum_hi;
       halves_of(add_pair(add_pair(sum_pair[0], sum_pair[1]), add_pair(sum_pair[2], sum_pair[3])), sum_lo, sum_hi);
       row_sum = row_sum * correction + (sum_lo + sum_hi);
-      // P(h) goes where P(h - 2) was: the PV of step h - 2 must have read it
-      if (h >= 2) {
-        ok = mbar_wait(&sh->pv_done[chain][h & 1], ((h >> 1) & 1) ^ 1, &sh->abort, args.status, ERR_SOFTMAX);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) continue;
-        fence_after_sync();
-      }
+      // P(h) goes where P(h - 2) was.  The product that read that was issued before the scores of step h, and a commit waits for
+      // everything its thread has issued: s_full(h) says that it has been read.
       tmem_store16(tmem_chain + P_COL + (h & 1) * 32 + sub * 16, v);   // keys 2 j and 2 j + 1 of the step in column j
       if (h > 0 && __any_sync(0xffffffffu, correction != 1.0f)) {
         // O still takes the step before: wait for its PV, then rescale
