@@ -13,17 +13,17 @@
 // turn them into float16 tiles in the 128-byte swizzle (four the keys', four the values'; two threads a key), and those are
 // what the products read.  Eight codes take 10 instructions (a byte permutation and a subtraction a pair, an exclusive or for
 // four).
-// The softmax is bound by the latency of its instructions more than by their number: with a thread a row (eight warps, as the
-// kernel over bfloat16 pages has) leaving out the exponentials, the scales' products or the conversion saved 8 to 10 % each.
-// So two threads share a row, each with 32 of a step's keys: twice the warps to hide latency with, half the unrolled code (a
-// prompt of 2,048 tokens, 28 heads: 66 us and 58).  Now issue slots and shared memory's bandwidth bound it together: a step of
-// 64 keys takes about 2,800 clocks of two chains, in which an SM issues 64 % of what it could, and 190 KB go to and from
-// shared memory (queries and keys of the first product 96, values 32, codes 16, conversion 48), 1,500 clocks of its bandwidth,
-// beside 1,024 each of the tensor pipe and of the special-function units.  They agree on the row's base through a barrier of their two warps that says whether anyone's
-// has to move (rarely), and only then exchange their maxima.
+// The softmax bounds it (with scores passed through untouched, 40 heads' 512 tokens over 8,192 keys took 60 % of the time), and
+// what bounds the softmax is the latency of its instructions and how fast they are fetched.  So it has sixteen warps (with
+// eight, a thread a row, a prompt of 2,048 tokens took 66 us where these took 58), a warp has sixteen rows and all 64 keys of a
+// step, as fragments: the four lanes of a row agree on its base by shuffles, and only where one has to move (two warps a row,
+// each with half of the keys, met at a barrier every step: 8 % of the time).  And the code is kept small, by loops that stay
+// loops: with the tries of every wait unrolled and 64 codes converted in one piece the kernel was 128 KB instead of 60, a warp
+// waited for its next instruction as long as for anything else, and the time was 154 us instead of 128 (as measured then).
 //
 // Roles: warp 0 brings key codes (and the queries), warp 3 value codes (and owns tensor memory), warps 1 and 2 issue the products
-// of a chain each, warps 4..11 and 12..19 are the softmax and epilogue of a chain each, warps 20..23 convert keys, 24..27 values.
+// of a chain each, warps 4..11 and 12..19 are the softmax and epilogue of a chain each (a warp reaches the 32 lanes of tensor memory
+// that its number modulo 4 says: two share them, sixteen rows each), warps 20..23 convert keys, 24..27 values.
 // Registers a thread: 72 at launch, 96 in the softmax warpgroups, 40 in the others (16 x 96 + 12 x 40 = 28 x 72).
 // Barriers: raw_k / raw_v full[raw stage] (TMA) and free (converters, an arrival a warp); k_full / v_full[stage] (converters;
 // v_full also says that the tile's scales lie in shared memory), k_free / v_free[stage] (commits of both chains); q_ready[chain]
@@ -132,6 +132,19 @@ __device__ __forceinline__ void umma_a_in_tmem(unsigned leader, unsigned tmem_d,
 template <int REGISTERS> __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGISTERS)); }
 template <int REGISTERS> __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGISTERS)); }
 
+// As mbar_wait, in less code (see above).
+__device__ __forceinline__ bool wait_bar(unsigned long long* bar, unsigned parity, volatile int* abort, int* status, int who) {
+  if (mbar_test_wait(bar, parity)) return true;
+#pragma unroll 1
+  for (unsigned tries = 0; tries < WAIT_LIMIT; ++tries) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if (*abort) return false;
+  }
+  *abort = 1;
+  if (status != nullptr && *status == 0) *status = who;
+  return false;
+}
+
 struct Args {
   const float* k_scales;
   const float* v_scales;
@@ -191,8 +204,6 @@ struct Shared {
   float k_scale[STAGES][KEYS], v_scale[STAGES][KEYS];
   int v_top[STAGES][2];   // per 32 keys: the exponent of the largest value scale
   int v_bad[STAGES][2];   // whether one of them is no finite number
-  float row_max[2][2][BM], row_sum[2][2][BM];   // [chain][key half]: what the two threads of a row tell each other
-  int row_top[2][2][BM];
   unsigned long long q_full, q_ready[2], s_full[2], s_read[2], p_full[2][2], pv_done[2][2], pv_last[2], stagger;
   unsigned long long raw_k_full[RAW_STAGES], raw_k_free[RAW_STAGES], raw_v_full[RAW_STAGES], raw_v_free[RAW_STAGES];
   unsigned long long k_full[STAGES], k_free[STAGES], v_full[STAGES], v_free[STAGES];
@@ -202,56 +213,58 @@ struct Shared {
 constexpr size_t SMEM = 2 * Q_BYTES + 2 * STAGES * KV_TILE + 2 * RAW_STAGES * RAW_TILE + sizeof(Shared);
 static_assert(SMEM <= 232448, "more than an SM's shared memory");
 
-// 32 lanes x 16 columns of 32-bit.
-__device__ __forceinline__ void tmem_store16(unsigned taddr, const unsigned (&r)[32]) {
+// 16 lanes x 64 columns of 32-bit as the fragments of a matrix: r[4 j + 2 m + c] is row lane / 4 + 8 m, column 8 j + 2 (lane % 4) + c.
+__device__ __forceinline__ void tmem_load_fragments(unsigned taddr, unsigned (&r)[32]) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+      "tcgen05.ld.sync.aligned.16x256b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_store_fragments(unsigned taddr, const unsigned (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.16x256b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+        "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]),
+        "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]),
+        "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+// 16 lanes x 32 columns, two 16-bit elements in each: r[2 j + m] is row lane / 4 + 8 m, column 4 j + lane % 4.
+__device__ __forceinline__ void tmem_store_pairs(unsigned taddr, const unsigned (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.16x128b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
       ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
         "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
-// This thread's share (every other run of 32 columns) of its output row.
-__device__ __noinline__ void rescale_output_row(unsigned tmem_o, int half, float correction) {
-  for (int c = half; c < D / 32; c += 2) {
+// A warp's sixteen output rows.
+__device__ __noinline__ void rescale_output_rows(unsigned tmem_o, float upper, float lower) {
+  for (int c = 0; c < D; c += 64) {
     unsigned o[32];
-    tmem_load32(tmem_o + c * 32, o);
+    tmem_load_fragments(tmem_o + c, o);
     tmem_wait_load();
 #pragma unroll
-    for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * correction);
-    tmem_store32(tmem_o + c * 32, o);
+    for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * ((j & 2) ? lower : upper));
+    tmem_store_fragments(tmem_o + c, o);
   }
-}
-// The barriers of the two warps that share 32 rows.
-__device__ __forceinline__ bool pair_any(int id, bool mine) {
-  unsigned any;
-  __syncwarp();
-  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %2, 0;\n\tbarrier.cta.red.or.pred.aligned q, %1, 64, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
-               : "=r"(any) : "r"(id), "r"(mine ? 1u : 0u) : "memory");
-  return any != 0;
-}
-__device__ __forceinline__ void pair_sync(int id) {
-  __syncwarp();
-  asm volatile("barrier.cta.sync.aligned %0, 64;" ::"r"(id) : "memory");
 }
 
 // A converting thread's share: 16-byte chunks first ... first + COUNT - 1 of its key's codes, and the float16 they become.
 constexpr int RAW_CHUNKS = D / 16, MY_CHUNKS = RAW_CHUNKS / 2;
-__device__ __forceinline__ void read_codes(const unsigned char* raw, int row, int first, uint4 (&codes)[MY_CHUNKS]) {
+__device__ __forceinline__ void convert_chunk(const unsigned char* raw, unsigned char* tile, int row, int chunk) {
   // rows of 128 bytes in the 128-byte swizzle, rows of 64 bytes in the 64-byte one
-  const int exchanged = D == 128 ? row & 7 : (row >> 1) & 3;
+  const uint4 codes = *reinterpret_cast<const uint4*>(raw + row * D + ((chunk ^ (D == 128 ? row & 7 : (row >> 1) & 3)) << 4));
+  unsigned char* half = tile + (chunk / 4) * KV_HALF + row * 128;
+  const unsigned w[4] = {codes.x ^ 0x80808080u, codes.y ^ 0x80808080u, codes.z ^ 0x80808080u, codes.w ^ 0x80808080u};
 #pragma unroll
-  for (int c = 0; c < MY_CHUNKS; ++c) codes[c] = *reinterpret_cast<const uint4*>(raw + row * D + (((first + c) ^ exchanged) << 4));
-}
-__device__ __forceinline__ void write_halves(unsigned char* tile, int row, int first, const uint4 (&codes)[MY_CHUNKS]) {
-#pragma unroll
-  for (int c = 0; c < MY_CHUNKS; ++c) {
-    unsigned char* half = tile + ((first + c) / 4) * KV_HALF + row * 128;
-    const unsigned w[4] = {codes[c].x ^ 0x80808080u, codes[c].y ^ 0x80808080u, codes[c].z ^ 0x80808080u, codes[c].w ^ 0x80808080u};
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-      *reinterpret_cast<uint4*>(half + (((2 * ((first + c) % 4) + i) ^ (row & 7)) << 4)) =
-          make_uint4(codes_to_half<0x4140>(w[2 * i]), codes_to_half<0x4342>(w[2 * i]), codes_to_half<0x4140>(w[2 * i + 1]), codes_to_half<0x4342>(w[2 * i + 1]));
-  }
+  for (int i = 0; i < 2; ++i)
+    *reinterpret_cast<uint4*>(half + (((2 * (chunk % 4) + i) ^ (row & 7)) << 4)) =
+        make_uint4(codes_to_half<0x4140>(w[2 * i]), codes_to_half<0x4342>(w[2 * i]), codes_to_half<0x4140>(w[2 * i + 1]), codes_to_half<0x4342>(w[2 * i + 1]));
 }
 
 __global__ void __launch_bounds__(THREADS, 1)
@@ -368,6 +381,7 @@ portions_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       unsigned long long* const free_again = for_keys ? sh->raw_k_free : sh->raw_v_free;
       const CUtensorMap* const map = for_keys ? &map_k : &map_v;
       int issued = 0, within = 0, chunk = 0;
+#pragma unroll 1
       for (int i = 0; i < num_tiles; ++i) {
         const int s = i % RAW_STAGES;
         if (within == tiles_per_chunk) {
@@ -381,7 +395,7 @@ portions_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         const int y = page < 0 ? nowhere : page << args.page_shift;
         int ok = 1;
         if (lane == 0) {
-          ok = mbar_wait(&free_again[s], ((i / RAW_STAGES) & 1) ^ 1, &sh->abort, args.status, ERR_PRODUCER) ? 1 : 0;
+          ok = wait_bar(&free_again[s], ((i / RAW_STAGES) & 1) ^ 1, &sh->abort, args.status, ERR_PRODUCER) ? 1 : 0;
           if (ok) mbar_expect_tx(&full[s], RAW_TILE);
         }
         ok = __shfl_sync(0xffffffffu, ok, 0);
@@ -392,10 +406,12 @@ portions_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       if (lane == 0 && sh->abort) {   // copies may still be in flight: wait for the buffers armed last
         for (int i = max(0, issued - RAW_STAGES); i < issued; ++i) {
           bool landed = false;
+#pragma unroll 1
           for (unsigned tries = 0; tries < WAIT_LIMIT && !landed; ++tries) landed = mbar_try_wait(&full[i % RAW_STAGES], (i / RAW_STAGES) & 1);
           if (!landed && args.status != nullptr) *args.status = ERR_DRAIN;
         }
         bool landed = !for_keys || num_tiles <= 0;
+#pragma unroll 1
         for (unsigned tries = 0; tries < WAIT_LIMIT && !landed; ++tries) landed = mbar_try_wait(&sh->q_full, 0);
       }
     } else {
@@ -405,7 +421,7 @@ portions_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       if (steps > 0) {
         const unsigned leader = elect_one();
         auto wait_for = [&](unsigned long long* bar, unsigned parity) {
-          return __all_sync(0xffffffffu, mbar_wait(bar, parity, &sh->abort, args.status, ERR_MMA)) != 0;
+          return __all_sync(0xffffffffu, wait_bar(bar, parity, &sh->abort, args.status, ERR_MMA)) != 0;
         };
         const unsigned idesc_s = half_descriptor(BM, KEYS, false);
         const unsigned idesc_o = half_descriptor(BM, D, true);
@@ -430,6 +446,7 @@ portions_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         // the later chain starts most of a step behind the earlier one, where that is not most of its time
         if (ok && c == 1 && steps_0 > 4) ok = wait_for(&sh->stagger, 0);
         if (ok) issue_scores(0);
+#pragma unroll 1
         for (int h = 0; h < steps && ok; ++h) {
           if (h + 1 < steps) {
             ok = wait_for(&sh->s_read[c], h & 1);
@@ -481,6 +498,7 @@ portions_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       place = scale_at(next_pages, 1);
       ahead = load_page(2, row);
     }
+#pragma unroll 1
     for (int i = 0; i < num_tiles; ++i) {
       const int st = i % STAGES, rs = i % RAW_STAGES;
       float next_k = 0.f, next_v = 0.f;
@@ -492,13 +510,9 @@ portions_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         place = scale_at(ahead, i + 2);
         ahead = load_page(i + 3, row);
       }
-      uint4 codes[MY_CHUNKS];
-      bool ok = mbar_wait(&raw_full[rs], (i / RAW_STAGES) & 1, &sh->abort, args.status, ERR_CONVERT);
+      bool ok = wait_bar(&raw_full[rs], (i / RAW_STAGES) & 1, &sh->abort, args.status, ERR_CONVERT);
       if (!__all_sync(0xffffffffu, ok)) break;
-      read_codes(raw + rs * RAW_TILE, row, first, codes);
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&raw_free[rs]);
-      ok = mbar_wait(&free_again[st], ((i / STAGES) & 1) ^ 1, &sh->abort, args.status, ERR_CONVERT);
+      ok = wait_bar(&free_again[st], ((i / STAGES) & 1) ^ 1, &sh->abort, args.status, ERR_CONVERT);
       if (!__all_sync(0xffffffffu, ok)) break;
       if (scales) {   // the softmax threads have read the scales of the tile that was here: its products are done
         sh->k_scale[st][row] = k_scale;
@@ -512,39 +526,48 @@ portions_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         k_scale = next_k;
         v_scale = next_v;
       }
-      write_halves(tiles + st * KV_TILE, row, first, codes);
+#pragma unroll 1
+      for (int c = 0; c < MY_CHUNKS; ++c) convert_chunk(raw + rs * RAW_TILE, tiles + st * KV_TILE, row, first + c);
       fence_async_shared();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&full[st]);
+      if (lane == 0) {
+        mbar_arrive(&raw_free[rs]);
+        mbar_arrive(&full[st]);
+      }
     }
   } else {
-    // ---- softmax and epilogue: two threads a row, each with 32 of a step's 64 keys
+    // ---- softmax and epilogue: a warp has sixteen rows, four lanes a row, and a lane two rows
     more_registers<96>();
-    const int chain = (warp - 4) >> 3, sub = ((warp - 4) >> 2) & 1, quarter = warp & 3;
-    const int pair = 1 + chain * 4 + quarter;   // the barrier of the two warps that share these rows
-    const int row = quarter * 32 + lane;
-    const int token = tile_start + chain * args.tokens + row / args.group, head = kv_head * args.group + row % args.group;
-    const bool there = row < args.tokens * args.group && token < q_len;
+    const int chain = (warp - 4) >> 3, t = lane & 3;
+    const int row0 = (warp & 3) * 32 + ((warp - 4) >> 2 & 1) * 16;   // this warp's first row, among the tensor memory lanes that it reaches
     const int my_steps = chain == 0 ? steps_0 : steps_1;
-    // a row that is not there (128 is no multiple of the group, or the portion ends) has zeros for a query and sees what the
-    // chain's last token sees, so that it takes the same turns; nobody reads it
-    const int last = pos0 + min(token, tile_start + chain * args.tokens + (chain == 0 ? tokens_0 : tokens_1) - 1);
-    const int first = first_visible_key(max(last, 0), args.window);
-    const unsigned lane_base = static_cast<unsigned>(quarter * 32) << 16;
-    const unsigned tmem_chain = sh->tmem_base + chain * CHAIN_COLS + lane_base, tmem_o = tmem_chain + O_COL;
-    float most = -INFINITY, base = -INFINITY, row_sum = 0.f, factor = 0.f;
-    int exponent = LEAST_EXPONENT;
+    const int chain_tokens = chain == 0 ? tokens_0 : tokens_1;
+    // Row lane % 16 of the warp's is this lane's where queries come in and outputs leave.
+    const int moved = row0 + (lane & 15), moved_token = chain * args.tokens + moved / args.group;
+    const bool there = moved < args.tokens * args.group && tile_start + moved_token < q_len;
+    // Between them it has rows lane / 4 and lane / 4 + 8.  A row that is not there (128 is no multiple of the group, or the
+    // portion ends) has zeros for a query and sees what the chain's last token sees, so that it takes the same turns; nobody
+    // reads it.
+    int first[2], last[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      last[r] = pos0 + tile_start + chain * args.tokens + min((row0 + (lane >> 2) + 8 * r) / args.group, chain_tokens - 1);
+      first[r] = first_visible_key(max(last[r], 0), args.window);
+    }
+    const int latest_first = max(first[0], first[1]), earliest_last = min(last[0], last[1]);
+    const unsigned tmem_chain = sh->tmem_base + chain * CHAIN_COLS + (static_cast<unsigned>(row0) << 16), tmem_o = tmem_chain + O_COL;
+    float most[2] = {-INFINITY, -INFINITY}, base[2] = {-INFINITY, -INFINITY}, row_sum[2] = {0.f, 0.f}, factor[2] = {0.f, 0.f};
+    int exponent[2] = {LEAST_EXPONENT, LEAST_EXPONENT};
     bool ok = true;
-    if (my_steps > 0) {
-      // the query's row, half of it each: scaled so that its largest element lies in [2^14, 2^15), then float16
-      ok = mbar_wait(&sh->q_full, 0, &sh->abort, args.status, ERR_SOFTMAX);
+    if (num_tiles > 0) {   // a chain without steps as well: its outputs leave by way of the tile that the queries land in
+      ok = wait_bar(&sh->q_full, 0, &sh->abort, args.status, ERR_SOFTMAX);
       ok = __all_sync(0xffffffffu, ok);
-      constexpr int MINE = HALVES * 4;   // 16-byte chunks of this thread
-      unsigned char* q_row = q_tiles + chain * Q_BYTES + row * 128;
-      auto chunk_of = [&](int c) { return reinterpret_cast<uint4*>(q_row + ((sub * MINE + c) / 8) * Q_HALF + ((((sub * MINE + c) % 8) ^ (row & 7)) << 4)); };
-      uint4 x[MINE];
-      unsigned top = 0u;   // the largest magnitude's upper sixteen bits
-      if (ok) {
+      if (ok && my_steps > 0) {   // the query's row, half of it each of two lanes: scaled so that its largest element lies in [2^14, 2^15), then float16
+        constexpr int MINE = HALVES * 4;   // 16-byte chunks of this thread
+        unsigned char* q_row = q_tiles + chain * Q_BYTES + moved * 128;
+        auto chunk_of = [&](int c) { return reinterpret_cast<uint4*>(q_row + (((lane >> 4) * MINE + c) / 8) * Q_HALF + (((((lane >> 4) * MINE + c) % 8) ^ (moved & 7)) << 4)); };
+        uint4 x[MINE];
+        unsigned top = 0u;   // the largest magnitude's upper sixteen bits
 #pragma unroll
         for (int c = 0; c < MINE; ++c) {
           x[c] = *chunk_of(c);
@@ -560,14 +583,12 @@ portions_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
             for (int i = 0; i < 4; ++i) top = max(top, max(finite_bits(__uint_as_float(w[i] << 16)), finite_bits(__uint_as_float(w[i] & 0xffff0000u))) >> 16);
           }
         }
-        sh->row_top[chain][sub][row] = static_cast<int>(top);
-      }
-      pair_sync(pair);   // on every path: the partner waits for it
-      if (ok) {
-        top = max(top, static_cast<unsigned>(sh->row_top[chain][sub ^ 1][row]));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 16));
         const int e = min(max(static_cast<int>(top >> 7) - 127, -100), 126);
         const float lift = args.scale_log2 < 0.f ? -power_of_two(14 - e) : power_of_two(14 - e);
-        factor = fmaxf(fabsf(args.scale_log2) * power_of_two(e - 14), 1e-38f);   // a hidden key's -inf has to stay one
+        const float own_factor = fmaxf(fabsf(args.scale_log2) * power_of_two(e - 14), 1e-38f);   // a hidden key's -inf has to stay one
+#pragma unroll
+        for (int r = 0; r < 2; ++r) factor[r] = __shfl_sync(0xffffffffu, own_factor, (lane >> 2) + 8 * r);
 #pragma unroll
         for (int c = 0; c < MINE; ++c) {
           const unsigned w[4] = {x[c].x, x[c].y, x[c].z, x[c].w};
@@ -582,182 +603,196 @@ portions_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       }
     }
     unsigned phase = 0;   // of the stage
-    for (int h = 0, st = 0; h < my_steps; ++h, st = st + 1 == STAGES ? 0 : st + 1, phase ^= st == 0 ? 1u : 0u) {
-      if (ok) ok = mbar_wait(&sh->v_full[st], phase, &sh->abort, args.status, ERR_SOFTMAX);   // the tile's scales
-      if (ok) ok = mbar_wait(&sh->s_full[chain], h & 1, &sh->abort, args.status, ERR_SOFTMAX);
+#pragma unroll 1
+    for (int h = 0, st = 0; h < my_steps && ok; ++h, st = st + 1 == STAGES ? 0 : st + 1, phase ^= st == 0 ? 1u : 0u) {
+      ok = wait_bar(&sh->v_full[st], phase, &sh->abort, args.status, ERR_SOFTMAX);   // the tile's scales
+      if (ok) ok = wait_bar(&sh->s_full[chain], h & 1, &sh->abort, args.status, ERR_SOFTMAX);
       ok = __all_sync(0xffffffffu, ok);   // the warp stays together: the tensor-memory accesses below are warp-wide
-      unsigned v[32];
-      const int key_base = (tile_lo + h) * KEYS + sub * 32;
-      const bool edge = key_base < first || key_base + 31 > last;   // only steps at the edge of the row's range pay for masking
-      float step_max = -INFINITY;
-      int top = LEAST_EXPONENT;
-      if (ok) {
-        fence_after_sync();
-        tmem_load32(tmem_chain + sub * 32, v);
-        top = sh->v_top[st][sub];
-        float4 scale[8];
+      if (!ok) break;
+      unsigned v[32];   // [4 j + 2 r + c]: row r, key 8 j + 2 t + c of the step
+      const int key_base = (tile_lo + h) * KEYS;
+      const bool edge = key_base < latest_first || key_base + KEYS - 1 > earliest_last;   // only steps at the edge of a row's range pay for masking
+      fence_after_sync();
+      tmem_load_fragments(tmem_chain, v);
+      int top[2];
+      top[0] = top[1] = max(sh->v_top[st][0], sh->v_top[st][1]);
+      float2 scale[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) scale[j] = *reinterpret_cast<const float4*>(sh->k_scale[st] + sub * 32 + 4 * j);   // while the scores come
-        tmem_wait_load();
-        fence_before_sync();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sh->s_read[chain]);    // the scores are in registers: their columns may take the next step
+      for (int j = 0; j < 8; ++j) scale[j] = *reinterpret_cast<const float2*>(sh->k_scale[st] + 8 * j + 2 * t);   // while the scores come
+      tmem_wait_load();
+      fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh->s_read[chain]);    // the scores are in registers: their columns may take the next step
 #pragma unroll
-        for (int j = 0; j < 32; j += 4) {
-          const float4 s = scale[j / 4];
-          float x[4];
-          halves_of(mul_pair(pair_of(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), pair_of(s.x, s.y)), x[0], x[1]);
-          halves_of(mul_pair(pair_of(__uint_as_float(v[j + 2]), __uint_as_float(v[j + 3])), pair_of(s.z, s.w)), x[2], x[3]);
+      for (int i = 0; i < 32; i += 2) {
+        float x0, x1;
+        halves_of(mul_pair(pair_of(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), pair_of(scale[i / 4].x, scale[i / 4].y)), x0, x1);
+        v[i] = __float_as_uint(x0);
+        v[i + 1] = __float_as_uint(x1);
+      }
+      const float* v_scale = sh->v_scale[st] + 2 * t;
+      if (__builtin_expect(edge, 0)) {
+        unsigned top_bits[2] = {0u, 0u};
 #pragma unroll
-          for (int i = 0; i < 4; ++i) v[j + i] = __float_as_uint(x[i]);
+        for (int i = 0; i < 32; ++i) {
+          const int r = (i >> 1) & 1, within = 8 * (i / 4) + (i & 1), key = key_base + 2 * t + within;
+          if (key < first[r] || key > last[r]) v[i] = 0xff800000u;   // -inf
+          else top_bits[r] = max(top_bits[r], finite_bits(v_scale[within]));
         }
-        if (edge) {
-          const float* v_scale = sh->v_scale[st] + sub * 32;
-          unsigned top_bits = 0u;
+        top[0] = static_cast<int>(top_bits[0] >> 23) - 127;
+        top[1] = static_cast<int>(top_bits[1] >> 23) - 127;
+      }
+      float step_max[2];
+      bool moves = false;
 #pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            const int key = key_base + j;
-            if (key < first || key > last) v[j] = 0xff800000u;   // -inf
-            else top_bits = max(top_bits, finite_bits(v_scale[j]));
-          }
-          top = static_cast<int>(top_bits >> 23) - 127;
-        }
-        float part_max[2] = {-INFINITY, -INFINITY};
+      for (int r = 0; r < 2; ++r) {
+        float part[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-        for (int j = 0; j < 32; j += 4)
-#pragma unroll
-          for (int a = 0; a < 2; ++a) part_max[a] = max3(part_max[a], __uint_as_float(v[j + 2 * a]), __uint_as_float(v[j + 2 * a + 1]));
-        step_max = fmaxf(part_max[0], part_max[1]) * factor;
-        top = min(top - SCALE_BITS, MOST_EXPONENT);
+        for (int j = 0; j < 8; ++j) part[j & 1] = max3(part[j & 1], __uint_as_float(v[4 * j + 2 * r]), __uint_as_float(v[4 * j + 2 * r + 1]));
+        step_max[r] = fmaxf(part[0], part[1]) * factor[r];
+        top[r] = min(top[r] - SCALE_BITS, MOST_EXPONENT);
+        moves = moves || step_max[r] > most[r] + BASE_LAG || top[r] > exponent[r] || most[r] == -INFINITY;
       }
       // The base follows the largest score lazily (2^6), and the largest value scale at once: the weights stay below 2^15.
-      // Both threads of a row have the same; the warps that share the rows ask each other whether any row's has to move (on
-      // every path: the partner waits).
-      float correction = 1.0f;
-      const bool moves = !ok || step_max > most + BASE_LAG || top > exponent || most == -INFINITY;
-      if (pair_any(pair, moves)) {
-        sh->row_max[chain][sub][row] = ok ? step_max : -INFINITY;
-        sh->row_top[chain][sub][row] = top;
-        pair_sync(pair);
-        most = fmaxf(most, fmaxf(step_max, sh->row_max[chain][sub ^ 1][row]));
-        exponent = max(exponent, max(top, sh->row_top[chain][sub ^ 1][row]));
-        const float next = most + static_cast<float>(exponent);
-        // a row that has seen no key yet has O = 0 and a sum of 0: nothing to rescale
-        correction = base == -INFINITY ? 1.0f : fast_exp2(base - next);
-        base = next;
+      // The four lanes of a row have the same.
+      bool rescales = false;
+      float correction[2] = {1.0f, 1.0f};
+      if (__builtin_expect(__any_sync(0xffffffffu, moves), 0)) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+#pragma unroll
+          for (int offset = 1; offset < 4; offset <<= 1) {
+            step_max[r] = fmaxf(step_max[r], __shfl_xor_sync(0xffffffffu, step_max[r], offset));
+            top[r] = max(top[r], __shfl_xor_sync(0xffffffffu, top[r], offset));
+          }
+          most[r] = fmaxf(most[r], step_max[r]);
+          exponent[r] = max(exponent[r], top[r]);
+          const float next = most[r] + static_cast<float>(exponent[r]);
+          // a row that has seen no key yet has O = 0 and a sum of 0: nothing to rescale
+          correction[r] = base[r] == -INFINITY ? 1.0f : fast_exp2(base[r] - next);
+          base[r] = next;
+          row_sum[r] *= correction[r];
+        }
+        rescales = h > 0 && __any_sync(0xffffffffu, correction[0] != 1.0f || correction[1] != 1.0f);
       }
-      if (!ok) {   // given up: the partner may still be a step behind, and must not wait for this warp's barriers
-        continue;
+      unsigned long long factor_pair[2], base_pair[2], sum_pair[4];
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const float from = base[r] == -INFINITY ? 0.f : -base[r];
+        factor_pair[r] = pair_of(factor[r], factor[r]);
+        base_pair[r] = pair_of(from, from);
+        sum_pair[r] = sum_pair[2 + r] = pair_of(0.f, 0.f);
       }
-      const float* v_scale = sh->v_scale[st] + sub * 32;
-      const float from = base == -INFINITY ? 0.f : base;
-      const unsigned long long factor_pair = pair_of(factor, factor), base_pair = pair_of(-from, -from);
-      unsigned long long sum_pair[4] = {pair_of(0.f, 0.f), pair_of(0.f, 0.f), pair_of(0.f, 0.f), pair_of(0.f, 0.f)};
       // one kind of instruction after the other over all elements: in the order of the elements each would wait for the one before
 #pragma unroll
-      for (int j = 0; j < 32; j += 2) {
+      for (int i = 0; i < 32; i += 2) {
         float x0, x1;
-        halves_of(fma_pair(pair_of(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), factor_pair, base_pair), x0, x1);
-        v[j] = __float_as_uint(x0);
-        v[j + 1] = __float_as_uint(x1);
+        halves_of(fma_pair(pair_of(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), factor_pair[(i >> 1) & 1], base_pair[(i >> 1) & 1]), x0, x1);
+        v[i] = __float_as_uint(x0);
+        v[i + 1] = __float_as_uint(x1);
       }
 #pragma unroll
-      for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(fast_exp2(__uint_as_float(v[j])));
+      for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(fast_exp2(__uint_as_float(v[i])));
 #pragma unroll
-      for (int j = 0; j < 32; j += 2)
-        sum_pair[(j >> 1) & 3] = add_pair(sum_pair[(j >> 1) & 3], pair_of(__uint_as_float(v[j]), __uint_as_float(v[j + 1])));
+      for (int i = 0; i < 32; i += 2)
+        sum_pair[(i >> 1) & 3] = add_pair(sum_pair[(i >> 1) & 3], pair_of(__uint_as_float(v[i]), __uint_as_float(v[i + 1])));
+      unsigned weights[16];
 #pragma unroll
-      for (int j = 0; j < 32; j += 4) {
-        const float4 s = *reinterpret_cast<const float4*>(v_scale + j);
+      for (int j = 0; j < 8; ++j) {
+        const float2 s = *reinterpret_cast<const float2*>(v_scale + 8 * j);
 #pragma unroll
-        for (int i = 0; i < 4; i += 2) {
+        for (int r = 0; r < 2; ++r) {
           float w0, w1;
-          halves_of(mul_pair(pair_of(__uint_as_float(v[j + i]), __uint_as_float(v[j + i + 1])), i == 0 ? pair_of(s.x, s.y) : pair_of(s.z, s.w)), w0, w1);
-          v[(j + i) / 2] = pack_half(w0, w1);   // over the weights already used
+          halves_of(mul_pair(pair_of(__uint_as_float(v[4 * j + 2 * r]), __uint_as_float(v[4 * j + 2 * r + 1])), pair_of(s.x, s.y)), w0, w1);
+          weights[2 * j + r] = pack_half(w0, w1);
         }
       }
-      if (edge && sh->v_bad[st][sub]) {   // rare: a key that the row does not see has no part in it, not even a scale of NaN
+      if (__builtin_expect(edge && (sh->v_bad[st][0] || sh->v_bad[st][1]), 0)) {   // rare: a key that the row does not see has no part in it, not even a scale of NaN
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const int key = key_base + 2 * j;
-          if (key < first || key > last) v[j] &= 0xffff0000u;
-          if (key + 1 < first || key + 1 > last) v[j] &= 0x0000ffffu;
+        for (int i = 0; i < 16; ++i) {
+          const int key = key_base + 8 * (i / 2) + 2 * t;
+          if (key < first[i & 1] || key > last[i & 1]) weights[i] &= 0xffff0000u;
+          if (key + 1 < first[i & 1] || key + 1 > last[i & 1]) weights[i] &= 0x0000ffffu;
         }
       }
-      float sum_lo, sum_hi;
-      halves_of(add_pair(add_pair(sum_pair[0], sum_pair[1]), add_pair(sum_pair[2], sum_pair[3])), sum_lo, sum_hi);
-      row_sum = row_sum * correction + (sum_lo + sum_hi);
       // P(h) goes where P(h - 2) was.  The product that read that was issued before the scores of step h, and a commit waits for
       // everything its thread has issued: s_full(h) says that it has been read.
-      tmem_store16(tmem_chain + P_COL + (h & 1) * 32 + sub * 16, v);   // keys 2 j and 2 j + 1 of the step in column j
-      if (h > 0 && __any_sync(0xffffffffu, correction != 1.0f)) {
+      tmem_store_pairs(tmem_chain + P_COL + (h & 1) * 32, weights);   // keys 2 j and 2 j + 1 of the step in column j
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        float sum_lo, sum_hi;
+        halves_of(add_pair(sum_pair[r], sum_pair[2 + r]), sum_lo, sum_hi);
+        row_sum[r] += sum_lo + sum_hi;
+      }
+      if (__builtin_expect(rescales, 0)) {
         // O still takes the step before: wait for its PV, then rescale
-        ok = mbar_wait(&sh->pv_done[chain][(h - 1) & 1], ((h - 1) >> 1) & 1, &sh->abort, args.status, ERR_SOFTMAX);
+        ok = wait_bar(&sh->pv_done[chain][(h - 1) & 1], ((h - 1) >> 1) & 1, &sh->abort, args.status, ERR_SOFTMAX);
         ok = __all_sync(0xffffffffu, ok);
-        if (!ok) continue;
+        if (!ok) break;
         fence_after_sync();
-        rescale_output_row(tmem_o, sub, correction);
+        rescale_output_rows(tmem_o, correction[0], correction[1]);
       }
       tmem_wait_store();
       fence_before_sync();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh->p_full[chain][h & 1]);
     }
-    if (ok && my_steps > 0) ok = mbar_wait(&sh->pv_last[chain], 0, &sh->abort, args.status, ERR_SOFTMAX);
+    if (ok && my_steps > 0) ok = wait_bar(&sh->pv_last[chain], 0, &sh->abort, args.status, ERR_SOFTMAX);
     ok = __all_sync(0xffffffffu, ok);
     fence_after_sync();
-    if (my_steps > 0) {
-      sh->row_sum[chain][sub][row] = row_sum;
-      pair_sync(pair);   // on every path
-      row_sum += sh->row_sum[chain][sub ^ 1][row];
-    }
-    // Outputs leave by way of the chain's query tile, which no product reads any more: a thread has a row, but 32 rows' pieces
-    // of 16 bytes would be 32 lines a store.  64 elements of a row a turn, 32 of each of its two threads.
-    const int token_head = there && ok ? (start + token) * args.num_heads + head : -1;
-    if (ok && args.splits > 1 && there && sub == 0) {
-      float* ml = args.partial_ml + 2 * (static_cast<size_t>(split) * args.num_tokens * args.num_heads + token_head);
-      ml[0] = my_steps > 0 ? base : -INFINITY;
-      ml[1] = my_steps > 0 ? row_sum : 0.f;
-    }
-    const bool nothing = row_sum == 0.f;   // a row that sees nothing is zeros
-    const float inv = nothing ? 0.f : 1.0f / row_sum;
+#pragma unroll
+    for (int r = 0; r < 2; ++r)
+#pragma unroll
+      for (int offset = 1; offset < 4; offset <<= 1) row_sum[r] += __shfl_xor_sync(0xffffffffu, row_sum[r], offset);
+    // Outputs leave by way of the chain's query tile, which no product reads any more: 64 elements of the warp's rows a turn, so
+    // that a store writes whole lines.
+    const int token_head = there && ok ? (start + tile_start + moved_token) * args.num_heads + kv_head * args.group + moved % args.group : -1;
     const bool partial = args.splits > 1;
+    bool nothing[2];
+    float inv[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      nothing[r] = row_sum[r] == 0.f;   // a row that sees nothing is zeros
+      inv[r] = nothing[r] ? 0.f : 1.0f / row_sum[r];
+      const int at = __shfl_sync(0xffffffffu, token_head, (lane >> 2) + 8 * r);
+      if (partial && at >= 0 && t == 0)
+        *reinterpret_cast<float2*>(args.partial_ml + 2 * (static_cast<size_t>(split) * args.num_tokens * args.num_heads + at)) =
+            make_float2(my_steps > 0 ? base[r] : -INFINITY, my_steps > 0 ? row_sum[r] : 0.f);
+    }
     if (my_steps > 0 || !partial) {
-      const int row_bytes = partial ? 256 : 128, lanes = row_bytes / 16;   // of 64 elements: lanes a row
+      const int row_bytes = partial ? 256 : 128, lanes = row_bytes / 16, spread = partial ? 1 : 0;   // of 64 elements: lanes a row
       unsigned char* stage = q_tiles + chain * Q_BYTES;
+#pragma unroll 1
       for (int turn = 0; turn < D / 64; ++turn) {
         unsigned o[32];
         if (my_steps > 0 && ok) {
-          tmem_load32(tmem_o + turn * 64 + sub * 32, o);
+          tmem_load_fragments(tmem_o + turn * 64, o);
           tmem_wait_load();
         } else {
 #pragma unroll
           for (int j = 0; j < 32; ++j) o[j] = 0u;
         }
-        unsigned char* mine = stage + row * row_bytes;
-        if (partial) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            *reinterpret_cast<uint4*>(mine + (((sub * 8 + j) ^ (row & 7)) << 4)) = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
-        } else {
+        for (int r = 0; r < 2; ++r) {
+          const int row = row0 + (lane >> 2) + 8 * r;
+          unsigned char* mine = stage + row * row_bytes;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            unsigned packed[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float x = nothing ? 0.f : __uint_as_float(o[8 * j + 2 * i]) * inv, y = nothing ? 0.f : __uint_as_float(o[8 * j + 2 * i + 1]) * inv;
-              const __nv_bfloat162 two = __floats2bfloat162_rn(x, y);
-              packed[i] = *reinterpret_cast<const unsigned*>(&two);
+          for (int j = 0; j < 8; ++j) {
+            if (partial) {
+              *reinterpret_cast<uint2*>(mine + (((2 * j + (t >> 1)) ^ ((row & 7) << 1)) << 4) + 8 * (t & 1)) = make_uint2(o[4 * j + 2 * r], o[4 * j + 2 * r + 1]);
+            } else {
+              const float x = nothing[r] ? 0.f : __uint_as_float(o[4 * j + 2 * r]) * inv[r], y = nothing[r] ? 0.f : __uint_as_float(o[4 * j + 2 * r + 1]) * inv[r];
+              *reinterpret_cast<__nv_bfloat162*>(mine + ((j ^ (row & 7)) << 4) + 4 * t) = __floats2bfloat162_rn(x, y);
             }
-            *reinterpret_cast<uint4*>(mine + (((sub * 4 + j) ^ (row & 7)) << 4)) = make_uint4(packed[0], packed[1], packed[2], packed[3]);
           }
         }
-        pair_sync(pair);
-        const int piece = lane & (lanes - 1), rows_at_once = 32 / lanes;   // of this warp's 16 of the 32 rows
+        __syncwarp();
+        const int piece = lane & (lanes - 1), rows_at_once = 32 / lanes;
+#pragma unroll 1
         for (int i = 0; i < 16 / rows_at_once; ++i) {
-          const int within = sub * 16 + i * rows_at_once + lane / lanes, from = quarter * 32 + within;
+          const int within = i * rows_at_once + lane / lanes, from = row0 + within;
           const int at = __shfl_sync(0xffffffffu, token_head, within);
-          const uint4 v = *reinterpret_cast<const uint4*>(stage + from * row_bytes + ((piece ^ (from & 7)) << 4));
+          const uint4 v = *reinterpret_cast<const uint4*>(stage + from * row_bytes + ((piece ^ ((from & 7) << spread)) << 4));
           if (at >= 0) {
             if (partial)
               *reinterpret_cast<uint4*>(args.partial_o + (static_cast<size_t>(split) * args.num_tokens * args.num_heads + at) * D + turn * 64 + piece * 4) = v;
@@ -765,7 +800,7 @@ portions_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
               *reinterpret_cast<uint4*>(args.out + static_cast<size_t>(at) * D + turn * 64 + piece * 8) = v;
           }
         }
-        pair_sync(pair);   // the tile is written again in the next turn
+        __syncwarp();   // the tile is written again in the next turn
       }
     }
   }
