@@ -919,9 +919,10 @@ SHRIKE_API int shrike_attention_q8_tc_tokens(int group) { return group >= 1 && g
 // How many CTAs should share the keys of a query tile, for a batch whose portions make `tiles` query tiles over block tables of
 // `keys` keys: the GPU holds one CTA per SM, so the time is that of the rounds of CTAs, each its key tiles and about CTA_START
 // of their time for a CTA's start and end, and a split launch pays COMBINE more for the second kernel.  Measured (40 heads, 512
-// tokens over 8,192 keys, 88 CTAs' worth of query tiles): unsplit 205 us, two splits 210, three 156, five 156, eight 186.
+// tokens over 8,192 keys, 88 CTAs' worth of query tiles): unsplit 164 us, two splits 171, three 128, four 146, five 131, six
+// 150, eight 161; 12 heads, 475 tokens over 1,115 keys, 24 CTAs' worth: unsplit 28.5, two 22.8, four 19.5, six 18.6.
 SHRIKE_API int shrike_attention_q8_tc_splits(int tiles, int num_kv_heads, long long keys) {
-  constexpr long long CTA_START = 6, COMBINE = 4;
+  constexpr long long CTA_START = 8, COMBINE = 4;
   const long long ctas = static_cast<long long>(num_kv_heads) * tiles, capacity = shrike_device().sm_count;
   const long long key_tiles = (keys + tcq8::KEYS - 1) / tcq8::KEYS;
   int best = 1;
