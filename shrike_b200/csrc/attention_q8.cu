@@ -539,11 +539,13 @@ split_keys_kernel(const Args args) {
   const int kv_head = blockIdx.y % args.num_kv_heads, tile = blockIdx.y / args.num_kv_heads;
   const int group = args.num_heads / args.num_kv_heads;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  wait_for_previous();
-  int start, q_len, context;
-  if (!entry_of(args, seq, start, q_len, context)) return;
+  int start, q_len, context;   // metadata, and so is the block table: written before the step's kernels
+  const bool mine = entry_of(args, seq, start, q_len, context);
   const int rows = q_len * group, row0 = tile * ROWS;
-  if (row0 >= rows) return;
+  if (!mine || row0 >= rows) {
+    wait_for_previous();
+    return;
+  }
   const int pos0 = context - q_len;
   const int tile_rows = min(ROWS, rows - row0);
   const int last_key = pos0 + (row0 + tile_rows - 1) / group, first_key = first_visible_key(pos0 + row0 / group, args.window);
@@ -571,6 +573,7 @@ split_keys_kernel(const Args args) {
   auto place_at = [&](int page, int step) { return place_of(args, page, kv_head, step * KEYS + lane); };
   int page = page_at(begin), next_page = page_at(begin + WARPS), ahead = page_at(begin + 2 * WARPS);
   Place place = place_at(page, begin), next = place_at(next_page, begin + WARPS);
+  wait_for_previous();   // the query and the newest keys come from the kernel before this one
   if (begin < mine_hi) load_keys(place, 0, 0);
   copies_commit();
   if (begin < mine_hi) load_codes<32>(args.v_codes, row_bytes, head_at, place.row, ring_at + TILE, lane);
@@ -726,12 +729,14 @@ portion_rows_kernel(const Args args) {
   const int seq = blockIdx.z, kv_head = blockIdx.y;
   const int group = args.num_heads / args.num_kv_heads;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  wait_for_previous();
-  int start, q_len, context;
-  if (!entry_of(args, seq, start, q_len, context)) return;
+  int start, q_len, context;   // metadata, as above
+  const bool mine = entry_of(args, seq, start, q_len, context);
   const int rows = q_len * group;
   const int tiles = (rows + WARPS * ROWS - 1) / (WARPS * ROWS);
-  if (static_cast<int>(blockIdx.x) >= tiles) return;
+  if (!mine || static_cast<int>(blockIdx.x) >= tiles) {
+    wait_for_previous();
+    return;
+  }
   const int cta_row0 = (tiles - 1 - static_cast<int>(blockIdx.x)) * WARPS * ROWS;   // the longest first
   const int row0 = cta_row0 + warp * ROWS;
   const int pos0 = context - q_len;
@@ -755,6 +760,7 @@ portion_rows_kernel(const Args args) {
   auto page_at = [&](int step) { return page_of(args, table, step * KEYS + lane, last_key); };
   auto place_at = [&](int page, int step) { return place_of(args, page, kv_head, step * KEYS + lane); };
   int page = page_at(step_lo), ahead = page_at(step_lo + 1);
+  wait_for_previous();
   if (step_lo < step_hi) load_step(place_at(page, step_lo), ring_at);
   copies_commit();
   r.begin(args, row0, rows, start, group, kv_head, pos0, shared_q, lane);

@@ -815,23 +815,42 @@ portions_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
 // Adds up the splits of every query row of the portions: out = sum_s O_s 2^(base_s - M) / sum_s l_s 2^(base_s - M) with M the
 // largest base.  One warp per (token, head), lanes over the splits first (bases and sums), then over the head size.  Tokens of
 // one-token sequences belong to the other kernel and are left alone.
+// The splits' rows are asked for four at a time, the first four before their weights are known.
 __global__ void __launch_bounds__(256)
 combine_portions_kernel(const Args args) {
+  constexpr int VEC = D / 32, AT_ONCE = 4;
   let_dependents_start();
-  wait_for_previous();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int token = blockIdx.y * 8 + warp, head = blockIdx.x;
-  if (token >= args.num_tokens || token >= args.q_start[args.num_seqs]) return;   // rows behind the last sequence stay as they are
-  const int seq = args.seq_of_token[token];
-  if (seq < 0 || seq >= args.num_seqs) return;
-  if (args.skip_single && args.q_start[seq + 1] - args.q_start[seq] == 1) return;
+  bool mine = token < args.num_tokens && token < args.q_start[args.num_seqs];   // rows behind the last sequence stay as they are
+  if (mine) {
+    const int seq = args.seq_of_token[token];
+    mine = seq >= 0 && seq < args.num_seqs && !(args.skip_single && args.q_start[seq + 1] - args.q_start[seq] == 1);
+  }
+  wait_for_previous();
+  if (!mine) return;
   const size_t token_head = static_cast<size_t>(token) * args.num_heads + head;
   const size_t slice = static_cast<size_t>(args.num_tokens) * args.num_heads;
-  float m = -INFINITY, l = 0.f;                       // lane s holds split s (at most 32 splits)
-  if (lane < args.splits) {
-    m = args.partial_ml[2 * (lane * slice + token_head)];
-    l = args.partial_ml[2 * (lane * slice + token_head) + 1];
-  }
+  const float* rows = args.partial_o + token_head * D + lane * VEC;
+  float v[AT_ONCE][VEC];
+  auto load = [&](int first) {   // what a split that saw no key of this row left there is whatever it is
+#pragma unroll
+    for (int i = 0; i < AT_ONCE; ++i)
+      if (first + i < args.splits) {
+        const float* src = rows + (first + i) * slice * D;
+        if constexpr (VEC == 4) {
+          const float4 x = *reinterpret_cast<const float4*>(src);
+          v[i][0] = x.x; v[i][1] = x.y; v[i][2] = x.z; v[i][3] = x.w;
+        } else {
+          const float2 x = *reinterpret_cast<const float2*>(src);
+          v[i][0] = x.x; v[i][1] = x.y;
+        }
+      }
+  };
+  load(0);
+  float2 ml = make_float2(-INFINITY, 0.f);            // lane s holds split s (at most 32 splits)
+  if (lane < args.splits) ml = *reinterpret_cast<const float2*>(args.partial_ml + 2 * (lane * slice + token_head));
+  const float m = ml.x, l = ml.y;
   float base = m;
 #pragma unroll
   for (int offset = 16; offset > 0; offset >>= 1) base = fmaxf(base, __shfl_xor_sync(0xffffffffu, base, offset));
@@ -839,20 +858,29 @@ combine_portions_kernel(const Args args) {
   float total = l != l ? l : weight == 0.f ? 0.f : l * weight;   // a score that is no number makes the row none
 #pragma unroll
   for (int offset = 16; offset > 0; offset >>= 1) total += __shfl_xor_sync(0xffffffffu, total, offset);
-  float acc[D / 32];
+  float acc[VEC];
 #pragma unroll
-  for (int c = 0; c < D / 32; ++c) acc[c] = 0.f;
-  for (int s = 0; s < args.splits; ++s) {
-    const float w = __shfl_sync(0xffffffffu, weight, s);
-    if (w == 0.f) continue;                           // its output row may never have been written
-    const float* src = args.partial_o + (s * slice + token_head) * D;
+  for (int c = 0; c < VEC; ++c) acc[c] = 0.f;
+  for (int first = 0; first < args.splits; first += AT_ONCE) {
+    if (first > 0) load(first);
 #pragma unroll
-    for (int c = 0; c < D / 32; ++c) acc[c] += src[c * 32 + lane] * w;
+    for (int i = 0; i < AT_ONCE; ++i) {
+      const float w = __shfl_sync(0xffffffffu, weight, (first + i) & 31);
+      if (first + i < args.splits && w != 0.f)
+#pragma unroll
+        for (int c = 0; c < VEC; ++c) acc[c] += v[i][c] * w;
+    }
   }
   const float inv = total == 0.f ? 0.f : 1.0f / total;
-  __nv_bfloat16* dst = args.out + token_head * D;
+  unsigned packed[VEC / 2];
 #pragma unroll
-  for (int c = 0; c < D / 32; ++c) dst[c * 32 + lane] = __float2bfloat16_rn(acc[c] * inv);
+  for (int c = 0; c < VEC; c += 2) {
+    const __nv_bfloat162 two = __floats2bfloat162_rn(acc[c] * inv, acc[c + 1] * inv);
+    packed[c / 2] = *reinterpret_cast<const unsigned*>(&two);
+  }
+  __nv_bfloat16* dst = args.out + token_head * D + lane * VEC;
+  if constexpr (VEC == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(packed[0], packed[VEC / 2 - 1]);
+  else *reinterpret_cast<unsigned*>(dst) = packed[0];
 }
 
 // Tensor maps, kept by what they describe (host only).
@@ -919,8 +947,8 @@ SHRIKE_API int shrike_attention_q8_tc_tokens(int group) { return group >= 1 && g
 // How many CTAs should share the keys of a query tile, for a batch whose portions make `tiles` query tiles over block tables of
 // `keys` keys: the GPU holds one CTA per SM, so the time is that of the rounds of CTAs, each its key tiles and about CTA_START
 // of their time for a CTA's start and end, and a split launch pays COMBINE more for the second kernel.  Measured (40 heads, 512
-// tokens over 8,192 keys, 88 CTAs' worth of query tiles): unsplit 164 us, two splits 171, three 128, four 146, five 131, six
-// 150, eight 161; 12 heads, 475 tokens over 1,115 keys, 24 CTAs' worth: unsplit 28.5, two 22.8, four 19.5, six 18.6.
+// tokens over 8,192 keys, 88 CTAs' worth of query tiles): unsplit 164 us, two splits 170, three 127, four 145, five 131, six
+// 148, eight 159; 12 heads, 475 tokens over 1,115 keys, 24 CTAs' worth: unsplit 28.5, two 22.0, four 18.0, six 17.2.
 SHRIKE_API int shrike_attention_q8_tc_splits(int tiles, int num_kv_heads, long long keys) {
   constexpr long long CTA_START = 8, COMBINE = 4;
   const long long ctas = static_cast<long long>(num_kv_heads) * tiles, capacity = shrike_device().sm_count;
