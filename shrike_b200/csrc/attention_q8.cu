@@ -23,8 +23,11 @@
 //
 // Two forms.  Few rows (single tokens): the rows' keys are dealt to `splits` CTAs and to each CTA's four warps, each with its
 // own ring of cp.async copies (no barrier in the loop); the warps' results meet in shared memory, those of up to eight CTAs in
-// the shared memory of their cluster, and the clusters' in global memory, where the last CTA to arrive adds them up in order.  Many rows (portions): four warps of 8 NT rows each
-// share one ring of key tiles.
+// the shared memory of their cluster, and the clusters' in global memory, where the last CTA to arrive adds them up in order.
+// Bound by memory at many keys (64 sequences of 4,096 keys, 40 heads of 128: 85 us, 5.0 TB/s; with the products left out the
+// copies alone take 71), and by the chain metadata, page, codes, products, merges at few (one sequence of 517 keys: 5.5 us).
+// Metadata and pages are looked up while the kernel before still runs (that sequence: 6.1 us without).  Many rows (portions):
+// four warps of 8 NT rows each share one ring of key tiles.
 #include <cuda_fp16.h>
 
 #include "attention_q8.cuh"
@@ -540,9 +543,12 @@ split_keys_kernel(const Args args) {
   const int group = args.num_heads / args.num_kv_heads;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   int start, q_len, context;   // metadata, and so is the block table: written before the step's kernels
-  const bool mine = entry_of(args, seq, start, q_len, context);
+  if (!entry_of(args, seq, start, q_len, context)) {
+    wait_for_previous();
+    return;
+  }
   const int rows = q_len * group, row0 = tile * ROWS;
-  if (!mine || row0 >= rows) {
+  if (row0 >= rows) {
     wait_for_previous();
     return;
   }
@@ -555,8 +561,8 @@ split_keys_kernel(const Args args) {
 
   uint2* shared_q = reinterpret_cast<uint2*>(smem + WARPS * RING);
   // A warp's ring: three tiles that keys and values go through in turn (K0 V0 K1 V1 ...), so that each is asked for a whole step
-  // before it is used, and two steps' scales.  (Two tiles for keys and one for values: a value tile then has half a step, and
-  // a batch of 64 sequences of 4,096 keys takes 91 us instead of 85.)
+  // before it is used, and two steps' scales.  Four warps' rings are 50 KB at a head size of 128: an SM holds four CTAs.  (One
+  // tile more a warp left room for three: 96 us instead of 89 for 64 sequences of 4,096 keys, as it was then.)
   unsigned char* ring = smem + warp * RING;
   const float* scales = reinterpret_cast<const float*>(ring + 3 * TILE);
   const unsigned ring_at = smem_u32(ring), scales_at = ring_at + 3 * TILE;
@@ -572,8 +578,8 @@ split_keys_kernel(const Args args) {
   auto page_at = [&](int step) { return page_of(args, table, step * KEYS + lane, step < mine_hi ? last_key : -1); };
   auto place_at = [&](int page, int step) { return place_of(args, page, kv_head, step * KEYS + lane); };
   int page = page_at(begin), next_page = page_at(begin + WARPS), ahead = page_at(begin + 2 * WARPS);
-  Place place = place_at(page, begin), next = place_at(next_page, begin + WARPS);
   wait_for_previous();   // the query and the newest keys come from the kernel before this one
+  Place place = place_at(page, begin), next = place_at(next_page, begin + WARPS);
   if (begin < mine_hi) load_keys(place, 0, 0);
   copies_commit();
   if (begin < mine_hi) load_codes<32>(args.v_codes, row_bytes, head_at, place.row, ring_at + TILE, lane);

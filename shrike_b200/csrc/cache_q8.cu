@@ -82,8 +82,9 @@ struct Pages {
 };
 
 // ---- store of rows as they are
-// LANES threads a row (a head of a token's keys or values), four elements each a turn; a block is 256 threads.  Measured: see
-// the launcher.
+// LANES threads a row (a head of a token's keys or values), four elements each a turn (two turns above 128 elements), 8, 16 or
+// 32 lanes by the head size, so that few are idle; a block is 256 threads.  Bound by the latency of a dependent chain (slot and
+// row, the maximum over the lanes, codes): 2,048 tokens of 4 heads of 128 in bfloat16, 6.3 MB in and out, take 5 us.
 template <typename T, int LANES>
 __global__ void __launch_bounds__(256)
 kv_write_q8_kernel(const T* __restrict__ k_new, const T* __restrict__ v_new, long long k_stride, long long v_stride, const Pages keys,
@@ -222,7 +223,7 @@ rope_kv_write_q8_kernel(const float* __restrict__ qkv, const float* __restrict__
 
 // ---- reading back
 // A thread takes 16 codes of a key and the 16 of its value: two 16-byte loads that do not wait for one another, two to four
-// 16-byte stores each.  Bound by memory.
+// 16-byte stores each.  Bound by memory: 32,768 tokens of 8 heads of 128 to bfloat16, 204 MB, take 34.5 us, 5.9 TB/s.
 template <typename T> __device__ __forceinline__ void read_chunk(const Pages& from, long long row, long long scale_at, int within, T* out) {
   uint4 words = make_uint4(0u, 0u, 0u, 0u);
   float scale = 0.f;

@@ -736,7 +736,7 @@ class CudaOps(QuantisedCacheOps):
         `keep_first` (with a window): the sequence's first `keep_first` keys stay visible to every later query.
         `early_metadata`: `block_table`, `q_start`, `ctx_len` and `seq_of_token` were last written by a copy or an earlier step
         (which have finished), not by a kernel of this step; they are then read while the kernel before this one runs.  In
-        bfloat16 (heads of up to 256) they always are, and have to be such.
+        bfloat16 (heads of up to 256) and over 8-bit pages they always are, and have to be such.
         With `QuantisedPages` for keys and values: heads of up to 256, a window or a chunk, and none of the other changes to
         scores; `max_q_len` is needed, and a query that sees no key (a context shorter than its new tokens) gets zeros."""
         if quantised(keys, values):

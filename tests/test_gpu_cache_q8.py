@@ -237,6 +237,14 @@ def test_rows_that_see_nothing_are_zeros(dtype, dim, tensor_cores, splits):
 
 
 @pytest.mark.parametrize("dtype,dim,tensor_cores", FORMS)
+@pytest.mark.parametrize("splits", [1, 3])
+@pytest.mark.parametrize("ctx_lens", [[30, 700, 12], [1, 300, 60], [54, 90, 2]])
+def test_whole_runs_of_rows_that_see_nothing(dtype, dim, tensor_cores, splits, ctx_lens):
+    """Contexts so short that a kernel's first run of 18 tokens (128 rows of seven heads) sees nothing and its second does."""
+    check_attention(dtype, 7, 1, dim, 16, [60, 37, 19], ctx_lens, seed=5, splits=(splits, 1), tensor_cores=tensor_cores, portion_splits=splits)
+
+
+@pytest.mark.parametrize("dtype,dim,tensor_cores", FORMS)
 @pytest.mark.parametrize("options", [{}, {"window": 30}])
 def test_what_a_row_does_not_see_has_no_part_in_it(dtype, dim, tensor_cores, options):
     """Keys and values stored from infinities, NaN and the largest numbers: rows before them are what they would be without,
