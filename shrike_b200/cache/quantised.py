@@ -12,23 +12,28 @@ import torch
 
 MOST_HEAD_DIM = 256   # of the kernels over 8-bit pages
 _INT8, _FLOAT32 = torch.int8, torch.float32
+look_pages = None   # the same questions as `_look_here`, natively, once the kernels are loaded (`ops/quantised_cache.py`)
+
+
+def _look_here(codes, scales):
+    """The codes' sizes; None: not a pool's codes and scales."""
+    dims = codes.shape
+    if not (len(dims) == 4 and codes.dtype is _INT8 and scales.dtype is _FLOAT32 and scales.shape == (dims[0], dims[2], dims[1])
+            and codes.is_contiguous() and scales.is_contiguous() and codes.device == scales.device):
+        return None
+    return tuple(dims)
 
 
 class QuantisedPages:
     """`codes` int8 [pages, page_size, kv heads, head size], `scales` float32 [pages, kv heads, page_size], on one device."""
 
-    __slots__ = ("codes", "scales", "dims", "device_index", "served")
+    __slots__ = ("codes", "scales", "dims")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor):
-        dims = codes.shape
-        if not (len(dims) == 4 and codes.dtype is _INT8 and scales.dtype is _FLOAT32 and scales.shape == (dims[0], dims[2], dims[1])
-                and codes.is_contiguous() and scales.is_contiguous() and codes.device == scales.device):
+        dims = (look_pages or _look_here)(codes, scales)
+        if dims is None:
             self._refuse(codes, scales)
         self.codes, self.scales, self.dims = codes, scales, dims   # (pages, page_size, kv heads, head size)
-        self.device_index = codes.get_device()   # -1: not on a GPU
-        pages, page_size, _heads, dim = dims
-        # whether the kernels take them: their head sizes, and slots that are 32-bit numbers
-        self.served = not dim % 16 and 16 <= dim <= MOST_HEAD_DIM and pages * page_size <= 0x7FFFFFFF
 
     @staticmethod
     def _refuse(codes, scales):

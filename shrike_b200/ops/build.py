@@ -13,7 +13,9 @@ from __future__ import annotations
 
 import ctypes
 import fcntl
+import functools
 import hashlib
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -187,6 +189,29 @@ def attention_q8_library(head_dim: int) -> ctypes.CDLL:
     return load_library(f"shrike_attention_q8_d{head_dim}", ATTENTION_Q8_SOURCES, {"SHRIKE_HEAD_DIM": head_dim})
 
 
+def _tensor_look_path() -> Path:
+    import re
+    import sysconfig
+
+    import torch
+
+    torch_dir = Path(torch.__file__).resolve().parent
+    built_for = re.sub(r"\W", "_", f"{torch.__version__}_{sys.implementation.cache_tag}")
+    flags = [f"-DSHRIKE_BUILT_FOR={built_for}", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", f"-I{torch_dir / 'include'}",
+             f"-I{torch_dir / 'include' / 'torch' / 'csrc' / 'api' / 'include'}", f"-I{sysconfig.get_paths()['include']}",
+             "-Xlinker", "--no-as-needed", f"-L{torch_dir / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10"]
+    return compile_library("shrike_tensor_look", ["tensor_look.cpp"], None, flags)
+
+
+@functools.lru_cache(maxsize=None)
+def tensor_look():
+    """The Python module of `tensor_look.cpp`."""
+    spec = importlib.util.spec_from_file_location("shrike_tensor_look", _tensor_look_path())
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    return module
+
+
 def tensor_core_gemm_library() -> ctypes.CDLL:
     return load_library("shrike_gemm_tcgen05", ["gemm_tcgen05.cu"])
 
@@ -202,7 +227,8 @@ def decode_step_library() -> ctypes.CDLL:
 def build_all(head_dims=(16, 32, 48, 64, 128, 256)) -> list[Path]:
     """Everything the package can load, for the usual head sizes."""
     built = [compile_library("shrike_core", CORE_SOURCES), compile_library("shrike_gemm_tcgen05", ["gemm_tcgen05.cu"]),
-             compile_library("shrike_layer_program", ["layer_program.cu"]), compile_library("shrike_decode_step", ["decode_step.cu"])]
+             compile_library("shrike_layer_program", ["layer_program.cu"]), compile_library("shrike_decode_step", ["decode_step.cu"]),
+             _tensor_look_path()]
     for head_dim in head_dims:
         built.append(compile_library(f"shrike_attention_d{head_dim}", ATTENTION_SOURCES,
                                      {"SHRIKE_HEAD_DIM": head_dim}))

@@ -8,11 +8,13 @@ belong on one stream at a time, captured launch sequences included.
 from __future__ import annotations
 
 import ctypes
+import functools
 import struct
 from dataclasses import dataclass
 
 import torch
 
+from ..cache import quantised as quantised_pages
 from ..cache.quantised import MOST_HEAD_DIM, QuantisedPages
 from . import build
 
@@ -21,9 +23,8 @@ _P, _I, _F, _LL = _c.c_void_p, _c.c_int, _c.c_float, _c.c_longlong
 DTYPE_CODE = {torch.float32: 0, torch.bfloat16: 1}
 # The launchers take their arguments as one packed structure (ShrikeCacheQ8, ShrikeAttentionQ8): a call of thirty arguments takes
 # ctypes two microseconds, this a third of one.
-_CACHE_CALL = struct.Struct("=8Q2q6i")
 _ATTENTION_CALL = struct.Struct("=14Q16if")
-_pack_cache, _pack_attention = _CACHE_CALL.pack, _ATTENTION_CALL.pack
+_pack_attention = _ATTENTION_CALL.pack
 _INT32 = torch.int32
 _device = getattr(torch._C, "_cuda_getDevice", None)          # the current device's number, and its current stream's handle:
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)   # asking torch for the objects costs more than a launch
@@ -45,6 +46,14 @@ class QuantisedPlan:
     portion_scratch: torch.Tensor | None = None
     lib: object = None
     launches: int = 0
+
+
+@functools.lru_cache(maxsize=None)
+def _look():
+    """The native module, which pages made from now on use too."""
+    module = build.tensor_look()
+    quantised_pages.look_pages = module.pages
+    return module
 
 
 def _error(text):
@@ -102,8 +111,8 @@ class QuantisedCacheOps:
         return lib
 
     # ---- checks
-    # A call of the engine's takes longer on the host than its kernel takes for few tokens, so what is right is seen in one
-    # expression of cheap questions; which of them failed is looked up only then.
+    # A call takes longer on the host than its kernel takes for few tokens, so its tensors are looked at in one native call
+    # (`tensor_look.cpp`: 0.3 us where the same questions from here take 2.5); what did not fit is looked up only then.
     def _q8_stream(self):
         """The current device and the handle of its current stream (or of the one that is held)."""
         device = _device()
@@ -156,26 +165,17 @@ class QuantisedCacheOps:
     def _kv_write_q8(self, k_new, v_new, keys, values, slots):
         device = _device()
         stream = _raw_stream(device) if self._held_stream is None else self._held_stream
-        pages, page_size, heads, dim = dims = keys.dims
-        codes, value_codes, dtype = keys.codes.data_ptr(), values.codes.data_ptr(), self.dtype
-        n = k_new.shape[0]
-        width = heads * dim
-        if not (keys.served and dims == values.dims and keys.device_index == device and values.device_index == device
-                and not (codes | value_codes) % 16 and slots.get_device() == device and slots.dtype is _INT32 and slots.numel() == n
-                and slots.is_contiguous()):
+        call = _look().cache(k_new, v_new, keys.codes, keys.scales, values.codes, values.scales, slots, device, self.code, stream, 1)
+        if call is None:
+            n, (_pages, _page_size, heads, dim) = k_new.shape[0], keys.dims
             self._q8_refuse(device, (), [(slots, n, "slots")], (keys, values, None, None))
-        if (k_new.dtype is dtype and v_new.dtype is dtype and k_new.get_device() == device and v_new.get_device() == device
-                and k_new.shape == v_new.shape == (n, width) and k_new.is_contiguous() and v_new.is_contiguous()):
-            k_stride = v_stride = width
-        else:
-            k_stride = self._q8_rows(device, k_new, n, width, "new keys")
-            v_stride = self._q8_rows(device, v_new, n, width, "new values")
-        if n == 0:
+            self._q8_rows(device, k_new, n, heads * dim, "new keys")
+            self._q8_rows(device, v_new, n, heads * dim, "new values")
+            raise _error("kv_write: the tensors do not fit 8-bit pages")
+        if not call:   # no rows
             return
         self.launches += 1
-        code = self.core.shrike_kv_write_q8(_pack_cache(
-            k_new.data_ptr(), v_new.data_ptr(), codes, value_codes, keys.scales.data_ptr(), values.scales.data_ptr(), slots.data_ptr(),
-            stream, k_stride, v_stride, self.code, n, heads, dim, pages, page_size))
+        code = self.core.shrike_kv_write_q8(call)
         if code:
             _failed(code, "kv_write_q8")
 
@@ -214,24 +214,16 @@ class QuantisedCacheOps:
             raise _error("kv_read reads 8-bit pages; a cache in the engine's type is indexed as it is")
         device = _device()
         stream = _raw_stream(device) if self._held_stream is None else self._held_stream
-        pages, page_size, heads, dim = dims = keys.dims
-        codes, value_codes = keys.codes.data_ptr(), values.codes.data_ptr()
-        n, dtype = slots.numel(), self.dtype
-        k_at, v_at = k_out.data_ptr(), v_out.data_ptr()
-        if not (keys.served and dims == values.dims and keys.device_index == device and values.device_index == device
-                and slots.get_device() == device and slots.dtype is _INT32 and slots.is_contiguous() and k_out.dtype is dtype
-                and v_out.dtype is dtype and k_out.shape == v_out.shape == (n, heads * dim) and k_out.get_device() == device
-                and v_out.get_device() == device and k_out.is_contiguous() and v_out.is_contiguous()
-                and not (k_at | v_at | codes | value_codes) % 16):
-            self._q8_refuse(device, [(k_out, dtype, "keys read"), (v_out, dtype, "values read")], [(slots, n, "slots")],
+        call = _look().cache(k_out, v_out, keys.codes, keys.scales, values.codes, values.scales, slots, device, self.code, stream, 0)
+        if call is None:
+            n, (_pages, _page_size, heads, dim) = slots.numel(), keys.dims
+            self._q8_refuse(device, [(k_out, self.dtype, "keys read"), (v_out, self.dtype, "values read")], [(slots, n, "slots")],
                             (keys, values, None, None))
             raise _error(f"keys and values read must be [{n}, {heads * dim}], are {list(k_out.shape)} and {list(v_out.shape)}")
-        if n == 0:
+        if not call:
             return
         self.launches += 1
-        code = self.core.shrike_kv_read_q8(_pack_cache(
-            k_at, v_at, codes, value_codes, keys.scales.data_ptr(), values.scales.data_ptr(), slots.data_ptr(), stream, 0, 0, self.code,
-            n, heads, dim, pages, page_size))
+        code = self.core.shrike_kv_read_q8(call)
         if code:
             _failed(code, "kv_read_q8")
 
@@ -329,20 +321,11 @@ class QuantisedCacheOps:
                             scale, window, out, max_q_len, min_q_len, q_lens, max_ctx_len):
         device = _device()
         stream = _raw_stream(device) if self._held_stream is None else self._held_stream
-        pages, page_size, heads, dim = dims = keys.dims
-        codes, value_codes = keys.codes.data_ptr(), values.codes.data_ptr()
-        num_seqs, max_blocks = block_table.shape
-        n, dtype = q.shape[0], self.dtype
-        q_at, out_at = q.data_ptr(), out.data_ptr()
-        if not (keys.served and dims == values.dims and keys.device_index == device and values.device_index == device
-                and heads == num_kv_heads and dim == head_dim and not num_heads % heads and q.dtype is dtype and out.dtype is dtype
-                and q.shape == out.shape == (n, num_heads * head_dim) and q.get_device() == device and out.get_device() == device
-                and q.is_contiguous() and out.is_contiguous() and not (q_at | out_at | codes | value_codes) % 16
-                and block_table.dtype is _INT32 and block_table.get_device() == device and block_table.is_contiguous()
-                and q_start.dtype is _INT32 and q_start.get_device() == device and q_start.numel() == num_seqs + 1
-                and q_start.is_contiguous() and ctx_len.dtype is _INT32 and ctx_len.get_device() == device
-                and ctx_len.numel() == num_seqs and ctx_len.is_contiguous() and max_q_len >= 1):
-            self._q8_refuse(device, [(q, dtype, "q"), (out, dtype, "attention output")], [
+        found = _look().attention(q, out, keys.codes, keys.scales, values.codes, values.scales, block_table, q_start, ctx_len, device,
+                                  self.code, num_heads, num_kv_heads, head_dim)
+        if found is None or max_q_len < 1:
+            num_seqs, max_blocks = block_table.shape
+            self._q8_refuse(device, [(q, self.dtype, "q"), (out, self.dtype, "attention output")], [
                 (block_table, num_seqs * max_blocks, "block table"), (q_start, num_seqs + 1, "query starts"),
                 (ctx_len, num_seqs, "context lengths")], (keys, values, num_kv_heads, head_dim))
             if num_heads % num_kv_heads:
@@ -350,15 +333,15 @@ class QuantisedCacheOps:
             if max_q_len < 1:
                 raise _error("paged_attention over 8-bit pages needs max_q_len, the longest entry of the batch")
             raise _error(f"q {list(q.shape)} and output {list(out.shape)} must be [tokens, {num_heads * head_dim}]")
+        n, num_seqs, max_blocks, out_at, at = found
         if n == 0 or num_seqs == 0:
             return
+        pages, page_size, _heads, _dim = keys.dims
         window = window or 0
         plan = self.q8_plan(num_heads, num_kv_heads, head_dim, num_seqs, max_blocks, page_size, max_q_len, min_q_len, window, n, q_lens, max_ctx_len)
         tc, has_portions = plan.tc_portions, plan.has_portions
         if tc and not self._q8_ints_fit(device, seq_of_token, n):
             self._q8_refuse(device, (), [(seq_of_token, n, "sequences of tokens")])
-        at = (q_at, codes, keys.scales.data_ptr(), value_codes, values.scales.data_ptr(), block_table.data_ptr(), q_start.data_ptr(),
-              ctx_len.data_ptr())
         sizes = (max_blocks, self.code, n, num_seqs, num_heads, num_kv_heads, page_size, pages, window, plan.has_single)
         self.launches += plan.launches
         if tc:

@@ -1,6 +1,7 @@
 """The 8-bit cache's host side, without a GPU: pages, pools, the engine's option, what the calls refuse and how they are cut."""
 
 import math
+import struct
 
 import numpy as np
 import pytest
@@ -8,6 +9,7 @@ import torch
 
 import shrike_b200.models  # noqa: F401
 from shrike_b200 import SamplingParams
+from shrike_b200.cache import quantised
 from shrike_b200.cache.quantised import QuantisedPages
 from shrike_b200.cli import parse_args
 from shrike_b200.config import parse_config
@@ -150,6 +152,37 @@ def test_pages_say_what_is_wrong():
             QuantisedPages(bad_codes, bad_scales)
     with pytest.raises(ValueError, match="are on"):
         QuantisedPages(codes, scales.to("meta"))
+
+
+def test_the_native_look_at_tensors_sees_what_the_plain_one_sees():
+    look = quantised_cache._look()
+    codes, scales = torch.zeros(3, 16, 2, 64, dtype=torch.int8), torch.zeros(3, 2, 16)
+    pairs = [(codes, scales), (codes.float(), scales), (codes[0], scales), (codes[:, ::2], scales), (codes, scales.half()), (codes, scales[:2]),
+             (codes, torch.zeros(3, 16, 2)), (codes, torch.zeros(3, 2, 32)[..., ::2]), (codes, scales.to("meta")), (codes[:0], scales[:0]),
+             (codes.to("meta"), scales.to("meta"))]
+    for pair in pairs:
+        assert look.pages(*pair) == quantised._look_here(*pair)
+    assert look.pages(codes, None) is None
+    with pytest.raises(TypeError):
+        look.pages(codes)
+
+
+def test_a_store_s_arguments_as_the_launcher_gets_them():
+    look = quantised_cache._look()
+    keys, values = (QuantisedPages.zeros(5, 16, 3, 32, "cpu") for _ in range(2))
+    wide, slots = torch.zeros(4, 300), torch.zeros(4, dtype=torch.int32)
+    k, v = wide[:, 1: 97], wide[:, 100: 196]
+    pools = (keys.codes, keys.scales, values.codes, values.scales)
+    got = struct.unpack("=8Q2q6i", look.cache(k, v, *pools, slots, -1, 0, 77, 1))
+    assert got == (k.data_ptr(), v.data_ptr(), keys.codes.data_ptr(), values.codes.data_ptr(), keys.scales.data_ptr(), values.scales.data_ptr(),
+                   slots.data_ptr(), 77, 300, 300, 0, 4, 3, 32, 5, 16)
+    assert look.cache(k, v, *pools, slots, -1, 0, 77, 0) is None            # read back: dense rows on 16 bytes
+    assert look.cache(k[:0], v[:0], *pools, slots[:0], -1, 0, 77, 1) == b""
+    for args in ((k, v, *pools, slots, 0, 0, 77, 1), (k, v, *pools, slots, -1, 1, 77, 1), (k.to("meta"), v, *pools, slots, -1, 0, 77, 1),
+                 (k, v[:3], *pools, slots, -1, 0, 77, 1), (k, v, *pools, slots[1:], -1, 0, 77, 1), (k, None, *pools, slots, -1, 0, 77, 1)):
+        assert look.cache(*args) is None
+    with pytest.raises(TypeError):
+        look.cache(k, v, *pools, slots, -1, 0, "stream", 1)
 
 
 class Library:
