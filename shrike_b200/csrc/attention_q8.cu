@@ -876,6 +876,15 @@ SHRIKE_API int shrike_attention_q8_resident_ctas(int dtype, int group) {
 SHRIKE_API int shrike_attention_q8_row_floats() { return attnq8::D + 2; }
 SHRIKE_API int shrike_attention_q8_max_splits() { return attnq8::MAX_SPLITS; }
 
+// Query rows of a CTA of the form for many.
+SHRIKE_API int shrike_attention_q8_portion_rows() { return attnq8::WARPS * 8 * attnq8::PORTION_NT; }
+// Whether a batch's single tokens should run on the form for many rows too, `ctas` CTAs with theirs over block tables of `keys`
+// keys, instead of a launch of their own after it: while the CTAs find room beside one another, and while the keys, which that
+// form does not split, are few.  Measured, us, two launches and one (float32): 28 heads of 128, 196 CTAs over 250 keys 24.7 and
+// 21.9, 248 CTAs 27.3 and 28.2; 40 heads, 104 CTAs 22.8 and 21.5, 360 CTAs 29.0 and 30.4, over 1,000 keys 85 and 95; 6 heads of 32,
+// a portion of 16 tokens and a single one over 64 keys 7.2 and 4.5, over 1,000 keys 34.5 and 30.6.
+SHRIKE_API int shrike_attention_q8_one_launch(long long ctas, long long keys) { return 2 * ctas <= 3ll * shrike_device().sm_count && keys <= 1024 ? 1 : 0; }
+
 // q and out [tokens, heads * D] of `dtype`, 16-byte aligned; codes [pages, page_size, kv heads, D], 16-byte aligned, scales
 // [pages, kv heads, page_size].  `has_single`: entries of one token (every entry, where has_portions is 0: then `max_q_len`
 // tokens at most) run on the few-rows form with `splits` CTAs a row tile; `has_portions`: the longer ones (all of them where

@@ -944,26 +944,41 @@ static int map_queries(const void* base, long long tokens, int heads, int group,
 // Tokens of a query tile for groups of `group` heads a kv head: what the caller counts the portions' tiles in; 0: not served.
 SHRIKE_API int shrike_attention_q8_tc_tokens(int group) { return group >= 1 && group <= 64 ? 2 * (tcq8::BM / group) : 0; }
 
-// How many CTAs should share the keys of a query tile, for a batch whose portions make `tiles` query tiles over block tables of
-// `keys` keys: the GPU holds one CTA per SM, so the time is that of the rounds of CTAs, each its key tiles and about CTA_START
-// of their time for a CTA's start and end, and a split launch pays COMBINE more for the second kernel.  Measured (40 heads, 512
-// tokens over 8,192 keys, 88 CTAs' worth of query tiles): unsplit 164 us, two splits 170, three 127, four 145, five 131, six
-// 148, eight 159; 12 heads, 475 tokens over 1,115 keys, 24 CTAs' worth: unsplit 28.5, two 22.0, four 18.0, six 17.2.
-SHRIKE_API int shrike_attention_q8_tc_splits(int tiles, int num_kv_heads, long long keys) {
+// The time of a batch whose portions make `tiles` query tiles over block tables of `keys` keys, in a key tile's time, and how
+// many CTAs should share the keys of a query tile for it: the GPU holds one CTA per SM, so the time is that of the rounds of
+// CTAs, each its key tiles and about CTA_START of their time for a CTA's start and end, and a split launch pays COMBINE more for
+// the second kernel.  Measured (40 heads, 512 tokens over 8,192 keys, 88 CTAs' worth of query tiles): unsplit 164 us, two splits
+// 170, three 127, four 145, five 131, six 148, eight 159; 12 heads, 475 tokens over 1,115 keys, 24 CTAs' worth: unsplit 28.5, two
+// 22.0, four 18.0, six 17.2.
+static long long portions_time(int tiles, int num_kv_heads, long long keys, int& splits) {
   constexpr long long CTA_START = 8, COMBINE = 4;
   const long long ctas = static_cast<long long>(num_kv_heads) * tiles, capacity = shrike_device().sm_count;
   const long long key_tiles = (keys + tcq8::KEYS - 1) / tcq8::KEYS;
-  int best = 1;
-  long long best_cost = -1;
+  long long least = -1;
   for (int s = 1; s <= 32 && (s == 1 || key_tiles / s >= 2); ++s) {
     const long long rounds = (ctas * s + capacity - 1) / capacity;
-    const long long cost = rounds * ((key_tiles + s - 1) / s + CTA_START) + (s > 1 ? COMBINE : 0);
-    if (best_cost < 0 || cost < best_cost) {
-      best_cost = cost;
-      best = s;
+    const long long time = rounds * ((key_tiles + s - 1) / s + CTA_START) + (s > 1 ? COMBINE : 0);
+    if (least < 0 || time < least) {
+      least = time;
+      splits = s;
     }
   }
-  return best;
+  return least;
+}
+SHRIKE_API int shrike_attention_q8_tc_splits(int tiles, int num_kv_heads, long long keys) {
+  int splits = 1;
+  portions_time(tiles, num_kv_heads, keys, splits);
+  return splits;
+}
+// Whether a batch's single tokens should be portions too (`all_tiles` query tiles then, `tiles` without them) instead of a launch
+// of their own, which comes after the portions' and takes at least OWN_LAUNCH: a single token then wastes most of its CTA's rows,
+// but the CTA runs beside the others where there are SMs left.  Measured, us, two launches and one: 28 heads, a portion of 64
+// tokens beside 8 single tokens over 250 keys 18.0 and 12.1, over 1,000 keys 23.3 and 18.1; 40 heads, portions of up to 70 tokens
+// beside 30 (288 CTAs) over 150 keys 19.0 and 20.2, one of 64 tokens beside 8 over 1,000 keys 26.4 and 27.4.
+SHRIKE_API int shrike_attention_q8_tc_one_launch(int all_tiles, int tiles, int num_kv_heads, long long keys) {
+  constexpr long long OWN_LAUNCH = 8;
+  int splits;
+  return portions_time(all_tiles, num_kv_heads, keys, splits) <= portions_time(tiles, num_kv_heads, keys, splits) + OWN_LAUNCH ? 1 : 0;
 }
 
 // Portions (q_len > 1) of a batch; entries with q_len == 1 are skipped when skip_single.  `tiles`: the query tiles of
@@ -1031,6 +1046,7 @@ SHRIKE_API int shrike_paged_attention_q8_tc(const ShrikeAttentionQ8* call) {
 
 SHRIKE_API int shrike_attention_q8_tc_tokens(int) { return 0; }
 SHRIKE_API int shrike_attention_q8_tc_splits(int, int, long long) { return 1; }
+SHRIKE_API int shrike_attention_q8_tc_one_launch(int, int, int, long long) { return 0; }
 SHRIKE_API int shrike_paged_attention_q8_tc(const ShrikeAttentionQ8*) { return SHRIKE_BAD_ARGUMENT; }
 
 #endif

@@ -99,9 +99,12 @@ class QuantisedCacheOps:
             lib.shrike_paged_attention_q8.restype = _I
             lib.shrike_attention_q8_tc_tokens.argtypes = [_I]
             lib.shrike_attention_q8_tc_splits.argtypes = [_I, _I, _LL]
-            for name in ("shrike_paged_attention_q8_tc", "shrike_attention_q8_tc_tokens", "shrike_attention_q8_tc_splits"):
+            lib.shrike_attention_q8_tc_one_launch.argtypes = [_I, _I, _I, _LL]
+            lib.shrike_attention_q8_one_launch.argtypes = [_LL, _LL]
+            for name in ("shrike_paged_attention_q8_tc", "shrike_attention_q8_tc_tokens", "shrike_attention_q8_tc_splits",
+                         "shrike_attention_q8_tc_one_launch", "shrike_attention_q8_one_launch"):
                 getattr(lib, name).restype = _I
-            for name in ("row_floats", "max_splits"):
+            for name in ("row_floats", "max_splits", "portion_rows"):
                 getattr(lib, f"shrike_attention_q8_{name}").argtypes = []
                 getattr(lib, f"shrike_attention_q8_{name}").restype = _I
             lib.shrike_attention_q8_resident_ctas.argtypes = [_I, _I]
@@ -242,6 +245,20 @@ class QuantisedCacheOps:
             return held[1]
         lib = self._q8_lib(head_dim)
         has_single, has_portions = min_q_len <= 1, max_q_len > 1
+        # Up to 64 keys the mma.sync kernel is done before the other has set up (us, 28 heads of 128, mma.sync and tcgen05: one
+        # portion of 16 tokens 5.6 and 7.4, of 64 7.3 and 9.1, four of 64 7.8 and 9.2; one of 5 tokens over 100 keys 8.9 and 8.3,
+        # of 256 over 256 17.1 and 13.8, of 16 over 600 27.9 and 12.5).
+        tile_tokens, table_keys = lib.shrike_attention_q8_tc_tokens(num_heads // num_kv_heads), max_blocks * page_size
+        tc_portions = bool(has_portions and tile_tokens and self.tensor_core_attention and self.dtype == torch.bfloat16
+                           and page_size in (8, 16, 32, 64) and num_tokens > 0 and not short and table_keys > self.SHORT_CONTEXT)
+        if has_single and has_portions and q_lens is not None:   # single tokens as portions, one launch for all
+            if tc_portions:
+                tiles = sum(-(-q // tile_tokens) for q in q_lens)
+                has_single = not lib.shrike_attention_q8_tc_one_launch(tiles, sum(-(-q // tile_tokens) for q in q_lens if q > 1), num_kv_heads, table_keys)
+            else:
+                group, cta_rows = num_heads // num_kv_heads, lib.shrike_attention_q8_portion_rows()
+                ctas = num_kv_heads * sum(-(-q * group // cta_rows) for q in q_lens)
+                has_single = not lib.shrike_attention_q8_one_launch(ctas, table_keys)
         splits, cluster, scratch, arrivals = 1, 1, None, None
         if has_single:
             group = num_heads // num_kv_heads
@@ -266,19 +283,13 @@ class QuantisedCacheOps:
                     self._q8_arrivals = torch.zeros(max(pairs, 4096), dtype=torch.int32, device=self.device)
                     self.generation += 1
                 scratch, arrivals = self._q8_scratch, self._q8_arrivals
-        tc_portions, tiles, portion_splits, portion_scratch = False, 0, 1, None
-        rows = lib.shrike_attention_q8_tc_tokens(num_heads // num_kv_heads)
-        # Up to 64 keys the mma.sync kernel is done before the other has set up (us, 28 heads of 128, mma.sync and tcgen05: one
-        # portion of 16 tokens 5.6 and 7.4, of 64 7.3 and 9.1, four of 64 7.8 and 9.2; one of 5 tokens over 100 keys 8.9 and 8.3,
-        # of 256 over 256 17.1 and 13.8, of 16 over 600 27.9 and 12.5).
-        if (has_portions and rows and self.tensor_core_attention and self.dtype == torch.bfloat16 and page_size in (8, 16, 32, 64)
-                and num_tokens > 0 and not short and max_blocks * page_size > self.SHORT_CONTEXT):
-            tc_portions = True
+        tiles, portion_splits, portion_scratch = 0, 1, None
+        if tc_portions:
             if q_lens is not None:
-                tiles = sum(-(-q // rows) for q in q_lens if q > 1 or not has_single)
+                tiles = sum(-(-q // tile_tokens) for q in q_lens if q > 1 or not has_single)
             else:   # lengths that are not known: what the tokens can make at most
-                tiles = num_tokens // rows + num_seqs
-            portion_splits = self.portion_splits or lib.shrike_attention_q8_tc_splits(tiles, num_kv_heads, max_blocks * page_size)
+                tiles = num_tokens // tile_tokens + num_seqs
+            portion_splits = self.portion_splits or lib.shrike_attention_q8_tc_splits(tiles, num_kv_heads, table_keys)
             each = num_tokens * num_heads * (head_dim + 2)
             portion_splits = max(1, min(portion_splits, 32, self.PORTION_SCRATCH_FLOATS // each)) if num_tokens <= 8 * 65535 else 1
             if portion_splits > 1:

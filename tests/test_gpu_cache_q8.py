@@ -200,6 +200,20 @@ def test_portions_beside_single_tokens(dtype, dim, known, options):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,kv_heads,dim", [(6, 3, 32), (14, 2, 64), (7, 1, 128)])
+@pytest.mark.parametrize("options", [{}, {"window": 70}, {"chunk": 48}])
+@pytest.mark.parametrize("q_lens,ctx_lens,one", [([1, 20, 1, 50, 0, 1], [300, 90, 1, 70, 9, 33], True), ([30, 1], [31, 500], True),
+                                                 ([9] + [1] * 400, [60] + [70] * 400, False)])
+def test_single_tokens_in_the_portions_launch_or_in_their_own(dtype, heads, kv_heads, dim, options, q_lens, ctx_lens, one):
+    """Few single tokens run beside the portions in one launch, many after them in their own."""
+    ops = cuda_ops(dtype)
+    ops.q8_splits, ops.tensor_core_attention, ops.portion_splits = None, True, 0
+    plan = ops.q8_plan(heads, kv_heads, dim, len(q_lens), -(-max(ctx_lens) // 16) + 2, 16, max(q_lens), 1, 0, sum(q_lens), q_lens, max(ctx_lens))
+    assert plan.has_portions and plan.has_single != one
+    check_attention(dtype, heads, kv_heads, dim, 16, q_lens, ctx_lens, seed=6, **options)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_large_scores(dtype):
     """Scores of some hundreds: one key takes all the weight."""
     check_attention(dtype, 4, 2, 64, 16, [1, 20, 1], [300, 90, 5], q_scale=60.0)
