@@ -823,6 +823,17 @@ static int resident() {
   return per_sm * shrike_device().sm_count;
 }
 
+template <typename T>
+static int resident_many() {
+  static PerDevice raised;
+  if (shrike_raise_smem(raised, portion_rows_kernel<T, PORTION_NT>, portion_rows_smem<T, PORTION_NT>()) != 0) return shrike_device().sm_count;
+  int per_sm = 0;
+  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, portion_rows_kernel<T, PORTION_NT>, THREADS, portion_rows_smem<T, PORTION_NT>()) != cudaSuccess ||
+      per_sm < 1)
+    per_sm = 1;
+  return per_sm * shrike_device().sm_count;
+}
+
 template <typename T, int NT>
 static int launch_few(const Args& args, int num_seqs, int tokens, cudaStream_t stream) {
   static PerDevice raised;
@@ -880,10 +891,17 @@ SHRIKE_API int shrike_attention_q8_max_splits() { return attnq8::MAX_SPLITS; }
 SHRIKE_API int shrike_attention_q8_portion_rows() { return attnq8::WARPS * 8 * attnq8::PORTION_NT; }
 // Whether a batch's single tokens should run on the form for many rows too, `ctas` CTAs with theirs over block tables of `keys`
 // keys, instead of a launch of their own after it: while the CTAs find room beside one another, and while the keys, which that
-// form does not split, are few.  Measured, us, two launches and one (float32): 28 heads of 128, 196 CTAs over 250 keys 24.7 and
-// 21.9, 248 CTAs 27.3 and 28.2; 40 heads, 104 CTAs 22.8 and 21.5, 360 CTAs 29.0 and 30.4, over 1,000 keys 85 and 95; 6 heads of 32,
-// a portion of 16 tokens and a single one over 64 keys 7.2 and 4.5, over 1,000 keys 34.5 and 30.6.
-SHRIKE_API int shrike_attention_q8_one_launch(long long ctas, long long keys) { return 2 * ctas <= 3ll * shrike_device().sm_count && keys <= 1024 ? 1 : 0; }
+// form does not split, are few or not many more than the `longest` portion's CTAs walk in any case (a single token of many keys
+// beside a short portion would be walked for long by one CTA: 53 us for 1,000 keys, 28 heads of 128 in float32, which its own
+// launch takes 12 for).  Measured, us, two launches and one (float32): 28
+// heads of 128, 196 CTAs over 250 keys 24.7 and 21.9, 248 CTAs 27.3 and 28.2 (296 find room); 40 heads, 104 CTAs 22.8 and 21.5, 360
+// CTAs 29.0 and 30.4; 6 heads of 32, a portion of 16 tokens and a single one over 64 keys 7.2 and 4.5, over 250 keys 13.3 and 9.7, one of 475 tokens and 20 single
+// ones over 483 keys 25.0 and 20.3.
+SHRIKE_API int shrike_attention_q8_one_launch(int dtype, long long ctas, long long keys, long long longest) {
+  using namespace attnq8;
+  if (keys > 256 && 2 * keys > 3 * longest) return 0;
+  return 4 * ctas <= 3ll * (dtype == SHRIKE_F32 ? resident_many<float>() : resident_many<__nv_bfloat16>()) ? 1 : 0;
+}
 
 // q and out [tokens, heads * D] of `dtype`, 16-byte aligned; codes [pages, page_size, kv heads, D], 16-byte aligned, scales
 // [pages, kv heads, page_size].  `has_single`: entries of one token (every entry, where has_portions is 0: then `max_q_len`

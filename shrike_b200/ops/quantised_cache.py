@@ -100,7 +100,7 @@ class QuantisedCacheOps:
             lib.shrike_attention_q8_tc_tokens.argtypes = [_I]
             lib.shrike_attention_q8_tc_splits.argtypes = [_I, _I, _LL]
             lib.shrike_attention_q8_tc_one_launch.argtypes = [_I, _I, _I, _LL]
-            lib.shrike_attention_q8_one_launch.argtypes = [_LL, _LL]
+            lib.shrike_attention_q8_one_launch.argtypes = [_I, _LL, _LL, _LL]
             for name in ("shrike_paged_attention_q8_tc", "shrike_attention_q8_tc_tokens", "shrike_attention_q8_tc_splits",
                          "shrike_attention_q8_tc_one_launch", "shrike_attention_q8_one_launch"):
                 getattr(lib, name).restype = _I
@@ -258,7 +258,7 @@ class QuantisedCacheOps:
             else:
                 group, cta_rows = num_heads // num_kv_heads, lib.shrike_attention_q8_portion_rows()
                 ctas = num_kv_heads * sum(-(-q * group // cta_rows) for q in q_lens)
-                has_single = not lib.shrike_attention_q8_one_launch(ctas, table_keys)
+                has_single = not lib.shrike_attention_q8_one_launch(self.code, ctas, table_keys, max_q_len)
         splits, cluster, scratch, arrivals = 1, 1, None, None
         if has_single:
             group = num_heads // num_kv_heads

@@ -202,8 +202,8 @@ def test_portions_beside_single_tokens(dtype, dim, known, options):
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("heads,kv_heads,dim", [(6, 3, 32), (14, 2, 64), (7, 1, 128)])
 @pytest.mark.parametrize("options", [{}, {"window": 70}, {"chunk": 48}])
-@pytest.mark.parametrize("q_lens,ctx_lens,one", [([1, 20, 1, 50, 0, 1], [300, 90, 1, 70, 9, 33], True), ([30, 1], [31, 500], True),
-                                                 ([9] + [1] * 400, [60] + [70] * 400, False)])
+@pytest.mark.parametrize("q_lens,ctx_lens,one", [([1, 20, 1, 50, 0, 1], [190, 90, 1, 70, 9, 33], True), ([30, 1], [31, 200], True),
+                                                 ([9] + [1] * 200, [60] + [70] * 199 + [300], False)])
 def test_single_tokens_in_the_portions_launch_or_in_their_own(dtype, heads, kv_heads, dim, options, q_lens, ctx_lens, one):
     """Few single tokens run beside the portions in one launch, many after them in their own."""
     ops = cuda_ops(dtype)
