@@ -978,6 +978,7 @@ SHRIKE_API int shrike_attention_q8_tc_splits(int tiles, int num_kv_heads, long l
 SHRIKE_API int shrike_attention_q8_tc_one_launch(int all_tiles, int tiles, int num_kv_heads, long long keys) {
   constexpr long long OWN_LAUNCH = 8;
   int splits;
+  if (all_tiles > 65535) return 0;   // more than a launch takes
   return portions_time(all_tiles, num_kv_heads, keys, splits) <= portions_time(tiles, num_kv_heads, keys, splits) + OWN_LAUNCH ? 1 : 0;
 }
 
