@@ -889,6 +889,10 @@ SHRIKE_API int shrike_attention_q8_max_splits() { return attnq8::MAX_SPLITS; }
 
 // Query rows of a CTA of the form for many.
 SHRIKE_API int shrike_attention_q8_portion_rows() { return attnq8::WARPS * 8 * attnq8::PORTION_NT; }
+// CTAs of that form that the device holds at once, for queries of `dtype`.
+SHRIKE_API int shrike_attention_q8_resident_portions(int dtype) {
+  return dtype == SHRIKE_F32 ? attnq8::resident_many<float>() : attnq8::resident_many<__nv_bfloat16>();
+}
 // Whether a batch's single tokens should run on the form for many rows too, `ctas` CTAs with theirs over block tables of `keys`
 // keys, instead of a launch of their own after it: while the CTAs find room beside one another, and while the keys, which that
 // form does not split, are few or not many more than the `longest` portion's CTAs walk in any case (a single token of many keys
@@ -898,9 +902,8 @@ SHRIKE_API int shrike_attention_q8_portion_rows() { return attnq8::WARPS * 8 * a
 // CTAs 29.0 and 30.4; 6 heads of 32, a portion of 16 tokens and a single one over 64 keys 7.2 and 4.5, over 250 keys 13.3 and 9.7, one of 475 tokens and 20 single
 // ones over 483 keys 25.0 and 20.3.
 SHRIKE_API int shrike_attention_q8_one_launch(int dtype, long long ctas, long long keys, long long longest) {
-  using namespace attnq8;
   if (keys > 256 && 2 * keys > 3 * longest) return 0;
-  return 4 * ctas <= 3ll * (dtype == SHRIKE_F32 ? resident_many<float>() : resident_many<__nv_bfloat16>()) ? 1 : 0;
+  return 4 * ctas <= 3ll * shrike_attention_q8_resident_portions(dtype) ? 1 : 0;
 }
 
 // q and out [tokens, heads * D] of `dtype`, 16-byte aligned; codes [pages, page_size, kv heads, D], 16-byte aligned, scales

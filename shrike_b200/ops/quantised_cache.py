@@ -104,6 +104,7 @@ class QuantisedCacheOps:
             for name in ("shrike_paged_attention_q8_tc", "shrike_attention_q8_tc_tokens", "shrike_attention_q8_tc_splits",
                          "shrike_attention_q8_tc_one_launch", "shrike_attention_q8_one_launch"):
                 getattr(lib, name).restype = _I
+            lib.shrike_attention_q8_resident_portions.argtypes, lib.shrike_attention_q8_resident_portions.restype = [_I], _I
             for name in ("row_floats", "max_splits", "portion_rows"):
                 getattr(lib, f"shrike_attention_q8_{name}").argtypes = []
                 getattr(lib, f"shrike_attention_q8_{name}").restype = _I
@@ -260,15 +261,13 @@ class QuantisedCacheOps:
                 ctas = num_kv_heads * sum(-(-q * group // cta_rows) for q in q_lens)
                 has_single = not lib.shrike_attention_q8_one_launch(self.code, ctas, table_keys, max_q_len)
         splits, cluster, scratch, arrivals = 1, 1, None, None
+        group, few_tokens = num_heads // num_kv_heads, 1
+        rows = lib.shrike_attention_q8_tile_rows(group)
+        if has_portions and not tc_portions and self._few_rows_serve(lib, num_heads, num_kv_heads, table_keys, window, num_seqs, max_q_len, q_lens):
+            has_single, has_portions, few_tokens = True, False, max_q_len
         if has_single:
-            group = num_heads // num_kv_heads
-            rows = lib.shrike_attention_q8_tile_rows(group)
-            pairs = num_seqs * num_kv_heads * -(-group // rows)
-            keys = max_blocks * page_size
-            if window > 0:
-                keys = min(keys, window)
-            elif window < 0:
-                keys = min(keys, -window)
+            pairs = num_seqs * num_kv_heads * -(-group * few_tokens // rows)
+            keys = table_keys if not window else min(table_keys, abs(window) + few_tokens - 1)
             most = lib.shrike_attention_q8_max_splits()
             splits, cluster = self.q8_splits or self.q8_few_row_splits(keys, pairs, lib.shrike_attention_q8_resident_ctas(self.code, group))
             share = rows * lib.shrike_attention_q8_row_floats() * pairs
@@ -305,13 +304,45 @@ class QuantisedCacheOps:
         self._q8_plans[key] = (self.generation, plan)
         return plan
 
+    # A key of the form for many rows, which all four warps of a CTA walk with 16 rows each, in keys of the other, which they
+    # share with 8 rows each.
+    Q8_MANY_ROWS_KEY = 5.6
+    Q8_EMPTY_KEYS = 90   # an empty CTA's time, in keys
+
+    def _few_rows_serve(self, lib, num_heads, num_kv_heads, table_keys, window, num_seqs, max_q_len, q_lens) -> bool:
+        """Whether the form for few rows, which splits the keys, serves a batch with portions sooner than the form for many, which
+        walks them once for 64 rows.  Its grid has a place for the longest entry's row tiles in every entry: the empty ones' CTAs
+        take some time too.  Measured, us, many and few rows (float32, 28 heads of 128): 2 tokens over 40 keys 7.0 and 4.7, over 8,000
+        375 and 14; 128 over 136 12.8 and 12.0; 400 over 408 31.5 and 36.5; 3 portions of up to 64 beside 9 single tokens over 72 keys
+        10.5 and 15.6, over 500 46 and 26."""
+        group = num_heads // num_kv_heads
+        rows, many_rows = lib.shrike_attention_q8_tile_rows(group), lib.shrike_attention_q8_portion_rows()
+        grid = num_kv_heads * -(-max_q_len * group // rows)
+        if grid > 65535 or grid * num_seqs > 1 << 20:
+            return False
+        lens = q_lens if q_lens is not None else [max_q_len] * num_seqs
+        keys = table_keys if not window else min(table_keys, abs(window) + max_q_len - 1)
+        pairs = num_kv_heads * sum(-(-q * group // rows) for q in lens)
+        ctas = num_kv_heads * sum(-(-q * group // many_rows) for q in lens)
+        resident = lib.shrike_attention_q8_resident_ctas(self.code, group)
+        few, splits = self.q8_few_row_time(keys, pairs, resident)
+        few += self.Q8_EMPTY_KEYS * splits * (grid * num_seqs - pairs) / resident
+        many = max(1.0, ctas / lib.shrike_attention_q8_resident_portions(self.code)) * (keys * self.Q8_MANY_ROWS_KEY + self.Q8_START_KEYS)
+        return few < many
+
     # What a CTA costs beside its keys, in keys: its start alone, with its share's way through a cluster's shared memory, and
     # with the clusters' way through global memory.
     Q8_START_KEYS, Q8_CLUSTER_KEYS, Q8_GLOBAL_KEYS = 160, 320, 640
 
     @classmethod
     def q8_few_row_splits(cls, keys: int, pairs: int, resident: int):
-        """(splits, cluster): CTAs that share the `keys` of each of `pairs` (entry, kv head, row tile) where the device holds
+        """(splits, cluster) of `q8_few_row_time`."""
+        best = cls.q8_few_row_time(keys, pairs, resident)[1]
+        return best, min(best, 8)
+
+    @classmethod
+    def q8_few_row_time(cls, keys: int, pairs: int, resident: int):
+        """(time in keys, splits): CTAs that share the `keys` of each of `pairs` (entry, kv head, row tile) where the device holds
         `resident` at once, and how many of them form a cluster (all up to eight: a cluster adds up in shared memory, 2 us
         sooner than through global memory).  The count with the least time: no less than a CTA's own, and about that of all
         CTAs' work, whose contexts are of uneven lengths (three quarters of the longest, say), with half a CTA's at the end.
@@ -326,7 +357,7 @@ class QuantisedCacheOps:
             time = max(each, 0.75 * pairs * splits * each / resident + 0.5 * each)
             if least is None or time < least:
                 best, least = splits, time
-        return best, min(best, 8)
+        return least, best
 
     def _paged_attention_q8(self, q, keys, values, block_table, q_start, ctx_len, seq_of_token, num_heads, num_kv_heads, head_dim,
                             scale, window, out, max_q_len, min_q_len, q_lens, max_ctx_len):

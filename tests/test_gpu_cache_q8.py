@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from shrike_b200.cache.quantised import QuantisedPages
+from shrike_b200.ops.cuda_ops import CudaOps
 from tests import cache_q8_oracle as oracle
 from tests.gpu_common import cuda_ops
 
@@ -140,8 +141,10 @@ def attend(ops, case, heads, kv_heads, dim, q_lens, ctx_lens, window=None, chunk
 
 
 def check_attention(dtype, heads, kv_heads, dim, page, q_lens, ctx_lens, seed=0, q_scale=1.0, splits=None, known=True, tensor_cores=True,
-                    portion_splits=0, **options):
+                    portion_splits=0, many_rows_key=CudaOps.Q8_MANY_ROWS_KEY, **options):
     ops = cuda_ops(dtype)
+    ops.Q8_MANY_ROWS_KEY = many_rows_key   # of the rule between the forms for few rows and for many
+    ops._q8_plans.clear()
     ops.q8_splits, ops.tensor_core_attention, ops.portion_splits = splits, tensor_cores, portion_splits
     case = oracle.pages_case(heads, kv_heads, dim, page, q_lens, ctx_lens, dtype, seed, DEV, q_scale)
     got = attend(ops, case, heads, kv_heads, dim, q_lens, ctx_lens, known=known, **options)
@@ -182,6 +185,15 @@ def test_portions(dtype, heads, kv_heads, dim, page, options):
     check_attention(dtype, heads, kv_heads, dim, page, q_lens, ctx_lens, seed=dim, tensor_cores=False, **options)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,kv_heads,dim,page", HEADS)
+@pytest.mark.parametrize("options", [{}, {"window": 40}, {"chunk": 48}])
+@pytest.mark.parametrize("many_rows_key,splits", [(0.0, None), (1e9, None), (1e9, (8, 4))])
+def test_portions_as_many_rows_and_as_few(dtype, heads, kv_heads, dim, page, options, many_rows_key, splits):
+    check_attention(dtype, heads, kv_heads, dim, page, [40, 1, 0, 9, 2], [170, 60, 5, 9, 300], seed=8, tensor_cores=False,
+                    many_rows_key=many_rows_key, splits=splits, **options)
+
+
 @pytest.mark.parametrize("heads,kv_heads,dim,page", [(7, 1, 128, 16), (14, 2, 64, 8), (40, 8, 128, 64), (2, 2, 64, 32), (64, 1, 128, 16), (25, 1, 64, 16)])
 @pytest.mark.parametrize("splits", [1, 2, 5])
 @pytest.mark.parametrize("options", [{}, {"window": 40}, {"window": 300}, {"chunk": 48}])
@@ -209,7 +221,7 @@ def test_single_tokens_in_the_portions_launch_or_in_their_own(dtype, heads, kv_h
     ops = cuda_ops(dtype)
     ops.q8_splits, ops.tensor_core_attention, ops.portion_splits = None, True, 0
     plan = ops.q8_plan(heads, kv_heads, dim, len(q_lens), -(-max(ctx_lens) // 16) + 2, 16, max(q_lens), 1, 0, sum(q_lens), q_lens, max(ctx_lens))
-    assert plan.has_portions and plan.has_single != one
+    assert (not one and not plan.tc_portions) or plan.has_single + plan.has_portions == (1 if one else 2)
     check_attention(dtype, heads, kv_heads, dim, 16, q_lens, ctx_lens, seed=6, **options)
 
 

@@ -195,7 +195,8 @@ class Library:
         def launcher(*args):
             self.calls.append(name)
             return {"shrike_attention_q8_tile_rows": 8, "shrike_attention_q8_resident_ctas": 592, "shrike_attention_q8_row_floats": 66,
-                    "shrike_attention_q8_max_splits": 64, "shrike_attention_q8_tc_tokens": 32, "shrike_attention_q8_tc_splits": 3, "shrike_attention_q8_portion_rows": 64}.get(name, 0)
+                    "shrike_attention_q8_max_splits": 64, "shrike_attention_q8_tc_tokens": 32, "shrike_attention_q8_tc_splits": 3, "shrike_attention_q8_portion_rows": 64,
+                    "shrike_attention_q8_resident_portions": 444}.get(name, 0)
         return launcher
 
 
