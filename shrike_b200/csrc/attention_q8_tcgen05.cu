@@ -32,6 +32,8 @@
 // Built once per head size; serves head sizes 64 and 128, page sizes 8, 16, 32, 64, and groups of up to 64 heads.
 #include <cuda_fp16.h>
 
+#include <algorithm>
+
 #include "attention_q8.cuh"
 #include "blackwell.cuh"
 
@@ -965,6 +967,10 @@ static long long portions_time(int tiles, int num_kv_heads, long long keys, int&
   }
   return least;
 }
+SHRIKE_API int shrike_attention_q8_tc_time(int tiles, int num_kv_heads, long long keys) {
+  int splits;
+  return static_cast<int>(std::min(portions_time(tiles, num_kv_heads, keys, splits), 0x7fffffffll));
+}
 SHRIKE_API int shrike_attention_q8_tc_splits(int tiles, int num_kv_heads, long long keys) {
   int splits = 1;
   portions_time(tiles, num_kv_heads, keys, splits);
@@ -1046,6 +1052,7 @@ SHRIKE_API int shrike_paged_attention_q8_tc(const ShrikeAttentionQ8* call) {
 #else  // other head sizes: the mma.sync kernel serves them
 
 SHRIKE_API int shrike_attention_q8_tc_tokens(int) { return 0; }
+SHRIKE_API int shrike_attention_q8_tc_time(int, int, long long) { return 0; }
 SHRIKE_API int shrike_attention_q8_tc_splits(int, int, long long) { return 1; }
 SHRIKE_API int shrike_attention_q8_tc_one_launch(int, int, int, long long) { return 0; }
 SHRIKE_API int shrike_paged_attention_q8_tc(const ShrikeAttentionQ8*) { return SHRIKE_BAD_ARGUMENT; }

@@ -87,6 +87,7 @@ class QuantisedCacheOps:
             getattr(lib, name).restype = _I
         self._q8_libs, self._q8_plans = {}, {}
         self._q8_scratch = self._q8_arrivals = self._q8_portion_scratch = None
+        self.q8_few_rows = None   # None: the rule of `_few_rows_serve`; whether the form for few rows takes portions (tests)
         self.q8_splits = None   # None: the rule of `q8_few_row_splits`; (splits, cluster) for few rows (tests)
 
     def _q8_lib(self, head_dim: int):
@@ -100,6 +101,7 @@ class QuantisedCacheOps:
             lib.shrike_attention_q8_tc_tokens.argtypes = [_I]
             lib.shrike_attention_q8_tc_splits.argtypes = [_I, _I, _LL]
             lib.shrike_attention_q8_tc_one_launch.argtypes = [_I, _I, _I, _LL]
+            lib.shrike_attention_q8_tc_time.argtypes, lib.shrike_attention_q8_tc_time.restype = [_I, _I, _LL], _I
             lib.shrike_attention_q8_one_launch.argtypes = [_I, _LL, _LL, _LL]
             for name in ("shrike_paged_attention_q8_tc", "shrike_attention_q8_tc_tokens", "shrike_attention_q8_tc_splits",
                          "shrike_attention_q8_tc_one_launch", "shrike_attention_q8_one_launch"):
@@ -240,7 +242,7 @@ class QuantisedCacheOps:
         short = 0 < max_ctx_len <= self.SHORT_CONTEXT
         shape = (num_tokens, short, tuple(q_lens) if q_lens is not None else None) if max_q_len > 1 else None
         key = (num_heads, num_kv_heads, head_dim, num_seqs, max_blocks, page_size, min_q_len <= 1, window, shape, self.q8_splits,
-               self.tensor_core_attention, self.portion_splits)
+               self.tensor_core_attention, self.portion_splits, self.q8_few_rows)
         held = self._q8_plans.get(key)
         if held is not None and held[0] == self.generation:   # the scratch has not moved since
             return held[1]
@@ -263,8 +265,9 @@ class QuantisedCacheOps:
         splits, cluster, scratch, arrivals = 1, 1, None, None
         group, few_tokens = num_heads // num_kv_heads, 1
         rows = lib.shrike_attention_q8_tile_rows(group)
-        if has_portions and not tc_portions and self._few_rows_serve(lib, num_heads, num_kv_heads, table_keys, window, num_seqs, max_q_len, q_lens):
-            has_single, has_portions, few_tokens = True, False, max_q_len
+        if has_portions and self._few_rows_serve(lib, num_heads, num_kv_heads, table_keys, window, num_seqs, num_tokens, max_q_len, q_lens,
+                                                 tile_tokens if tc_portions else 0, has_single):
+            has_single, has_portions, tc_portions, few_tokens = True, False, False, max_q_len
         if has_single:
             pairs = num_seqs * num_kv_heads * -(-group * few_tokens // rows)
             keys = table_keys if not window else min(table_keys, abs(window) + few_tokens - 1)
@@ -304,31 +307,40 @@ class QuantisedCacheOps:
         self._q8_plans[key] = (self.generation, plan)
         return plan
 
-    # A key of the form for many rows, which all four warps of a CTA walk with 16 rows each, in keys of the other, which they
-    # share with 8 rows each.
-    Q8_MANY_ROWS_KEY = 5.6
-    Q8_EMPTY_KEYS = 90   # an empty CTA's time, in keys
+    # In keys of the form for few rows, which a CTA's four warps share with 8 rows each: a key of the mma.sync form for many, which
+    # all of them walk with 16 rows each; the tcgen05 kernel's unit of time, and a launch of the single tokens' own after it; a CTA
+    # that finds nothing to do.
+    Q8_MANY_ROWS_KEY, Q8_TC_UNIT, Q8_OWN_LAUNCH, Q8_EMPTY_KEYS = 5.6, 50, 400, 90
 
-    def _few_rows_serve(self, lib, num_heads, num_kv_heads, table_keys, window, num_seqs, max_q_len, q_lens) -> bool:
-        """Whether the form for few rows, which splits the keys, serves a batch with portions sooner than the form for many, which
-        walks them once for 64 rows.  Its grid has a place for the longest entry's row tiles in every entry: the empty ones' CTAs
-        take some time too.  Measured, us, many and few rows (float32, 28 heads of 128): 2 tokens over 40 keys 7.0 and 4.7, over 8,000
-        375 and 14; 128 over 136 12.8 and 12.0; 400 over 408 31.5 and 36.5; 3 portions of up to 64 beside 9 single tokens over 72 keys
-        10.5 and 15.6, over 500 46 and 26."""
+    def _few_rows_serve(self, lib, num_heads, num_kv_heads, table_keys, window, num_seqs, num_tokens, max_q_len, q_lens, tile_tokens,
+                        own_launch) -> bool:
+        """Whether the form for few rows, which splits the keys, serves a batch with portions sooner than the tcgen05 kernel (query
+        tiles of `tile_tokens` tokens) or, where that does not serve (0), the mma.sync form for many rows, which walks the keys
+        once for 64 rows.  The grid has a place for the longest entry's row tiles in every entry: the empty ones' CTAs take some
+        time too.
+        Measured, us, tcgen05 and few rows (28 heads of 128): 2 tokens over 100 keys 7.9 and 4.6, over 16,000 19.8 and 18.0; 5 over
+        16,000 20.0 and 28.9; 16 over 1,000 11.2 and 10.2, over 4,000 14.5 and 18.5; 48 over 300 14.2 and 8.5, over 1,000 13.7 and
+        18.1; 8 portions of 4 tokens over 4,000 32.5 and 17.7.  mma.sync and few rows (float32, 28 heads of 128): 2 tokens over 40
+        keys 7.0 and 4.7, over 8,000 375 and 14; 128 over 136 12.8 and 12.0; 400 over 408 31.5 and 36.5; 3 portions of up to 64
+        beside 9 single tokens over 72 keys 10.5 and 15.6, over 500 46 and 26."""
         group = num_heads // num_kv_heads
-        rows, many_rows = lib.shrike_attention_q8_tile_rows(group), lib.shrike_attention_q8_portion_rows()
+        rows = lib.shrike_attention_q8_tile_rows(group)
         grid = num_kv_heads * -(-max_q_len * group // rows)
-        if grid > 65535 or grid * num_seqs > 1 << 20:
+        if grid > 65535 or grid * num_seqs > 1 << 20 or num_seqs > 65535:
             return False
+        if self.q8_few_rows is not None:
+            return self.q8_few_rows
         lens = q_lens if q_lens is not None else [max_q_len] * num_seqs
         keys = table_keys if not window else min(table_keys, abs(window) + max_q_len - 1)
         pairs = num_kv_heads * sum(-(-q * group // rows) for q in lens)
-        ctas = num_kv_heads * sum(-(-q * group // many_rows) for q in lens)
         resident = lib.shrike_attention_q8_resident_ctas(self.code, group)
         few, splits = self.q8_few_row_time(keys, pairs, resident)
         few += self.Q8_EMPTY_KEYS * splits * (grid * num_seqs - pairs) / resident
-        many = max(1.0, ctas / lib.shrike_attention_q8_resident_portions(self.code)) * (keys * self.Q8_MANY_ROWS_KEY + self.Q8_START_KEYS)
-        return few < many
+        if tile_tokens:
+            tiles = num_tokens // tile_tokens + num_seqs if q_lens is None else sum(-(-q // tile_tokens) for q in q_lens if q > 1 or not own_launch)
+            return few < lib.shrike_attention_q8_tc_time(tiles, num_kv_heads, keys) * self.Q8_TC_UNIT + (self.Q8_OWN_LAUNCH if own_launch else 0)
+        ctas = num_kv_heads * sum(-(-q * group // lib.shrike_attention_q8_portion_rows()) for q in lens)
+        return few < max(1.0, ctas / lib.shrike_attention_q8_resident_portions(self.code)) * (keys * self.Q8_MANY_ROWS_KEY + self.Q8_START_KEYS)
 
     # What a CTA costs beside its keys, in keys: its start alone, with its share's way through a cluster's shared memory, and
     # with the clusters' way through global memory.

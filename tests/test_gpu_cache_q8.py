@@ -6,7 +6,6 @@ import pytest
 import torch
 
 from shrike_b200.cache.quantised import QuantisedPages
-from shrike_b200.ops.cuda_ops import CudaOps
 from tests import cache_q8_oracle as oracle
 from tests.gpu_common import cuda_ops
 
@@ -141,10 +140,9 @@ def attend(ops, case, heads, kv_heads, dim, q_lens, ctx_lens, window=None, chunk
 
 
 def check_attention(dtype, heads, kv_heads, dim, page, q_lens, ctx_lens, seed=0, q_scale=1.0, splits=None, known=True, tensor_cores=True,
-                    portion_splits=0, many_rows_key=CudaOps.Q8_MANY_ROWS_KEY, **options):
+                    portion_splits=0, few_rows=False, **options):
     ops = cuda_ops(dtype)
-    ops.Q8_MANY_ROWS_KEY = many_rows_key   # of the rule between the forms for few rows and for many
-    ops._q8_plans.clear()
+    ops.q8_few_rows = few_rows
     ops.q8_splits, ops.tensor_core_attention, ops.portion_splits = splits, tensor_cores, portion_splits
     case = oracle.pages_case(heads, kv_heads, dim, page, q_lens, ctx_lens, dtype, seed, DEV, q_scale)
     got = attend(ops, case, heads, kv_heads, dim, q_lens, ctx_lens, known=known, **options)
@@ -188,10 +186,19 @@ def test_portions(dtype, heads, kv_heads, dim, page, options):
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("heads,kv_heads,dim,page", HEADS)
 @pytest.mark.parametrize("options", [{}, {"window": 40}, {"chunk": 48}])
-@pytest.mark.parametrize("many_rows_key,splits", [(0.0, None), (1e9, None), (1e9, (8, 4))])
-def test_portions_as_many_rows_and_as_few(dtype, heads, kv_heads, dim, page, options, many_rows_key, splits):
-    check_attention(dtype, heads, kv_heads, dim, page, [40, 1, 0, 9, 2], [170, 60, 5, 9, 300], seed=8, tensor_cores=False,
-                    many_rows_key=many_rows_key, splits=splits, **options)
+@pytest.mark.parametrize("few_rows,splits", [(True, None), (True, (8, 4)), (None, None)])
+def test_portions_as_few_rows_and_as_the_rule_has_them(dtype, heads, kv_heads, dim, page, options, few_rows, splits):
+    check_attention(dtype, heads, kv_heads, dim, page, [40, 1, 0, 9, 2], [170, 60, 5, 9, 300], seed=8, few_rows=few_rows, splits=splits, **options)
+
+
+def test_which_form_the_rule_takes():
+    """Few tokens over any keys, and more over few: the form that splits keys for few rows; else tcgen05, or mma.sync."""
+    for dtype, dim, many in ((torch.bfloat16, 128, "tcgen05"), (torch.float32, 128, "mma")):
+        ops = cuda_ops(dtype)
+        ops.q8_splits, ops.tensor_core_attention, ops.portion_splits, ops.q8_few_rows = None, True, 0, None
+        for tokens, keys, few in ((2, 160, True), (4, 1008, True), (48, 320, True), (2000, 2000, False)):
+            plan = ops.q8_plan(28, 4, dim, 1, keys // 16, 16, tokens, tokens, 0, tokens, [tokens], keys)
+            assert plan.has_single == few and plan.tc_portions == (not few and many == "tcgen05")
 
 
 @pytest.mark.parametrize("heads,kv_heads,dim,page", [(7, 1, 128, 16), (14, 2, 64, 8), (40, 8, 128, 64), (2, 2, 64, 32), (64, 1, 128, 16), (25, 1, 64, 16)])
@@ -219,7 +226,7 @@ def test_portions_beside_single_tokens(dtype, dim, known, options):
 def test_single_tokens_in_the_portions_launch_or_in_their_own(dtype, heads, kv_heads, dim, options, q_lens, ctx_lens, one):
     """Few single tokens run beside the portions in one launch, many after them in their own."""
     ops = cuda_ops(dtype)
-    ops.q8_splits, ops.tensor_core_attention, ops.portion_splits = None, True, 0
+    ops.q8_splits, ops.tensor_core_attention, ops.portion_splits, ops.q8_few_rows = None, True, 0, False
     plan = ops.q8_plan(heads, kv_heads, dim, len(q_lens), -(-max(ctx_lens) // 16) + 2, 16, max(q_lens), 1, 0, sum(q_lens), q_lens, max(ctx_lens))
     assert (not one and not plan.tc_portions) or plan.has_single + plan.has_portions == (1 if one else 2)
     check_attention(dtype, heads, kv_heads, dim, 16, q_lens, ctx_lens, seed=6, **options)
@@ -240,13 +247,14 @@ FORMS = [(torch.bfloat16, 128, True), (torch.bfloat16, 64, True), (torch.bfloat1
 
 @pytest.mark.parametrize("dtype,dim,tensor_cores", FORMS)
 @pytest.mark.parametrize("splits", [0, 3])
-def test_rows_that_see_nothing_are_zeros(dtype, dim, tensor_cores, splits):
+@pytest.mark.parametrize("few_rows", [False, True])
+def test_rows_that_see_nothing_are_zeros(dtype, dim, tensor_cores, splits, few_rows):
     """A context shorter than the new tokens: the first of them lie before position 0.  An entry without tokens is left out, and
     rows behind the last sequence stay as they are."""
     heads, kv_heads, page = 6, 2, 16
     q_lens, ctx_lens = [5, 90, 0, 1, 1, 40], [3, 70, 9, 0, 4, 400]
     ops = cuda_ops(dtype)
-    ops.tensor_core_attention, ops.portion_splits, ops.q8_splits = tensor_cores, splits, (2, 2) if splits else None
+    ops.tensor_core_attention, ops.portion_splits, ops.q8_splits, ops.q8_few_rows = tensor_cores, splits, (2, 2) if splits else None, few_rows
     case = oracle.pages_case(heads, kv_heads, dim, page, q_lens, ctx_lens, dtype, 3, DEV)
     more = 3
     q = torch.cat([case["q"], rnd(more, heads * dim, dtype=dtype)])
@@ -272,12 +280,14 @@ def test_whole_runs_of_rows_that_see_nothing(dtype, dim, tensor_cores, splits, c
 
 @pytest.mark.parametrize("dtype,dim,tensor_cores", FORMS)
 @pytest.mark.parametrize("options", [{}, {"window": 30}])
-def test_what_a_row_does_not_see_has_no_part_in_it(dtype, dim, tensor_cores, options):
+@pytest.mark.parametrize("few_rows", [False, True])
+def test_what_a_row_does_not_see_has_no_part_in_it(dtype, dim, tensor_cores, options, few_rows):
     """Keys and values stored from infinities, NaN and the largest numbers: rows before them are what they would be without,
     rows that see them are NaN, or large."""
     heads, kv_heads, page = 4, 2, 16
     q_lens, ctx_lens = [100, 1, 33], [150, 140, 33]
     ops = cuda_ops(dtype)
+    ops.q8_few_rows = few_rows
     ops.tensor_core_attention = tensor_cores
     case = oracle.pages_case(heads, kv_heads, dim, page, q_lens, ctx_lens, dtype, 7, DEV)
     bad = {0: 120, 2: 20}   # sequence -> the position that is spoilt
@@ -327,11 +337,13 @@ def test_scales_of_any_sign(scale):
 
 
 @pytest.mark.parametrize("dtype,dim", [(torch.bfloat16, 128), (torch.bfloat16, 64), (torch.float32, 64)])
-def test_pools_beyond_32_bit_offsets(dtype, dim):
+@pytest.mark.parametrize("few_rows", [False, True])
+def test_pools_beyond_32_bit_offsets(dtype, dim, few_rows):
     """Pages whose codes lie more than 2^31 and 2^32 bytes into the pool: stored, read back and attended over."""
     heads, kv_heads, page = 16, 8, 64
     pages = (1 << 32) // (page * kv_heads * dim) + 40
     ops = cuda_ops(dtype)
+    ops.q8_few_rows = few_rows
     keys, values = (QuantisedPages(torch.empty(pages, page, kv_heads, dim, dtype=torch.int8, device=DEV),
                                    torch.full((pages, kv_heads, page), math.nan, device=DEV)) for _ in range(2))
     ctx_lens, q_lens = [200, 333, 130], [1, 120, 1]
@@ -365,11 +377,13 @@ def test_pools_beyond_32_bit_offsets(dtype, dim):
 
 
 @pytest.mark.parametrize("dtype,dim,tensor_cores", FORMS)
-def test_a_layer_captured_and_replayed_and_on_another_stream(dtype, dim, tensor_cores):
+@pytest.mark.parametrize("few_rows", [False, True])
+def test_a_layer_captured_and_replayed_and_on_another_stream(dtype, dim, tensor_cores, few_rows):
     """Rotation and store, then attention, as a layer has them: captured once, replayed with other positions, contexts and pages."""
     heads, kv_heads, page = 4, 2, 16
     q_lens, first = [40, 1, 1], [30, 200, 5]
     ops = cuda_ops(dtype)
+    ops.q8_few_rows = few_rows
     ops.tensor_core_attention = tensor_cores
     n, width = sum(q_lens), (heads + 2 * kv_heads) * dim
     inv_freq = (10000.0 ** (-torch.arange(0, dim, 2).double() / dim)).float().to(DEV)

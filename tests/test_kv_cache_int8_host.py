@@ -196,7 +196,7 @@ class Library:
             self.calls.append(name)
             return {"shrike_attention_q8_tile_rows": 8, "shrike_attention_q8_resident_ctas": 592, "shrike_attention_q8_row_floats": 66,
                     "shrike_attention_q8_max_splits": 64, "shrike_attention_q8_tc_tokens": 32, "shrike_attention_q8_tc_splits": 3, "shrike_attention_q8_portion_rows": 64,
-                    "shrike_attention_q8_resident_portions": 444}.get(name, 0)
+                    "shrike_attention_q8_resident_portions": 444, "shrike_attention_q8_tc_time": 0}.get(name, 0)
         return launcher
 
 
@@ -212,6 +212,7 @@ def calls(monkeypatch):
     ops._held_stream, ops.tensor_core_attention, ops.status = None, True, torch.zeros(4, dtype=torch.int32)
     ops._q8_libs, ops._q8_plans = {64: lib}, {}
     ops._q8_scratch = ops._q8_arrivals = ops._q8_portion_scratch = ops.q8_splits = None
+    ops.q8_few_rows = False
     return ops, lib
 
 
