@@ -308,9 +308,9 @@ class QuantisedCacheOps:
         return plan
 
     # In keys of the form for few rows, which a CTA's four warps share with 8 rows each: a key of the mma.sync form for many, which
-    # all of them walk with 16 rows each; the tcgen05 kernel's unit of time, and a launch of the single tokens' own after it; a CTA
+    # all of them walk with 16 rows each; the tcgen05 kernel's unit of time; the least that a launch of the single tokens' own after it takes; a CTA
     # that finds nothing to do.
-    Q8_MANY_ROWS_KEY, Q8_TC_UNIT, Q8_OWN_LAUNCH, Q8_EMPTY_KEYS = 5.6, 50, 400, 90
+    Q8_MANY_ROWS_KEY, Q8_TC_UNIT, Q8_OWN_LAUNCH, Q8_EMPTY_KEYS = 5.6, 55, 400, 90
 
     def _few_rows_serve(self, lib, num_heads, num_kv_heads, table_keys, window, num_seqs, num_tokens, max_q_len, q_lens, tile_tokens,
                         own_launch) -> bool:
@@ -338,7 +338,11 @@ class QuantisedCacheOps:
         few += self.Q8_EMPTY_KEYS * splits * (grid * num_seqs - pairs) / resident
         if tile_tokens:
             tiles = num_tokens // tile_tokens + num_seqs if q_lens is None else sum(-(-q // tile_tokens) for q in q_lens if q > 1 or not own_launch)
-            return few < lib.shrike_attention_q8_tc_time(tiles, num_kv_heads, keys) * self.Q8_TC_UNIT + (self.Q8_OWN_LAUNCH if own_launch else 0)
+            many = lib.shrike_attention_q8_tc_time(tiles, num_kv_heads, keys) * self.Q8_TC_UNIT
+            if own_launch:
+                singles = num_kv_heads * -(-group // rows) * sum(q == 1 for q in lens)
+                many += max(self.Q8_OWN_LAUNCH, self.q8_few_row_time(keys, singles, resident)[0])
+            return few < many
         ctas = num_kv_heads * sum(-(-q * group // lib.shrike_attention_q8_portion_rows()) for q in lens)
         return few < max(1.0, ctas / lib.shrike_attention_q8_resident_portions(self.code)) * (keys * self.Q8_MANY_ROWS_KEY + self.Q8_START_KEYS)
 
