@@ -21,7 +21,7 @@
 // meet in a bank.  Four codes become two registers of float16 pairs by a byte permutation (1024 + code + 128, exact) and a
 // subtraction; the weights go from the scores' layout to an operand's through movmatrix.
 //
-// Two forms.  Few rows (single tokens): the rows' keys are dealt to `splits` CTAs and to each CTA's four warps, each with its
+// Two forms.  Few rows (single tokens, and small portions, eight or sixteen rows a tile): the rows' keys are dealt to `splits` CTAs and to each CTA's four warps, each with its
 // own ring of cp.async copies (no barrier in the loop); the warps' results meet in shared memory, those of up to eight CTAs in
 // the shared memory of their cluster, and the clusters' in global memory, where the last CTA to arrive adds them up in order.
 // Bound by memory at many keys (64 sequences of 4,096 keys, 40 heads of 128: 85 us, 5.0 TB/s; with the products left out the

@@ -34,8 +34,8 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)   # asking to
 class QuantisedPlan:
     """How a batch's attention over 8-bit pages is cut."""
 
-    has_single: bool      # entries of one token run on the form for few rows
-    has_portions: bool    # longer ones on the form for many
+    has_single: bool      # the form for few rows runs: single tokens, or every entry where has_portions is False
+    has_portions: bool    # a form for many rows runs: longer entries, or every entry where has_single is False
     tc_portions: bool     # which is the tcgen05 kernel, else the mma.sync one
     splits: int           # CTAs that share the keys of a row tile of the former
     cluster: int          # how many of them form a thread-block cluster
@@ -240,7 +240,7 @@ class QuantisedCacheOps:
         batch of that shape (and of its `context_class`).  `q_lens`: every entry's length, if they are known; `max_ctx_len`: the
         longest context, or 0."""
         short = 0 < max_ctx_len <= self.SHORT_CONTEXT
-        shape = (num_tokens, short, tuple(q_lens) if q_lens is not None else None) if max_q_len > 1 else None
+        shape = (num_tokens, short, max_q_len, tuple(q_lens) if q_lens is not None else None) if max_q_len > 1 else None
         key = (num_heads, num_kv_heads, head_dim, num_seqs, max_blocks, page_size, min_q_len <= 1, window, shape, self.q8_splits,
                self.tensor_core_attention, self.portion_splits, self.q8_few_rows)
         held = self._q8_plans.get(key)

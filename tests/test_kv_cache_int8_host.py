@@ -352,6 +352,23 @@ def test_plans_are_kept_by_shape_until_the_scratch_moves(calls):
     assert not ops.q8_plan(4, 2, 64, 3, 64, 5, 40, 1, 0, 42, [40, 1, 1]).tc_portions   # pages of five tokens: the other kernel
 
 
+def test_plans_of_unknown_lengths_differ_by_the_longest(calls):
+    """The form for few rows has a place for the longest entry's rows in every entry, in its grid and in its scratch."""
+    ops, _lib = calls
+    ops.q8_few_rows, ops.q8_splits = True, (64, 8)
+    ops.tensor_core_attention = False
+    needs = []
+    for longest in (2, 4000, 2):
+        plan = ops.q8_plan(4, 2, 64, 3, 1024, 16, longest, 1, 0, 4002)
+        assert plan.has_single and not plan.has_portions
+        pairs = 3 * 2 * -(-2 * longest // 8)
+        assert plan.splits % plan.cluster == 0
+        if plan.splits > plan.cluster:
+            assert plan.scratch.numel() >= plan.splits // plan.cluster * 8 * 66 * pairs and plan.arrivals.numel() >= pairs
+        needs.append(pairs)
+    assert needs[1] > needs[0]
+
+
 def test_codes_of_bfloat16_elements_fall_on_the_right_side_of_every_border():
     """The store's shorter form for bfloat16 (a 32-bit product, and halves of the largest element apart), for every pair of
     significands, against integers: 127 x / a to the nearest, halves to even."""
