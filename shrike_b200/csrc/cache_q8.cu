@@ -4,24 +4,12 @@
 // scale s = a / 127 (rounded once): x_i is about c_i s.  A row of zeros has scale 0; a row that holds an infinity or a NaN has
 // scale NaN and codes 0, so that whatever reads it gets NaN and nothing else.  Pages: codes int8 [pages, page size, kv heads,
 // D], scales float32 [pages, kv heads, page size]: the attention reads the scales of one head, and a page's lie together.
+#include "codes_q8.cuh"
 #include "common.cuh"
 
 namespace cacheq8 {
 
-// The code of x in a row of largest magnitude a (finite, above zero), `inv` about 127 / a.  The first guess may be one off near
-// a border between two codes; d = 127 x - q a, formed without the rounding of the product q a, tells on which side x lies.  On
-// the border itself (x = a / 2 always lies on one) d is exact and the even code is taken.
-__device__ __forceinline__ int code_of(float x, float a, float inv) {
-  const float q = rintf(__fmul_rn(x, inv));
-  const float p = __fmul_rn(q, a), e = __fmaf_rn(q, a, -p);
-  const float d = __fsub_rn(__fmaf_rn(127.f, x, -p), e);
-  const float twice = fabsf(d) * 2.f;
-  int code = static_cast<int>(q);
-  if (twice > a || (twice == a && (code & 1))) code += d > 0.f ? 1 : -1;
-  return code;
-}
-
-// The same for bfloat16 elements.  With X and A the eight-bit significands of x and a, and x smaller by 2^s, 127 x / a lies at
+// `code_of` for bfloat16 elements, in fewer steps.  With X and A the eight-bit significands of x and a, and x smaller by 2^s, 127 x / a lies at
 // least 1 / (510 2^s) from a border it does not lie on, and the product below is off by 2^-23 of up to 127 / 2^s: it decides
 // rightly.  127 x / a lies on a border where 254 X is an odd multiple of A: where A is 254 (the product is exact then, and
 // rounds to the even code) or x = a / 2.
