@@ -432,6 +432,17 @@ struct Rows {
           sum[nt][r] += p[j][r];
         }
       }
+      // A value that is no number makes the rows that see it none: by way of their sums, since its weight may be zero in 32 bits,
+      // here or where shares are added up.
+      if (odd_scale) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const int key = key0 + 8 * j + key_of(g);
+            if (!(fabsf(v_scale[j]) < INFINITY) && key >= first[nt][r] && key <= last[nt][r]) sum[nt][r] = __int_as_float(0x7fffffff);
+          }
+      }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         float x = p[j][0] * v_scale[j], y = p[j][1] * v_scale[j];
@@ -512,7 +523,7 @@ __device__ __forceinline__ bool entry_of(const Args& args, int seq, int& start, 
 // whose largest base is `base`.
 __device__ __forceinline__ void add_share(float m, float l, const float4& v, float base, float& total, float (&acc)[4]) {
   const float weight = m == -INFINITY ? 0.f : fast_exp2(m - base);
-  if (l != l) total = l;   // a score that is no number: the row is none either, whatever the others hold
+  if (l != l) total = l;   // a score or a value that is no number: the row is none either, whatever the others hold
   if (weight == 0.f) return;
   total += l * weight;
   acc[0] += v.x * weight; acc[1] += v.y * weight; acc[2] += v.z * weight; acc[3] += v.w * weight;

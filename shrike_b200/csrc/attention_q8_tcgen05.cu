@@ -204,8 +204,7 @@ __device__ __forceinline__ Work find_work(const Args& args, int work, int rows) 
 
 struct Shared {
   float k_scale[STAGES][KEYS], v_scale[STAGES][KEYS];
-  int v_top[STAGES][2];   // per 32 keys: the exponent of the largest value scale
-  int v_bad[STAGES][2];   // whether one of them is no finite number
+  int4 v_info[STAGES];   // x, y: of each 32 keys the exponent of the largest value scale; z, w: whether one of them is no finite number
   unsigned long long q_full, q_ready[2], s_full[2], s_read[2], p_full[2][2], pv_done[2][2], pv_last[2], stagger;
   unsigned long long raw_k_full[RAW_STAGES], raw_k_free[RAW_STAGES], raw_v_full[RAW_STAGES], raw_v_free[RAW_STAGES];
   unsigned long long k_full[STAGES], k_free[STAGES], v_full[STAGES], v_free[STAGES];
@@ -522,8 +521,9 @@ portions_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         const unsigned top = __reduce_max_sync(0xffffffffu, finite_bits(v_scale));
         const bool bad = __any_sync(0xffffffffu, !(fabsf(v_scale) < INFINITY));
         if (lane == 0) {
-          sh->v_top[st][row >> 5] = static_cast<int>(top >> 23) - 127;
-          sh->v_bad[st][row >> 5] = bad ? 1 : 0;
+          int* info = reinterpret_cast<int*>(&sh->v_info[st]) + (row >> 5);
+          info[0] = static_cast<int>(top >> 23) - 127;
+          info[2] = bad ? 1 : 0;
         }
         k_scale = next_k;
         v_scale = next_v;
@@ -617,7 +617,8 @@ portions_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       fence_after_sync();
       tmem_load_fragments(tmem_chain, v);
       int top[2];
-      top[0] = top[1] = max(sh->v_top[st][0], sh->v_top[st][1]);
+      const int4 info = sh->v_info[st];
+      top[0] = top[1] = max(info.x, info.y);
       float2 scale[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) scale[j] = *reinterpret_cast<const float2*>(sh->k_scale[st] + 8 * j + 2 * t);   // while the scores come
@@ -709,12 +710,21 @@ portions_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
           weights[2 * j + r] = pack_half(w0, w1);
         }
       }
-      if (__builtin_expect(edge && (sh->v_bad[st][0] || sh->v_bad[st][1]), 0)) {   // rare: a key that the row does not see has no part in it, not even a scale of NaN
+      if (__builtin_expect((info.z | info.w) != 0, 0)) {   // rare: a value that is no number
+        // A key that a row does not see has no part in it, not even a scale of NaN.
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const int key = key_base + 8 * (i / 2) + 2 * t;
           if (key < first[i & 1] || key > last[i & 1]) weights[i] &= 0xffff0000u;
           if (key + 1 < first[i & 1] || key + 1 > last[i & 1]) weights[i] &= 0x0000ffffu;
+        }
+        // The rows that see it are none either: by way of their sums, since its weight may be zero where splits are added up.
+#pragma unroll 1
+        for (int i = 0; i < 16; ++i) {
+          const int within = 8 * (i >> 1) + (i & 1), key = key_base + 2 * t + within;
+          if (fabsf(v_scale[within]) < INFINITY) continue;
+          if (key >= first[0] && key <= last[0]) row_sum[0] = __int_as_float(0x7fffffff);
+          if (key >= first[1] && key <= last[1]) row_sum[1] = __int_as_float(0x7fffffff);
         }
       }
       // P(h) goes where P(h - 2) was.  The product that read that was issued before the scores of step h, and a commit waits for
@@ -857,7 +867,7 @@ combine_portions_kernel(const Args args) {
 #pragma unroll
   for (int offset = 16; offset > 0; offset >>= 1) base = fmaxf(base, __shfl_xor_sync(0xffffffffu, base, offset));
   const float weight = m == -INFINITY ? 0.f : fast_exp2(m - base);   // a split that saw no key of this row has base -inf
-  float total = l != l ? l : weight == 0.f ? 0.f : l * weight;   // a score that is no number makes the row none
+  float total = l != l ? l : weight == 0.f ? 0.f : l * weight;   // a score or a value that is no number makes the row none
 #pragma unroll
   for (int offset = 16; offset > 0; offset >>= 1) total += __shfl_xor_sync(0xffffffffu, total, offset);
   float acc[VEC];

@@ -8,6 +8,7 @@ import torch
 from shrike_b200.cache.quantised import QuantisedPages
 from tests import cache_q8_oracle as oracle
 from tests.gpu_common import cuda_ops
+from tests.test_gpu_cache_q8 import FORMS, attend
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -53,3 +54,59 @@ def test_codes_beside_the_borders(dim, fused, dtype):
         codes, scales = oracle.quantise(x.view(n, heads, dim))
         assert torch.equal(pool.codes[at // page, at % page], codes)
         assert torch.equal(pool.scales[at // page, :, at % page], scales)
+
+
+@pytest.mark.parametrize("dtype,dim,tensor_cores", FORMS)
+@pytest.mark.parametrize("splits", [1, 3])
+@pytest.mark.parametrize("few_rows", [False, True])
+@pytest.mark.parametrize("options", [{}, {"window": 90}])
+def test_a_value_that_is_no_number_reaches_every_row_that_sees_it(dtype, dim, tensor_cores, splits, few_rows, options):
+    """However small its key's weight: 2^-300 of the others', zero in 32 bits."""
+    heads, kv_heads, page = 4, 2, 16
+    q_lens, ctx_lens, bad = [100, 1, 1, 70], [150, 700, 90, 400], [120, 655, 89, 340]
+    ops = cuda_ops(dtype)
+    ops.tensor_core_attention, ops.portion_splits, ops.q8_splits, ops.q8_few_rows = tensor_cores, splits, (splits, 1), few_rows
+    case = oracle.pages_case(heads, kv_heads, dim, page, q_lens, ctx_lens, dtype, 9, DEV)
+    case["q"].view(-1, dim)[:, 0] = 16.0
+    for s, position in enumerate(bad):
+        page_id, within = int(case["table"][s, position // page]), position % page
+        case["codes_k"][page_id, within] = 0
+        case["codes_k"][page_id, within, :, 0] = -127
+        case["scales_k"][page_id, :, within] = 0.125 * dim ** 0.5   # a score of -254, against some units
+        case["scales_v"][page_id, :, within] = math.nan
+        case["sequences"][s][0][0][position] = case["codes_k"][page_id, within]
+        case["sequences"][s][0][1][position] = 0.125 * dim ** 0.5
+        case["sequences"][s][1][1][position] = 0.0
+    got = attend(ops, case, heads, kv_heads, dim, q_lens, ctx_lens, **options)
+    want, bound = oracle.attention(case["q"], case["sequences"], q_lens, ctx_lens, heads, kv_heads, dim, dim ** -0.5, **options)
+    position = torch.cat([torch.arange(c - n, c) for n, c in zip(q_lens, ctx_lens)])
+    spoilt = torch.repeat_interleave(torch.tensor(bad), torch.tensor(q_lens))
+    sees = ((position >= spoilt) & (position < spoilt + options.get("window", 1 << 30))).to(DEV)
+    assert torch.isnan(got[sees]).all()
+    assert ((got.double() - want).abs() <= bound)[~sees].all()
+    ops.check_status()
+
+
+@pytest.mark.parametrize("dtype,dim,tensor_cores", FORMS)
+@pytest.mark.parametrize("few_rows", [False, True])
+def test_a_value_that_is_no_number_among_keys_of_no_weight(dtype, dim, tensor_cores, few_rows):
+    """All keys of a share score 2^-300 of the others': the share has no weight, and its NaN still counts."""
+    heads, kv_heads, page = 4, 2, 16
+    q_lens, ctx_lens = [70, 1], [400, 400]
+    ops = cuda_ops(dtype)
+    ops.tensor_core_attention, ops.portion_splits, ops.q8_splits, ops.q8_few_rows = tensor_cores, 3, (4, 2), few_rows
+    case = oracle.pages_case(heads, kv_heads, dim, page, q_lens, ctx_lens, dtype, 9, DEV)
+    case["q"].view(-1, dim)[:, 0] = 16.0
+    for s in range(2):
+        ids = case["table"][s, : 192 // page].long()   # the first 192 keys: a share of any form, and more
+        case["codes_k"][ids] = 0
+        case["codes_k"][ids, :, :, 0] = -127
+        case["scales_k"][ids] = 0.125 * dim ** 0.5
+    fine = attend(ops, case, heads, kv_heads, dim, q_lens, ctx_lens)
+    assert torch.isfinite(fine).all()
+    case["scales_v"][int(case["table"][0, 40 // page]), 1, 40 % page] = math.nan   # heads 2 and 3 of the portion
+    case["scales_v"][int(case["table"][1, 7 // page]), 0, 7] = math.nan             # heads 0 and 1 of the single token
+    got = attend(ops, case, heads, kv_heads, dim, q_lens, ctx_lens)
+    none = torch.isnan(got.view(71, 2, -1))
+    assert none[:70, 1].all() and none[70, 0].all() and not none[:70, 0].any() and not none[70, 1].any()
+    ops.check_status()
