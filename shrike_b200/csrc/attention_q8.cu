@@ -116,7 +116,9 @@ __device__ __forceinline__ int swizzle(int row) {
 }
 __device__ __forceinline__ int chunk_at(int row, int chunk) { return row * D + ((chunk ^ swizzle(row)) << 4); }
 
-// F's range: sums of 2^(z - m) stay within float32 for any count of keys, and weights of 2^-20 of the largest above its least.
+// F's range: sums of 2^(z - m) stay within float32 for any count of keys, and weights of 2^-19 of the largest above its least.
+// The largest scale that a store leaves is below 2^122: a weight is then below 2^15 if the base does not lag, and where a step's
+// largest scale is above F's range it does not.
 constexpr int LEAST_EXPONENT = -93, MOST_EXPONENT = 107, SCALE_BITS = 8;
 constexpr float BASE_LAG = 6.0f;   // float16's largest power of two is 2^15: 2^9 times 2^6
 // A magnitude's bits (which order as the magnitudes do), 0 for infinities and NaN.

@@ -653,7 +653,7 @@ portions_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
 #pragma unroll
         for (int j = 0; j < 8; ++j) part[j & 1] = max3(part[j & 1], __uint_as_float(v[4 * j + 2 * r]), __uint_as_float(v[4 * j + 2 * r + 1]));
         step_max[r] = fmaxf(part[0], part[1]) * factor[r];
-        top[r] = min(top[r] - SCALE_BITS, MOST_EXPONENT);
+        top[r] -= SCALE_BITS;   // above MOST_EXPONENT the base never lags: the weights have no room for it
         moves = moves || step_max[r] > most[r] + BASE_LAG || top[r] > exponent[r] || most[r] == -INFINITY;
       }
       // The base follows the largest score lazily (2^6), and the largest value scale at once: the weights stay below 2^15.
@@ -669,7 +669,7 @@ portions_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
             top[r] = max(top[r], __shfl_xor_sync(0xffffffffu, top[r], offset));
           }
           most[r] = fmaxf(most[r], step_max[r]);
-          exponent[r] = max(exponent[r], top[r]);
+          exponent[r] = max(exponent[r], min(top[r], MOST_EXPONENT));
           const float next = most[r] + static_cast<float>(exponent[r]);
           // a row that has seen no key yet has O = 0 and a sum of 0: nothing to rescale
           correction[r] = base[r] == -INFINITY ? 1.0f : fast_exp2(base[r] - next);

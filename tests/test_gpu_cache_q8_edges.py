@@ -110,3 +110,32 @@ def test_a_value_that_is_no_number_among_keys_of_no_weight(dtype, dim, tensor_co
     none = torch.isnan(got.view(71, 2, -1))
     assert none[:70, 1].all() and none[70, 0].all() and not none[:70, 0].any() and not none[70, 1].any()
     ops.check_status()
+
+
+@pytest.mark.parametrize("dtype,dim,tensor_cores", FORMS)
+@pytest.mark.parametrize("few_rows", [False, True])
+@pytest.mark.parametrize("size", [1e34, 1e36, 3e38])
+def test_the_largest_values(dtype, dim, tensor_cores, few_rows, size):
+    """Values of up to about float32's largest number under scores that grow along the keys, so that a base which lagged would show."""
+    heads, kv_heads, page = 4, 2, 16
+    q_lens, ctx_lens = [150, 1, 1], [700, 900, 70]
+    ops = cuda_ops(dtype)
+    ops.tensor_core_attention, ops.portion_splits, ops.q8_splits, ops.q8_few_rows = tensor_cores, 1, (1, 1), few_rows
+    case = oracle.pages_case(heads, kv_heads, dim, page, q_lens, ctx_lens, dtype, 21, DEV)
+    case["q"].view(-1, dim)[:, 0] = 4.0
+    for s, context in enumerate(ctx_lens):
+        (key_codes, key_scales), (codes, scales) = case["sequences"][s]
+        for j in range(context):   # the first element's part of the score: up to 4 more from the first key to the last
+            key_codes[j, :, 0] = ((j + 1) * dim ** 0.5 / context / key_scales[j]).round().clamp(0, 127).to(torch.int8)
+        scales.copy_(torch.where(torch.arange(context, device=DEV)[:, None] % 5 == 4, 1.0, size / 127))   # ordinary ones among them
+        ids = case["table"][s].long()
+        for j in range(context):
+            at = ids[j // page], j % page
+            case["codes_k"][at], case["scales_v"][at[0], :, at[1]] = key_codes[j], scales[j]
+    got = attend(ops, case, heads, kv_heads, dim, q_lens, ctx_lens)
+    want, bound = oracle.attention(case["q"], case["sequences"], q_lens, ctx_lens, heads, kv_heads, dim, dim ** -0.5)
+    # under F = 107 what is below 2^-19 of the largest weight is below 2^-126, zero: that much of a key's value, and of a sum
+    lost = torch.repeat_interleave(torch.tensor(ctx_lens), torch.tensor(q_lens)).double().to(DEV)[:, None] * 2.0 ** -18 * size
+    assert torch.isfinite(got).all()
+    assert ((got.double() - want).abs() <= bound + lost).all()
+    ops.check_status()
