@@ -146,6 +146,10 @@ __device__ __forceinline__ float4 load_peer4(unsigned address) {
   return v;
 }
 
+// x 2^d for d <= 0, also where 2^d is below float32's range: a sum under the least exponent F (a row whose values were all zeros
+// so far) becomes one under a large one, 2^200 smaller.  Outputs need not go that far: they are nothing beside the values that F rose for.
+__device__ __forceinline__ float scale_sum(float x, float d) { return x * fast_exp2(fmaxf(d, -126.f)) * fast_exp2(fminf(d + 126.f, 0.f)); }
+
 // 2^e for e in [-126, 127].
 __device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e + 127) << 23); }
 
@@ -415,9 +419,10 @@ struct Rows {
           exponent[nt][r] = max(exponent[nt][r], min(static_cast<int>(top[r] >> 23) - 127 - SCALE_BITS, MOST_EXPONENT));
           most[nt][r] = fmaxf(most[nt][r], largest[r]);
           const float next = most[nt][r] + static_cast<float>(exponent[nt][r]);
-          correction[r] = base[nt][r] == next ? 1.f : fast_exp2(base[nt][r] - (next == -INFINITY ? 0.f : next));
+          const float down = base[nt][r] == next ? 0.f : base[nt][r] - (next == -INFINITY ? 0.f : next);
+          correction[r] = fast_exp2(down);
           base[nt][r] = next;
-          sum[nt][r] *= correction[r];
+          sum[nt][r] = scale_sum(sum[nt][r], down);
         }
 #pragma unroll
         for (int i = 0; i < BLOCKS_V * 2; ++i)
@@ -526,8 +531,8 @@ __device__ __forceinline__ bool entry_of(const Args& args, int seq, int& start, 
 __device__ __forceinline__ void add_share(float m, float l, const float4& v, float base, float& total, float (&acc)[4]) {
   const float weight = m == -INFINITY ? 0.f : fast_exp2(m - base);
   if (l != l) total = l;   // a score or a value that is no number: the row is none either, whatever the others hold
+  if (m != -INFINITY) total += scale_sum(l, m - base);
   if (weight == 0.f) return;
-  total += l * weight;
   acc[0] += v.x * weight; acc[1] += v.y * weight; acc[2] += v.z * weight; acc[3] += v.w * weight;
 }
 __device__ __forceinline__ void leave_share(float* share, int rows, int row, int element, float base, float total, const float (&acc)[4]) {
@@ -724,7 +729,7 @@ split_keys_kernel(const Args args) {
 #pragma unroll
       for (int c = 0; c < 8; ++c) next = fmaxf(next, ml[c].x);
       const float down = base == -INFINITY ? 0.f : fast_exp2(base - next);
-      total *= down;
+      total = base == -INFINITY ? total : scale_sum(total, base - next);
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[e] *= down;
       base = next;

@@ -70,6 +70,8 @@ __device__ __forceinline__ float fast_exp2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// x 2^d for d <= 0, also where 2^d is below float32's range (as in attention_q8.cu).
+__device__ __forceinline__ float scale_sum(float x, float d) { return x * fast_exp2(fmaxf(d, -126.f)) * fast_exp2(fminf(d + 126.f, 0.f)); }
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -672,9 +674,10 @@ portions_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
           exponent[r] = max(exponent[r], min(top[r], MOST_EXPONENT));
           const float next = most[r] + static_cast<float>(exponent[r]);
           // a row that has seen no key yet has O = 0 and a sum of 0: nothing to rescale
-          correction[r] = base[r] == -INFINITY ? 1.0f : fast_exp2(base[r] - next);
+          const float base_was = base[r];
+          correction[r] = base_was == -INFINITY ? 1.0f : fast_exp2(base_was - next);
           base[r] = next;
-          row_sum[r] *= correction[r];
+          row_sum[r] = base_was == -INFINITY ? row_sum[r] : scale_sum(row_sum[r], base_was - next);
         }
         rescales = h > 0 && __any_sync(0xffffffffu, correction[0] != 1.0f || correction[1] != 1.0f);
       }
@@ -867,7 +870,7 @@ combine_portions_kernel(const Args args) {
 #pragma unroll
   for (int offset = 16; offset > 0; offset >>= 1) base = fmaxf(base, __shfl_xor_sync(0xffffffffu, base, offset));
   const float weight = m == -INFINITY ? 0.f : fast_exp2(m - base);   // a split that saw no key of this row has base -inf
-  float total = l != l ? l : weight == 0.f ? 0.f : l * weight;   // a score or a value that is no number makes the row none
+  float total = l != l ? l : m == -INFINITY ? 0.f : scale_sum(l, m - base);   // a score or a value that is no number makes the row none
 #pragma unroll
   for (int offset = 16; offset > 0; offset >>= 1) total += __shfl_xor_sync(0xffffffffu, total, offset);
   float acc[VEC];

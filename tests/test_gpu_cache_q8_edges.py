@@ -139,3 +139,28 @@ def test_the_largest_values(dtype, dim, tensor_cores, few_rows, size):
     assert torch.isfinite(got).all()
     assert ((got.double() - want).abs() <= bound + lost).all()
     ops.check_status()
+
+
+@pytest.mark.parametrize("dtype,dim,tensor_cores", FORMS)
+@pytest.mark.parametrize("few_rows", [False, True])
+@pytest.mark.parametrize("splits", [1, 3])
+@pytest.mark.parametrize("size", [1.0, 1e20, 1e36])
+def test_keys_without_values_before_large_ones(dtype, dim, tensor_cores, few_rows, splits, size):
+    """Keys whose values are zeros have their part in the sums, however large the values behind them (or beside them, in another
+    share of the keys) are."""
+    heads, kv_heads, page = 4, 2, 16
+    q_lens, ctx_lens, zeros = [90, 1, 1, 40], [700, 900, 70, 300], [350, 800, 32, 64]
+    ops = cuda_ops(dtype)
+    ops.tensor_core_attention, ops.portion_splits, ops.q8_splits, ops.q8_few_rows = tensor_cores, splits, (4 * splits, 2 * splits), few_rows
+    case = oracle.pages_case(heads, kv_heads, dim, page, q_lens, ctx_lens, dtype, 22, DEV)
+    for s, context in enumerate(ctx_lens):
+        scales = case["sequences"][s][1][1]
+        scales.mul_(size)
+        scales[: zeros[s]] = 0
+        for j in range(context):
+            case["scales_v"][int(case["table"][s, j // page]), :, j % page] = scales[j]
+    got = attend(ops, case, heads, kv_heads, dim, q_lens, ctx_lens)
+    want, bound = oracle.attention(case["q"], case["sequences"], q_lens, ctx_lens, heads, kv_heads, dim, dim ** -0.5)
+    lost = torch.repeat_interleave(torch.tensor(ctx_lens), torch.tensor(q_lens)).double().to(DEV)[:, None] * 2.0 ** -18 * 40 * size if size > 1e30 else 0.0
+    assert ((got.double() - want).abs() <= bound + lost).all()
+    ops.check_status()
