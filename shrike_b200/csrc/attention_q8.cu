@@ -264,7 +264,7 @@ struct Rows {
       }
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const int e = min(max(static_cast<int>(top >> 23) - 127, -100), 126);
+      const int e = max(static_cast<int>(top >> 23) - 127, -100);
       const float lift = args.scale_log2 < 0.f ? -power_of_two(14 - e) : power_of_two(14 - e);
 #pragma unroll
       for (int s = 0; s < STEPS_K; ++s) {

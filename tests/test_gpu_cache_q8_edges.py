@@ -164,3 +164,24 @@ def test_keys_without_values_before_large_ones(dtype, dim, tensor_cores, few_row
     lost = torch.repeat_interleave(torch.tensor(ctx_lens), torch.tensor(q_lens)).double().to(DEV)[:, None] * 2.0 ** -18 * 40 * size if size > 1e30 else 0.0
     assert ((got.double() - want).abs() <= bound + lost).all()
     ops.check_status()
+
+
+@pytest.mark.parametrize("few_rows", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_the_largest_queries(dtype, few_rows):
+    """Queries of the type's largest number over keys as small as that: scores of some units."""
+    heads, kv_heads, dim, page = 4, 2, 64, 16
+    q_lens, ctx_lens = [70, 1], [200, 300]
+    ops = cuda_ops(dtype)
+    ops.q8_few_rows = few_rows
+    case = oracle.pages_case(heads, kv_heads, dim, page, q_lens, ctx_lens, dtype, 23, DEV)
+    top = torch.finfo(dtype).max
+    q = case["q"].view(-1, dim)
+    q.copy_(torch.where(q > 0, top, -top) * (torch.arange(dim, device=DEV) % 16 == 0))
+    case["scales_k"].mul_(1.0 / 2.0 ** 127)
+    for keys, _values in case["sequences"]:
+        keys[1].mul_(1.0 / 2.0 ** 127)
+    got = attend(ops, case, heads, kv_heads, dim, q_lens, ctx_lens)
+    want, bound = oracle.attention(case["q"], case["sequences"], q_lens, ctx_lens, heads, kv_heads, dim, dim ** -0.5)
+    assert ((got.double() - want).abs() <= bound).all()
+    ops.check_status()
