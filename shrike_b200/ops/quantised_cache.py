@@ -28,6 +28,7 @@ _pack_attention = _ATTENTION_CALL.pack
 _INT32 = torch.int32
 _device = getattr(torch._C, "_cuda_getDevice", None)          # the current device's number, and its current stream's handle:
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)   # asking torch for the objects costs more than a launch
+_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", None)
 
 
 @dataclass(frozen=True, slots=True)
@@ -79,6 +80,8 @@ class QuantisedCacheOps:
     """Mixed into `CudaOps`."""
 
     Q8_SCRATCH_FLOATS = 64 << 20   # at most 256 MiB for the shares of split rows: fewer splits beyond that
+    _q8_captured = frozenset()     # names of the buffers that a capture has seen,
+    _q8_kept = ()                  # and such buffers that are no longer in use
 
     def _declare_q8_core(self, lib):
         lib.shrike_kv_write_q8.argtypes = lib.shrike_kv_read_q8.argtypes = [_c.c_char_p]
@@ -115,6 +118,26 @@ class QuantisedCacheOps:
             lib.shrike_attention_q8_resident_ctas.restype = lib.shrike_attention_q8_tile_rows.restype = _I
             self._q8_libs[head_dim] = lib
         return lib
+
+    def _q8_buffer(self, name: str, need: int, least: int, most: int) -> torch.Tensor:
+        """The object's buffer `name` with at least `need` elements, float32, or int32 zeros for the arrivals.  It grows to twice its
+        size (up to `most`): few calls move it, and each move makes captured launch sequences stale (`generation`).  The old one is
+        given back, unless a capture has seen it: whoever holds that sequence may replay it, and what its kernels write has to stay
+        theirs.  With the doubling those that are kept are no larger than the one in use, all together."""
+        held = getattr(self, name)
+        if held is not None and held.numel() >= need:
+            return held
+        size = max(need, least, min(2 * held.numel() if held is not None else 0, most))
+        if name in self._q8_captured:
+            self._q8_kept = (*self._q8_kept, held)
+            self._q8_captured -= {name}
+        self._q8_plans.clear()   # plans hold the buffers that they were made with
+        held = None
+        setattr(self, name, None)
+        make, dtype = (torch.zeros, _INT32) if name == "_q8_arrivals" else (torch.empty, torch.float32)
+        setattr(self, name, make(size, dtype=dtype, device=self.device))
+        self.generation += 1
+        return getattr(self, name)
 
     # ---- checks
     # A call takes longer on the host than its kernel takes for few tokens, so its tensors are looked at in one native call
@@ -277,14 +300,8 @@ class QuantisedCacheOps:
             if splits > most or splits // cluster * share > self.Q8_SCRATCH_FLOATS:
                 splits = cluster * max(1, min(most // cluster, self.Q8_SCRATCH_FLOATS // share))
             if splits > cluster:
-                need = splits // cluster * share
-                if self._q8_scratch is None or self._q8_scratch.numel() < need:
-                    self._q8_scratch = torch.empty(max(need, 1 << 20), dtype=torch.float32, device=self.device)
-                    self.generation += 1
-                if self._q8_arrivals is None or self._q8_arrivals.numel() < pairs:
-                    self._q8_arrivals = torch.zeros(max(pairs, 4096), dtype=torch.int32, device=self.device)
-                    self.generation += 1
-                scratch, arrivals = self._q8_scratch, self._q8_arrivals
+                scratch = self._q8_buffer("_q8_scratch", splits // cluster * share, 1 << 20, self.Q8_SCRATCH_FLOATS)
+                arrivals = self._q8_buffer("_q8_arrivals", pairs, 4096, 1 << 20)
         tiles, portion_splits, portion_scratch = 0, 1, None
         if tc_portions:
             if q_lens is not None:
@@ -295,11 +312,7 @@ class QuantisedCacheOps:
             each = num_tokens * num_heads * (head_dim + 2)
             portion_splits = max(1, min(portion_splits, 32, self.PORTION_SCRATCH_FLOATS // each)) if num_tokens <= 8 * 65535 else 1
             if portion_splits > 1:
-                need = portion_splits * each
-                if self._q8_portion_scratch is None or self._q8_portion_scratch.numel() < need:
-                    self._q8_portion_scratch = torch.empty(max(need, 1 << 22), dtype=torch.float32, device=self.device)
-                    self.generation += 1
-                portion_scratch = self._q8_portion_scratch
+                portion_scratch = self._q8_buffer("_q8_portion_scratch", portion_splits * each, 1 << 22, self.PORTION_SCRATCH_FLOATS)
         plan = QuantisedPlan(has_single, has_portions, tc_portions, splits, cluster, scratch, arrivals, tiles, portion_splits, portion_scratch, lib,
                              int(has_single) + int(has_portions) + (portion_splits > 1))
         if len(self._q8_plans) >= 4096:
@@ -398,6 +411,8 @@ class QuantisedCacheOps:
         window = window or 0
         plan = self.q8_plan(num_heads, num_kv_heads, head_dim, num_seqs, max_blocks, page_size, max_q_len, min_q_len, window, n, q_lens, max_ctx_len)
         tc, has_portions = plan.tc_portions, plan.has_portions
+        if stream and (plan.scratch is not None or plan.portion_scratch is not None) and _capturing():   # the default stream never is
+            self._q8_captured |= {"_q8_" + name for name in ("scratch", "arrivals", "portion_scratch") if getattr(plan, name) is not None}
         if tc and not self._q8_ints_fit(device, seq_of_token, n):
             self._q8_refuse(device, (), [(seq_of_token, n, "sequences of tokens")])
         sizes = (max_blocks, self.code, n, num_seqs, num_heads, num_kv_heads, page_size, pages, window, plan.has_single)

@@ -1,0 +1,68 @@
+"""Plans and workspaces of the calls over 8-bit pages, without a GPU."""
+
+import weakref
+
+import pytest
+import torch
+
+from shrike_b200.ops import quantised_cache
+from tests.test_kv_cache_int8_host import arguments, calls  # noqa: F401  (a fixture)
+
+
+@pytest.fixture
+def ops(calls):  # noqa: F811
+    return calls[0]
+
+
+def portions(ops, tokens):
+    return ops.q8_plan(4, 2, 64, 1, 1 << 16, 16, tokens, tokens, 0, tokens, [tokens])
+
+
+def test_a_buffer_that_has_grown_is_given_back(ops):
+    first = portions(ops, 40_000)
+    held, size, generation = weakref.ref(first.portion_scratch), first.portion_scratch.numel(), ops.generation
+    for tokens in (39_999, 39_998, 20):   # plans of their own, over the same buffer
+        assert portions(ops, tokens).portion_scratch is first.portion_scratch
+    assert ops.generation == generation
+    del first
+    more = portions(ops, 40_100)
+    assert held() is None and ops.generation == generation + 1
+    # to twice its size, or the most there may be: the next ones do not move it
+    assert more.portion_scratch.numel() == min(2 * size, ops.PORTION_SCRATCH_FLOATS)
+    generation = ops.generation
+    portions(ops, 41_000)
+    assert ops.generation == generation
+    few = ops.q8_plan(4, 2, 64, 1, 4096, 16, 1, 1)   # the other buffers
+    assert few.scratch is ops._q8_scratch and few.arrivals is ops._q8_arrivals and not few.arrivals.any()
+
+
+def test_a_buffer_that_a_capture_has_seen_is_kept(ops, monkeypatch):
+    monkeypatch.setattr(quantised_cache, "_raw_stream", lambda device: 5)
+    capturing = False
+    monkeypatch.setattr(quantised_cache, "_capturing", lambda: capturing)
+    (keys, values), _rows, _q, _out, _index = arguments()
+    tokens = 40_000
+    q, out = (torch.zeros(tokens, 4 * 64, dtype=torch.bfloat16) for _ in range(2))
+    table, owner = torch.zeros(1, 1 << 16, dtype=torch.int32), torch.zeros(tokens, dtype=torch.int32)
+
+    def attend(count):
+        ops.paged_attention(q[:count], keys, values, table, torch.tensor([0, count], dtype=torch.int32), torch.tensor([count], dtype=torch.int32),
+                            owner[:count], 4, 2, 64, 0.125, None, out[:count], max_q_len=count, min_q_len=count, q_lens=[count])
+
+    attend(22_000)
+    before = weakref.ref(ops._q8_portion_scratch)
+    capturing = True
+    attend(22_000)
+    capturing = False
+    ops._q8_portion_scratch, keep = ops._q8_portion_scratch[:22_000], before   # as if it had been made for less
+    small = ops._q8_portion_scratch
+    ops._q8_plans.clear()
+    attend(tokens)
+    assert any(x is small for x in ops._q8_kept) and ops._q8_portion_scratch is not small and keep() is not None
+    second = weakref.ref(ops._q8_portion_scratch)
+    ops._q8_portion_scratch = ops._q8_portion_scratch[:10].clone()
+    ops._q8_plans.clear()
+    assert second() is None
+    third = weakref.ref(ops._q8_portion_scratch)
+    attend(tokens)   # no capture has seen this one
+    assert third() is None and len(ops._q8_kept) == 1

@@ -185,3 +185,36 @@ def test_the_largest_queries(dtype, few_rows):
     want, bound = oracle.attention(case["q"], case["sequences"], q_lens, ctx_lens, heads, kv_heads, dim, dim ** -0.5)
     assert ((got.double() - want).abs() <= bound).all()
     ops.check_status()
+
+
+def test_a_captured_call_keeps_its_workspace_when_a_larger_one_is_needed():
+    """A sequence captured over split rows is replayed after the workspace has grown and the memory has found other users."""
+    heads, kv_heads, dim, page = 8, 1, 64, 16
+    ops = cuda_ops(torch.bfloat16)
+    ops.q8_splits = (64, 1)
+    case = oracle.pages_case(heads, kv_heads, dim, page, [1], [4000], torch.bfloat16, 4, DEV)
+    out = torch.empty_like(case["q"])
+
+    def call():
+        ops.paged_attention(case["q"], QuantisedPages(case["codes_k"], case["scales_k"]), QuantisedPages(case["codes_v"], case["scales_v"]),
+                            case["table"], case["q_start"], case["ctx_len"], case["seq_of"], heads, kv_heads, dim, dim ** -0.5, None, out,
+                            max_q_len=1, min_q_len=1)
+
+    call()
+    want = out.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    old, count = ops._q8_scratch, 200
+    many = oracle.pages_case(heads, kv_heads, dim, page, [1] * count, [70] * count, torch.bfloat16, 5, DEV)
+    ops.q8_plan(heads, kv_heads, dim, 4000, 20, page, 1, 1)   # as a batch of many sequences asks for
+    assert ops._q8_scratch.numel() > old.numel() and any(x is old for x in ops._q8_kept)
+    del old
+    others = [torch.full((1 << 20,), 7.0, device=DEV) for _ in range(8)]
+    out.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want) and all((x == 7.0).all() for x in others)
+    got = attend(ops, many, heads, kv_heads, dim, [1] * count, [70] * count)
+    expected, bound = oracle.attention(many["q"], many["sequences"], [1] * count, [70] * count, heads, kv_heads, dim, dim ** -0.5)
+    assert ((got.double() - expected).abs() <= bound).all()
