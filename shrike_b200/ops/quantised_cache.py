@@ -89,7 +89,8 @@ class QuantisedCacheOps:
         for name in ("shrike_kv_write_q8", "shrike_rope_kv_write_q8", "shrike_kv_read_q8"):
             getattr(lib, name).restype = _I
         self._q8_libs, self._q8_plans = {}, {}
-        self._q8_scratch = self._q8_arrivals = self._q8_portion_scratch = None
+        self._q8_scratch = self._q8_portion_scratch = None
+        self._q8_arrivals = torch.zeros(4096, dtype=_INT32, device=self.device)   # more than the rule for splits ever asks for
         self.q8_few_rows = None   # None: the rule of `_few_rows_serve`; whether the form for few rows takes portions (tests)
         self.q8_splits = None   # None: the rule of `q8_few_row_splits`; (splits, cluster) for few rows (tests)
 
@@ -128,6 +129,8 @@ class QuantisedCacheOps:
         if held is not None and held.numel() >= need:
             return held
         size = max(need, least, min(2 * held.numel() if held is not None else 0, most))
+        if name == "_q8_arrivals" and self._q8_stream()[1] and _capturing():   # its zeros would be written by the replay, not now
+            raise _error(f"attention over 8-bit pages needs {size} counters that are zero: make such a call once before it is captured")
         if name in self._q8_captured:
             self._q8_kept = (*self._q8_kept, held)
             self._q8_captured -= {name}

@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from shrike_b200.ops import quantised_cache
+from shrike_b200.ops.cuda_ops import CudaOps, KernelError
 from tests.test_kv_cache_int8_host import arguments, calls  # noqa: F401  (a fixture)
 
 
@@ -66,3 +67,24 @@ def test_a_buffer_that_a_capture_has_seen_is_kept(ops, monkeypatch):
     third = weakref.ref(ops._q8_portion_scratch)
     attend(tokens)   # no capture has seen this one
     assert third() is None and len(ops._q8_kept) == 1
+
+
+def test_counters_are_not_made_while_a_call_is_captured(ops, monkeypatch):
+    """Their zeros would be written when the sequence is replayed, and calls before that would count from anything."""
+    monkeypatch.setattr(quantised_cache, "_raw_stream", lambda device: 5)
+    monkeypatch.setattr(quantised_cache, "_capturing", lambda: True)
+    ops.q8_splits = (64, 1)
+    ops._q8_arrivals = torch.zeros(4096, dtype=torch.int32)
+    assert ops.q8_plan(4, 2, 64, 2000, 64, 16, 1, 1).arrivals is ops._q8_arrivals
+    with pytest.raises(KernelError, match="once before it is captured"):
+        ops.q8_plan(4, 2, 64, 2100, 64, 16, 1, 1)
+    monkeypatch.setattr(quantised_cache, "_capturing", lambda: False)
+    assert ops.q8_plan(4, 2, 64, 2100, 64, 16, 1, 1).arrivals.numel() >= 4200
+
+
+@pytest.mark.parametrize("resident", [148, 296, 592])
+def test_the_counters_made_at_first_are_enough_for_the_rule(resident):
+    for keys in (600, 1024, 5000, 65536, 1 << 20):
+        for pairs in range(1, 8192):
+            splits, cluster = CudaOps.q8_few_row_splits(keys, pairs, resident)
+            assert splits == cluster or pairs <= 4096

@@ -218,3 +218,32 @@ def test_a_captured_call_keeps_its_workspace_when_a_larger_one_is_needed():
     got = attend(ops, many, heads, kv_heads, dim, [1] * count, [70] * count)
     expected, bound = oracle.attention(many["q"], many["sequences"], [1] * count, [70] * count, heads, kv_heads, dim, dim ** -0.5)
     assert ((got.double() - expected).abs() <= bound).all()
+
+
+def test_the_first_call_of_all_may_be_a_captured_one():
+    """Its counters are there already: a call before the first replay counts from zero, and so does a second sequence."""
+    heads, kv_heads, dim, page = 8, 1, 64, 16
+    torch.randint(1, 1000, (1 << 16,), dtype=torch.int32, device=DEV)   # what fresh memory may hold
+    ops = cuda_ops(torch.bfloat16)
+    ops.q8_splits = (64, 8)
+    cases = [oracle.pages_case(heads, kv_heads, dim, page, [1], [3000 + 500 * i], torch.bfloat16, i, DEV) for i in range(3)]
+    outs = [torch.zeros_like(case["q"]) for case in cases]
+
+    def call(i):
+        case = cases[i]
+        ops.paged_attention(case["q"], QuantisedPages(case["codes_k"], case["scales_k"]), QuantisedPages(case["codes_v"], case["scales_v"]),
+                            case["table"], case["q_start"], case["ctx_len"], case["seq_of"], heads, kv_heads, dim, dim ** -0.5, None, outs[i],
+                            max_q_len=1, min_q_len=1)
+
+    ops._q8_lib(dim)   # compiled, if it has to be, before a capture
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    for i, graph in enumerate(graphs):
+        with torch.cuda.graph(graph):
+            call(i)
+    call(2)
+    graphs[1].replay()
+    graphs[0].replay()
+    torch.cuda.synchronize()
+    for i, case in enumerate(cases):
+        want, bound = oracle.attention(case["q"], case["sequences"], [1], [3000 + 500 * i], heads, kv_heads, dim, dim ** -0.5)
+        assert ((outs[i].double() - want).abs() <= bound).all()
