@@ -395,6 +395,8 @@ class QuantisedCacheOps:
                             scale, window, out, max_q_len, min_q_len, q_lens, max_ctx_len):
         device = _device()
         stream = _raw_stream(device) if self._held_stream is None else self._held_stream
+        if device != self.status.get_device():   # workspaces are on the object's device: another one's kernels may not reach them
+            raise _error(f"these kernels were made for {self.status.device}: they are called on the current device cuda:{device}")
         found = _look().attention(q, out, keys.codes, keys.scales, values.codes, values.scales, block_table, q_start, ctx_len, device,
                                   self.code, num_heads, num_kv_heads, head_dim)
         if found is None or max_q_len < 1:

@@ -88,3 +88,26 @@ def test_the_counters_made_at_first_are_enough_for_the_rule(resident):
         for pairs in range(1, 8192):
             splits, cluster = CudaOps.q8_few_row_splits(keys, pairs, resident)
             assert splits == cluster or pairs <= 4096
+
+
+def test_attention_on_another_device_than_the_object_s_is_refused(ops, monkeypatch):
+    """Tensors and current device agree, but the workspaces and the status word are on the first device."""
+    (keys, values), _rows, q, out, index = arguments()
+    table = torch.zeros(3, 8, dtype=torch.int32)
+    args = q, keys, values, table, index, index[1:], index[:3], 4, 2, 64, 0.125, None, out
+    ops.paged_attention(*args, max_q_len=1, min_q_len=1)
+    launches = ops.launches
+
+    class Elsewhere:
+        device = torch.device("cuda:1")
+
+        def get_device(self):
+            return 1
+
+        def data_ptr(self):
+            return 0
+
+    ops.status = Elsewhere()
+    with pytest.raises(KernelError, match="made for cuda:1"):
+        ops.paged_attention(*args, max_q_len=1, min_q_len=1)
+    assert ops.launches == launches
