@@ -277,26 +277,27 @@ class QuantisedCacheOps:
         # Up to 64 keys the mma.sync kernel is done before the other has set up (us, 28 heads of 128, mma.sync and tcgen05: one
         # portion of 16 tokens 5.6 and 7.4, of 64 7.3 and 9.1, four of 64 7.8 and 9.2; one of 5 tokens over 100 keys 8.9 and 8.3,
         # of 256 over 256 17.1 and 13.8, of 16 over 600 27.9 and 12.5).
-        tile_tokens, table_keys = lib.shrike_attention_q8_tc_tokens(num_heads // num_kv_heads), max_blocks * page_size
+        group, cta_rows = num_heads // num_kv_heads, lib.shrike_attention_q8_portion_rows()
+        tile_tokens, table_keys = lib.shrike_attention_q8_tc_tokens(group), max_blocks * page_size
+        tc_keys = self._keys_of_tile(table_keys, window, tile_tokens, max_q_len, 64)   # key tiles are 64 keys each, wherever a window begins
         tc_portions = bool(has_portions and tile_tokens and self.tensor_core_attention and self.dtype == torch.bfloat16
                            and page_size in (8, 16, 32, 64) and num_tokens > 0 and not short and table_keys > self.SHORT_CONTEXT)
         if has_single and has_portions and q_lens is not None:   # single tokens as portions, one launch for all
             if tc_portions:
                 tiles = sum(-(-q // tile_tokens) for q in q_lens)
-                has_single = not lib.shrike_attention_q8_tc_one_launch(tiles, sum(-(-q // tile_tokens) for q in q_lens if q > 1), num_kv_heads, table_keys)
+                has_single = not lib.shrike_attention_q8_tc_one_launch(tiles, sum(-(-q // tile_tokens) for q in q_lens if q > 1), num_kv_heads, tc_keys)
             else:
-                group, cta_rows = num_heads // num_kv_heads, lib.shrike_attention_q8_portion_rows()
                 ctas = num_kv_heads * sum(-(-q * group // cta_rows) for q in q_lens)
-                has_single = not lib.shrike_attention_q8_one_launch(self.code, ctas, table_keys, max_q_len)
-        splits, cluster, scratch, arrivals = 1, 1, None, None
-        group, few_tokens = num_heads // num_kv_heads, 1
+                has_single = not lib.shrike_attention_q8_one_launch(
+                    self.code, ctas, self._keys_of_tile(table_keys, window, self._tokens_of_rows(cta_rows, group), max_q_len), max_q_len)
+        splits, cluster, scratch, arrivals, few_tokens = 1, 1, None, None, 1
         rows = lib.shrike_attention_q8_tile_rows(group)
         if has_portions and self._few_rows_serve(lib, num_heads, num_kv_heads, table_keys, window, num_seqs, num_tokens, max_q_len, q_lens,
-                                                 tile_tokens if tc_portions else 0, has_single):
+                                                 tile_tokens if tc_portions else 0, tc_keys, has_single):
             has_single, has_portions, tc_portions, few_tokens = True, False, False, max_q_len
         if has_single:
             pairs = num_seqs * num_kv_heads * -(-group * few_tokens // rows)
-            keys = table_keys if not window else min(table_keys, abs(window) + few_tokens - 1)
+            keys = self._keys_of_tile(table_keys, window, self._tokens_of_rows(rows, group), few_tokens)
             most = lib.shrike_attention_q8_max_splits()
             splits, cluster = self.q8_splits or self.q8_few_row_splits(keys, pairs, lib.shrike_attention_q8_resident_ctas(self.code, group))
             share = rows * lib.shrike_attention_q8_row_floats() * pairs
@@ -311,7 +312,7 @@ class QuantisedCacheOps:
                 tiles = sum(-(-q // tile_tokens) for q in q_lens if q > 1 or not has_single)
             else:   # lengths that are not known: what the tokens can make at most
                 tiles = num_tokens // tile_tokens + num_seqs
-            portion_splits = self.portion_splits or lib.shrike_attention_q8_tc_splits(tiles, num_kv_heads, table_keys)
+            portion_splits = self.portion_splits or lib.shrike_attention_q8_tc_splits(tiles, num_kv_heads, tc_keys)
             each = num_tokens * num_heads * (head_dim + 2)
             portion_splits = max(1, min(portion_splits, 32, self.PORTION_SCRATCH_FLOATS // each)) if num_tokens <= 8 * 65535 else 1
             if portion_splits > 1:
@@ -323,15 +324,26 @@ class QuantisedCacheOps:
         self._q8_plans[key] = (self.generation, plan)
         return plan
 
+    @staticmethod
+    def _tokens_of_rows(rows: int, group: int) -> int:
+        """The tokens that `rows` rows belong to at most, `group` rows a token."""
+        return (rows + group - 2) // group + 1
+
+    @staticmethod
+    def _keys_of_tile(table_keys: int, window: int, tokens: int, max_q_len: int, step: int = 1) -> int:
+        """The keys that a tile of `tokens` tokens (of entries of up to `max_q_len`) can see of those that the block tables hold, in
+        steps of `step` keys: what its CTAs walk, and what is worth dealing to several of them."""
+        return table_keys if not window else min(table_keys, abs(window) + min(tokens, max_q_len) - 1 + step - 1)
+
     # In keys of the form for few rows, which a CTA's four warps share with 8 rows each: a key of the mma.sync form for many, which
     # all of them walk with 16 rows each; the tcgen05 kernel's unit of time; the least that a launch of the single tokens' own after it takes; a CTA
     # that finds nothing to do.
     Q8_MANY_ROWS_KEY, Q8_TC_UNIT, Q8_OWN_LAUNCH, Q8_EMPTY_KEYS = 5.6, 55, 400, 90
 
     def _few_rows_serve(self, lib, num_heads, num_kv_heads, table_keys, window, num_seqs, num_tokens, max_q_len, q_lens, tile_tokens,
-                        own_launch) -> bool:
+                        tc_keys, own_launch) -> bool:
         """Whether the form for few rows, which splits the keys, serves a batch with portions sooner than the tcgen05 kernel (query
-        tiles of `tile_tokens` tokens) or, where that does not serve (0), the mma.sync form for many rows, which walks the keys
+        tiles of `tile_tokens` tokens, which see `tc_keys` keys) or, where that does not serve (0), the mma.sync form for many rows, which walks the keys
         once for 64 rows.  The grid has a place for the longest entry's row tiles in every entry: the empty ones' CTAs take some
         time too.
         Measured, us, tcgen05 and few rows (28 heads of 128): 2 tokens over 100 keys 7.9 and 4.6, over 16,000 19.8 and 18.0; 5 over
@@ -347,20 +359,22 @@ class QuantisedCacheOps:
         if self.q8_few_rows is not None:
             return self.q8_few_rows
         lens = q_lens if q_lens is not None else [max_q_len] * num_seqs
-        keys = table_keys if not window else min(table_keys, abs(window) + max_q_len - 1)
+        keys = self._keys_of_tile(table_keys, window, self._tokens_of_rows(rows, group), max_q_len)
         pairs = num_kv_heads * sum(-(-q * group // rows) for q in lens)
         resident = lib.shrike_attention_q8_resident_ctas(self.code, group)
         few, splits = self.q8_few_row_time(keys, pairs, resident)
         few += self.Q8_EMPTY_KEYS * splits * (grid * num_seqs - pairs) / resident
         if tile_tokens:
             tiles = num_tokens // tile_tokens + num_seqs if q_lens is None else sum(-(-q // tile_tokens) for q in q_lens if q > 1 or not own_launch)
-            many = lib.shrike_attention_q8_tc_time(tiles, num_kv_heads, keys) * self.Q8_TC_UNIT
+            many = lib.shrike_attention_q8_tc_time(tiles, num_kv_heads, tc_keys) * self.Q8_TC_UNIT
             if own_launch:
                 singles = num_kv_heads * -(-group // rows) * sum(q == 1 for q in lens)
                 many += max(self.Q8_OWN_LAUNCH, self.q8_few_row_time(keys, singles, resident)[0])
             return few < many
-        ctas = num_kv_heads * sum(-(-q * group // lib.shrike_attention_q8_portion_rows()) for q in lens)
-        return few < max(1.0, ctas / lib.shrike_attention_q8_resident_portions(self.code)) * (keys * self.Q8_MANY_ROWS_KEY + self.Q8_START_KEYS)
+        cta_rows = lib.shrike_attention_q8_portion_rows()
+        ctas = num_kv_heads * sum(-(-q * group // cta_rows) for q in lens)
+        many_keys = self._keys_of_tile(table_keys, window, self._tokens_of_rows(cta_rows, group), max_q_len)
+        return few < max(1.0, ctas / lib.shrike_attention_q8_resident_portions(self.code)) * (many_keys * self.Q8_MANY_ROWS_KEY + self.Q8_START_KEYS)
 
     # What a CTA costs beside its keys, in keys: its start alone, with its share's way through a cluster's shared memory, and
     # with the clusters' way through global memory.

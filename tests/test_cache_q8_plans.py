@@ -7,7 +7,7 @@ import torch
 
 from shrike_b200.ops import quantised_cache
 from shrike_b200.ops.cuda_ops import CudaOps, KernelError
-from tests.test_kv_cache_int8_host import arguments, calls  # noqa: F401  (a fixture)
+from tests.test_kv_cache_int8_host import Library, arguments, calls  # noqa: F401  (a fixture)
 
 
 @pytest.fixture
@@ -111,3 +111,53 @@ def test_attention_on_another_device_than_the_object_s_is_refused(ops, monkeypat
     with pytest.raises(KernelError, match="made for cuda:1"):
         ops.paged_attention(*args, max_q_len=1, min_q_len=1)
     assert ops.launches == launches
+
+
+class Weighing(Library):
+    """A library that keeps what it was asked to weigh."""
+
+    def __init__(self, **answers):
+        super().__init__()
+        self.asked, self.answers = [], answers
+
+    def __getattr__(self, name):
+        plain = super().__getattr__(name)
+
+        def launcher(*args):
+            self.asked.append((name.replace("shrike_attention_q8_", ""), args))
+            return self.answers.get(name.replace("shrike_attention_q8_", ""), plain(*args))
+        return launcher
+
+    def keys(self, name):
+        return [args[-2] if name == "one_launch" else args[-1] for asked, args in self.asked if asked == name]
+
+
+@pytest.mark.parametrize("window", [200, -200])
+def test_windowed_portions_are_weighed_by_the_keys_that_they_see(ops, window):
+    """Not by those of the block tables: 64 tokens behind a window of 200 over 8,192 keys are no reason for many splits."""
+    lib = ops._q8_libs[64] = Weighing(tc_one_launch=0, one_launch=0, resident_ctas=592)
+    ops.q8_few_rows = None
+    q_lens = [64, 1, 1]
+    seen = 200 + 32 - 1 + 63   # a query tile of the stand-in has 32 tokens, a key tile 64 keys
+    ops.q8_plan(4, 2, 64, 3, 512, 16, 64, 1, window, 66, q_lens)
+    ops.q8_few_rows = False
+    ops.q8_plan(4, 2, 64, 3, 512, 16, 64, 1, window, 66, q_lens)
+    for name in ("tc_one_launch", "tc_time", "tc_splits"):
+        assert lib.keys(name) and set(lib.keys(name)) == {seen}, name
+    short = ops.q8_plan(4, 2, 64, 3, 512, 16, 5, 1, window, 7, [5, 1, 1])   # a tile has no more tokens than the longest entry
+    assert short.tc_portions and lib.keys("tc_splits")[-1] == 200 + 5 - 1 + 63
+    ops.tensor_core_attention = False
+    ops.q8_plan(4, 2, 64, 3, 512, 16, 64, 1, window, 66, q_lens)
+    assert lib.keys("one_launch") == [200 + 33 - 1]   # 64 rows of two heads: up to 33 tokens
+    ops.tensor_core_attention = True
+    ops.q8_plan(4, 2, 64, 3, 512, 16, 64, 1, 0, 66, q_lens)
+    ops.q8_plan(4, 2, 64, 3, 512, 16, 64, 1, 9000, 66, q_lens)
+    assert lib.keys("tc_splits")[-2:] == [8192, 8192] and lib.keys("tc_one_launch")[-2:] == [8192, 8192]
+
+
+def test_few_rows_behind_a_window_are_split_by_the_keys_that_they_see(ops):
+    ops._q8_libs[64] = Weighing(resident_ctas=592)
+    ops.q8_few_rows = True
+    for tokens in (1, 100):   # eight rows of two heads: up to five tokens
+        plan = ops.q8_plan(4, 2, 64, 1, 4096, 16, tokens, tokens, 64, tokens, [tokens])
+        assert plan.has_single and plan.splits <= 2
