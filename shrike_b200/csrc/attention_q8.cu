@@ -147,7 +147,8 @@ __device__ __forceinline__ float4 load_peer4(unsigned address) {
 }
 
 // x 2^d for d <= 0, also where 2^d is below float32's range: a sum under the least exponent F (a row whose values were all zeros
-// so far) becomes one under a large one, 2^200 smaller.  Outputs need not go that far: they are nothing beside the values that F rose for.
+// so far) becomes one under a large one, 2^200 smaller.  Outputs need not go that far: they are nothing beside the values that F
+// rose for.
 __device__ __forceinline__ float scale_sum(float x, float d) { return x * fast_exp2(fmaxf(d, -126.f)) * fast_exp2(fminf(d + 126.f, 0.f)); }
 
 // 2^e for e in [-126, 127].
@@ -385,8 +386,22 @@ struct Rows {
     // order above all finite bits)
     unsigned all_top = max(max(__float_as_uint(v_scale[0]), __float_as_uint(v_scale[1])), max(__float_as_uint(v_scale[2]), __float_as_uint(v_scale[3])));
     const bool odd_scale = all_top >= 0x7f800000u, careful = edge && __any_sync(0xffffffffu, odd_scale);
+    if (odd_scale) {
+      all_top = max(max(finite_bits(v_scale[0]), finite_bits(v_scale[1])), max(finite_bits(v_scale[2]), finite_bits(v_scale[3])));
+      // A value that is no number makes the rows that see it none: by way of their sums, since its weight may be zero in 32 bits,
+      // here or where shares are added up.
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (!(fabsf(v_scale[j]) < INFINITY)) {
+          const int key = key0 + 8 * j + key_of(g);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+              if (key >= first[nt][r] && key <= last[nt][r]) sum[nt][r] = __int_as_float(0x7fffffff);
+        }
+    }
     if (edge) all_top = 0u;
-    else if (odd_scale) all_top = max(max(finite_bits(v_scale[0]), finite_bits(v_scale[1])), max(finite_bits(v_scale[2]), finite_bits(v_scale[3])));
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       float largest[2] = {-INFINITY, -INFINITY};
@@ -419,7 +434,7 @@ struct Rows {
           exponent[nt][r] = max(exponent[nt][r], min(static_cast<int>(top[r] >> 23) - 127 - SCALE_BITS, MOST_EXPONENT));
           most[nt][r] = fmaxf(most[nt][r], largest[r]);
           const float next = most[nt][r] + static_cast<float>(exponent[nt][r]);
-          const float down = base[nt][r] == next ? 0.f : base[nt][r] - (next == -INFINITY ? 0.f : next);
+          const float down = fmaxf(base[nt][r], -1e30f) - fmaxf(next, -1e30f);   // 0 for a row that has seen no key yet
           correction[r] = fast_exp2(down);
           base[nt][r] = next;
           sum[nt][r] = scale_sum(sum[nt][r], down);
@@ -438,17 +453,6 @@ struct Rows {
           p[j][r] = fast_exp2(fmaf(s[nt][j >> 1][2 * (j & 1) + r], factor[nt][r], -from));
           sum[nt][r] += p[j][r];
         }
-      }
-      // A value that is no number makes the rows that see it none: by way of their sums, since its weight may be zero in 32 bits,
-      // here or where shares are added up.
-      if (odd_scale) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            const int key = key0 + 8 * j + key_of(g);
-            if (!(fabsf(v_scale[j]) < INFINITY) && key >= first[nt][r] && key <= last[nt][r]) sum[nt][r] = __int_as_float(0x7fffffff);
-          }
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -516,6 +520,25 @@ struct Rows {
 #pragma unroll
         for (int offset = 4; offset < 32; offset <<= 1) sum[nt][r] += __shfl_xor_sync(0xffffffffu, sum[nt][r], offset);
   }
+  // Rows that others are added to: half of F leaves the base.  Bases of rows with equally large scores are then within 2^100 of one
+  // another, whatever their values' sizes, and the sum of one whose values are all zeros is not lost beside another's.
+  __device__ __forceinline__ void meet() {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      float factor[2];
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const int half = exponent[nt][r] / 2;
+        factor[r] = power_of_two(half);
+        base[nt][r] -= static_cast<float>(half);
+        sum[nt][r] *= factor[r];
+      }
+#pragma unroll
+      for (int i = 0; i < BLOCKS_V * 2; ++i)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) o[nt][i][c] *= factor[c & 1];
+    }
+  }
 };
 
 // Which entry this is, and whether it is this launch's.
@@ -531,8 +554,8 @@ __device__ __forceinline__ bool entry_of(const Args& args, int seq, int& start, 
 __device__ __forceinline__ void add_share(float m, float l, const float4& v, float base, float& total, float (&acc)[4]) {
   const float weight = m == -INFINITY ? 0.f : fast_exp2(m - base);
   if (l != l) total = l;   // a score or a value that is no number: the row is none either, whatever the others hold
-  if (m != -INFINITY) total += scale_sum(l, m - base);
   if (weight == 0.f) return;
+  total += l * weight;
   acc[0] += v.x * weight; acc[1] += v.y * weight; acc[2] += v.z * weight; acc[3] += v.w * weight;
 }
 __device__ __forceinline__ void leave_share(float* share, int rows, int row, int element, float base, float total, const float (&acc)[4]) {
@@ -634,6 +657,7 @@ split_keys_kernel(const Args args) {
   }
   copies_wait<0>();
   r.finish();
+  r.meet();
   __syncthreads();
   // the warps' rows meet: [warp][ROWS][D + 4] (four more, so that the stores of a quad fall into different banks), and
   // [warp][ROWS][base, sum]
@@ -729,7 +753,7 @@ split_keys_kernel(const Args args) {
 #pragma unroll
       for (int c = 0; c < 8; ++c) next = fmaxf(next, ml[c].x);
       const float down = base == -INFINITY ? 0.f : fast_exp2(base - next);
-      total = base == -INFINITY ? total : scale_sum(total, base - next);
+      total *= down;
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[e] *= down;
       base = next;

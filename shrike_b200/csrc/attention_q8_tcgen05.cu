@@ -62,6 +62,7 @@ constexpr unsigned CHAIN_COLS = 256, P_COL = 64, O_COL = 128, TMEM_COLS = 512;  
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr int LEAST_EXPONENT = -93, MOST_EXPONENT = 107, SCALE_BITS = 8;   // as in attention_q8.cu
 constexpr float BASE_LAG = 6.0f;
+constexpr int NOT_FINITE = 4096;   // above any exponent
 
 enum : int { ERR_PRODUCER = 61, ERR_CONVERT = 62, ERR_MMA = 63, ERR_SOFTMAX = 64, ERR_DRAIN = 65, ERR_ALIGNMENT = 66 };
 
@@ -206,7 +207,7 @@ __device__ __forceinline__ Work find_work(const Args& args, int work, int rows) 
 
 struct Shared {
   float k_scale[STAGES][KEYS], v_scale[STAGES][KEYS];
-  int4 v_info[STAGES];   // x, y: of each 32 keys the exponent of the largest value scale; z, w: whether one of them is no finite number
+  int4 v_top[STAGES];   // of each 32 keys the exponent of the largest value scale: x, y with NOT_FINITE added where one is no finite number; z, w
   unsigned long long q_full, q_ready[2], s_full[2], s_read[2], p_full[2][2], pv_done[2][2], pv_last[2], stagger;
   unsigned long long raw_k_full[RAW_STAGES], raw_k_free[RAW_STAGES], raw_v_full[RAW_STAGES], raw_v_free[RAW_STAGES];
   unsigned long long k_full[STAGES], k_free[STAGES], v_full[STAGES], v_free[STAGES];
@@ -255,6 +256,19 @@ __device__ __noinline__ void rescale_output_rows(unsigned tmem_o, float upper, f
     for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * ((j & 2) ? lower : upper));
     tmem_store_fragments(tmem_o + c, o);
   }
+}
+
+// Which of two rows see a value that is no finite number among 16 keys of a step: bits 0 and 1.  `key`: the first of them, two side by
+// side of every eight.  Rare, and out of the loop's code.
+__device__ __noinline__ unsigned rows_of_no_number(const float* v_scale, int key, int first_0, int last_0, int first_1, int last_1) {
+  unsigned rows = 0u;
+#pragma unroll 1
+  for (int i = 0; i < 16; ++i) {
+    const int within = 8 * (i >> 1) + (i & 1), at = key + within;
+    if (fabsf(v_scale[within]) < INFINITY) continue;
+    rows |= (at >= first_0 && at <= last_0 ? 1u : 0u) | (at >= first_1 && at <= last_1 ? 2u : 0u);
+  }
+  return rows;
 }
 
 // A converting thread's share: 16-byte chunks first ... first + COUNT - 1 of its key's codes, and the float16 they become.
@@ -523,9 +537,9 @@ portions_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         const unsigned top = __reduce_max_sync(0xffffffffu, finite_bits(v_scale));
         const bool bad = __any_sync(0xffffffffu, !(fabsf(v_scale) < INFINITY));
         if (lane == 0) {
-          int* info = reinterpret_cast<int*>(&sh->v_info[st]) + (row >> 5);
-          info[0] = static_cast<int>(top >> 23) - 127;
-          info[2] = bad ? 1 : 0;
+          int* tops = reinterpret_cast<int*>(&sh->v_top[st]) + (row >> 5);
+          tops[0] = static_cast<int>(top >> 23) - 127 + (bad ? NOT_FINITE : 0);
+          tops[2] = static_cast<int>(top >> 23) - 127;
         }
         k_scale = next_k;
         v_scale = next_v;
@@ -619,8 +633,9 @@ portions_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       fence_after_sync();
       tmem_load_fragments(tmem_chain, v);
       int top[2];
-      const int4 info = sh->v_info[st];
-      top[0] = top[1] = max(info.x, info.y);
+      const int2 tops = *reinterpret_cast<const int2*>(&sh->v_top[st]);
+      const int tile_top = max(tops.x, tops.y);
+      top[0] = top[1] = tile_top;
       float2 scale[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) scale[j] = *reinterpret_cast<const float2*>(sh->k_scale[st] + 8 * j + 2 * t);   // while the scores come
@@ -663,6 +678,7 @@ portions_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       bool rescales = false;
       float correction[2] = {1.0f, 1.0f};
       if (__builtin_expect(__any_sync(0xffffffffu, moves), 0)) {
+        if (tile_top >= NOT_FINITE / 2 && !edge) top[0] = top[1] = max(sh->v_top[st].z, sh->v_top[st].w) - SCALE_BITS;
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
 #pragma unroll
@@ -677,7 +693,7 @@ portions_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
           const float base_was = base[r];
           correction[r] = base_was == -INFINITY ? 1.0f : fast_exp2(base_was - next);
           base[r] = next;
-          row_sum[r] = base_was == -INFINITY ? row_sum[r] : scale_sum(row_sum[r], base_was - next);
+          row_sum[r] = scale_sum(row_sum[r], fmaxf(base_was, -1e30f) - fmaxf(next, -1e30f));
         }
         rescales = h > 0 && __any_sync(0xffffffffu, correction[0] != 1.0f || correction[1] != 1.0f);
       }
@@ -713,7 +729,7 @@ portions_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
           weights[2 * j + r] = pack_half(w0, w1);
         }
       }
-      if (__builtin_expect((info.z | info.w) != 0, 0)) {   // rare: a value that is no number
+      if (__builtin_expect(tile_top >= NOT_FINITE / 2, 0)) {   // rare: a value that is no number
         // A key that a row does not see has no part in it, not even a scale of NaN.
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
@@ -722,13 +738,9 @@ portions_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
           if (key + 1 < first[i & 1] || key + 1 > last[i & 1]) weights[i] &= 0x0000ffffu;
         }
         // The rows that see it are none either: by way of their sums, since its weight may be zero where splits are added up.
-#pragma unroll 1
-        for (int i = 0; i < 16; ++i) {
-          const int within = 8 * (i >> 1) + (i & 1), key = key_base + 2 * t + within;
-          if (fabsf(v_scale[within]) < INFINITY) continue;
-          if (key >= first[0] && key <= last[0]) row_sum[0] = __int_as_float(0x7fffffff);
-          if (key >= first[1] && key <= last[1]) row_sum[1] = __int_as_float(0x7fffffff);
-        }
+        const unsigned none = rows_of_no_number(v_scale, key_base + 2 * t, first[0], last[0], first[1], last[1]);
+        if (none & 1u) row_sum[0] = __int_as_float(0x7fffffff);
+        if (none & 2u) row_sum[1] = __int_as_float(0x7fffffff);
       }
       // P(h) goes where P(h - 2) was.  The product that read that was issued before the scores of step h, and a commit waits for
       // everything its thread has issued: s_full(h) says that it has been read.
