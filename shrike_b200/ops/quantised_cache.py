@@ -282,6 +282,9 @@ class QuantisedCacheOps:
         tc_keys = self._keys_of_tile(table_keys, window, tile_tokens, max_q_len, 64)   # key tiles are 64 keys each, wherever a window begins
         tc_portions = bool(has_portions and tile_tokens and self.tensor_core_attention and self.dtype == torch.bfloat16
                            and page_size in (8, 16, 32, 64) and num_tokens > 0 and not short and table_keys > self.SHORT_CONTEXT)
+        if tc_portions:   # no more query tiles than a grid takes, and rows that 32 bits count: the other form has no such limits
+            tiles = num_tokens // tile_tokens + num_seqs if q_lens is None else sum(-(-q // tile_tokens) for q in q_lens if q > 1 or not has_single)
+            tc_portions = tiles <= 65535 and num_tokens * num_heads <= 0x7FFFFFFF
         if has_single and has_portions and q_lens is not None:   # single tokens as portions, one launch for all
             if tc_portions:
                 tiles = sum(-(-q // tile_tokens) for q in q_lens)

@@ -161,3 +161,15 @@ def test_few_rows_behind_a_window_are_split_by_the_keys_that_they_see(ops):
     for tokens in (1, 100):   # eight rows of two heads: up to five tokens
         plan = ops.q8_plan(4, 2, 64, 1, 4096, 16, tokens, tokens, 64, tokens, [tokens])
         assert plan.has_single and plan.splits <= 2
+
+
+def test_more_query_tiles_than_a_grid_takes_go_to_the_other_form(ops):
+    """The stand-in's tiles have 32 tokens: 65,535 of them are served, one more would be refused."""
+    most = 65535 * 32
+    for tokens, tc in ((most, True), (most + 1, False)):
+        for q_lens in ([tokens], [tokens, 1]):
+            plan = ops.q8_plan(4, 2, 64, len(q_lens), 1 << 18, 16, tokens, min(q_lens), 0, sum(q_lens), q_lens)
+            assert plan.tc_portions == tc and plan.has_portions
+    assert not ops.q8_plan(4, 2, 64, 2, 1 << 18, 16, most, 1, 0, most + 1, None).tc_portions   # what unknown lengths may make
+    ops._q8_libs[64] = Weighing(tc_tokens=256)
+    assert not ops.q8_plan(256, 256, 64, 1, 1 << 20, 16, 1 << 23, 1 << 23, 0, 1 << 23, [1 << 23]).tc_portions   # 2^31 rows
