@@ -162,15 +162,16 @@ struct Place {
   long long scale;
 };
 // The page of a key, -1 if the key lies behind `last_key`: to be asked for a step before its place is formed, since the answer
-// takes as long as a quarter of a step.
-__device__ __forceinline__ int page_of(const Args& args, const int* table, int key, int last_key) {
-  const int block = args.page_shift >= 0 ? key >> args.page_shift : key / args.page_size;
-  return key <= last_key && block < args.max_blocks ? table[block] : -1;
+// takes as long as a quarter of a step.  A context near 2^31, which no table holds, makes steps whose keys pass 32 bits: as
+// unsigned numbers they lie behind every table.
+__device__ __forceinline__ int page_of(const Args& args, const int* table, unsigned key, int last_key) {
+  const unsigned block = args.page_shift >= 0 ? key >> args.page_shift : key / static_cast<unsigned>(args.page_size);
+  return static_cast<int>(key) <= last_key && block < static_cast<unsigned>(args.max_blocks) ? table[block] : -1;
 }
 // The key's place, given its page; nowhere if that is not one of the pool's.
-__device__ __forceinline__ Place place_of(const Args& args, int page, int kv_head, int key) {
+__device__ __forceinline__ Place place_of(const Args& args, int page, int kv_head, unsigned key) {
   Place at{0, false, 0};
-  const int within = args.page_shift >= 0 ? key & (args.page_size - 1) : key % args.page_size;
+  const int within = static_cast<int>(args.page_shift >= 0 ? key & (args.page_size - 1) : key % static_cast<unsigned>(args.page_size));
   if (page >= 0 && page < args.num_pages) {
     at.row = page * args.page_size + within;
     at.there = true;
@@ -616,8 +617,8 @@ split_keys_kernel(const Args args) {
   R r;
   // this warp's steps: mine_lo + warp, + WARPS, ...
   const int begin = mine_lo + warp;
-  auto page_at = [&](int step) { return page_of(args, table, step * KEYS + lane, step < mine_hi ? last_key : -1); };
-  auto place_at = [&](int page, int step) { return place_of(args, page, kv_head, step * KEYS + lane); };
+  auto page_at = [&](int step) { return page_of(args, table, static_cast<unsigned>(step) * KEYS + lane, step < mine_hi ? last_key : -1); };
+  auto place_at = [&](int page, int step) { return place_of(args, page, kv_head, static_cast<unsigned>(step) * KEYS + lane); };
   int page = page_at(begin), next_page = page_at(begin + WARPS), ahead = page_at(begin + 2 * WARPS);
   wait_for_previous();   // the query and the newest keys come from the kernel before this one
   Place place = place_at(page, begin), next = place_at(next_page, begin + WARPS);
@@ -805,8 +806,8 @@ portion_rows_kernel(const Args args) {
     load_scales(args, place, to + 2 * TILE, threadIdx.x);
   };
   R r;
-  auto page_at = [&](int step) { return page_of(args, table, step * KEYS + lane, last_key); };
-  auto place_at = [&](int page, int step) { return place_of(args, page, kv_head, step * KEYS + lane); };
+  auto page_at = [&](int step) { return page_of(args, table, static_cast<unsigned>(step) * KEYS + lane, last_key); };
+  auto place_at = [&](int page, int step) { return place_of(args, page, kv_head, static_cast<unsigned>(step) * KEYS + lane); };
   int page = page_at(step_lo), ahead = page_at(step_lo + 1);
   wait_for_previous();
   if (step_lo < step_hi) load_step(place_at(page, step_lo), ring_at);
@@ -961,6 +962,7 @@ SHRIKE_API int shrike_paged_attention_q8(const ShrikeAttentionQ8* call) {
   if (num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads || num_kv_heads > 65535 || max_blocks <= 0 || page_size <= 0 ||
       num_pages <= 0 || static_cast<long long>(num_pages) * page_size > 0x7fffffff ||
       static_cast<long long>(max_blocks) * page_size > 0x7fffffff - 4096 || max_q_len < 1 || num_seqs > 65535 || splits < 1 ||
+      static_cast<long long>(max_q_len) * (num_heads / num_kv_heads) > 0x7fffffff - 4096 ||
       cluster < 1 || cluster > 8 || splits % cluster || splits > attnq8::MAX_SPLITS ||
       (splits > cluster && (scratch == nullptr || arrivals == nullptr)) ||
       (reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(k_codes) |

@@ -356,15 +356,15 @@ portions_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
   // The first page ids (metadata): the loaders' a chunk of 32 at a time (lane l: page l of the chunk, several tiles' worth), the
   // converting threads' their own key's.
   const int* table = args.block_table + static_cast<size_t>(seq) * args.max_blocks;
-  auto page_of = [&](int key) -> int {   // of a key that some row sees; -1 for one that none does
-    const int block = key >> args.page_shift;
-    return key <= hi && block < args.max_blocks ? table[block] : -1;
+  auto page_of = [&](unsigned key) -> int {   // of a key that some row sees; -1 for one that none does, or that passes 32 bits
+    const unsigned block = key >> args.page_shift;
+    return static_cast<int>(key) <= hi && block < static_cast<unsigned>(args.max_blocks) ? table[block] : -1;
   };
   const int pages_per_tile = KEYS >> args.page_shift, tiles_per_chunk = 32 / pages_per_tile;
   auto load_chunk = [&](int chunk) -> int {
-    return chunk * tiles_per_chunk < num_tiles ? page_of(tile_lo * KEYS + ((chunk * 32 + lane) << args.page_shift)) : -1;
+    return chunk * tiles_per_chunk < num_tiles ? page_of(static_cast<unsigned>(tile_lo) * KEYS + (static_cast<unsigned>(chunk * 32 + lane) << args.page_shift)) : -1;
   };
-  auto load_page = [&](int i, int row) -> int { return i < num_tiles ? page_of((tile_lo + i) * KEYS + row) : -1; };
+  auto load_page = [&](int i, int row) -> int { return i < num_tiles ? page_of(static_cast<unsigned>(tile_lo + i) * KEYS + row) : -1; };
   const bool scales = warp == 24 || warp == 25;   // the converting warps that bring the tiles' scales
   int chunk_pages = -1, next_pages = -1;          // chunks 0 and 1, or this thread's pages of tiles 0 and 1
   if (warp == 0 || warp == 3) {

@@ -247,3 +247,23 @@ def test_the_first_call_of_all_may_be_a_captured_one():
     for i, case in enumerate(cases):
         want, bound = oracle.attention(case["q"], case["sequences"], [1], [3000 + 500 * i], heads, kv_heads, dim, dim ** -0.5)
         assert ((outs[i].double() - want).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("dtype,dim,tensor_cores", FORMS)
+@pytest.mark.parametrize("few_rows", [False, True])
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("options", [{"window": 64}, {"chunk": 96}])
+def test_a_context_that_no_table_holds(dtype, dim, tensor_cores, few_rows, new, options):
+    """Keys near 2^31 have no page: the rows that see nothing else are zeros, and the other sequences' are what they are without."""
+    heads, kv_heads, page = 4, 2, 16
+    q_lens, ctx_lens = [new, new, 1], [300, new, 90]
+    ops = cuda_ops(dtype)
+    ops.tensor_core_attention, ops.portion_splits, ops.q8_splits, ops.q8_few_rows = tensor_cores, 2, (2, 2), few_rows
+    case = oracle.pages_case(heads, kv_heads, dim, page, q_lens, ctx_lens, dtype, 24, DEV)
+    plain = attend(ops, case, heads, kv_heads, dim, q_lens, ctx_lens, **options)
+    case["ctx_len"][1] = 2 ** 31 - 1
+    got = attend(ops, case, heads, kv_heads, dim, q_lens, ctx_lens, **options)
+    torch.cuda.synchronize()
+    assert (got[new: 2 * new] == 0).all()
+    assert torch.equal(got[:new], plain[:new]) and torch.equal(got[2 * new:], plain[2 * new:])
+    ops.check_status()
