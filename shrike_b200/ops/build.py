@@ -189,13 +189,17 @@ def attention_q8_library(head_dim: int) -> ctypes.CDLL:
     return load_library(f"shrike_attention_q8_d{head_dim}", ATTENTION_Q8_SOURCES, {"SHRIKE_HEAD_DIM": head_dim})
 
 
-def _tensor_look_path() -> Path:
+def _tensor_look_path() -> Path | None:
+    """None: Python's or torch's headers are not there."""
     import re
     import sysconfig
 
     import torch
 
     torch_dir = Path(torch.__file__).resolve().parent
+    if not all(header.is_file() for header in (Path(sysconfig.get_paths()["include"]) / "Python.h",
+                                               torch_dir / "include" / "torch" / "csrc" / "autograd" / "python_variable.h")):
+        return None
     built_for = re.sub(r"\W", "_", f"{torch.__version__}_{sys.implementation.cache_tag}")
     flags = [f"-DSHRIKE_BUILT_FOR={built_for}", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", f"-I{torch_dir / 'include'}",
              f"-I{torch_dir / 'include' / 'torch' / 'csrc' / 'api' / 'include'}", f"-I{sysconfig.get_paths()['include']}",
@@ -205,8 +209,11 @@ def _tensor_look_path() -> Path:
 
 @functools.lru_cache(maxsize=None)
 def tensor_look():
-    """The Python module of `tensor_look.cpp`."""
-    spec = importlib.util.spec_from_file_location("shrike_tensor_look", _tensor_look_path())
+    """The Python module of `tensor_look.cpp`; None where it cannot be built."""
+    path = _tensor_look_path()
+    if path is None:
+        return None
+    spec = importlib.util.spec_from_file_location("shrike_tensor_look", path)
     module = importlib.util.module_from_spec(spec)
     spec.loader.exec_module(module)
     return module
@@ -227,8 +234,10 @@ def decode_step_library() -> ctypes.CDLL:
 def build_all(head_dims=(16, 32, 48, 64, 128, 256)) -> list[Path]:
     """Everything the package can load, for the usual head sizes."""
     built = [compile_library("shrike_core", CORE_SOURCES), compile_library("shrike_gemm_tcgen05", ["gemm_tcgen05.cu"]),
-             compile_library("shrike_layer_program", ["layer_program.cu"]), compile_library("shrike_decode_step", ["decode_step.cu"]),
-             _tensor_look_path()]
+             compile_library("shrike_layer_program", ["layer_program.cu"]), compile_library("shrike_decode_step", ["decode_step.cu"])]
+    look = _tensor_look_path()
+    if look is not None:   # a Python module against torch's headers: the calls over 8-bit pages do without it, at 3 us more each
+        built.append(look)
     for head_dim in head_dims:
         built.append(compile_library(f"shrike_attention_d{head_dim}", ATTENTION_SOURCES,
                                      {"SHRIKE_HEAD_DIM": head_dim}))

@@ -25,7 +25,9 @@ DTYPE_CODE = {torch.float32: 0, torch.bfloat16: 1}
 # ctypes two microseconds, this a third of one.
 _ATTENTION_CALL = struct.Struct("=14Q16if")
 _pack_attention = _ATTENTION_CALL.pack
+_CACHE_CALL = struct.Struct("=8Q2q6i")
 _INT32 = torch.int32
+_DTYPES = {code: dtype for dtype, code in DTYPE_CODE.items()}
 _device = getattr(torch._C, "_cuda_getDevice", None)          # the current device's number, and its current stream's handle:
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)   # asking torch for the objects costs more than a launch
 _capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", None)
@@ -49,10 +51,73 @@ class QuantisedPlan:
     launches: int = 0
 
 
+class PlainLook:
+    """What `tensor_look.cpp` answers, asked from Python: for where that cannot be built (no headers of Python or torch)."""
+
+    @staticmethod
+    def _tensors(*tensors) -> bool:
+        return all(isinstance(x, torch.Tensor) for x in tensors)
+
+    @staticmethod
+    def _ints(tensor, count, device) -> bool:
+        return tensor.get_device() == device and not tensor.is_meta and tensor.dtype is _INT32 and tensor.numel() == count and tensor.is_contiguous()
+
+    @staticmethod
+    def _both_fit(keys, values, device) -> bool:
+        if keys.dim() != 4 or keys.shape != values.shape or any(x.get_device() != device or x.is_meta or x.data_ptr() % 16 for x in (keys, values)):
+            return False
+        pages, page_size, _heads, dim = keys.shape
+        return dim % 16 == 0 and 16 <= dim <= MOST_HEAD_DIM and pages * page_size <= 0x7FFFFFFF
+
+    @staticmethod
+    def _rows(x, dtype, n, width, device) -> bool:
+        return (x.shape == (n, width) and x.dtype is dtype and x.get_device() == device and not x.is_meta and (width <= 1 or x.stride(1) == 1)
+                and (n <= 1 or x.stride(0) >= 0))
+
+    @classmethod
+    def pages(cls, codes, scales):
+        return quantised_pages._look_here(codes, scales) if cls._tensors(codes, scales) else None
+
+    @classmethod
+    def cache(cls, k, v, key_codes, key_scales, value_codes, value_scales, slots, device, code, stream, stores):
+        """The launcher's arguments (`ShrikeCacheQ8`), empty for no rows."""
+        if (not cls._tensors(k, v, key_codes, key_scales, value_codes, value_scales, slots)
+                or not cls._both_fit(key_codes, value_codes, device) or k.dim() != 2):
+            return None
+        pages, page_size, heads, dim = key_codes.shape
+        n, width, dtype = k.shape[0] if stores else slots.numel(), heads * dim, _DTYPES[code]
+        if not cls._ints(slots, n, device) or not all(cls._rows(x, dtype, n, width, device) for x in (k, v)) or n > 0x7FFFFFFF:
+            return None
+        if not stores and not all(x.is_contiguous() and x.data_ptr() % 16 == 0 for x in (k, v)):
+            return None
+        if n == 0:
+            return b""
+        return _CACHE_CALL.pack(*(x.data_ptr() for x in (k, v, key_codes, value_codes, key_scales, value_scales, slots)), stream,
+                                *(x.stride(0) if n > 1 else width for x in (k, v)), code, n, heads, dim, pages, page_size)
+
+    @classmethod
+    def attention(cls, q, out, key_codes, key_scales, value_codes, value_scales, table, starts, context, device, code, heads, kv_heads, dim):
+        """(tokens, sequences, blocks a sequence, out's address, (the addresses that a launch begins with))."""
+        if not cls._tensors(q, out, key_codes, key_scales, value_codes, value_scales, table, starts, context):
+            return None
+        if (not cls._both_fit(key_codes, value_codes, device) or key_codes.shape[2:] != (kv_heads, dim) or kv_heads <= 0 or heads <= 0
+                or heads % kv_heads or q.dim() != 2 or q.shape[1] != heads * dim or q.shape != out.shape or table.dim() != 2):
+            return None
+        if any(x.dtype is not _DTYPES[code] or x.get_device() != device or x.is_meta or not x.is_contiguous() or x.data_ptr() % 16 for x in (q, out)):
+            return None
+        sequences = table.shape[0]
+        if not (cls._ints(table, table.numel(), device) and cls._ints(starts, sequences + 1, device) and cls._ints(context, sequences, device)):
+            return None
+        return (q.shape[0], sequences, table.shape[1], out.data_ptr(),
+                tuple(x.data_ptr() for x in (q, key_codes, key_scales, value_codes, value_scales, table, starts, context)))
+
+
 @functools.lru_cache(maxsize=None)
 def _look():
     """The native module, which pages made from now on use too."""
     module = build.tensor_look()
+    if module is None:
+        return PlainLook
     quantised_pages.look_pages = module.pages
     return module
 
