@@ -2,6 +2,7 @@
 // than to launch.
 #pragma once
 #include <cuda_runtime.h>
+#include <stddef.h>
 
 struct ShrikeAttentionQ8 {
   const void* q;
@@ -24,3 +25,5 @@ struct ShrikeAttentionQ8 {
   int splits, cluster, tiles;
   float scale;
 };
+// As the caller packs them: fourteen addresses, sixteen 32-bit integers and a 32-bit number side by side.
+static_assert(offsetof(ShrikeAttentionQ8, max_blocks) == 14 * 8 && offsetof(ShrikeAttentionQ8, scale) == 14 * 8 + 16 * 4, "packed");

@@ -4,6 +4,7 @@
 // scale s = a / 127 (rounded once): x_i is about c_i s.  A row of zeros has scale 0; a row that holds an infinity or a NaN has
 // scale NaN and codes 0, so that whatever reads it gets NaN and nothing else.  Pages: codes int8 [pages, page size, kv heads,
 // D], scales float32 [pages, kv heads, page size]: the attention reads the scales of one head, and a page's lie together.
+#include "cache_q8_call.cuh"
 #include "codes_q8.cuh"
 #include "common.cuh"
 
@@ -265,21 +266,13 @@ static bool good_pages(const void* codes, const void* scales) {
 
 using namespace cacheq8;
 
-// The arguments of a store or a reading back, packed by the caller (a call with a dozen arguments costs more to make than the
-// kernel takes for a token): rows k and v, `k_stride` / `v_stride` elements apart where they are stored, dense where they are read.
-struct ShrikeCacheQ8 {
-  void *k, *v, *k_codes, *v_codes;
-  float *k_scales, *v_scales;
-  const int* slots;
-  cudaStream_t stream;
-  long long k_stride, v_stride;
-  int dtype, n, kv_heads, dim, pages, page_size;
-};
-
 // Stores n rows of kv_heads * dim elements of `dtype`.  Rows whose slot is not one of the pool's are left out; the others' slots
 // have to differ from one another.
 SHRIKE_API int shrike_kv_write_q8(const ShrikeCacheQ8* call) {
-  const auto [k_new, v_new, k_codes, v_codes, k_scales, v_scales, slots, stream, k_stride, v_stride, dtype, n, kv_heads, dim, pages, page_size] = *call;
+  const auto [k_new, v_new, k_codes, v_codes, k_scale_at, v_scale_at, slot_at, stream_at, k_stride, v_stride, dtype, n, kv_heads, dim, pages, page_size] = *call;
+  float *const k_scales = static_cast<float*>(k_scale_at), *const v_scales = static_cast<float*>(v_scale_at);
+  const int* const slots = static_cast<const int*>(slot_at);
+  const cudaStream_t stream = static_cast<cudaStream_t>(stream_at);
   const long long num_slots = static_cast<long long>(pages) * page_size;
   if (n <= 0) return SHRIKE_OK;
   if (kv_heads <= 0 || dim <= 0 || dim % 16 || dim > 256 || page_size <= 0 || !good_pages(k_codes, k_scales) ||
@@ -333,7 +326,10 @@ SHRIKE_API int shrike_rope_kv_write_q8(const float* qkv, const float* bias, cons
 // Reads n rows of kv_heads * dim elements of `dtype` back to k and v, 16-byte aligned and dense; rows whose slot is not one of
 // the pool's become zeros.
 SHRIKE_API int shrike_kv_read_q8(const ShrikeCacheQ8* call) {
-  const auto [k_out, v_out, k_codes, v_codes, k_scales, v_scales, slots, stream, k_stride, v_stride, dtype, n, kv_heads, dim, pages, page_size] = *call;
+  const auto [k_out, v_out, k_codes, v_codes, k_scale_at, v_scale_at, slot_at, stream_at, k_stride, v_stride, dtype, n, kv_heads, dim, pages, page_size] = *call;
+  float *const k_scales = static_cast<float*>(k_scale_at), *const v_scales = static_cast<float*>(v_scale_at);
+  const int* const slots = static_cast<const int*>(slot_at);
+  const cudaStream_t stream = static_cast<cudaStream_t>(stream_at);
   const long long num_slots = static_cast<long long>(pages) * page_size;
   if (n <= 0) return SHRIKE_OK;
   if (kv_heads <= 0 || dim <= 0 || dim % 16 || page_size <= 0 || !good_pages(k_codes, k_scales) || !good_pages(v_codes, v_scales) ||

@@ -7,18 +7,11 @@
 
 #include <torch/csrc/autograd/python_variable.h>
 
+#include "cache_q8_call.cuh"
+
 namespace {
 
 constexpr int MOST_HEAD_DIM = 256;
-
-// The launchers' arguments, as cache_q8.cu declares them.
-struct ShrikeCacheQ8 {
-  const void *k, *v, *k_codes, *v_codes, *k_scales, *v_scales, *slots;
-  unsigned long long stream;
-  long long k_stride, v_stride;
-  int dtype, n, kv_heads, dim, pages, page_size;
-};
-static_assert(sizeof(ShrikeCacheQ8) == 104, "the launcher's structure");
 
 const at::Tensor* tensor_of(PyObject* x) { return THPVariable_Check(x) ? &THPVariable_Unpack(x) : nullptr; }
 long long device_of(const at::Tensor& t) { return t.is_cuda() ? t.get_device() : t.is_cpu() ? -1 : -2; }
@@ -97,7 +90,7 @@ PyObject* look_cache(PyObject*, PyObject* const* args, Py_ssize_t count) {
     if (!stores && !(k.is_contiguous() && v.is_contiguous() && on_16_bytes(k) && on_16_bytes(v))) Py_RETURN_NONE;
     if (n == 0) return PyBytes_FromStringAndSize(nullptr, 0);
     const ShrikeCacheQ8 call{k.data_ptr(), v.data_ptr(), codes.data_ptr(), value_codes.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(),
-                             slots.data_ptr(), x[2], n > 1 ? k.stride(0) : width, n > 1 ? v.stride(0) : width, static_cast<int>(x[1]),
+                             slots.data_ptr(), reinterpret_cast<void*>(static_cast<uintptr_t>(x[2])), n > 1 ? k.stride(0) : width, n > 1 ? v.stride(0) : width, static_cast<int>(x[1]),
                              static_cast<int>(n), static_cast<int>(codes.size(2)), static_cast<int>(codes.size(3)), static_cast<int>(codes.size(0)),
                              static_cast<int>(codes.size(1))};
     return PyBytes_FromStringAndSize(reinterpret_cast<const char*>(&call), sizeof(call));

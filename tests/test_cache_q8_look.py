@@ -90,3 +90,7 @@ def test_everything_else_is_built_without_the_headers(without_headers, monkeypat
     monkeypatch.setattr(build, "compile_library", lambda name, *args, **options: built.append(name))
     build.build_all((64,))
     assert "shrike_core" in built and "shrike_attention_q8_d64" in built and "shrike_tensor_look" not in built
+
+
+def test_the_calls_are_packed_as_the_launchers_declare_them():
+    assert quantised_cache._CACHE_CALL.size == 104 and quantised_cache._ATTENTION_CALL.size == 14 * 8 + 17 * 4   # asserted beside the structures too
