@@ -156,6 +156,7 @@ class QuantisedCacheOps:
         self._q8_libs, self._q8_plans = {}, {}
         self._q8_scratch = self._q8_portion_scratch = None
         self._q8_arrivals = torch.zeros(4096, dtype=_INT32, device=self.device)   # more than the rule for splits ever asks for
+        torch.cuda.current_stream(self.device).synchronize()   # zeros before the first call, whichever stream that is on
         self.q8_few_rows = None   # None: the rule of `_few_rows_serve`; whether the form for few rows takes portions (tests)
         self.q8_splits = None   # None: the rule of `q8_few_row_splits`; (splits, cluster) for few rows (tests)
 
