@@ -5,7 +5,8 @@
 // Codes are integers up to 127: exact in float16.  Both products run on mma.sync m16n8k16 with float16 operands and 32-bit
 // sums, and nothing but the queries and the weights is ever rounded:
 //   queries   scaled by a power of two per row (largest magnitude in [2^14, 2^15)); bfloat16 queries are then exact, float32
-//             ones are split in two float16 parts (22 bits) whose products are added in the accumulator
+//             ones are split in two float16 parts (22 bits) whose products are added in the accumulator.  A score leaves
+//             float32's range, and its row is NaN, where keys are of 2^105 (4e31) and more: (q . c) s^k with q of 2^15
 //   weights   w_j = p_j s^v_j.  The base m of the exponentials is a row's largest score (it may lag by up to 2^6) plus an
 //             exponent F that puts the largest value scale the row has seen at 2^8 ... 2^9 (the sums and the outputs are all in
 //             units of 2^m, so F costs nothing): float16 then keeps 11 bits of a weight down to 2^-22 of the largest possible
@@ -24,8 +25,9 @@
 // Two forms.  Few rows (single tokens, and small portions, eight or sixteen rows a tile): the rows' keys are dealt to `splits` CTAs and to each CTA's four warps, each with its
 // own ring of cp.async copies (no barrier in the loop); the warps' results meet in shared memory, those of up to eight CTAs in
 // the shared memory of their cluster, and the clusters' in global memory, where the last CTA to arrive adds them up in order.
-// Bound by memory at many keys (64 sequences of 4,096 keys, 40 heads of 128: 85 us, 5.0 TB/s; with the products left out the
-// copies alone take 71), and by the chain metadata, page, codes, products, merges at few (one sequence of 517 keys: 5.5 us).
+// Bound by memory at many keys (64 sequences of 4,096 keys, 40 heads of 128: 85 us, 5.0 TB/s, with warm caches, where with the
+// products left out the copies alone take 71; 95 us, 4.5 TB/s, where every pass finds other data), and by the chain metadata,
+// page, codes, products, merges at few (one sequence of 517 keys: 5.6 us).
 // Metadata and pages are looked up while the kernel before still runs (that sequence: 6.1 us without).  Many rows (portions):
 // four warps of 8 NT rows each share one ring of key tiles.
 #include <cuda_fp16.h>
@@ -38,6 +40,7 @@
 #endif
 
 namespace attnq8 {
+using namespace q8;
 
 constexpr int D = SHRIKE_HEAD_DIM;
 static_assert(D % 16 == 0 && D >= 16 && D <= 256, "head sizes are multiples of 16 up to 256");
@@ -51,7 +54,6 @@ constexpr int TILE = KEYS * D;           // bytes of a step's key (or value) cod
 constexpr int SCALES = 2 * KEYS * 4;     // of both kinds of a step's scales
 constexpr int RING = 3 * TILE + 2 * SCALES;   // a warp's share of the few-rows form
 constexpr int STEP_BYTES = 2 * TILE + SCALES;   // a step of the other form: keys, values, scales
-constexpr float LOG2E = 1.4426950408889634f;
 constexpr int MAX_SPLITS = 64;
 
 struct Args {
@@ -73,11 +75,6 @@ struct Args {
   int* arrivals;       // [(entry, kv head, row tile)]: CTAs that have left their share; zero between launches
 };
 
-__device__ __forceinline__ float fast_exp2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 __device__ __forceinline__ unsigned smem_u32(const void* p) { return static_cast<unsigned>(__cvta_generic_to_shared(p)); }
 __device__ __forceinline__ void copy16(unsigned dst, const void* src, bool there) {   // zeros where there is nothing
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
@@ -94,18 +91,8 @@ __device__ __forceinline__ void mma(float (&c)[4], const unsigned (&a)[4], unsig
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ unsigned pack_half(float lo, float hi) {
-  const __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const unsigned*>(&h);
-}
 __device__ __forceinline__ float low_half(unsigned v) { return __low2float(*reinterpret_cast<const __half2*>(&v)); }
 __device__ __forceinline__ float high_half(unsigned v) { return __high2float(*reinterpret_cast<const __half2*>(&v)); }
-// Two codes, biased by 128 in bytes 0, 1 (or 2, 3) of `biased`, as float16: byte b under 0x64 is 1024 + b.
-template <int SELECT> __device__ __forceinline__ unsigned codes_to_half(unsigned biased) {
-  const unsigned raw = __byte_perm(biased, 0x64646464u, SELECT), offset = 0x64806480u;   // 1152 twice
-  const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&raw), *reinterpret_cast<const __half2*>(&offset));
-  return *reinterpret_cast<const unsigned*>(&h);
-}
 // The key of column n of a group of eight columns.
 __device__ __forceinline__ constexpr int key_of(int n) { return n ^ ((n >> 1) & 1); }
 // What the 16-byte chunks of a row are exchanged by.
@@ -115,17 +102,6 @@ __device__ __forceinline__ int swizzle(int row) {
   return 0;
 }
 __device__ __forceinline__ int chunk_at(int row, int chunk) { return row * D + ((chunk ^ swizzle(row)) << 4); }
-
-// F's range: sums of 2^(z - m) stay within float32 for any count of keys, and weights of 2^-19 of the largest above its least.
-// The largest scale that a store leaves is below 2^122: a weight is then below 2^15 if the base does not lag, and where a step's
-// largest scale is above F's range it does not.
-constexpr int LEAST_EXPONENT = -93, MOST_EXPONENT = 107, SCALE_BITS = 8;
-constexpr float BASE_LAG = 6.0f;   // float16's largest power of two is 2^15: 2^9 times 2^6
-// A magnitude's bits (which order as the magnitudes do), 0 for infinities and NaN.
-__device__ __forceinline__ unsigned finite_bits(float x) {
-  const unsigned bits = __float_as_uint(x) & 0x7fffffffu;
-  return bits < 0x7f800000u ? bits : 0u;
-}
 
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -145,14 +121,6 @@ __device__ __forceinline__ float4 load_peer4(unsigned address) {
   asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(address) : "memory");
   return v;
 }
-
-// x 2^d for d <= 0, also where 2^d is below float32's range: a sum under the least exponent F (a row whose values were all zeros
-// so far) becomes one under a large one, 2^200 smaller.  Outputs need not go that far: they are nothing beside the values that F
-// rose for.
-__device__ __forceinline__ float scale_sum(float x, float d) { return x * fast_exp2(fmaxf(d, -126.f)) * fast_exp2(fminf(d + 126.f, 0.f)); }
-
-// 2^e for e in [-126, 127].
-__device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e + 127) << 23); }
 
 // Where a lane's key lies: its row among all codes, its place among the scales, and whether it exists.  A key that does not
 // has scales of zero and whatever codes the pool's first row holds: codes are finite whatever they are, so it counts as zeros.

@@ -45,6 +45,7 @@
 
 namespace tcq8 {
 using namespace bw;
+using namespace q8;
 
 constexpr int D = SHRIKE_HEAD_DIM;
 constexpr int BM = 128;                         // query rows of one chain
@@ -59,20 +60,10 @@ constexpr int KV_TILE = HALVES * KV_HALF;
 constexpr int RAW_TILE = KEYS * D;             // a tile's codes
 constexpr int WARPS = 28, THREADS = WARPS * 32;
 constexpr unsigned CHAIN_COLS = 256, P_COL = 64, O_COL = 128, TMEM_COLS = 512;   // as in attention_tcgen05.cu
-constexpr float LOG2E = 1.4426950408889634f;
-constexpr int LEAST_EXPONENT = -93, MOST_EXPONENT = 107, SCALE_BITS = 8;   // as in attention_q8.cu
-constexpr float BASE_LAG = 6.0f;
 constexpr int NOT_FINITE = 4096;   // above any exponent
 
 enum : int { ERR_PRODUCER = 61, ERR_CONVERT = 62, ERR_MMA = 63, ERR_SOFTMAX = 64, ERR_DRAIN = 65, ERR_ALIGNMENT = 66 };
 
-__device__ __forceinline__ float fast_exp2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-// x 2^d for d <= 0, also where 2^d is below float32's range (as in attention_q8.cu).
-__device__ __forceinline__ float scale_sum(float x, float d) { return x * fast_exp2(fmaxf(d, -126.f)) * fast_exp2(fminf(d + 126.f, 0.f)); }
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -100,21 +91,6 @@ __device__ __forceinline__ unsigned long long mul_pair(unsigned long long a, uns
   unsigned long long d;
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
-}
-__device__ __forceinline__ unsigned pack_half(float lo, float hi) {
-  const __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const unsigned*>(&h);
-}
-__device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e + 127) << 23); }
-__device__ __forceinline__ unsigned finite_bits(float x) {
-  const unsigned bits = __float_as_uint(x) & 0x7fffffffu;
-  return bits < 0x7f800000u ? bits : 0u;
-}
-// Two codes, biased by 128 in bytes 0, 1 (or 2, 3) of `biased`, as float16: byte b under 0x64 is 1024 + b.
-template <int SELECT> __device__ __forceinline__ unsigned codes_to_half(unsigned biased) {
-  const unsigned raw = __byte_perm(biased, 0x64646464u, SELECT), offset = 0x64806480u;   // 1152 twice
-  const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&raw), *reinterpret_cast<const __half2*>(&offset));
-  return *reinterpret_cast<const unsigned*>(&h);
 }
 // kind::f16 instruction descriptor: D float32, A and B float16, A K-major; B K-major or MN-major.
 __device__ __forceinline__ unsigned half_descriptor(int m, int n, bool b_mn_major) {

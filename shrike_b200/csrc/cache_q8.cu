@@ -128,7 +128,9 @@ kv_write_q8_kernel(const T* __restrict__ k_new, const T* __restrict__ v_new, lon
 // ---- bias, rotation and store of a fused q/k/v projection
 // As rope_kv_write_kernel (its formulas, its order of operations: queries get the same bits), with keys and values into 8-bit
 // pages.  A warp owns a head at a time, since a row's largest magnitude is needed before its first code; a block is one
-// token (a slice of its heads where tokens are few) and forms the token's angles once.
+// token (a slice of its heads where tokens are few) and forms the token's angles once.  Its accesses are an element a lane wide,
+// queries included: 28 heads of 128 over 4 kv heads in bfloat16 take 2.2 us for a token, 10.6 for 512 and 21.6 for 2,048 (55 MB:
+// 8.3 at the measured bandwidth), where the store into bfloat16 pages takes 1.3, 4.9 and 10.7.
 template <typename T>
 __global__ void __launch_bounds__(256)
 rope_kv_write_q8_kernel(const float* __restrict__ qkv, const float* __restrict__ bias, const int* __restrict__ positions,
