@@ -65,3 +65,21 @@ def test_batches_with_padding_rows(tmp_path, monkeypatch, dtype, key, count):
                 assert margin < 2 * tol, f"token {position}: engine {a}, plain {b}, gap {margin}"
                 break
     engine._check_kernels()
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("key", ["A", "B", "C"])
+def test_what_a_pool_held_before_has_no_part_in_it(tmp_path, dtype, key):
+    """Places that nobody has written hold any codes and scales of NaN: the same tokens as from an empty pool."""
+    folder = make_model_folder(tmp_path, key)
+    prompts = [random_tokens(TINY[key]["vocab_size"], n, 90 + n) for n in (1, 17, 40, 5)]
+    outs = []
+    for poison in (False, True):
+        engine = LLMEngine(str(folder), block_size=PAGE_SIZES[key], num_blocks=64, max_tokens_per_step=24, dtype=dtype, kv_cache="int8")
+        if poison:
+            for codes, scales in zip(engine.runner.storage.kv, engine.runner.storage.scales):
+                codes.random_(-127, 128)
+                scales.fill_(float("nan"))
+        outs.append(engine.generate(prompts, SamplingParams(max_new_tokens=8, ignore_eos=True)))
+        engine._check_kernels()
+    assert outs[0] == outs[1]
