@@ -4,7 +4,9 @@ import pytest
 import torch
 
 from shrike_b200 import SamplingParams
+from shrike_b200.cache import quantised
 from shrike_b200.engine.llm_engine import LLMEngine
+from shrike_b200.ops import quantised_cache
 from tests.gpu_common import TOL, cuda_ops
 from tests.helpers import make_model_folder, random_tokens
 from tests.plain import plain_model as pm
@@ -83,3 +85,13 @@ def test_what_a_pool_held_before_has_no_part_in_it(tmp_path, dtype, key):
         outs.append(engine.generate(prompts, SamplingParams(max_new_tokens=8, ignore_eos=True)))
         engine._check_kernels()
     assert outs[0] == outs[1]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_the_calls_without_the_native_module(monkeypatch, dtype):
+    """The same launches where what a call asks of its tensors is asked from Python."""
+    monkeypatch.setattr(quantised_cache, "_look", lambda: quantised_cache.PlainLook)
+    monkeypatch.setattr(quantised, "look_pages", None)
+    check_store_and_read_back(dtype, 33, 3, 32, 8)
+    check_attention(dtype, 7, 1, 128, 16, [1, 1, 1], [1, 300, 517])
+    check_attention(dtype, 14, 2, 64, 16, [70, 1, 2], [300, 40, 129], window=40)
